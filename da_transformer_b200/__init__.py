@@ -17,7 +17,13 @@ from .dag_loss import (  # noqa: F401
 )
 
 from .criterion_glue import dag_loss_mean, dag_match, glat_alignment  # noqa: F401
-from .graph_ops import dag_links_from_heads, dag_node_passing_prob, dag_viterbi_decode  # noqa: F401
+from .graph_ops import (  # noqa: F401
+    dag_links_from_heads,
+    dag_node_passing_prob,
+    dag_relative_buckets,
+    dag_viterbi_decode,
+)
+from .policy_loss import dag_policy_loss, dag_preference_loss  # noqa: F401
 from .torch_twins import (  # noqa: F401
     torch_dag_best_alignment,
     torch_dag_logsoftmax_gather_inplace,

@@ -26,10 +26,12 @@ EXPORTS = (
     "dat_links_from_heads", "dat_links_from_heads_backward", "dat_node_passing_prob",
     "dat_viterbi_decode", "dat_viterbi_decode_workspace_bytes", "dat_dag_loss_fast_flagged",
     "dat_upload_links", "dat_upload_links_bytes", "dat_upload_links_head_rows",
+    "dat_links_from_heads_biased", "dat_links_from_heads_biased_backward", "dat_links_bias_workspace_bytes",
+    "dat_policy_loss", "dat_policy_loss_backward", "dat_policy_loss_workspace_bytes", "dat_preference_loss",
 )
 
 _lib = None
-_vp, _i64, _i32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int
+_vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int, ctypes.c_float
 
 
 def _declare(lib):
@@ -90,6 +92,22 @@ def _declare(lib):
     lib.dat_logsoftmax_gather_backward_fused.restype = _i32
     lib.dat_logsoftmax_gather_backward_fused.argtypes = [_vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64,
                                                          _i64, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp]
+    lib.dat_links_from_heads_biased.restype = _i32
+    lib.dat_links_from_heads_biased.argtypes = [_vp] * 4 + [_i32] + [_vp] * 5 + [_i32] * 4 + [_vp]
+    lib.dat_links_bias_workspace_bytes.restype = ctypes.c_size_t
+    lib.dat_links_bias_workspace_bytes.argtypes = [_i32] * 4
+    lib.dat_links_from_heads_biased_backward.restype = _i32
+    lib.dat_links_from_heads_biased_backward.argtypes = [_vp] * 5 + [_i32] + [_vp] * 8 + [_i32] * 4 + [_vp]
+    lib.dat_policy_loss_workspace_bytes.restype = ctypes.c_size_t
+    lib.dat_policy_loss_workspace_bytes.argtypes = [_i32] * 2
+    lib.dat_policy_loss.restype = _i32
+    lib.dat_policy_loss.argtypes = [_vp, _vp, _i32, _vp, _vp, _vp, _i64, _i64, _vp, _vp, _vp, _f32, _f32, _f32, _vp, _f32,
+                                    _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]
+    lib.dat_policy_loss_backward.restype = _i32
+    lib.dat_policy_loss_backward.argtypes = [_vp, _vp, _i32, _vp, _vp, _f32, _vp, _vp, _vp, _i32, _vp, _vp,
+                                             _i32, _i32, _i32, _vp]
+    lib.dat_preference_loss.restype = _i32
+    lib.dat_preference_loss.argtypes = [_vp] * 6 + [ctypes.c_double] * 2 + [_i32] + [_vp] * 5 + [_i32, _vp]
 
 
 def lib():
@@ -126,6 +144,12 @@ def require_cuda(*tensors):
     for t in tensors:
         if t is not None and not t.is_cuda:
             raise RuntimeError("all tensors of the custom cuda operations must be CUDA tensors")
+
+
+def require_same_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise RuntimeError(f"{name} is on {t.device}, expected {device}")
 
 
 def stream_ptr(device):

@@ -15,33 +15,28 @@
 // HBM-bound.  Algorithmic bytes: forward reads the upper triangle of content once
 // (~ B*L*L*H*4 / 2) and writes B*L*K*4; backward reads the same triangle plus the band gradient and
 // writes the dense [B,L,L,H] gradient once (zeros included, like autograd's result).
-#include "dat_common.cuh"
+#include "links_common.cuh"
 
 namespace dat {
 
 constexpr int kLinksThreads = 128;   // 256 and 64 threads per vertex row were slower (0.25 / 0.26 against 0.22 ms forward)
 
-struct LinksMask {
-    const int64_t *bound_end;      // [B, L]: successors j <= bound_end[b,i] (decoding), or null
-    const unsigned char *nonpad;   // [B, L]: successor j allowed iff nonpad[b,j] != 0 (training), or null
-};
-
-// first / last successor of vertex i inside the band and the graph: j in [i+1, jhi]
-__device__ __forceinline__ int links_jhi(int i, int L, int K, const LinksMask &mk, int64_t row) {
-    int jhi = i + K < L - 1 ? i + K : L - 1;
-    if (mk.bound_end) {
-        const int64_t be = mk.bound_end[row];
-        jhi = be < jhi ? (int)be : jhi;
-    }
-    return jhi;
-}
-
-// Stages content[b,i,j,:] for j in [i+1, jhi] into sm[(j-i-1)*H + h]; masked columns become -inf.
+// Stages content[b,i,j,:] (+ bias) for j in [i+1, jhi] into sm[(j-i-1)*H + h]; masked columns become -inf.
+template <bool kBias>
 __device__ __forceinline__ void links_stage_row(const float *__restrict__ crow, float *sm, int i, int jhi,
-                                                int H, const unsigned char *np_row) {
+                                                int H, const unsigned char *np_row, const LinksBias &lb) {
     const int n = (jhi - i) * H;   // may be <= 0
     const float *src = crow + (size_t)(i + 1) * H;
-    if ((H & 3) == 0) {
+    if (kBias) {
+        bool bad = false;
+        for (int x = threadIdx.x; x < n; x += kLinksThreads) {
+            const int d = x / H;
+            const float t = links_bias1(lb, d, x - d * H, H, bad);
+            const bool dead = (np_row && !np_row[i + 1 + d]) || t == -INFINITY;   // also where the score is +inf or NaN
+            sm[x] = dead ? -INFINITY : __ldg(src + x) + t;
+        }
+        if (bad && lb.status) atomicOr(lb.status, DAT_STATUS_BAD_INDEX);
+    } else if ((H & 3) == 0) {
         const float4 *s4 = reinterpret_cast<const float4 *>(src);
         float4 *d4 = reinterpret_cast<float4 *>(sm);
         for (int x = threadIdx.x; x < n / 4; x += kLinksThreads) {
@@ -88,8 +83,9 @@ __device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, f
     __syncthreads();
 }
 
+template <bool kBias>
 __global__ void __launch_bounds__(kLinksThreads)
-links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk,
+links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk, LinksBias lb,
                  float *__restrict__ links, float *__restrict__ head_lse, int L, int H, int K) {
     extern __shared__ __align__(16) float lsm[];
     const int64_t row = blockIdx.x;          // b * L + i
@@ -104,7 +100,7 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
     const int jhi = links_jhi(i, L, K, mk, row);
     const int nj = jhi - i > 0 ? jhi - i : 0;
     const unsigned char *np_row = mk.nonpad ? mk.nonpad + b * L : nullptr;
-    links_stage_row(content + row * (size_t)L * H, sm, i, jhi, H, np_row);
+    links_stage_row<kBias>(content + row * (size_t)L * H, sm, i, jhi, H, np_row, lb);
     if (tid < H) gate_s[tid] = log_gates[row * H + tid];
     __syncthreads();
     links_head_lse(sm, nj, H, part_m, part_s, lse_s);
@@ -136,10 +132,11 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
 //     d / d c[j,h] = G[j] p[j,h] - exp(c[j,h] - lse_h) * S_h
 // grad_content is written for the whole [L,H] row (zeros outside the valid successors); it may alias
 // content (a CTA has its row in shared memory before it writes).
+template <bool kBias>
 __global__ void __launch_bounds__(kLinksThreads)
 links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
                  const float *__restrict__ log_gates, const float *__restrict__ links,
-                 const float *__restrict__ head_lse, LinksMask mk, float *grad_content,
+                 const float *__restrict__ head_lse, LinksMask mk, LinksBias lb, float *grad_content,
                  float *__restrict__ grad_log_gates, int L, int H, int K) {
     extern __shared__ __align__(16) float lsm[];
     const int64_t row = blockIdx.x;
@@ -156,7 +153,7 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
     const int jhi = links_jhi(i, L, K, mk, row);
     const int nj = jhi - i > 0 ? jhi - i : 0;
     const unsigned char *np_row = mk.nonpad ? mk.nonpad + b * L : nullptr;
-    links_stage_row(content + row * (size_t)L * H, sm, i, jhi, H, np_row);
+    links_stage_row<kBias>(content + row * (size_t)L * H, sm, i, jhi, H, np_row, lb);
     for (int d = tid; d < nj; d += kLinksThreads) {
         gl_s[d] = grad_links[row * (size_t)K + d];
         lk_s[d] = links[row * (size_t)K + d];
@@ -476,6 +473,44 @@ static size_t links_smem_bwd(int L, int H) {
     return ((size_t)(L - 1) * H + 2 * (size_t)(L - 1) + kLinksThreads + 3 * H) * sizeof(float) + 16;
 }
 
+// The kernels of one CTA per vertex row, any head count up to kLinksThreads.
+template <bool kBias>
+int links_fwd_rows(const float *content, const float *log_gates, const LinksMask &mk, const LinksBias &lb, float *links,
+                   float *head_lse, int bsz, int prelen, int heads, int translen, cudaStream_t st, const DeviceInfo &di,
+                   const char *who) {
+    DAT_REQUIRE(heads <= kLinksThreads, DAT_ERR_UNSUPPORTED, "%s: heads=%d exceeds %d", who, heads, kLinksThreads);
+    const size_t smem = links_smem_fwd(prelen, heads);
+    DAT_REQUIRE(smem <= (size_t)di.max_smem_optin, DAT_ERR_UNSUPPORTED,
+                "%s: prelen*heads = %d*%d needs %zu bytes of shared memory", who, prelen, heads, smem);
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(links_fwd_kernel<kBias>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)smem) != cudaSuccess)
+        return check_launch(who);
+    links_fwd_kernel<kBias><<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, st>>>(
+        content, log_gates, mk, lb, links, head_lse, prelen, heads, translen);
+    return check_launch(who);
+}
+template <bool kBias>
+int links_bwd_rows(const float *grad_links, const float *content, const float *log_gates, const float *links,
+                   const float *head_lse, const LinksMask &mk, const LinksBias &lb, float *grad_content,
+                   float *grad_log_gates, int bsz, int prelen, int heads, int translen, cudaStream_t st,
+                   const DeviceInfo &di, const char *who) {
+    DAT_REQUIRE(heads <= kLinksThreads, DAT_ERR_UNSUPPORTED, "%s: heads=%d exceeds %d", who, heads, kLinksThreads);
+    const size_t smem = links_smem_bwd(prelen, heads);
+    DAT_REQUIRE(smem <= (size_t)di.max_smem_optin, DAT_ERR_UNSUPPORTED,
+                "%s: prelen*heads = %d*%d needs %zu bytes of shared memory", who, prelen, heads, smem);
+    if (smem > 48 * 1024 && cudaFuncSetAttribute(links_bwd_kernel<kBias>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 (int)smem) != cudaSuccess)
+        return check_launch(who);
+    links_bwd_kernel<kBias><<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, st>>>(
+        grad_links, content, log_gates, links, head_lse, mk, lb, grad_content, grad_log_gates, prelen, heads, translen);
+    return check_launch(who);
+}
+template int links_fwd_rows<true>(const float *, const float *, const LinksMask &, const LinksBias &, float *, float *,
+                                  int, int, int, int, cudaStream_t, const DeviceInfo &, const char *);
+template int links_bwd_rows<true>(const float *, const float *, const float *, const float *, const float *,
+                                  const LinksMask &, const LinksBias &, float *, float *, int, int, int, int,
+                                  cudaStream_t, const DeviceInfo &, const char *);
+
 }  // namespace dat
 
 extern "C" {
@@ -506,17 +541,8 @@ int dat_links_from_heads(const float *content, const float *log_gates, const int
         }
         return check_launch(who);
     }
-    const size_t smem = links_smem_fwd(prelen, heads);
-    DAT_REQUIRE(smem <= (size_t)di.max_smem_optin, DAT_ERR_UNSUPPORTED,
-                "%s: prelen*heads = %d*%d needs %zu bytes of shared memory", who, prelen, heads, smem);
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(links_fwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-            cudaSuccess)
-        return check_launch(who);
-    const LinksMask mk{bound_end, nonpad};
-    links_fwd_kernel<<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, static_cast<cudaStream_t>(stream)>>>(
-        content, log_gates, mk, links, head_lse, prelen, heads, translen);
-    return check_launch(who);
+    return links_fwd_rows<false>(content, log_gates, LinksMask{bound_end, nonpad}, LinksBias{}, links, head_lse, bsz,
+                                 prelen, heads, translen, static_cast<cudaStream_t>(stream), di, who);
 }
 
 int dat_links_from_heads_backward(const float *grad_links, const float *content, const float *log_gates,
@@ -550,18 +576,9 @@ int dat_links_from_heads_backward(const float *grad_links, const float *content,
 #undef DAT_LINKS_BWD
         return check_launch(who);
     }
-    const size_t smem = links_smem_bwd(prelen, heads);
-    DAT_REQUIRE(smem <= (size_t)di.max_smem_optin, DAT_ERR_UNSUPPORTED,
-                "%s: prelen*heads = %d*%d needs %zu bytes of shared memory", who, prelen, heads, smem);
-    if (smem > 48 * 1024 &&
-        cudaFuncSetAttribute(links_bwd_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) !=
-            cudaSuccess)
-        return check_launch(who);
-    const LinksMask mk{bound_end, nonpad};
-    links_bwd_kernel<<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, static_cast<cudaStream_t>(stream)>>>(
-        grad_links, content, log_gates, links, head_lse, mk, grad_content, grad_log_gates, prelen, heads,
-        translen);
-    return check_launch(who);
+    return links_bwd_rows<false>(grad_links, content, log_gates, links, head_lse, LinksMask{bound_end, nonpad},
+                                 LinksBias{}, grad_content, grad_log_gates, bsz, prelen, heads, translen,
+                                 static_cast<cudaStream_t>(stream), di, who);
 }
 
 }  // extern "C"

@@ -1,0 +1,558 @@
+// Clipped policy loss with a KL term over the vertices' logits, forward and backward, for sm_100a.
+//
+// A step of a sampled path takes a token at a vertex and a transition to the next vertex, so that
+//     lp[b,l] = log softmax(x[b,l,:])[token] (+ link_logp[b,l])
+// and with r = exp(lp - old), advantage A and the active vertices N,
+//     term = -min(r A, clip(r, 1-low, 1+high) A),     loss = 1/N sum_active (term + beta KL).
+// KL, one of
+//     full      sum_v p_v (log p_v - log q_v) over the vocabulary, q = softmax(y) of the reference model,
+//     estimate  e^u - u - 1, u = ref_logp - lp.
+// Gradient of the loss with respect to x_v of an active vertex, with delta the one-hot of the token:
+//     1/N [ c (delta_v - p_v) + beta p_v (d_v - E_p d) ],   d = x - y (full KL only),
+//     c = -A r where the clip does not hold the term, 0 where it does, + beta (1 - e^u) with the estimate.
+//
+// HBM-bound: the logits of the active vertices are read once and the dense gradient is written once.  To read
+// them once the gradient is written by the forward, while the row is still in the L2 cache (one CTA per row: a
+// row and its reference are at most a few hundred KB, all rows in flight a few ten MB of the 126 MB), scaled by
+// the gradient that the caller expects the loss to receive (1, or a loss scale).  The backward compares that
+// with what arrives, on the device, and computes the gradient again from the logits where they differ.
+//
+// Numerics: fp32 with exact differences to the running maximum; log-probabilities, ratios and the KL of a row
+// are put together in 64 bits by one thread (a 32-bit log-probability near -10 carries 5e-7, which would show
+// in the ratio), sums over rows in 64 bits in a fixed order.  d is taken relative to its value at v = 0, so
+// that a constant between the two models' logits does not cancel.
+#include "dat_common.cuh"
+
+namespace dat {
+
+constexpr int kPoThreads = 256;
+constexpr int kPoWarps = kPoThreads / 32;
+constexpr int kPoChunk = 256;   // rows whose results are summed together
+constexpr int kPoSums = 5;      // terms, KL, ratios, clipped, active
+
+// start of the caller's workspace
+struct PolicyHead {
+    double inv_n;      // 1 / active rows (1 / max(1, n))
+    float scale;       // gradient that the forward assumed for the loss
+    int chunks_done;
+};
+
+struct PolicyArgs {
+    const void *x, *y;            // logits [rows, V]; y null without the full KL
+    const int64_t *tokens;        // [rows]
+    const float *old_logp;        // [rows]
+    const float *advantage;
+    int64_t adv_b, adv_l;         // strides of the advantage
+    const float *link_logp;       // [rows] or null
+    const float *ref_logp;        // [rows] or null
+    const unsigned char *mask;    // [rows] or null
+    float beta, clip_low, clip_high;
+    float *loss;                  // [1]
+    double *stats;                // [kPoSums]
+    float *logp, *kl;             // [rows]
+    float4 *row_state;            // [rows]: M, 1 / S, c / N, E_p d (for the backward), or null
+    void *grad;                   // [rows, V] or null
+    PolicyHead *head;
+    int *done;                    // [chunks]
+    float4 *row_sums;             // [rows]: term, KL, ratio, clipped
+    double *chunk_sums;           // [chunks, kPoSums]
+    int32_t *status;
+    int64_t rows;
+    int L, V;
+    bool vec;                     // x, y and grad start on 16-byte boundaries
+};
+
+// counts the active rows and clears the counters
+__global__ void __launch_bounds__(1024)
+policy_prep_kernel(const unsigned char *__restrict__ mask, int64_t rows, PolicyHead *head, int *done, int chunks,
+                   const float *scale_ptr, float scale) {
+    __shared__ long long part[32];
+    const int tid = threadIdx.x;
+    long long n = 0;
+    if (mask)
+        for (int64_t r = tid; r < rows; r += 1024) n += mask[r] != 0;
+    for (int c = tid; c < chunks; c += 1024) done[c] = 0;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    if ((tid & 31) == 0) part[tid >> 5] = n;
+    __syncthreads();
+    if (tid == 0) {
+        long long t = 0;
+        for (int w = 0; w < 32; w++) t += part[w];
+        if (!mask) t = rows;
+        head->inv_n = 1.0 / (double)(t > 0 ? t : 1);
+        head->scale = scale_ptr ? *scale_ptr : scale;
+        head->chunks_done = 0;
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void policy_split(bool vec, const T *p, int V, int &head, int &nvec) {
+    constexpr int kVec = Elem<T>::kVec;
+    if (!vec) {
+        head = V;
+        nvec = 0;
+        return;
+    }
+    const int mis = (int)((reinterpret_cast<uintptr_t>(p) & 15u) / sizeof(T));
+    head = mis ? kVec - mis : 0;
+    if (head > V) head = V;
+    nvec = (V - head) / kVec;
+}
+
+// Running state of a thread over its share of a row.
+template <bool kRef>
+struct PolicyState {
+    float m = kNegBig, s = 0.f, t = 0.f;   // maximum, sum e^(x-m), sum e^(x-m) d
+    float my = kNegBig, sy = 0.f;          // the same of the reference
+    template <int N>
+    __device__ __forceinline__ void update(const float (&x)[N], const float (&y)[N], float off) {
+        float v = x[0];
+#pragma unroll
+        for (int i = 1; i < N; i++) v = fmaxf(v, x[i]);
+        if (v > m) {
+            const float f = ex2((m - v) * kLog2e);
+            s *= f;
+            if (kRef) t *= f;
+            m = v;
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            const float e = ex2((x[i] - m) * kLog2e);
+            s += e;
+            // where p = 0 (a score of -inf) d may be -inf or NaN: fmaxf makes it a number, the product 0
+            if (kRef) t = fmaf(e, fmaxf((x[i] - off) - y[i], kNegBig), t);
+        }
+        if (kRef) {
+            v = y[0];
+#pragma unroll
+            for (int i = 1; i < N; i++) v = fmaxf(v, y[i]);
+            if (v > my) {
+                sy *= ex2((my - v) * kLog2e);
+                my = v;
+            }
+#pragma unroll
+            for (int i = 0; i < N; i++) sy += ex2((y[i] - my) * kLog2e);
+        }
+    }
+};
+
+// d at v = 0, or 0 where that is no number
+template <typename T>
+__device__ __forceinline__ float policy_offset(const T *x, const T *y) {
+    const float o = Elem<T>::to_float(x[0]) - Elem<T>::to_float(y[0]);
+    return fabsf(o) < 1e30f ? o : 0.f;
+}
+
+// The gradient of one active row.  a = -c / (N S), w = beta / (N S), each times the loss's gradient; tok_c = c / N
+// times it, added at the token.
+template <typename T, bool kRef>
+__device__ __forceinline__ void policy_grad_row(const T *x, const T *y, T *g, bool vec, int V, float M, float a, float w,
+                                                float mean_d, float off, int64_t tok, float tok_c) {
+    constexpr int kVec = Elem<T>::kVec;
+    const int tid = threadIdx.x;
+    int head, nvec;
+    policy_split(vec, x, V, head, nvec);
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head), *yv = reinterpret_cast<const uint4 *>(kRef ? y + head : x);
+    uint4 *gv = reinterpret_cast<uint4 *>(g + head);
+    const float base = kRef ? fmaf(-w, mean_d, a) : a;
+    auto one = [&](float xe, float ye) {
+        const float e = ex2((xe - M) * kLog2e);
+        return e * (kRef ? fmaf(w, fmaxf((xe - off) - ye, kNegBig), base) : base);
+    };
+    constexpr int U = 2;
+    for (int v = tid; v < nvec; v += U * kPoThreads) {
+        uint4 ux[U], uy[U];
+#pragma unroll
+        for (int q = 0; q < U; q++)
+            if (v + q * kPoThreads < nvec) {
+                ux[q] = xv[v + q * kPoThreads];
+                if (kRef) uy[q] = yv[v + q * kPoThreads];
+            }
+#pragma unroll
+        for (int q = 0; q < U; q++)
+            if (v + q * kPoThreads < nvec) {
+                float fx[kVec], fy[kVec];
+                Elem<T>::unpack(ux[q], fx);
+                if (kRef) Elem<T>::unpack(uy[q], fy);
+#pragma unroll
+                for (int i = 0; i < kVec; i++) fx[i] = one(fx[i], kRef ? fy[i] : 0.f);
+                gv[v + q * kPoThreads] = Elem<T>::pack(fx);
+            }
+    }
+    for (int e = tid; e < head; e += kPoThreads)
+        g[e] = Elem<T>::from_float(one(Elem<T>::to_float(x[e]), kRef ? Elem<T>::to_float(y[e]) : 0.f));
+    for (int e = head + nvec * kVec + tid; e < V; e += kPoThreads)
+        g[e] = Elem<T>::from_float(one(Elem<T>::to_float(x[e]), kRef ? Elem<T>::to_float(y[e]) : 0.f));
+    __syncthreads();
+    if (tid == 0 && tok >= 0 && tok < V)
+        g[tok] = Elem<T>::from_float(tok_c + one(Elem<T>::to_float(x[tok]), kRef ? Elem<T>::to_float(y[tok]) : 0.f));
+}
+
+template <typename T>
+__device__ __forceinline__ void policy_zero_row(T *g, bool vec, int V) {
+    constexpr int kVec = Elem<T>::kVec;
+    int head, nvec;
+    policy_split(vec, g, V, head, nvec);
+    uint4 *gv = reinterpret_cast<uint4 *>(g + head);
+    for (int v = threadIdx.x; v < nvec; v += kPoThreads) gv[v] = make_uint4(0, 0, 0, 0);
+    for (int e = threadIdx.x; e < head; e += kPoThreads) g[e] = Elem<T>::from_float(0.f);
+    for (int e = head + nvec * kVec + threadIdx.x; e < V; e += kPoThreads) g[e] = Elem<T>::from_float(0.f);
+}
+
+// Sums the rows' results: the CTA that finishes the last row of a chunk adds the chunk's, the one that finishes
+// the last chunk adds the chunks', each in a fixed order.
+__device__ __forceinline__ void policy_sums(const PolicyArgs &a, int64_t row) {
+    __shared__ int last_s;
+    __shared__ double part[kPoSums][kPoWarps];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int chunk = (int)(row / kPoChunk);
+    const int chunks = (int)((a.rows + kPoChunk - 1) / kPoChunk);
+    const int64_t first = (int64_t)chunk * kPoChunk;
+    const int n = a.rows - first < kPoChunk ? (int)(a.rows - first) : kPoChunk;
+    if (tid == 0) {
+        __threadfence();
+        last_s = atomicAdd(a.done + chunk, 1) == n - 1;
+    }
+    __syncthreads();
+    if (!last_s) return;
+    __threadfence();
+    double s[kPoSums] = {};
+    if (tid < n && (!a.mask || a.mask[first + tid])) {
+        const float4 r = __ldcg(a.row_sums + first + tid);
+        s[0] = r.x;
+        s[1] = r.y;
+        s[2] = r.z;
+        s[3] = r.w;
+        s[4] = 1.0;
+    }
+#pragma unroll
+    for (int k = 0; k < kPoSums; k++) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) s[k] += __shfl_xor_sync(0xffffffffu, s[k], o);
+        if (lane == 0) part[k][warp] = s[k];
+    }
+    __syncthreads();
+    if (tid == 0) {
+        for (int k = 0; k < kPoSums; k++) {
+            double t = 0.0;
+            for (int w = 0; w < kPoWarps; w++) t += part[k][w];
+            a.chunk_sums[(int64_t)chunk * kPoSums + k] = t;
+        }
+        __threadfence();
+        last_s = atomicAdd(&a.head->chunks_done, 1) == chunks - 1;
+    }
+    __syncthreads();
+    if (!last_s) return;
+    __threadfence();
+    if (warp < kPoSums) {
+        double t = 0.0;
+        for (int c = lane; c < chunks; c += 32) t += __ldcg(a.chunk_sums + (int64_t)c * kPoSums + warp);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (lane == 0) {
+            a.stats[warp] = t;
+            part[warp][0] = t;
+        }
+    }
+    __syncthreads();
+    if (tid == 0) *a.loss = (float)((part[0][0] + (double)a.beta * part[1][0]) * a.head->inv_n);
+}
+
+template <typename T, bool kRef>
+__global__ void __launch_bounds__(kPoThreads)
+policy_fwd_kernel(PolicyArgs a) {
+    constexpr int kVec = Elem<T>::kVec;
+    __shared__ float red[5][kPoWarps];
+    __shared__ float row_s[4];   // coefficients of the row's gradient
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int64_t row = blockIdx.x;
+    const int V = a.V;
+    T *g = a.grad ? static_cast<T *>(a.grad) + row * V : nullptr;
+    if (a.mask && !a.mask[row]) {
+        if (g) policy_zero_row(g, a.vec, V);
+        if (tid == 0) {
+            a.logp[row] = 0.f;
+            a.kl[row] = 0.f;
+            if (a.row_state) a.row_state[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        policy_sums(a, row);
+        return;
+    }
+    const T *x = static_cast<const T *>(a.x) + row * V;
+    const T *y = kRef ? static_cast<const T *>(a.y) + row * V : nullptr;
+    const float off = kRef ? policy_offset(x, y) : 0.f;
+    int head, nvec;
+    policy_split(a.vec, x, V, head, nvec);
+    const uint4 *xv = reinterpret_cast<const uint4 *>(x + head), *yv = reinterpret_cast<const uint4 *>(kRef ? y + head : x);
+    PolicyState<kRef> st;
+    constexpr int U = 2;
+    int v = tid;
+    for (; v + (U - 1) * kPoThreads < nvec; v += U * kPoThreads) {
+        uint4 ux[U], uy[U];
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+            ux[q] = xv[v + q * kPoThreads];
+            if (kRef) uy[q] = yv[v + q * kPoThreads];
+        }
+        float fx[U * kVec], fy[U * kVec];
+#pragma unroll
+        for (int q = 0; q < U; q++) {
+            Elem<T>::unpack(ux[q], fx + q * kVec);
+            if (kRef) Elem<T>::unpack(uy[q], fy + q * kVec);
+        }
+        st.update(fx, fy, off);
+    }
+    for (; v < nvec; v += kPoThreads) {
+        float fx[kVec], fy[kVec];
+        Elem<T>::unpack(xv[v], fx);
+        if (kRef) Elem<T>::unpack(yv[v], fy);
+        st.update(fx, fy, off);
+    }
+    for (int part = 0; part < 2; part++) {
+        const int e0 = part ? head + nvec * kVec : 0, e1 = part ? V : head;
+        for (int e = e0 + tid; e < e1; e += kPoThreads) {
+            const float fx[1] = {Elem<T>::to_float(x[e])}, fy[1] = {kRef ? Elem<T>::to_float(y[e]) : 0.f};
+            st.update(fx, fy, off);
+        }
+    }
+    // the row's maxima, then its sums
+    const float wm = warp_max(st.m), wmy = kRef ? warp_max(st.my) : 0.f;
+    if (lane == 0) {
+        red[0][warp] = wm;
+        red[1][warp] = wmy;
+    }
+    __syncthreads();
+    float M = red[0][0], My = red[1][0];
+#pragma unroll
+    for (int w = 1; w < kPoWarps; w++) {
+        M = fmaxf(M, red[0][w]);
+        My = fmaxf(My, red[1][w]);
+    }
+    const float f = ex2((st.m - M) * kLog2e);
+    const float ws = warp_sum(st.s * f);
+    const float wt = kRef ? warp_sum(st.t * f) : 0.f, wsy = kRef ? warp_sum(st.sy * ex2((st.my - My) * kLog2e)) : 0.f;
+    if (lane == 0) {
+        red[2][warp] = ws;
+        red[3][warp] = wt;
+        red[4][warp] = wsy;
+    }
+    __syncthreads();
+    const int64_t tok = a.tokens[row];
+    if (tid == 0) {
+        double S = 0.0, Tt = 0.0, Sy = 0.0;
+        for (int w = 0; w < kPoWarps; w++) {
+            S += red[2][w];
+            Tt += red[3][w];
+            Sy += red[4][w];
+        }
+        const bool ok = tok >= 0 && tok < V;
+        if (!ok && a.status) atomicOr(a.status, DAT_STATUS_BAD_INDEX);
+        const int64_t b = row / a.L, l = row - b * a.L;
+        const double A = a.advantage[b * a.adv_b + l * a.adv_l];
+        const double log_s = log(S);
+        double lp = ok ? (double)(Elem<T>::to_float(x[tok])) - (double)M - log_s : __longlong_as_double(0x7ff8000000000000ll);
+        if (a.link_logp) lp += a.link_logp[row];
+        const double r = exp(lp - (double)a.old_logp[row]);
+        const double lo = 1.0 - (double)a.clip_low, hi = 1.0 + (double)a.clip_high;
+        const double ra = r * A, rc = (r < lo ? lo : r > hi ? hi : r) * A;
+        const double term = -(ra < rc ? ra : rc);
+        const bool clipped = (A > 0.0 && r > hi) || (A < 0.0 && r < lo);
+        double c = clipped ? 0.0 : -ra, kl = 0.0, mean_d = 0.0;
+        if (kRef) {
+            mean_d = Tt / S;
+            kl = mean_d - (((double)M - (double)off - (double)My) + log_s - log(Sy));
+        } else if (a.ref_logp) {
+            const double u = (double)a.ref_logp[row] - lp, eu = expm1(u);
+            kl = eu - u;
+            c -= (double)a.beta * eu;
+        }
+        a.logp[row] = (float)lp;
+        a.kl[row] = (float)kl;
+        a.row_sums[row] = make_float4((float)term, (float)kl, (float)r, clipped ? 1.f : 0.f);
+        const double inv_n = a.head->inv_n, up = inv_n * (double)a.head->scale;
+        if (a.row_state) a.row_state[row] = make_float4(M, (float)(1.0 / S), (float)(c * inv_n), (float)mean_d);
+        row_s[0] = (float)(-c * up / S);
+        row_s[1] = (float)((double)a.beta * up / S);
+        row_s[2] = (float)mean_d;
+        row_s[3] = (float)(c * up);
+    }
+    __syncthreads();
+    if (g) policy_grad_row<T, kRef>(x, y, g, a.vec, V, M, row_s[0], row_s[1], row_s[2], off, tok, row_s[3]);
+    policy_sums(a, row);
+}
+
+struct PolicyBackwardArgs {
+    const void *x, *y;
+    const int64_t *tokens;
+    const unsigned char *mask;
+    const float4 *row_state;
+    const PolicyHead *head;
+    const float *grad_loss;     // [1]
+    void *grad;                 // [rows, V]
+    float *grad_link;           // [rows] or null
+    float beta;
+    int64_t rows;
+    int V;
+    bool vec, written;          // written: grad holds the gradient for head->scale
+};
+
+template <typename T, bool kRef>
+__global__ void __launch_bounds__(kPoThreads)
+policy_bwd_kernel(PolicyBackwardArgs a) {
+    const float up = *a.grad_loss;
+    if (a.grad_link)
+        for (int64_t r = (int64_t)blockIdx.x * kPoThreads + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * kPoThreads)
+            a.grad_link[r] = a.row_state[r].z * up;
+    if (!a.grad || (a.written && up == a.head->scale)) return;
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        T *g = static_cast<T *>(a.grad) + row * a.V;
+        if (a.mask && !a.mask[row]) {
+            policy_zero_row(g, a.vec, a.V);
+            continue;
+        }
+        const T *x = static_cast<const T *>(a.x) + row * a.V, *y = kRef ? static_cast<const T *>(a.y) + row * a.V : nullptr;
+        const float4 st = a.row_state[row];
+        const float c = st.z * up;
+        policy_grad_row<T, kRef>(x, y, g, a.vec, a.V, st.x, -c * st.y, (float)((double)a.beta * a.head->inv_n * up * st.y),
+                                 st.w, kRef ? policy_offset(x, y) : 0.f, a.tokens[row], c);
+    }
+}
+
+static int64_t policy_chunks(int64_t rows) { return (rows + kPoChunk - 1) / kPoChunk; }
+
+struct PolicyWorkspace {
+    size_t done, sums, chunk, total;
+    explicit PolicyWorkspace(int64_t rows) {
+        const auto up = [](size_t n) { return (n + 15) / 16 * 16; };
+        done = up(sizeof(PolicyHead));
+        sums = up(done + (size_t)policy_chunks(rows) * sizeof(int));
+        chunk = up(sums + (size_t)rows * sizeof(float4));
+        total = up(chunk + (size_t)policy_chunks(rows) * kPoSums * sizeof(double));
+    }
+};
+
+static bool aligned16(const void *a, const void *b, const void *c) {
+    return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
+}
+
+template <typename T>
+static int policy_fwd_t(const PolicyArgs &a, cudaStream_t st, const char *who) {
+    if (a.y)
+        policy_fwd_kernel<T, true><<<(unsigned)a.rows, kPoThreads, 0, st>>>(a);
+    else
+        policy_fwd_kernel<T, false><<<(unsigned)a.rows, kPoThreads, 0, st>>>(a);
+    return check_launch(who);
+}
+
+template <typename T>
+static int policy_bwd_t(const PolicyBackwardArgs &a, const DeviceInfo &di, cudaStream_t st, const char *who) {
+    int64_t grid = (int64_t)di.sm_count * 6;
+    if (grid > a.rows) grid = a.rows;
+    if (a.y)
+        policy_bwd_kernel<T, true><<<(unsigned)grid, kPoThreads, 0, st>>>(a);
+    else
+        policy_bwd_kernel<T, false><<<(unsigned)grid, kPoThreads, 0, st>>>(a);
+    return check_launch(who);
+}
+
+}  // namespace dat
+
+extern "C" {
+
+size_t dat_policy_loss_workspace_bytes(int bsz, int prelen) {
+    if (bsz < 0 || prelen < 0) return 0;
+    return dat::PolicyWorkspace((int64_t)bsz * prelen).total;
+}
+
+int dat_policy_loss(const void *word_ins_out, const void *ref_logits, int dtype, const int64_t *tokens,
+                    const float *old_logp, const float *advantage, int64_t adv_stride_b, int64_t adv_stride_l,
+                    const float *link_logp, const float *ref_logp, const unsigned char *mask, float kl_coef,
+                    float clip_low, float clip_high, const float *grad_scale_ptr, float grad_scale, float *loss,
+                    double *stats, float *logp, float *kl, float *row_state, void *grad_logits, void *workspace,
+                    int32_t *status, int bsz, int prelen, int vocab, void *stream) {
+    using namespace dat;
+    const char *who = "dat_policy_loss";
+    DAT_REQUIRE(bsz >= 0 && prelen >= 0 && vocab >= 1, DAT_ERR_BAD_ARG, "%s: bad sizes bsz=%d prelen=%d vocab=%d", who, bsz,
+                prelen, vocab);
+    DAT_REQUIRE(loss && stats && workspace, DAT_ERR_BAD_ARG, "%s: null pointer", who);
+    DAT_REQUIRE(!(ref_logits && ref_logp), DAT_ERR_BAD_ARG, "%s: ref_logits and ref_logp exclude each other", who);
+    DAT_REQUIRE(clip_low >= 0.f && clip_high >= 0.f, DAT_ERR_BAD_ARG, "%s: negative clip range", who);
+    const int64_t rows = (int64_t)bsz * prelen;
+    DAT_REQUIRE(rows <= 0x7fffffff, DAT_ERR_UNSUPPORTED, "%s: bsz*prelen = %lld exceeds 2^31-1", who, (long long)rows);
+    DAT_REQUIRE(dtype == DAT_F32 || dtype == DAT_F16 || dtype == DAT_BF16, DAT_ERR_UNSUPPORTED,
+                "%s: unsupported dtype %d (fp32, fp16, bf16 only)", who, dtype);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (rows == 0) {
+        cudaMemsetAsync(loss, 0, sizeof(float), st);
+        cudaMemsetAsync(stats, 0, kPoSums * sizeof(double), st);
+        return check_launch(who);
+    }
+    DAT_REQUIRE(word_ins_out && tokens && old_logp && advantage && logp && kl, DAT_ERR_BAD_ARG, "%s: null pointer", who);
+    const PolicyWorkspace lay(rows);
+    unsigned char *ws = static_cast<unsigned char *>(workspace);
+    PolicyArgs a{};
+    a.x = word_ins_out;
+    a.y = ref_logits;
+    a.tokens = tokens;
+    a.old_logp = old_logp;
+    a.advantage = advantage;
+    a.adv_b = adv_stride_b;
+    a.adv_l = adv_stride_l;
+    a.link_logp = link_logp;
+    a.ref_logp = ref_logp;
+    a.mask = mask;
+    a.beta = kl_coef;
+    a.clip_low = clip_low;
+    a.clip_high = clip_high;
+    a.loss = loss;
+    a.stats = stats;
+    a.logp = logp;
+    a.kl = kl;
+    a.row_state = reinterpret_cast<float4 *>(row_state);
+    a.grad = grad_logits;
+    a.head = reinterpret_cast<PolicyHead *>(ws);
+    a.done = reinterpret_cast<int *>(ws + lay.done);
+    a.row_sums = reinterpret_cast<float4 *>(ws + lay.sums);
+    a.chunk_sums = reinterpret_cast<double *>(ws + lay.chunk);
+    a.status = status;
+    a.rows = rows;
+    a.L = prelen;
+    a.V = vocab;
+    a.vec = aligned16(word_ins_out, ref_logits, grad_logits);
+    policy_prep_kernel<<<1, 1024, 0, st>>>(mask, rows, a.head, a.done, (int)policy_chunks(rows), grad_scale_ptr, grad_scale);
+    if (int rc = check_launch(who)) return rc;
+    switch (dtype) {
+        case DAT_F32: return policy_fwd_t<float>(a, st, who);
+        case DAT_F16: return policy_fwd_t<__half>(a, st, who);
+        default: return policy_fwd_t<__nv_bfloat16>(a, st, who);
+    }
+}
+
+int dat_policy_loss_backward(const void *word_ins_out, const void *ref_logits, int dtype, const int64_t *tokens,
+                             const unsigned char *mask, float kl_coef, const float *row_state, const void *workspace,
+                             const float *grad_loss, int grad_written, void *grad_logits, float *grad_link, int bsz,
+                             int prelen, int vocab, void *stream) {
+    using namespace dat;
+    const char *who = "dat_policy_loss_backward";
+    DAT_REQUIRE(bsz >= 0 && prelen >= 0 && vocab >= 1, DAT_ERR_BAD_ARG, "%s: bad sizes bsz=%d prelen=%d vocab=%d", who, bsz,
+                prelen, vocab);
+    const int64_t rows = (int64_t)bsz * prelen;
+    if (rows == 0 || !(grad_logits || grad_link)) return DAT_OK;
+    DAT_REQUIRE(word_ins_out && tokens && row_state && workspace && grad_loss, DAT_ERR_BAD_ARG, "%s: null pointer", who);
+    DAT_REQUIRE(dtype == DAT_F32 || dtype == DAT_F16 || dtype == DAT_BF16, DAT_ERR_UNSUPPORTED,
+                "%s: unsupported dtype %d (fp32, fp16, bf16 only)", who, dtype);
+    DeviceInfo di;
+    if (!device_info(&di)) return DAT_ERR_NO_DEVICE;
+    const PolicyBackwardArgs a{word_ins_out, ref_logits, tokens, mask, reinterpret_cast<const float4 *>(row_state),
+                               static_cast<const PolicyHead *>(workspace), grad_loss, grad_logits, grad_link, kl_coef, rows,
+                               vocab, aligned16(word_ins_out, ref_logits, grad_logits), grad_written != 0};
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case DAT_F32: return policy_bwd_t<float>(a, di, st, who);
+        case DAT_F16: return policy_bwd_t<__half>(a, di, st, who);
+        default: return policy_bwd_t<__nv_bfloat16>(a, di, st, who);
+    }
+}
+
+}  // extern "C"

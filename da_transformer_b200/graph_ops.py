@@ -10,17 +10,28 @@ All call the C ABI of ``libdat_b200.so``; there is no CPU or PyTorch fallback.
 """
 import torch
 from torch.autograd import Function
+from torch.autograd.function import once_differentiable
 
-from ._native import check, lib, ptr, require_cuda, stream_ptr
+from ._native import check, lib, ptr, require_cuda, require_same_device, stream_ptr
 from .dag_loss import _status_word
 
-__all__ = ["DagLinksFromHeadsFunc", "dag_links_from_heads", "dag_node_passing_prob", "dag_viterbi_decode"]
+__all__ = ["DagLinksFromHeadsFunc", "DagBiasedLinksFunc", "dag_links_from_heads", "dag_relative_buckets",
+           "dag_node_passing_prob", "dag_viterbi_decode"]
 
 
 def _mask_u8(mask):
     if mask is None:
         return None
     return (mask if mask.dtype == torch.uint8 else mask.to(torch.uint8)).contiguous()
+
+
+def _mask_bytes(mask):
+    """The mask as uint8, without a copy where it is a bool tensor."""
+    if mask is None:
+        return None
+    if mask.dtype == torch.bool:
+        return mask.contiguous().view(torch.uint8)
+    return _mask_u8(mask)
 
 
 class DagLinksFromHeadsFunc(Function):
@@ -76,8 +87,105 @@ class DagLinksFromHeadsFunc(Function):
         return grad_content, grad_gates, None, None, None
 
 
+class DagBiasedLinksFunc(Function):
+    """``dag_links_from_heads`` with a learned relative position bias."""
+
+    @staticmethod
+    def forward(ctx, log_multi_content, log_gates, relative_bias, relative_buckets, nonpad_mask, bound_end,
+                max_transition_length):
+        if log_multi_content.dim() != 4 or log_multi_content.size(1) != log_multi_content.size(2):
+            raise RuntimeError("log_multi_content should be [batch, prelen, prelen, heads]")
+        bsz, prelen, _, heads = log_multi_content.shape
+        if log_gates.shape != (bsz, prelen, heads):
+            raise RuntimeError("log_gates should be [batch, prelen, heads]")
+        if relative_bias.dim() != 2 or relative_bias.size(0) < 1 or relative_bias.size(1) != heads:
+            raise RuntimeError("relative_bias should be [num_buckets, heads]")
+        for name, t in (("log_multi_content", log_multi_content), ("log_gates", log_gates),
+                        ("relative_bias", relative_bias)):
+            if t.dtype != torch.float32:
+                raise RuntimeError(f"dag_links_from_heads is implemented for float32 ({name} is {t.dtype})")
+        translen = min(int(max_transition_length), prelen - 1)
+        if translen < 1:
+            raise RuntimeError("max_transition_length must be at least 1 and prelen at least 2")
+        if relative_buckets.dim() != 1 or relative_buckets.dtype != torch.long or relative_buckets.numel() < translen:
+            raise RuntimeError(f"relative_buckets should be a long tensor with at least {translen} distances")
+        if nonpad_mask is not None and nonpad_mask.shape != (bsz, prelen):
+            raise RuntimeError("nonpad_mask should be [batch, prelen]")
+        if bound_end is not None and (bound_end.shape != (bsz, prelen) or bound_end.dtype != torch.long):
+            raise RuntimeError("bound_end should be a long tensor of shape [batch, prelen]")
+        require_cuda(log_multi_content, log_gates, relative_bias, relative_buckets, nonpad_mask, bound_end)
+        dev = log_multi_content.device
+        require_same_device(dev, log_gates=log_gates, relative_bias=relative_bias, relative_buckets=relative_buckets,
+                            nonpad_mask=nonpad_mask, bound_end=bound_end)
+        need_grad = any(ctx.needs_input_grad[:3])
+        with torch.cuda.device(dev):
+            content = log_multi_content.contiguous()
+            gates = log_gates.contiguous()
+            table = relative_bias.contiguous()
+            buckets = relative_buckets.contiguous()
+            nonpad = _mask_bytes(nonpad_mask)
+            bound_end = None if bound_end is None else bound_end.contiguous()
+            links = torch.empty(bsz, prelen, translen, dtype=torch.float32, device=dev)
+            head_lse = torch.empty(bsz, prelen, heads, dtype=torch.float32, device=dev) if need_grad else None
+            check(lib().dat_links_from_heads_biased(
+                ptr(content), ptr(gates), ptr(table), ptr(buckets), table.size(0), ptr(bound_end), ptr(nonpad),
+                ptr(links), ptr(head_lse), ptr(_status_word(dev)), bsz, prelen, heads, translen, stream_ptr(dev)),
+                "links_from_heads (biased)")
+        if need_grad:
+            ctx.save_for_backward(content, gates, table, buckets, links, head_lse, nonpad, bound_end)
+        return links
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_links):
+        content, gates, table, buckets, links, head_lse, nonpad, bound_end = ctx.saved_tensors
+        bsz, prelen, _, heads = content.shape
+        translen = links.size(2)
+        dev = content.device
+        L = lib()
+        with torch.cuda.device(dev):
+            grad_links = grad_links.to(torch.float32).contiguous()
+            grad_content = torch.empty_like(content)
+            grad_gates = torch.empty_like(gates)
+            grad_table = ws = None
+            if ctx.needs_input_grad[2]:
+                grad_table = torch.empty_like(table)
+                ws = torch.empty(max(L.dat_links_bias_workspace_bytes(bsz, prelen, heads, translen), 1),
+                                 dtype=torch.uint8, device=dev)
+            check(L.dat_links_from_heads_biased_backward(
+                ptr(grad_links), ptr(content), ptr(gates), ptr(table), ptr(buckets), table.size(0), ptr(links),
+                ptr(head_lse), ptr(bound_end), ptr(nonpad), ptr(grad_content), ptr(grad_gates), ptr(grad_table),
+                ptr(ws), bsz, prelen, heads, translen, stream_ptr(dev)), "links_from_heads_backward (biased)")
+        return grad_content, grad_gates, grad_table, None, None, None, None
+
+
+def dag_relative_buckets(num_distances, num_buckets, max_distance=128, device=None):
+    r"""Bucket of each distance ``1..num_distances`` between two vertices, for ``dag_links_from_heads``.
+
+    The first half of the buckets holds one distance each, the others grow geometrically up to
+    ``max_distance``, and the last one holds every distance beyond it.  Computed in whole numbers, so no
+    distance next to a border depends on a rounded logarithm.  Returns int64 [num_distances]."""
+    num_distances, num_buckets, max_distance = int(num_distances), int(num_buckets), int(max_distance)
+    exact = num_buckets // 2
+    if num_distances < 1 or num_buckets < 1 or max_distance <= exact:
+        raise RuntimeError("dag_relative_buckets needs num_distances >= 1, num_buckets >= 1 and "
+                           "max_distance > num_buckets // 2")
+    grown = num_buckets - exact
+    start = max(exact, 1)
+    out, k = [], 0
+    for d in range(num_distances):        # d = 0 is the distance 1
+        if d < exact:
+            out.append(d)
+            continue
+        # bucket exact + k begins where d >= start * (max_distance / start) ** (k / grown)
+        while k + 1 < grown and d ** grown >= start ** (grown - k - 1) * max_distance ** (k + 1):
+            k += 1
+        out.append(exact + k)
+    return torch.tensor(out, dtype=torch.long, device=device)
+
+
 def dag_links_from_heads(log_multi_content, log_gates, nonpad_mask=None, bound_end=None,
-                         max_transition_length=99999):
+                         max_transition_length=99999, relative_bias=None, relative_buckets=None):
     r"""Band links from per-head transition scores (glat_decomposed_with_link.py:380-404, the
     finite ``max_transition_length`` branch)::
 
@@ -88,7 +196,18 @@ def dag_links_from_heads(log_multi_content, log_gates, nonpad_mask=None, bound_e
     log_multi_content [B,L,L,H] fp32, log_gates [B,L,H] fp32.  The valid successors of a vertex are
     the later vertices inside the band that ``nonpad_mask`` ([B,L] bool, ``prev_output_tokens != pad``)
     allows, or, while decoding, those up to ``bound_end`` ([B,L] int64).  Returns links [B,L,K] fp32
-    with K = min(max_transition_length, L-1).  Differentiable in the first two arguments."""
+    with K = min(max_transition_length, L-1).  Differentiable in the first two arguments.
+
+    ``relative_bias`` [num_buckets,H] fp32 is a learned bias of the distance between two vertices:
+    ``relative_bias[relative_buckets[j-i-1]]`` is added to the scores of the transition i -> j
+    (``relative_buckets``: int64, one bucket for each distance 1..K or more, see ``dag_relative_buckets``).
+    Differentiable in it too; the gradient is summed in a fixed order.  A bucket outside the table forbids
+    the transitions of its distance and sets bit 4 of ``last_status()``."""
+    if (relative_bias is None) != (relative_buckets is None):
+        raise RuntimeError("relative_bias and relative_buckets are given together")
+    if relative_bias is not None:
+        return DagBiasedLinksFunc.apply(log_multi_content, log_gates, relative_bias, relative_buckets, nonpad_mask,
+                                        bound_end, max_transition_length)
     return DagLinksFromHeadsFunc.apply(log_multi_content, log_gates, nonpad_mask, bound_end,
                                        max_transition_length)
 

@@ -46,6 +46,13 @@ enum dat_dtype {
     DAT_BF16 = 2
 };
 
+/* kinds of dat_preference_loss */
+enum dat_preference_kind {
+    DAT_PREFERENCE_SIGMOID = 0,
+    DAT_PREFERENCE_HINGE = 1,
+    DAT_PREFERENCE_SQUARED = 2
+};
+
 /* bits OR-ed by the kernels into the optional device status word */
 #define DAT_STATUS_BAD_LENGTH 1 /* a sentence had invalid lengths                  */
 #define DAT_STATUS_NO_PATH 2    /* best alignment: a sentence has no finite path   */
@@ -340,6 +347,83 @@ size_t dat_upload_links_bytes(int bsz, int prelen, int translen, int max_output_
 int dat_upload_links_head_rows(int prelen, int translen, int max_output_length);
 int dat_upload_links(const float *host_links, float *dev_links, int bsz, int prelen, int translen,
                      int max_output_length, void *stream);
+
+/*
+ * dat_links_from_heads with a learned relative position bias (no counterpart in the reference):
+ * content[b,i,j,h] + bias_table[buckets[j-i-1], h] takes the place of content[b,i,j,h].
+ *   bias_table [num_buckets,heads] fp32, buckets [translen] int64: the bucket of each distance 1..translen.
+ * A bucket outside [0, num_buckets) forbids the transitions of its distance (-inf, no gradient) and sets
+ * DAT_STATUS_BAD_INDEX.  The other arguments are those of dat_links_from_heads.
+ */
+int dat_links_from_heads_biased(const float *content, const float *log_gates, const float *bias_table,
+                                const int64_t *buckets, int num_buckets, const int64_t *bound_end,
+                                const unsigned char *nonpad, float *links, float *head_lse, int32_t *status,
+                                int bsz, int prelen, int heads, int translen, void *stream);
+
+/*
+ * Gradient of dat_links_from_heads_biased.  grad_bias_table [num_buckets,heads] (NULL: not computed) is the sum
+ * of grad_content over all transitions of a bucket, added in a fixed order (the same bits every time).
+ * grad_content must not alias content.  workspace: dat_links_bias_workspace_bytes(...) bytes, 16-byte aligned.
+ */
+size_t dat_links_bias_workspace_bytes(int bsz, int prelen, int heads, int translen);
+int dat_links_from_heads_biased_backward(const float *grad_links, const float *content, const float *log_gates,
+                                         const float *bias_table, const int64_t *buckets, int num_buckets,
+                                         const float *links, const float *head_lse, const int64_t *bound_end,
+                                         const unsigned char *nonpad, float *grad_content, float *grad_log_gates,
+                                         float *grad_bias_table, void *workspace, int bsz, int prelen, int heads,
+                                         int translen, void *stream);
+
+/*
+ * Clipped policy loss with a KL term (no counterpart in the reference).  For the active vertices (mask[b,l] != 0,
+ * or all of them when mask is NULL; N of them):
+ *   lp    = log_softmax(word_ins_out[b,l,:])[tokens[b,l]] + link_logp[b,l]       (link_logp may be NULL)
+ *   r     = exp(lp - old_logp[b,l]),  A = advantage[b * adv_stride_b + l * adv_stride_l]
+ *   term  = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *   kl    = sum_v p_v (log p_v - log q_v), q = softmax(ref_logits[b,l,:])   with ref_logits, or
+ *           e^u - u - 1, u = ref_logp[b,l] - lp                             with ref_logp, or 0 with neither
+ *   loss  = (1/N) sum (term + kl_coef * kl)                                 (0 when N = 0)
+ * word_ins_out, ref_logits [bsz,prelen,vocab] contiguous, of one dtype DAT_F32/F16/BF16; tokens int64, the other
+ * per-vertex inputs fp32, all [bsz,prelen] contiguous but the advantage, which has element strides.  Nothing of an
+ * inactive vertex is read.  A token outside [0, vocab) makes its log-probability NaN and sets DAT_STATUS_BAD_INDEX.
+ * Outputs: loss (one fp32), stats [5] fp64 = sums over the active vertices of term, kl and r, the number of clipped
+ * and of active vertices; logp, kl [bsz,prelen] fp32 (0 where inactive).
+ * For the backward: row_state [bsz*prelen,4] fp32, and grad_logits (optional, like word_ins_out): d loss /
+ * d word_ins_out times *grad_scale_ptr (a device float) or, when that is NULL, times grad_scale, rounded once.
+ * workspace: dat_policy_loss_workspace_bytes(...) bytes, 16-byte aligned; the backward reads it.
+ */
+size_t dat_policy_loss_workspace_bytes(int bsz, int prelen);
+int dat_policy_loss(const void *word_ins_out, const void *ref_logits, int dtype, const int64_t *tokens,
+                    const float *old_logp, const float *advantage, int64_t adv_stride_b, int64_t adv_stride_l,
+                    const float *link_logp, const float *ref_logp, const unsigned char *mask, float kl_coef,
+                    float clip_low, float clip_high, const float *grad_scale_ptr, float grad_scale, float *loss,
+                    double *stats, float *logp, float *kl, float *row_state, void *grad_logits, void *workspace,
+                    int32_t *status, int bsz, int prelen, int vocab, void *stream);
+
+/*
+ * Gradient of dat_policy_loss's loss times *grad_loss (device).  grad_written != 0: grad_logits is what
+ * dat_policy_loss wrote; it is left as it is when *grad_loss equals the scale it was written for and written
+ * again otherwise.  grad_logits or grad_link ([bsz,prelen] fp32) may be NULL.
+ */
+int dat_policy_loss_backward(const void *word_ins_out, const void *ref_logits, int dtype, const int64_t *tokens,
+                             const unsigned char *mask, float kl_coef, const float *row_state, const void *workspace,
+                             const float *grad_loss, int grad_written, void *grad_logits, float *grad_link, int bsz,
+                             int prelen, int vocab, void *stream);
+
+/*
+ * Loss of paired log ratios (preference loss; no counterpart in the reference) of sentence log-likelihoods as
+ * dat_dag_loss returns them.  Rewards r = beta * (log p - log p_ref) / length, margin h = r_chosen - r_rejected:
+ *   DAT_PREFERENCE_SIGMOID  -(1-e) log sigmoid(h) - e log sigmoid(-h)
+ *   DAT_PREFERENCE_HINGE    (1-e) max(0, 1-h) + e max(0, 1+h)
+ *   DAT_PREFERENCE_SQUARED  (1-e) (h - 1/2)^2 + e (h + 1/2)^2                 e = smoothing
+ * loss: their mean over all pairs (one fp32; 0 for no pairs).  A pair with a value that is not finite, or a length
+ * below 1 (DAT_STATUS_BAD_LENGTH), adds nothing.  ref_* and *_length may be NULL, both or neither.
+ * rewards [2,pairs] fp32 (0 for such a pair); stats [6] fp64: sums of the losses, chosen and rejected rewards,
+ * number of pairs with h > 0, of pairs, of pairs left out; grad (optional) [2,pairs] fp32: d loss / d chosen, rejected.
+ */
+int dat_preference_loss(const float *chosen, const float *rejected, const float *ref_chosen,
+                        const float *ref_rejected, const int64_t *chosen_length, const int64_t *rejected_length,
+                        double beta, double smoothing, int kind, float *loss, float *rewards, double *stats,
+                        float *grad, int32_t *status, int pairs, void *stream);
 
 #ifdef __cplusplus
 }
