@@ -11,7 +11,7 @@
 // forward, the dense gradient backward.  A CTA owns a vertex at a time and keeps its scores in registers, a
 // thread the same distances and heads (16 bytes: four heads of one distance) for every vertex it meets, so that
 // the bias is expanded by distance once per CTA (shared memory, log2 units) and the table's gradient gathers in
-// places of its own; the partial sums of the CTAs are added in a fixed order (no atomics: results repeat bit for
+// its registers; the partial sums of the CTAs are added in a fixed order (no atomics: results repeat bit for
 // bit).  One exponential per score and direction:
 //   forward   e = exp(z - r_h), r_h the score of the nearest successor in place of the maximum over all of them:
 //             the sum is at least 1, and a vertex where it overflows (a score 60 above r_h) or whose nearest
@@ -25,13 +25,9 @@
 
 namespace dat {
 
-constexpr int kLbThreads = 128;
-constexpr int kLbSplits = 16;           // partial sums per distance and head that the last kernel adds
 constexpr float kLbTiny = 0x1p-80f;
 constexpr float kLbHuge = 0x1p+86f;
 constexpr int kLbMaxVec = 4096;         // score vectors per vertex: 512 threads with eight each
-
-__device__ __forceinline__ int lb_row_of_slot(int q, int L) { return (q & 1) ? L - 1 - (q >> 1) : (q >> 1); }
 
 // bias by distance in log2 units into shared memory; -inf for a bucket outside the table
 template <int NT>
@@ -43,21 +39,75 @@ __device__ __forceinline__ void lb_expand(const LinksBias &lb, float *bl, int H,
 
 __device__ __forceinline__ float4 lb_ninf4() { return make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY); }
 
-// sum (or maximum) of v over the CTA's threads of the same head group, in every thread
-template <int G, int NT, bool kMax>
-__device__ __forceinline__ void lb_reduce(float (&v)[4], float *red, bool synced_before) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & (G - 1);
-#pragma unroll
-    for (int o = G; o < 32; o <<= 1) {
-#pragma unroll
-        for (int k = 0; k < 4; k++) {
-            const float w = __shfl_xor_sync(0xffffffffu, v[k], o);
-            v[k] = kMax ? fmaxf(v[k], w) : v[k] + w;
-        }
+// One vertex of the walk: rows are dealt so that a CTA meets long and short rows in turn.
+struct LbRow {
+    int64_t row;   // b * L + i
+    int i, nj;     // vertex, successors inside the band (before the padding mask); nj < 0: no such row
+};
+__device__ __forceinline__ LbRow lb_row(int slot, int rows, int L, int K, const LinksMask &mk) {
+    LbRow r{0, 0, -1};
+    if (slot < rows) {
+        const int b = slot / L, q = slot - b * L;
+        r.i = (q & 1) ? L - 1 - (q >> 1) : (q >> 1);
+        r.row = (int64_t)b * L + r.i;
+        const int jhi = links_jhi(r.i, L, K, mk, r.row);
+        r.nj = jhi - r.i > 0 ? jhi - r.i : 0;
     }
-    float4 *r4 = reinterpret_cast<float4 *>(red);
-    if (!synced_before) __syncthreads();
-    if (lane < G) r4[warp * G + g] = make_float4(v[0], v[1], v[2], v[3]);
+    return r;
+}
+// bit u: the thread's vector tid + u * NT belongs to a valid successor; bit 31: so does the nearest successor
+template <int G, int NT, int U>
+__device__ __forceinline__ unsigned lb_live(const LbRow &r, int L, const LinksMask &mk) {
+    const int tid = threadIdx.x;
+    unsigned live = 0;
+    if (r.nj <= 0) return 0;
+    if (!mk.nonpad) {
+#pragma unroll
+        for (int u = 0; u < U; u++) live |= tid + u * NT < r.nj * G ? 1u << u : 0u;
+        return live | 0x80000000u;
+    }
+    const unsigned char *np = mk.nonpad + (r.row - r.i) + r.i + 1;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int v = tid + u * NT;
+        if (v < r.nj * G && np[v / G]) live |= 1u << u;
+    }
+    return np[0] ? live | 0x80000000u : live;
+}
+__device__ __forceinline__ void lb_copy16(float4 *dst, const float4 *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void lb_copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void lb_copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// the thread's vectors of a row on their way into the stage (each thread reads only what it copied itself)
+template <int G, int NT, int U>
+__device__ __forceinline__ void lb_fetch(const LbRow &r, unsigned live, const float *content, int L, float4 *stage) {
+    if (r.nj > 0) {
+        const float4 *src = reinterpret_cast<const float4 *>(content + (r.row * L + r.i + 1) * (int64_t)(4 * G));
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (live >> u & 1) lb_copy16(stage + threadIdx.x + u * NT, src + threadIdx.x + u * NT);
+    }
+    lb_copy_commit();
+}
+
+// Sum (or maximum) of v over the warp's lanes of the same head group, left in red[warp][4g + k].  Halving exchange:
+// two steps in which a lane hands over half of its values, then butterflies on what it keeps.
+template <int G, int NT, bool kMax>
+__device__ __forceinline__ void lb_reduce(const float (&v)[4], float *red) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & (G - 1);
+    const auto op = [](float a, float b) { return kMax ? fmaxf(a, b) : a + b; };
+    const bool up = lane & 16, up2 = lane & 8;
+    float a = up ? v[0] : v[2], b = up ? v[1] : v[3];                   // given away
+    a = op(up ? v[2] : v[0], __shfl_xor_sync(0xffffffffu, a, 16));      // kept: heads 0,1 below, 2,3 above
+    b = op(up ? v[3] : v[1], __shfl_xor_sync(0xffffffffu, b, 16));
+    float c = op(up2 ? b : a, __shfl_xor_sync(0xffffffffu, up2 ? a : b, 8));
+    if (G < 8) c = op(c, __shfl_xor_sync(0xffffffffu, c, 4));
+    if (G < 4) c = op(c, __shfl_xor_sync(0xffffffffu, c, 2));
+    if (G < 2) c = op(c, __shfl_xor_sync(0xffffffffu, c, 1));
+    if ((lane & 7) < G) red[warp * (4 * G) + 4 * g + (up ? 2 : 0) + (up2 ? 1 : 0)] = c;
 }
 template <int G, int NT, bool kMax>
 __device__ __forceinline__ void lb_collect(float (&v)[4], const float *red) {
@@ -88,91 +138,89 @@ __device__ __forceinline__ float lb_max_over_heads(float v) {
     for (int o = 1; o < G; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// t = c log2e + (b - r)
+__device__ __forceinline__ float4 lb_shifted(float4 c, float4 b, const float (&r)[4]) {
+    fadd2_rn(b.x, b.y, b.x, b.y, -r[0], -r[1]);
+    fadd2_rn(b.z, b.w, b.z, b.w, -r[2], -r[3]);
+    ffma2_rn(b.x, b.y, c.x, c.y, kLog2e, kLog2e);
+    ffma2_rn(b.z, b.w, c.z, c.w, kLog2e, kLog2e);
+    return b;
+}
 
-// G = H / 4 vectors per distance; thread t holds the vectors t, t + NT, ... of a vertex's row (U of them)
+// Shared memory of both kernels: the bias by distance [K * H], two rows of scores [K * H], red [2][NT / 32][H].
+// A row's scores are copied while the row before is worked on, its mask is read one row earlier still.
+// G = H / 4 vectors per distance; thread t holds the vectors t, t + NT, ... of a vertex's row (U of them).
 template <int G, int NT, int U>
 __global__ void __launch_bounds__(NT)
 lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk, LinksBias lb,
               float *__restrict__ links, float *__restrict__ head_lse, int B, int L, int K) {
     constexpr int H = 4 * G;
     extern __shared__ __align__(16) float lbsm[];
-    float *bl = lbsm;                                  // [K * H]
-    float *red = lbsm + (size_t)K * H;                 // [2][NT / 32][H]
+    float *bl = lbsm, *red = lbsm + (size_t)3 * K * H;
+    float4 *const bl4 = reinterpret_cast<float4 *>(bl);
     const int tid = threadIdx.x, lane = tid & 31, g = lane & (G - 1);
+    const int rows = B * L, step = gridDim.x;
+    int slot = blockIdx.x;
+    LbRow r0 = lb_row(slot, rows, L, K, mk), r1 = lb_row(slot + step, rows, L, K, mk);
+    unsigned live0 = lb_live<G, NT, U>(r0, L, mk), live1 = lb_live<G, NT, U>(r1, L, mk);
+    const auto nearest = [&](const LbRow &r) {
+        return r.nj > 0 ? __ldg(reinterpret_cast<const float4 *>(content + (r.row * L + r.i + 1) * (int64_t)H) + g) : lb_ninf4();
+    };
+    const auto gates_of = [&](const LbRow &r) {
+        return r.nj >= 0 ? __ldg(reinterpret_cast<const float4 *>(log_gates + r.row * H) + g) : lb_ninf4();
+    };
+    float4 near0 = nearest(r0), gate0 = gates_of(r0);
+    lb_fetch<G, NT, U>(r0, live0, content, L, bl4 + (size_t)K * G);
     lb_expand<NT>(lb, bl, H, K);
     __syncthreads();
-    const float4 *bl4 = reinterpret_cast<const float4 *>(bl);
-    const int64_t rows = (int64_t)B * L;
     int par = 0;
-    for (int64_t slot = blockIdx.x; slot < rows; slot += gridDim.x, par ^= 1) {
-        const int64_t b = slot / L;
-        const int i = lb_row_of_slot((int)(slot - b * L), L);
-        const int64_t row = b * L + i;
-        const int jhi = links_jhi(i, L, K, mk, row);
-        const int nj = jhi - i > 0 ? jhi - i : 0, nvec = nj * G;
-        const unsigned char *np = mk.nonpad ? mk.nonpad + b * L + i + 1 : nullptr;
-        const float4 *src = reinterpret_cast<const float4 *>(content + (row * L + i + 1) * (int64_t)H);
-        if (nj == 0) {   // the whole CTA: no barrier, so the next vertex takes the same half of red
-            for (int d = tid; d < K; d += NT) links[row * (int64_t)K + d] = -INFINITY;
-            if (head_lse && tid < H) head_lse[row * H + tid] = -INFINITY;
-            par ^= 1;
-            continue;
-        }
+    for (; r0.nj >= 0; slot += step, par ^= 1) {
+        float4 *const stage = bl4 + (size_t)(1 + par) * K * G;
+        lb_fetch<G, NT, U>(r1, live1, content, L, bl4 + (size_t)(2 - par) * K * G);
+        const float4 near1 = nearest(r1), gate1 = gates_of(r1);
+        const LbRow r2 = lb_row(slot + 2 * step, rows, L, K, mk);
+        const unsigned live2 = lb_live<G, NT, U>(r2, L, mk);
+        lb_copy_wait<1>();
+        // r_h in log2 units
+        const float4 b0 = bl4[g];
+        float r[4] = {fmaf(near0.x, kLog2e, b0.x), fmaf(near0.y, kLog2e, b0.y), fmaf(near0.z, kLog2e, b0.z),
+                      fmaf(near0.w, kLog2e, b0.w)};
+        const bool no_r = !(live0 >> 31) || !(fabsf(r[0]) < INFINITY && fabsf(r[1]) < INFINITY && fabsf(r[2]) < INFINITY &&
+                                              fabsf(r[3]) < INFINITY);
         float4 e4[U];
-        unsigned live = 0;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const int nvec = r0.nj * G;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int v = tid + u * NT;
-            const bool ok = v < nvec && !(np && !np[v / G]);
-            live |= ok ? 1u << u : 0u;
-            e4[u] = ok ? __ldg(src + v) : lb_ninf4();
-        }
-        // r_h in log2 units
-        float r[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-        if (!(np && !np[0])) {
-            const float4 c0 = __ldg(src + g), b0 = bl4[g];
-            r[0] = fmaf(c0.x, kLog2e, b0.x);
-            r[1] = fmaf(c0.y, kLog2e, b0.y);
-            r[2] = fmaf(c0.z, kLog2e, b0.z);
-            r[3] = fmaf(c0.w, kLog2e, b0.w);
-        }
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        const bool no_r = !(fabsf(r[0]) < INFINITY && fabsf(r[1]) < INFINITY && fabsf(r[2]) < INFINITY && fabsf(r[3]) < INFINITY);
-#pragma unroll
-        for (int u = 0; u < U; u++) {
-            if (u * NT + (tid & ~31) >= nvec) {     // nothing of this warp
-                e4[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                continue;
+            e4[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (live0 >> u & 1) {
+                const float4 t = lb_shifted(stage[v], bl4[v], r);
+                e4[u] = make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w));
+                fadd2_rn(sum[0], sum[1], sum[0], sum[1], e4[u].x, e4[u].y);
+                fadd2_rn(sum[2], sum[3], sum[2], sum[3], e4[u].z, e4[u].w);
             }
-            float4 t = bl4[min(tid + u * NT, K * G - 1)];
-            fadd2_rn(t.x, t.y, t.x, t.y, -r[0], -r[1]);
-            fadd2_rn(t.z, t.w, t.z, t.w, -r[2], -r[3]);
-            ffma2_rn(t.x, t.y, e4[u].x, e4[u].y, kLog2e, kLog2e);
-            ffma2_rn(t.z, t.w, e4[u].z, e4[u].w, kLog2e, kLog2e);
-            const bool ok = live >> u & 1;
-            e4[u] = ok ? make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w)) : make_float4(0.f, 0.f, 0.f, 0.f);
-            fadd2_rn(sum[0], sum[1], sum[0], sum[1], e4[u].x, e4[u].y);
-            fadd2_rn(sum[2], sum[3], sum[2], sum[3], e4[u].z, e4[u].w);
         }
-        const bool bad = no_r || !(fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3])) < kLbHuge) ||
-                         !(sum[0] + sum[1] + sum[2] + sum[3] < INFINITY);
+        const bool bad = (live0 & 0x7fffffffu) &&
+                         (no_r || !(fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3])) < kLbHuge) ||
+                          !(sum[0] + sum[1] + sum[2] + sum[3] < INFINITY));
         float *rd = red + par * (NT / 32) * H;
-        lb_reduce<G, NT, false>(sum, rd, true);
+        lb_reduce<G, NT, false>(sum, rd);
         if (__syncthreads_or(bad)) {
             // the exact maximum of each head takes the place of r_h
             float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int u = 0; u < U; u++) {
                 const int v = tid + u * NT;
-                if (live >> u & 1) {
-                    const float4 c = __ldg(src + v), t = bl4[v];
+                if (live0 >> u & 1) {
+                    const float4 c = stage[v], t = bl4[v];
                     m[0] = fmaxf(m[0], fmaf(c.x, kLog2e, t.x));
                     m[1] = fmaxf(m[1], fmaf(c.y, kLog2e, t.y));
                     m[2] = fmaxf(m[2], fmaf(c.z, kLog2e, t.z));
                     m[3] = fmaxf(m[3], fmaf(c.w, kLog2e, t.w));
                 }
             }
-            lb_reduce<G, NT, true>(m, rd, true);   // the sums that the slot held are not wanted
+            lb_reduce<G, NT, true>(m, rd);   // the sums that the place held are not wanted
             __syncthreads();
             lb_collect<G, NT, true>(m, rd);
             sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
@@ -182,56 +230,67 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             for (int u = 0; u < U; u++) {
                 const int v = tid + u * NT;
                 e4[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (live >> u & 1) {
-                    const float4 c = __ldg(src + v), t = bl4[v];
-                    e4[u] = make_float4(ex2(fmaf(c.x, kLog2e, t.x - r[0])), ex2(fmaf(c.y, kLog2e, t.y - r[1])),
-                                        ex2(fmaf(c.z, kLog2e, t.z - r[2])), ex2(fmaf(c.w, kLog2e, t.w - r[3])));
-                    sum[0] += e4[u].x;
-                    sum[1] += e4[u].y;
-                    sum[2] += e4[u].z;
-                    sum[3] += e4[u].w;
+                if (live0 >> u & 1) {
+                    const float4 t = lb_shifted(stage[v], bl4[v], r);
+                    e4[u] = make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w));
+                    fadd2_rn(sum[0], sum[1], sum[0], sum[1], e4[u].x, e4[u].y);
+                    fadd2_rn(sum[2], sum[3], sum[2], sum[3], e4[u].z, e4[u].w);
                 }
             }
-            lb_reduce<G, NT, false>(sum, rd, false);
+            __syncthreads();
+            lb_reduce<G, NT, false>(sum, rd);
             __syncthreads();
         }
         lb_collect<G, NT, false>(sum, rd);
         // f_h = exp(g_h) / S_h; a head without a finite score takes no part
+        const float g2[4] = {gate0.x * kLog2e, gate0.y * kLog2e, gate0.z * kLog2e, gate0.w * kLog2e};
         float f[4];
-        const float4 gate = __ldg(reinterpret_cast<const float4 *>(log_gates + row * H) + g);
-        const float gt[4] = {gate.x, gate.y, gate.z, gate.w};
+        bool some[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            const bool some = sum[k] > 0.f && sum[k] < INFINITY;
-            f[k] = some ? ex2(gt[k] * kLog2e) / sum[k] : 0.f;
-            if (head_lse && tid < G) head_lse[row * H + 4 * g + k] = some ? (r[k] + lg2(sum[k])) * kLn2 : -INFINITY;
+            some[k] = sum[k] > 0.f && sum[k] < INFINITY;
+            f[k] = some[k] ? __fdividef(ex2(g2[k]), sum[k]) : 0.f;
         }
-        float *out = links + row * (int64_t)K;
+        if (head_lse && tid < G) {
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                head_lse[r0.row * H + 4 * g + k] = some[k] ? (r[k] + lg2(sum[k])) * kLn2 : -INFINITY;
+        }
+        float *out = links + r0.row * (int64_t)K;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int v = tid + u * NT, d = v / G;
             if (u * NT + (tid & ~31) >= K * G) break;
-            const bool ok = live >> u & 1;
-            float q = lb_over_heads<G>(fmaf(e4[u].x, f[0], e4[u].y * f[1]) + fmaf(e4[u].z, f[2], e4[u].w * f[3]));
-            float link = lg2(q) * kLn2;
-            if (__any_sync(0xffffffffu, ok && q < kLbTiny)) {
-                float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                if (ok) {
-                    const float4 c = __ldg(src + v), bb = bl4[v];
-                    const float cc[4] = {c.x, c.y, c.z, c.w}, bk[4] = {bb.x, bb.y, bb.z, bb.w};
-#pragma unroll
-                    for (int k = 0; k < 4; k++)   // log2 of e f without the exponential's flush
-                        if (gt[k] > -INFINITY && sum[k] > 0.f && sum[k] < INFINITY)
-                            t[k] = fmaf(cc[k], kLog2e, bk[k] - r[k]) + (gt[k] * kLog2e - lg2(sum[k]));
+            const bool ok = live0 >> u & 1;
+            float link = -INFINITY;
+            if (u * NT + (tid & ~31) < nvec) {
+                float q = lb_over_heads<G>(fmaf(e4[u].x, f[0], e4[u].y * f[1]) + fmaf(e4[u].z, f[2], e4[u].w * f[3]));
+                link = ok ? lg2(q) * kLn2 : -INFINITY;
+                if (__any_sync(0xffffffffu, ok && q < kLbTiny)) {
+                    float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (ok) {   // log2 of e f without the exponential's flush
+                        const float4 z = lb_shifted(stage[v], bl4[v], r);
+                        if (some[0]) t[0] = z.x + (g2[0] - lg2(sum[0]));
+                        if (some[1]) t[1] = z.y + (g2[1] - lg2(sum[1]));
+                        if (some[2]) t[2] = z.z + (g2[2] - lg2(sum[2]));
+                        if (some[3]) t[3] = z.w + (g2[3] - lg2(sum[3]));
+                    }
+                    const float m = lb_max_over_heads<G>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+                    const float mm = m > -INFINITY ? m : 0.f;
+                    q = lb_over_heads<G>(ex2(t[0] - mm) + ex2(t[1] - mm) + ex2(t[2] - mm) + ex2(t[3] - mm));
+                    link = m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
                 }
-                const float m = lb_max_over_heads<G>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-                const float mm = m > -INFINITY ? m : 0.f;
-                q = lb_over_heads<G>(ex2(t[0] - mm) + ex2(t[1] - mm) + ex2(t[2] - mm) + ex2(t[3] - mm));
-                link = m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
             }
-            if (g == 0 && d < K) out[d] = ok ? link : -INFINITY;
+            if (g == 0 && d < K) out[d] = link;
         }
+        r0 = r1;
+        r1 = r2;
+        live0 = live1;
+        live1 = live2;
+        near0 = near1;
+        gate0 = gate1;
     }
+    lb_copy_wait<0>();
 }
 
 template <int G, int NT, int U>
@@ -242,147 +301,172 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
               int K) {
     constexpr int H = 4 * G;
     extern __shared__ __align__(16) float lbsm[];
-    float *bl = lbsm;                                       // [K * H]
-    float *acc = lbsm + (size_t)K * H;                      // [K * H]: this CTA's share of the gradient by distance
-    float *red = acc + (part ? (size_t)K * H : 0);          // [2][NT / 32][H]
+    float *bl = lbsm, *red = lbsm + (size_t)3 * K * H;
+    float4 *const bl4 = reinterpret_cast<float4 *>(bl);
     const int tid = threadIdx.x, lane = tid & 31, g = lane & (G - 1);
+    const int rows = B * L, step = gridDim.x;
+    int slot = blockIdx.x;
+    LbRow r0 = lb_row(slot, rows, L, K, mk), r1 = lb_row(slot + step, rows, L, K, mk);
+    unsigned live0 = lb_live<G, NT, U>(r0, L, mk), live1 = lb_live<G, NT, U>(r1, L, mk);
+    const auto of_row = [&](const float *p, const LbRow &r) {
+        return r.nj >= 0 ? __ldg(reinterpret_cast<const float4 *>(p + r.row * H) + g) : lb_ninf4();
+    };
+    float gd[U];   // the incoming gradient, a row ahead like the scores
+    const auto fetch_grad = [&](const LbRow &r, unsigned live, float (&to)[U]) {
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            to[u] = live >> u & 1 ? __ldg(grad_links + r.row * (int64_t)K + (tid + u * NT) / G) : 0.f;
+    };
+    float4 lse0 = of_row(head_lse, r0), gate0 = of_row(log_gates, r0);
+    fetch_grad(r0, live0, gd);
+    lb_fetch<G, NT, U>(r0, live0, content, L, bl4 + (size_t)K * G);
     lb_expand<NT>(lb, bl, H, K);
-    if (part)
-        for (int x = tid; x < K * H; x += NT) acc[x] = 0.f;
     __syncthreads();
-    const float4 *bl4 = reinterpret_cast<const float4 *>(bl);
-    float4 *acc4 = reinterpret_cast<float4 *>(acc);
-    const int64_t rows = (int64_t)B * L;
+    float4 acc[U];   // the gradient by distance of this CTA's rows
+#pragma unroll
+    for (int u = 0; u < U; u++) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
     int par = 0;
-    for (int64_t slot = blockIdx.x; slot < rows; slot += gridDim.x, par ^= 1) {
-        const int64_t b = slot / L;
-        const int i = lb_row_of_slot((int)(slot - b * L), L);
-        const int64_t row = b * L + i;
-        const int jhi = links_jhi(i, L, K, mk, row);
-        const int nj = jhi - i > 0 ? jhi - i : 0, nvec = nj * G;
-        const unsigned char *np = mk.nonpad ? mk.nonpad + b * L + i + 1 : nullptr;
-        const float4 *src = reinterpret_cast<const float4 *>(content + (row * L + i + 1) * (int64_t)H);
-        const float *gl = grad_links + row * (int64_t)K;
-        float4 s4[U], p4[U];
-        float gd[U];
-        unsigned live = 0;
+    for (; r0.nj >= 0; slot += step, par ^= 1) {
+        float4 *const stage = bl4 + (size_t)(1 + par) * K * G;
+        lb_fetch<G, NT, U>(r1, live1, content, L, bl4 + (size_t)(2 - par) * K * G);
+        const float4 lse1 = of_row(head_lse, r1), gate1 = of_row(log_gates, r1);
+        const LbRow r2 = lb_row(slot + 2 * step, rows, L, K, mk);
+        const unsigned live2 = lb_live<G, NT, U>(r2, L, mk);
+        // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
+        const float ls[4] = {lse0.x > -INFINITY ? lse0.x * kLog2e : INFINITY, lse0.y > -INFINITY ? lse0.y * kLog2e : INFINITY,
+                             lse0.z > -INFINITY ? lse0.z * kLog2e : INFINITY, lse0.w > -INFINITY ? lse0.w * kLog2e : INFINITY};
+        const float g2[4] = {gate0.x * kLog2e, gate0.y * kLog2e, gate0.z * kLog2e, gate0.w * kLog2e};
+        const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
+        lb_copy_wait<1>();
+        float4 p4[U];
+        float S[4] = {0.f, 0.f, 0.f, 0.f};
+        const int nvec = r0.nj * G;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int v = tid + u * NT;
-            const bool ok = v < nvec && !(np && !np[v / G]);
-            live |= ok ? 1u << u : 0u;
-            s4[u] = ok ? __ldg(src + v) : lb_ninf4();
-            gd[u] = ok ? __ldg(gl + v / G) : 0.f;
-        }
-        const float4 lse = __ldg(reinterpret_cast<const float4 *>(head_lse + row * H) + g);
-        const float4 gate = __ldg(reinterpret_cast<const float4 *>(log_gates + row * H) + g);
-        // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
-        const float ls[4] = {lse.x > -INFINITY ? lse.x * kLog2e : INFINITY, lse.y > -INFINITY ? lse.y * kLog2e : INFINITY,
-                             lse.z > -INFINITY ? lse.z * kLog2e : INFINITY, lse.w > -INFINITY ? lse.w * kLog2e : INFINITY};
-        const float g2[4] = {gate.x * kLog2e, gate.y * kLog2e, gate.z * kLog2e, gate.w * kLog2e};
-        const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
-        float S[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int u = 0; u < U; u++) {
+            p4[u] = make_float4(0.f, 0.f, 0.f, 0.f);
             if (u * NT + (tid & ~31) >= nvec) continue;   // nothing of this warp
-            float4 t = bl4[min(tid + u * NT, K * G - 1)];
-            fadd2_rn(t.x, t.y, t.x, t.y, -ls[0], -ls[1]);
-            fadd2_rn(t.z, t.w, t.z, t.w, -ls[2], -ls[3]);
-            ffma2_rn(t.x, t.y, s4[u].x, s4[u].y, kLog2e, kLog2e);
-            ffma2_rn(t.z, t.w, s4[u].z, s4[u].w, kLog2e, kLog2e);
-            if (!(live >> u & 1)) t = lb_ninf4();   // whatever the table holds
-            s4[u] = make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w));
-            float4 q = make_float4(s4[u].x * eg[0], s4[u].y * eg[1], s4[u].z * eg[2], s4[u].w * eg[3]);
+            const bool ok = live0 >> u & 1;
+            const float4 t = ok ? lb_shifted(stage[v], bl4[v], ls) : lb_ninf4();
+            const float4 soft = make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w));
+            if (v < K * G) stage[v] = soft;
+            float4 q = make_float4(soft.x * eg[0], soft.y * eg[1], soft.z * eg[2], soft.w * eg[3]);
             const float tot = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
             float w = tot >= kLbTiny ? __fdividef(gd[u], tot) : 0.f;
-            if (__any_sync(0xffffffffu, gd[u] != 0.f && tot < kLbTiny)) {
+            if (__any_sync(0xffffffffu, ok && tot < kLbTiny)) {
                 const float a[4] = {t.x + g2[0], t.y + g2[1], t.z + g2[2], t.w + g2[3]};
                 const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-                if (tot < kLbTiny) {   // the same lanes of a distance
+                if (tot < kLbTiny) {   // the same in all lanes of a distance
                     const float mm = m > -INFINITY ? m : 0.f;
                     q = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
                 }
                 const float tot2 = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
                 w = tot2 > 0.f ? gd[u] / tot2 : 0.f;
             }
-            p4[u] = make_float4(q.x * w, q.y * w, q.z * w, q.w * w);
+            // a link of -inf has w = 0 times a gradient that may be anything
+            p4[u] = w != 0.f ? make_float4(q.x * w, q.y * w, q.z * w, q.w * w) : p4[u];
             fadd2_rn(S[0], S[1], S[0], S[1], p4[u].x, p4[u].y);
             fadd2_rn(S[2], S[3], S[2], S[3], p4[u].z, p4[u].w);
         }
         float *rd = red + par * (NT / 32) * H;
-        lb_reduce<G, NT, false>(S, rd, true);
+        lb_reduce<G, NT, false>(S, rd);
+        fetch_grad(r1, live1, gd);
         // the places of the dense row that no valid successor has
-        float4 *rowv = reinterpret_cast<float4 *>(grad_content + row * (int64_t)L * H);
+        float4 *rowv = reinterpret_cast<float4 *>(grad_content + r0.row * (int64_t)L * H);
         const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int v = tid; v < (i + 1) * G; v += NT) rowv[v] = zero;
-        for (int v = (i + 1) * G + nvec + tid; v < L * G; v += NT) rowv[v] = zero;
+        for (int v = tid; v < (r0.i + 1) * G; v += NT) rowv[v] = zero;
+        for (int v = (r0.i + 1) * G + nvec + tid; v < L * G; v += NT) rowv[v] = zero;
         __syncthreads();
         lb_collect<G, NT, false>(S, rd);
         if (tid < G)
-            reinterpret_cast<float4 *>(grad_log_gates + row * H)[g] = make_float4(S[0], S[1], S[2], S[3]);
-        float4 *dst = rowv + (i + 1) * G;
+            reinterpret_cast<float4 *>(grad_log_gates + r0.row * H)[g] = make_float4(S[0], S[1], S[2], S[3]);
+        float4 *dst = rowv + (r0.i + 1) * G;
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int v = tid + u * NT;
             if (v >= nvec) break;
+            const float4 soft = stage[v];
             float4 o = p4[u];
-            ffma2_rn(o.x, o.y, s4[u].x, s4[u].y, -S[0], -S[1]);
-            ffma2_rn(o.z, o.w, s4[u].z, s4[u].w, -S[2], -S[3]);
+            ffma2_rn(o.x, o.y, soft.x, soft.y, -S[0], -S[1]);
+            ffma2_rn(o.z, o.w, soft.z, soft.w, -S[2], -S[3]);
             dst[v] = o;
-            if (part) {
-                float4 a = acc4[v];
-                fadd2_rn(a.x, a.y, a.x, a.y, o.x, o.y);
-                fadd2_rn(a.z, a.w, a.z, a.w, o.z, o.w);
-                acc4[v] = a;
-            }
+            fadd2_rn(acc[u].x, acc[u].y, acc[u].x, acc[u].y, o.x, o.y);
+            fadd2_rn(acc[u].z, acc[u].w, acc[u].z, acc[u].w, o.z, o.w);
+        }
+        r0 = r1;
+        r1 = r2;
+        live0 = live1;
+        live1 = live2;
+        lse0 = lse1;
+        gate0 = gate1;
+    }
+    lb_copy_wait<0>();
+    if (part) {
+        float4 *p = reinterpret_cast<float4 *>(part + (size_t)blockIdx.x * K * H);
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (tid + u * NT < K * G) p[tid + u * NT] = acc[u];
+    }
+}
+
+// by_distance[x] = sum of part[n][x] over the n CTAs, x = d * H + h: 32 columns per CTA, 16 lanes of rows each
+constexpr int kLbSumCols = 32, kLbSumLanes = 16;
+__global__ void __launch_bounds__(kLbSumCols * kLbSumLanes)
+lb_sum_kernel(const float *__restrict__ part, double *__restrict__ by_distance, int n, int KH) {
+    __shared__ double lane_s[kLbSumLanes][kLbSumCols];
+    const int c = threadIdx.x % kLbSumCols, q = threadIdx.x / kLbSumCols, x = blockIdx.x * kLbSumCols + c;
+    double acc = 0.0;
+    if (x < KH) {
+#pragma unroll 8
+        for (int k = q; k < n; k += kLbSumLanes) acc += (double)part[(size_t)k * KH + x];
+    }
+    lane_s[q][c] = acc;
+    __syncthreads();
+    if (q == 0 && x < KH) {
+#pragma unroll
+        for (int k = 1; k < kLbSumLanes; k++) acc += lane_s[k][c];
+        by_distance[x] = acc;
+    }
+}
+
+// The same sums from the dense gradient: by_distance[d * H + h] = sum of dc[b,i,i+1+d,h] over the vertices (b,i)
+__global__ void __launch_bounds__(kLbSumCols * kLbSumLanes)
+lb_diag_kernel(const float *__restrict__ grad_content, double *__restrict__ by_distance, int B, int L, int H, int K) {
+    __shared__ double lane_s[kLbSumLanes][kLbSumCols];
+    const int c = threadIdx.x % kLbSumCols, q = threadIdx.x / kLbSumCols, x = blockIdx.x * kLbSumCols + c;
+    double acc = 0.0;
+    if (x < K * H) {
+        const int n = L - 1 - x / H;   // vertices that have a successor at this distance
+        for (int b = 0; b < B; b++) {
+            const float *p = grad_content + ((int64_t)b * L * L + 1) * H + x;
+#pragma unroll 8
+            for (int i = q; i < n; i += kLbSumLanes) acc += (double)p[(int64_t)i * (L + 1) * H];
         }
     }
-    if (part) {
-        // a thread's own places: written by the thread that reads them
-        float4 *p = reinterpret_cast<float4 *>(part + (size_t)blockIdx.x * K * H);
-        for (int v = tid; v < K * G; v += NT) p[v] = acc4[v];
-    }
-}
-
-// sums[split][x] = sum of part[n][x] over the split's n, x = d * H + h
-__global__ void __launch_bounds__(kLbThreads)
-lb_sum_kernel(const float *__restrict__ part, double *__restrict__ sums, int n, int KH) {
-    const int x = blockIdx.x * kLbThreads + threadIdx.x;
-    if (x >= KH) return;
-    double acc = 0.0;
-#pragma unroll 8
-    for (int k = blockIdx.y; k < n; k += kLbSplits) acc += (double)part[(size_t)k * KH + x];
-    sums[(size_t)blockIdx.y * KH + x] = acc;
-}
-
-// sums[split][d * H + h] = sum of dc[b,i,i+1+d,h] over the split's vertices (b,i)
-__global__ void __launch_bounds__(kLbThreads)
-lb_diag_kernel(const float *__restrict__ grad_content, double *__restrict__ sums, int B, int L, int H, int K) {
-    const int x = blockIdx.x * kLbThreads + threadIdx.x;
-    if (x >= K * H) return;
-    const int d = x / H;
-    const int64_t rows = (int64_t)B * L;
-    double acc = 0.0;
-    for (int64_t row = blockIdx.y; row < rows; row += kLbSplits) {
-        const int i = (int)(row % L);
-        if (i + 1 + d < L) acc += (double)grad_content[(row * L + i + 1) * H + x];
-    }
-    sums[(size_t)blockIdx.y * K * H + x] = acc;
-}
-
-// grad_table[k, h] from the partial sums: one CTA per bucket, the distances dealt to P = 128 / H lanes of a head
-__global__ void __launch_bounds__(kLbThreads)
-lb_join_kernel(const double *__restrict__ sums, const int64_t *__restrict__ bucket, float *__restrict__ grad_table, int H,
-               int K) {
-    __shared__ double lane_s[kLbThreads];
-    const int k = blockIdx.x, P = kLbThreads / H, h = threadIdx.x % H, p = threadIdx.x / H;
-    double acc = 0.0;
-    if (p < P)
-        for (int d = p; d < K; d += P)
-            if (__ldg(bucket + d) == k) {
+    lane_s[q][c] = acc;
+    __syncthreads();
+    if (q == 0 && x < K * H) {
 #pragma unroll
-                for (int s = 0; s < kLbSplits; s++) acc += sums[((size_t)s * K + d) * H + h];
-            }
+        for (int k = 1; k < kLbSumLanes; k++) acc += lane_s[k][c];
+        by_distance[x] = acc;
+    }
+}
+
+// grad_table[k, h]: one CTA per bucket, the distances dealt to P lanes of a head
+constexpr int kLbJoinThreads = 256;
+__global__ void __launch_bounds__(kLbJoinThreads)
+lb_join_kernel(const double *__restrict__ by_distance, const int64_t *__restrict__ bucket, float *__restrict__ grad_table,
+               int H, int K) {
+    __shared__ double lane_s[kLbJoinThreads];
+    const int k = blockIdx.x, P = kLbJoinThreads / H, h = threadIdx.x % H, p = threadIdx.x / H;
+    double acc = 0.0;
+    if (p < P) {
+#pragma unroll 8
+        for (int d = p; d < K; d += P) {
+            const double v = by_distance[(size_t)d * H + h];
+            acc += __ldg(bucket + d) == k ? v : 0.0;
+        }
+    }
     lane_s[threadIdx.x] = acc;
     __syncthreads();
     if (p == 0) {
@@ -426,13 +510,11 @@ template <int G, int NT, int U>
 static int lb_launch(const LbArgs &a, bool backward, int &grid, cudaStream_t st, const DeviceInfo &di, const char *who) {
     const int H = 4 * G;
     const int64_t rows = (int64_t)a.B * a.L;
-    const size_t red = 2 * (NT / 32) * H * sizeof(float), table = (size_t)a.K * H * sizeof(float);
+    const size_t smem = ((size_t)3 * a.K * H + 2 * (NT / 32) * H) * sizeof(float);
     if (!backward) {
-        const size_t smem = table + red;
         if (int rc = lb_grid(lb_fwd_kernel<G, NT, U>, NT, smem, rows, di, grid, who)) return rc;
         lb_fwd_kernel<G, NT, U><<<grid, NT, smem, st>>>(a.content, a.log_gates, a.mk, a.lb, a.links, a.head_lse, a.B, a.L, a.K);
     } else {
-        const size_t smem = table * (a.part ? 2 : 1) + red;
         if (int rc = lb_grid(lb_bwd_kernel<G, NT, U>, NT, smem, rows, di, grid, who)) return rc;
         if (grid > di.sm_count * kLbMaxPerSm) grid = di.sm_count * kLbMaxPerSm;
         lb_bwd_kernel<G, NT, U><<<grid, NT, smem, st>>>(a.grad_links, a.content, a.log_gates, a.head_lse_in, a.mk, a.lb,
@@ -467,6 +549,8 @@ static int lb_check(const char *who, const float *table, const int64_t *bucket, 
                 "%s: bad sizes bsz=%d prelen=%d heads=%d translen=%d num_buckets=%d", who, bsz, prelen, heads, translen,
                 buckets);
     DAT_REQUIRE(table && bucket, DAT_ERR_BAD_ARG, "%s: null pointer", who);
+    DAT_REQUIRE((int64_t)bsz * prelen <= 0x3fffffff, DAT_ERR_UNSUPPORTED, "%s: bsz*prelen = %lld exceeds 2^30-1", who,
+                (long long)bsz * prelen);
     return DAT_OK;
 }
 
@@ -481,7 +565,7 @@ size_t dat_links_bias_workspace_bytes(int bsz, int prelen, int heads, int transl
     if (!device_info(&di)) return 0;
     int64_t n = (int64_t)di.sm_count * kLbMaxPerSm;
     if (n > (int64_t)bsz * prelen) n = (int64_t)bsz * prelen;
-    return (size_t)translen * heads * (kLbSplits * sizeof(double) + (size_t)n * sizeof(float));
+    return (size_t)translen * heads * (sizeof(double) + (size_t)n * sizeof(float)) + 16;
 }
 
 int dat_links_from_heads_biased(const float *content, const float *log_gates, const float *bias_table,
@@ -538,7 +622,8 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
     const LinksBias lb{bias_table, buckets, num_buckets, nullptr};
     const int KH = translen * heads;
     double *sums = static_cast<double *>(workspace);
-    const dim3 sgrid((unsigned)((KH + kLbThreads - 1) / kLbThreads), kLbSplits);
+    const unsigned sgrid = (unsigned)((KH + kLbSumCols - 1) / kLbSumCols);
+    constexpr int kSum = kLbSumCols * kLbSumLanes;
     if (lb_vector_form(heads, translen, content, log_gates, head_lse, grad_content) &&
         (reinterpret_cast<uintptr_t>(grad_log_gates) & 15) == 0) {
         LbArgs a{};
@@ -550,23 +635,23 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
         a.lb = lb;
         a.grad_content = grad_content;
         a.grad_log_gates = grad_log_gates;
-        a.part = grad_bias_table ? reinterpret_cast<float *>(sums + (size_t)kLbSplits * KH) : nullptr;
+        a.part = grad_bias_table ? reinterpret_cast<float *>(sums + (KH + 1) / 2 * 2) : nullptr;
         a.B = bsz;
         a.L = prelen;
         a.K = translen;
         int grid;
         if (int rc = lb_run(a, heads, true, grid, st, di, who)) return rc;
         if (!grad_bias_table) return DAT_OK;
-        lb_sum_kernel<<<sgrid, kLbThreads, 0, st>>>(a.part, sums, grid, KH);
+        lb_sum_kernel<<<sgrid, kSum, 0, st>>>(a.part, sums, grid, KH);
     } else {
         if (int rc = links_bwd_rows<true>(grad_links, content, log_gates, links, head_lse, mk, lb, grad_content,
                                           grad_log_gates, bsz, prelen, heads, translen, st, di, who))
             return rc;
         if (!grad_bias_table) return DAT_OK;
-        lb_diag_kernel<<<sgrid, kLbThreads, 0, st>>>(grad_content, sums, bsz, prelen, heads, translen);
+        lb_diag_kernel<<<sgrid, kSum, 0, st>>>(grad_content, sums, bsz, prelen, heads, translen);
     }
     if (int rc = check_launch(who)) return rc;
-    lb_join_kernel<<<(unsigned)num_buckets, kLbThreads, 0, st>>>(sums, buckets, grad_bias_table, heads, translen);
+    lb_join_kernel<<<(unsigned)num_buckets, kLbJoinThreads, 0, st>>>(sums, buckets, grad_bias_table, heads, translen);
     return check_launch(who);
 }
 
