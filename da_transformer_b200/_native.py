@@ -93,11 +93,11 @@ def _declare(lib):
     lib.dat_logsoftmax_gather_backward_fused.argtypes = [_vp, _i32, _vp, _i64, _i64, _i64, _vp, _i64,
                                                          _i64, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp]
     lib.dat_links_from_heads_biased.restype = _i32
-    lib.dat_links_from_heads_biased.argtypes = [_vp] * 4 + [_i32] + [_vp] * 5 + [_i32] * 4 + [_vp]
+    lib.dat_links_from_heads_biased.argtypes = [_vp] * 4 + [_i32] + [_vp] * 6 + [_i32] * 4 + [_vp]
     lib.dat_links_bias_workspace_bytes.restype = ctypes.c_size_t
     lib.dat_links_bias_workspace_bytes.argtypes = [_i32] * 4
     lib.dat_links_from_heads_biased_backward.restype = _i32
-    lib.dat_links_from_heads_biased_backward.argtypes = [_vp] * 5 + [_i32] + [_vp] * 8 + [_i32] * 4 + [_vp]
+    lib.dat_links_from_heads_biased_backward.argtypes = [_vp] * 5 + [_i32] + [_vp] * 10 + [_i32] * 4 + [_vp]
     lib.dat_policy_loss_workspace_bytes.restype = ctypes.c_size_t
     lib.dat_policy_loss_workspace_bytes.argtypes = [_i32] * 2
     lib.dat_policy_loss.restype = _i32

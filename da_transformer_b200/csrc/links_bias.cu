@@ -21,7 +21,10 @@
 // the 32-bit exponent flushes stays below 2^-40 of what it is added to.
 // Head counts of 4, 8, 16, 32 and up to 4096 score vectors per vertex; others take the kernels of links.cu (one
 // CTA per vertex, scores in shared memory) and a pass over the gradient's diagonals.
+#include <functional>
+
 #include "links_common.cuh"
+#include "umma.cuh"
 
 namespace dat {
 
@@ -409,6 +412,560 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     }
 }
 
+// ---------------------------------------------------------------------------------------------------
+// One warp per vertex, four neighbouring vertices at a time: what a vertex costs beside its scores (its place, the
+// reduction over the lanes, the gates) is paid by one warp and not by the four of a CTA per vertex.  A vertex's valid
+// scores are one piece of memory: one bulk asynchronous copy brings it into the warp's ring in shared memory while
+// the warp works on the vertex before, the exponentials and then the gradient take the scores' place, and a bulk
+// copy writes the gradient back (the zeros around it come from a block of zeros).  Rows are triangular, so a ring
+// little larger than the longest row holds two ordinary ones.
+// Used where a row has at most kLwMaxVec vectors and the bias table a few KB.
+// ---------------------------------------------------------------------------------------------------
+constexpr int kLwRows = 4;          // vertices of a group, a warp each
+constexpr int kLwMaxVec = 1024;     // score vectors per vertex
+constexpr int kLwMaxTable = 2048;   // floats of the bias table
+constexpr int kLwZeros = 2048;      // bytes of zeros
+constexpr int kLwU = 4;             // vectors of a lane taken together: loads first, then the arithmetic, then the stores
+constexpr int kLwPolls = 1 << 22;   // bound of a wait for a copy (never reached)
+constexpr uint32_t kLwFull = 0x7fc00d1eu;   // weight of a distance whose gradient is in the buffer already (no result of arithmetic)
+
+// span[b] = (last vertex that the mask allows, whether one between the first and it is not allowed); vertex 0 is
+// nobody's successor
+__global__ void __launch_bounds__(128)
+lw_span_kernel(const unsigned char *__restrict__ nonpad, int2 *__restrict__ span, int L) {
+    __shared__ int last_s[4], n_s[4];
+    const unsigned char *np = nonpad + (int64_t)blockIdx.x * L;
+    int last = -1, n = 0;
+    for (int j = 1 + threadIdx.x; j < L; j += 128)
+        if (np[j]) {
+            last = j;
+            n++;
+        }
+    last = __reduce_max_sync(0xffffffffu, last);
+    n = __reduce_add_sync(0xffffffffu, n);
+    if ((threadIdx.x & 31) == 0) {
+        last_s[threadIdx.x >> 5] = last;
+        n_s[threadIdx.x >> 5] = n;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 4; w++) {
+            last = max(last, last_s[w]);
+            n += n_s[w];
+        }
+        span[blockIdx.x] = make_int2(last, last >= 1 && n != last);
+    }
+}
+
+// The walk: groups of four neighbouring vertices, groups from the two ends of a sentence in turn.
+struct LwRow {
+    int64_t row;   // b * L + i
+    int i, nj;     // vertex, successors up to the last one that the masks allow
+    bool exists, holes;
+};
+__device__ __forceinline__ LwRow lw_row(int group, int groups, int L, int K, const LinksMask &mk, const int2 *span) {
+    LwRow r{0, 0, 0, false, false};
+    if (group >= groups) return r;
+    const int per = (L + kLwRows - 1) / kLwRows, b = group / per, q = group - b * per;
+    r.i = ((q & 1) ? per - 1 - (q >> 1) : (q >> 1)) * kLwRows + (threadIdx.x >> 5) % kLwRows;
+    if (r.i >= L) return r;
+    r.exists = true;
+    r.row = (int64_t)b * L + r.i;
+    int jhi = links_jhi(r.i, L, K, mk, r.row);
+    if (mk.nonpad) {
+        const int2 sp = __ldg(span + b);
+        jhi = min(jhi, sp.x);
+        r.holes = sp.y != 0;
+    }
+    r.nj = jhi - r.i > 0 ? jhi - r.i : 0;
+    return r;
+}
+
+// bias of vector v in log2 units, from the table in shared memory (its last row: -inf, for buckets outside)
+template <int G>
+__device__ __forceinline__ float4 lw_bias(const float4 *table, const unsigned short *bucket, int v) {
+    return table[bucket[v / G] * G + (v & (G - 1))];
+}
+template <int G, int NT>
+__device__ __forceinline__ void lw_load_table(const LinksBias &lb, float *table, unsigned short *bucket, int K) {
+    constexpr int H = 4 * G;
+    bool bad = false;
+    for (int x = threadIdx.x; x < lb.n * H; x += NT) table[x] = __ldg(lb.table + x) * kLog2e;
+    for (int x = threadIdx.x; x < H; x += NT) table[lb.n * H + x] = -INFINITY;
+    for (int d = threadIdx.x; d < K; d += NT) {
+        const int64_t k = __ldg(lb.bucket + d);
+        const bool ok = k >= 0 && k < lb.n;
+        bad |= !ok;
+        bucket[d] = (unsigned short)(ok ? k : lb.n);
+    }
+    if (bad && lb.status) atomicOr(lb.status, DAT_STATUS_BAD_INDEX);
+}
+
+// Shared memory, in bytes: table, buckets, zeros, barriers of the copies, then the rings.
+struct LwSmem {
+    int bucket, zeros, mbar, rings, ring;   // ring: bytes of one warp's
+};
+// dynamic shared memory of one CTA per SM (a little is left for what the kernels declare themselves) and of two
+static int lw_one(const DeviceInfo &di) { return di.max_smem_optin - 256; }
+static int lw_two(const DeviceInfo &di) { return (di.max_smem_optin + 1024) / 2 - 1024 - 256; }
+static int lw_row_bytes(int K, int H) { return K * H * 4 + (K + 8) * 4 / 16 * 16; }   // scores and the band's gradient
+static LwSmem lw_smem(int K, int H, int n, int warps, int avail) {
+    LwSmem m;
+    m.bucket = (n + 1) * H * 4;
+    m.zeros = (m.bucket + K * 2 + 15) / 16 * 16;
+    m.mbar = m.zeros + kLwZeros;
+    m.rings = m.mbar + (warps * 8 + 15) / 16 * 16;
+    m.ring = (avail - m.rings) / warps / 16 * 16;
+    return m;
+}
+
+__device__ __forceinline__ void lw_bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t mbar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(mbar)
+                 : "memory");
+}
+__device__ __forceinline__ void lw_bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void lw_bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// all bulk stores of this thread have read their shared memory
+__device__ __forceinline__ void lw_bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// A row in the ring: [window of the band's gradient (backward)][scores].  The window is the 16-byte pieces of
+// grad_links that lie before the row's end; the up to three values behind them are loaded singly (all of them where
+// grad_links does not start on a 16-byte boundary: wide = false).
+struct LwSlot {
+    int at, bytes;    // place in the ring
+    int window;       // bytes of the window
+    int skip;         // values of the window before the row's first
+    int whole;        // values of the row that the window holds
+};
+template <int G, bool kBackward>
+__device__ __forceinline__ LwSlot lw_slot(const LwRow &r, int K, bool wide) {
+    LwSlot s{0, 0, 0, 0, 0};
+    if (kBackward && r.nj > 0) {
+        const int64_t first = r.row * (int64_t)K, from = first & ~(int64_t)3, to = (first + r.nj) & ~(int64_t)3;
+        s.skip = (int)(first - from);
+        s.window = (s.skip + r.nj + 3) / 4 * 16;   // room for the single values too
+        s.whole = wide && to > first ? (int)(to - first) : 0;
+    }
+    s.bytes = s.window + r.nj * (16 * G);
+    return s;
+}
+// the place after `at + bytes` in the ring that keeps clear of [at, at + bytes), or -1
+__device__ __forceinline__ int lw_place(const LwSlot &cur, int need, int ring) {
+    if (cur.at + cur.bytes + need <= ring) return cur.at + cur.bytes;
+    return need <= cur.at ? 0 : -1;
+}
+
+// Lane 0: starts the copies of a row into its slot; the other lanes fetch the single values of the window.
+template <int G, bool kBackward>
+__device__ __forceinline__ void lw_issue(const LwRow &r, const LwSlot &s, unsigned char *ring, uint64_t *mbar,
+                                         const float *content, const float *grad_links, int L, int K) {
+    if (r.nj <= 0) return;
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) {
+        const uint32_t mb = umma::smem_u32(mbar), base = umma::smem_u32(ring) + s.at;
+        const uint32_t scores = r.nj * (16 * G);
+        const uint32_t win = kBackward && s.whole > 0 ? (s.skip + s.whole) * 4 : 0;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mb), "r"(scores + win) : "memory");
+        lw_bulk_load(base + s.window, content + (r.row * L + r.i + 1) * (int64_t)(4 * G), scores, mb);
+        if (win) lw_bulk_load(base, grad_links + (r.row * (int64_t)K - s.skip), win, mb);
+    }
+    if (kBackward) {
+        float *w = reinterpret_cast<float *>(ring + s.at) + s.skip;
+        for (int d = s.whole + lane; d < r.nj; d += 32) w[d] = __ldg(grad_links + r.row * (int64_t)K + d);
+    }
+}
+
+// sum or maximum over the lanes of a head group, in every lane: halving exchange, then each lane fetches its four
+template <int G, bool kMax>
+__device__ __forceinline__ void lw_reduce(float (&v)[4]) {
+    const int lane = threadIdx.x & 31, g = lane & (G - 1);
+    const auto op = [](float a, float b) { return kMax ? fmaxf(a, b) : a + b; };
+    const bool up = lane & 16, up2 = lane & 8;
+    float a = up ? v[0] : v[2], b = up ? v[1] : v[3];
+    a = op(up ? v[2] : v[0], __shfl_xor_sync(0xffffffffu, a, 16));
+    b = op(up ? v[3] : v[1], __shfl_xor_sync(0xffffffffu, b, 16));
+    float c = op(up2 ? b : a, __shfl_xor_sync(0xffffffffu, up2 ? a : b, 8));
+    if (G < 8) c = op(c, __shfl_xor_sync(0xffffffffu, c, 4));
+    if (G < 4) c = op(c, __shfl_xor_sync(0xffffffffu, c, 2));
+    if (G < 2) c = op(c, __shfl_xor_sync(0xffffffffu, c, 1));
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = __shfl_sync(0xffffffffu, c, (k >> 1) * 16 + (k & 1) * 8 + g);
+}
+
+// scores of masked places inside the span to -inf (each lane its own places)
+template <int G>
+__device__ __forceinline__ void lw_punch(const LwRow &r, float4 *buf, const LinksMask &mk) {
+    const unsigned char *np = mk.nonpad + r.row + 1;   // b * L + i + 1
+    for (int v = threadIdx.x & 31; v < r.nj * G; v += 32)
+        if (!np[v / G]) buf[v] = lb_ninf4();
+}
+
+// What both kernels begin with: table, barriers, zeros.
+template <int G, int NT>
+__device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, const LinksBias &lb, int K) {
+    lw_load_table<G, NT>(lb, reinterpret_cast<float *>(sm), reinterpret_cast<unsigned short *>(sm + lay.bucket), K);
+    for (int x = threadIdx.x; x < kLwZeros / 16; x += NT)
+        reinterpret_cast<float4 *>(sm + lay.zeros)[x] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (threadIdx.x < NT / 32) umma::mbar_init(reinterpret_cast<uint64_t *>(sm + lay.mbar) + threadIdx.x, 1);
+    umma::fence_smem_to_async();
+    __syncthreads();
+}
+
+// NG groups of four vertices at work in a CTA
+template <int G, int NG>
+__global__ void __launch_bounds__(NG * kLwRows * 32, 2)
+lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk,
+              const int2 *__restrict__ span, LinksBias lb, LwSmem lay, float *__restrict__ links,
+              float *__restrict__ head_lse, int B, int L, int K) {
+    constexpr int H = 4 * G;
+    extern __shared__ __align__(16) unsigned char lwsm[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & (G - 1);
+    const float4 *const table = reinterpret_cast<const float4 *>(lwsm);
+    const unsigned short *const bucket = reinterpret_cast<const unsigned short *>(lwsm + lay.bucket);
+    unsigned char *const ring = lwsm + lay.rings + warp * lay.ring;
+    uint64_t *const mbar = reinterpret_cast<uint64_t *>(lwsm + lay.mbar) + warp;
+    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
+    const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
+    int group = blockIdx.x * NG + warp / kLwRows;
+    LwRow r0 = lw_row(group, groups, L, K, mk, span), r1 = lw_row(group + step, groups, L, K, mk, span);
+    LwSlot s0 = lw_slot<G, false>(r0, K, false);
+    lw_issue<G, false>(r0, s0, ring, mbar, content, nullptr, L, K);
+    const auto gates_of = [&](const LwRow &r) {
+        return r.exists ? __ldg(reinterpret_cast<const float4 *>(log_gates + r.row * H) + g) : lb_ninf4();
+    };
+    float4 gate = gates_of(r0);
+    uint32_t phase = 0;
+    bool stalled = false;
+    for (; group < groups; group += step) {
+        if (r0.nj > 0) {
+            stalled |= !umma::mbar_wait(mbar, phase, kLwPolls);
+            phase ^= 1;
+        }
+        // the next row on its way, where the ring has room for it beside this one
+        LwSlot s1 = lw_slot<G, false>(r1, K, false);
+        s1.at = lw_place(s0, s1.bytes, lay.ring);
+        const bool later = s1.at < 0;
+        if (!later) lw_issue<G, false>(r1, s1, ring, mbar, content, nullptr, L, K);
+        const float4 gate1 = gates_of(r1);
+        const LwRow r2 = lw_row(group + 2 * step, groups, L, K, mk, span);
+        if (r0.exists) {
+            const int nvec = r0.nj * G;
+            float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at);
+            const float4 *const src = reinterpret_cast<const float4 *>(content + (r0.row * L + r0.i + 1) * (int64_t)H);
+            const unsigned char *const np = r0.holes ? mk.nonpad + r0.row + 1 : nullptr;
+            if (r0.holes) {
+                lw_punch<G>(r0, buf, mk);
+                __syncwarp();
+            }
+            // r_h in log2 units
+            float r[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
+            bool bad = false;
+            if (nvec > 0) {
+                const float4 c = buf[g], b0 = lw_bias<G>(table, bucket, g);
+                r[0] = fmaf(c.x, kLog2e, b0.x);
+                r[1] = fmaf(c.y, kLog2e, b0.y);
+                r[2] = fmaf(c.z, kLog2e, b0.z);
+                r[3] = fmaf(c.w, kLog2e, b0.w);
+                bad = !(fabsf(r[0]) < INFINITY && fabsf(r[1]) < INFINITY && fabsf(r[2]) < INFINITY && fabsf(r[3]) < INFINITY);
+                __syncwarp();   // before the nearest successor's place is written over
+            }
+            for (int v0 = lane; v0 < nvec; v0 += 32 * kLwU) {
+                float4 t[kLwU];
+#pragma unroll
+                for (int u = 0; u < kLwU; u++)
+                    if (v0 + 32 * u < nvec) t[u] = lb_shifted(buf[v0 + 32 * u], lw_bias<G>(table, bucket, v0 + 32 * u), r);
+#pragma unroll
+                for (int u = 0; u < kLwU; u++)
+                    if (v0 + 32 * u < nvec) {
+                        const float4 e = make_float4(ex2(t[u].x), ex2(t[u].y), ex2(t[u].z), ex2(t[u].w));
+                        buf[v0 + 32 * u] = e;
+                        fadd2_rn(sum[0], sum[1], sum[0], sum[1], e.x, e.y);
+                        fadd2_rn(sum[2], sum[3], sum[2], sum[3], e.z, e.w);
+                    }
+            }
+            bad |= !(fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3])) < kLbHuge) ||
+                   !(sum[0] + sum[1] + sum[2] + sum[3] < INFINITY);
+            if (__any_sync(0xffffffffu, bad)) {   // the exact maximum of each head takes the place of r_h
+                float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                for (int v = lane; v < nvec; v += 32)
+                    if (!(np && !np[v / G])) {
+                        const float4 c = __ldg(src + v), t = lw_bias<G>(table, bucket, v);
+                        m[0] = fmaxf(m[0], fmaf(c.x, kLog2e, t.x));
+                        m[1] = fmaxf(m[1], fmaf(c.y, kLog2e, t.y));
+                        m[2] = fmaxf(m[2], fmaf(c.z, kLog2e, t.z));
+                        m[3] = fmaxf(m[3], fmaf(c.w, kLog2e, t.w));
+                    }
+                __syncwarp();
+                lw_reduce<G, true>(m);
+                sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) r[k] = m[k] > -INFINITY ? m[k] : 0.f;
+                for (int v = lane; v < nvec; v += 32) {
+                    float4 e = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (!(np && !np[v / G])) {
+                        const float4 t = lb_shifted(__ldg(src + v), lw_bias<G>(table, bucket, v), r);
+                        e = make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w));
+                        fadd2_rn(sum[0], sum[1], sum[0], sum[1], e.x, e.y);
+                        fadd2_rn(sum[2], sum[3], sum[2], sum[3], e.z, e.w);
+                    }
+                    buf[v] = e;
+                }
+                __syncwarp();
+            }
+            lw_reduce<G, false>(sum);
+            // f_h = exp(g_h) / S_h; a head without a finite score takes no part
+            const float g2[4] = {gate.x * kLog2e, gate.y * kLog2e, gate.z * kLog2e, gate.w * kLog2e};
+            float f[4], ls[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool some = sum[k] > 0.f && sum[k] < INFINITY;
+                ls[k] = some ? lg2(sum[k]) : INFINITY;
+                f[k] = some ? __fdividef(ex2(g2[k]), sum[k]) : 0.f;
+            }
+            if (head_lse && lane < G) {
+                float4 o;
+                o.x = ls[0] < INFINITY ? (r[0] + ls[0]) * kLn2 : -INFINITY;
+                o.y = ls[1] < INFINITY ? (r[1] + ls[1]) * kLn2 : -INFINITY;
+                o.z = ls[2] < INFINITY ? (r[2] + ls[2]) * kLn2 : -INFINITY;
+                o.w = ls[3] < INFINITY ? (r[3] + ls[3]) * kLn2 : -INFINITY;
+                reinterpret_cast<float4 *>(head_lse + r0.row * H)[g] = o;
+            }
+            float *const out = links + r0.row * (int64_t)K;
+#pragma unroll 4
+            for (int v0 = 0; v0 < nvec; v0 += 32) {
+                const int v = v0 + lane, d = v / G;
+                const bool in = v < nvec;
+                const float4 e = in ? buf[v] : make_float4(0.f, 0.f, 0.f, 0.f);
+                float q = lb_over_heads<G>(fmaf(e.x, f[0], e.y * f[1]) + fmaf(e.z, f[2], e.w * f[3]));
+                float link = lg2(q) * kLn2;
+                if (__any_sync(0xffffffffu, in && q < kLbTiny)) {
+                    float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    if (in && !(np && !np[d])) {   // log2 of e f without the exponential's flush
+                        const float4 z = lb_shifted(__ldg(src + v), lw_bias<G>(table, bucket, v), r);
+                        if (ls[0] < INFINITY) t[0] = z.x + (g2[0] - ls[0]);
+                        if (ls[1] < INFINITY) t[1] = z.y + (g2[1] - ls[1]);
+                        if (ls[2] < INFINITY) t[2] = z.z + (g2[2] - ls[2]);
+                        if (ls[3] < INFINITY) t[3] = z.w + (g2[3] - ls[3]);
+                    }
+                    const float m = lb_max_over_heads<G>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+                    const float mm = m > -INFINITY ? m : 0.f;
+                    q = lb_over_heads<G>(ex2(t[0] - mm) + ex2(t[1] - mm) + ex2(t[2] - mm) + ex2(t[3] - mm));
+                    link = m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
+                }
+                if (g == 0 && in) out[d] = link;
+            }
+            for (int d = r0.nj + lane; d < K; d += 32) out[d] = -INFINITY;
+        }
+        // this row's place may be copied over from here on
+        umma::fence_smem_to_async();
+        __syncwarp();
+        if (later) {
+            s1.at = 0;
+            lw_issue<G, false>(r1, s1, ring, mbar, content, nullptr, L, K);
+        }
+        r0 = r1;
+        s0 = s1;
+        r1 = r2;
+        gate = gate1;
+    }
+    if (stalled && lb.status) atomicOr(lb.status, DAT_STATUS_STALLED);
+}
+
+// Backward.  With w_d = G_d / sum_h q the gradient of a score is soft_h (exp(g_h) w_d - S_h): the scores' place holds
+// soft and then the gradient itself, which the four rows' warps add to their sums by distance (registers of the 128
+// threads, UA vectors each).
+template <int G, int UA, int NG>
+__global__ void __launch_bounds__(NG * kLwRows * 32, UA <= 4 ? 2 : 1)
+lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ content,
+              const float *__restrict__ log_gates, const float *__restrict__ head_lse, LinksMask mk,
+              const int2 *__restrict__ span, LinksBias lb, LwSmem lay, float *__restrict__ grad_content,
+              float *__restrict__ grad_log_gates, float *__restrict__ part, int B, int L, int K) {
+    constexpr int H = 4 * G;
+    extern __shared__ __align__(16) unsigned char lwsm[];
+    __shared__ int2 row_at[NG * kLwRows];   // where a row's gradient lies (bytes from lwsm), its vectors
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane & (G - 1);
+    const float4 *const table = reinterpret_cast<const float4 *>(lwsm);
+    const unsigned short *const bucket = reinterpret_cast<const unsigned short *>(lwsm + lay.bucket);
+    unsigned char *const ring = lwsm + lay.rings + warp * lay.ring;
+    uint64_t *const mbar = reinterpret_cast<uint64_t *>(lwsm + lay.mbar) + warp;
+    const uint32_t zeros = umma::smem_u32(lwsm + lay.zeros);
+    const bool wide = (reinterpret_cast<uintptr_t>(grad_links) & 15) == 0;
+    const int set = warp / kLwRows, set_tid = tid - set * (kLwRows * 32);
+    const auto set_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(set + 1), "n"(kLwRows * 32) : "memory"); };
+    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
+    const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
+    int group = blockIdx.x * NG + set;
+    LwRow r0 = lw_row(group, groups, L, K, mk, span), r1 = lw_row(group + step, groups, L, K, mk, span);
+    LwSlot s0 = lw_slot<G, true>(r0, K, wide);
+    lw_issue<G, true>(r0, s0, ring, mbar, content, grad_links, L, K);
+    const auto of_row = [&](const float *p, const LwRow &r) {
+        return r.exists ? __ldg(reinterpret_cast<const float4 *>(p + r.row * H) + g) : lb_ninf4();
+    };
+    float4 lse = of_row(head_lse, r0), gate = of_row(log_gates, r0);
+    float4 acc[UA];
+#pragma unroll
+    for (int u = 0; u < UA; u++) acc[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+    uint32_t phase = 0;
+    bool stalled = false;
+    for (; group < groups; group += step) {
+        if (r0.nj > 0) {
+            stalled |= !umma::mbar_wait(mbar, phase, kLwPolls);
+            phase ^= 1;
+        }
+        __syncwarp();
+        const float4 lse1 = of_row(head_lse, r1), gate1 = of_row(log_gates, r1);
+        const LwRow r2 = lw_row(group + 2 * step, groups, L, K, mk, span);
+        const int nvec = r0.nj * G;
+        float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at + s0.window);
+        float *const weight = reinterpret_cast<float *>(ring + s0.at) + s0.skip;   // G_d, then w_d
+        if (r0.holes) {
+            lw_punch<G>(r0, buf, mk);
+            __syncwarp();
+        }
+        // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
+        const float ls[4] = {lse.x > -INFINITY ? lse.x * kLog2e : INFINITY, lse.y > -INFINITY ? lse.y * kLog2e : INFINITY,
+                             lse.z > -INFINITY ? lse.z * kLog2e : INFINITY, lse.w > -INFINITY ? lse.w * kLog2e : INFINITY};
+        const float g2[4] = {gate.x * kLog2e, gate.y * kLog2e, gate.z * kLog2e, gate.w * kLog2e};
+        const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
+        float S[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int v0 = lane; v0 - lane < nvec; v0 += 32 * kLwU) {
+            float4 t[kLwU];
+            float gd[kLwU];
+#pragma unroll
+            for (int u = 0; u < kLwU; u++) {
+                const int v = v0 + 32 * u;
+                t[u] = lb_ninf4();
+                gd[u] = 0.f;
+                if (v < nvec) {
+                    t[u] = lb_shifted(buf[v], lw_bias<G>(table, bucket, v), ls);
+                    gd[u] = weight[v / G];
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < kLwU; u++) {
+                const int v = v0 + 32 * u;
+                if (v - lane >= nvec) break;
+                const bool in = v < nvec;
+                float4 keep = make_float4(ex2(t[u].x), ex2(t[u].y), ex2(t[u].z), ex2(t[u].w)), q = keep;
+                fmul2_rn(q.x, q.y, q.x, q.y, eg[0], eg[1]);
+                fmul2_rn(q.z, q.w, q.z, q.w, eg[2], eg[3]);
+                const float tot = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
+                float w = tot >= kLbTiny ? __fdividef(gd[u], tot) : 0.f, mark = w;
+                if (__any_sync(0xffffffffu, in && tot < kLbTiny)) {
+                    const float a[4] = {t[u].x + g2[0], t[u].y + g2[1], t[u].z + g2[2], t[u].w + g2[3]};
+                    const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
+                    const bool tiny = tot < kLbTiny;   // the same in all lanes of a distance
+                    const float mm = m > -INFINITY ? m : 0.f;
+                    if (tiny) q = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
+                    const float tot2 = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
+                    if (tiny) {
+                        // p G in full where soft has lost it; soft S_h of such a place is below 2^-80 S_h and is
+                        // dropped: the second pass finds the mark and the product in the buffer
+                        w = tot2 > 0.f ? gd[u] / tot2 : 0.f;
+                        keep = tot2 > 0.f ? make_float4(q.x * w, q.y * w, q.z * w, q.w * w) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        mark = __uint_as_float(kLwFull);
+                    }
+                }
+                if (in) {
+                    buf[v] = keep;
+                    if (g == 0) weight[v / G] = mark;
+                }
+                ffma2_rn(S[0], S[1], q.x, q.y, w, w);
+                ffma2_rn(S[2], S[3], q.z, q.w, w, w);
+            }
+        }
+        __syncwarp();
+        // the next row on its way: the gradient of the row before this one has left its place
+        LwSlot s1 = lw_slot<G, true>(r1, K, wide);
+        s1.at = lw_place(s0, s1.bytes, lay.ring);
+        const bool later = s1.at < 0;
+        if (!later) {
+            lw_bulk_read();
+            __syncwarp();
+            lw_issue<G, true>(r1, s1, ring, mbar, content, grad_links, L, K);
+        }
+        if (r0.exists) {
+            lw_reduce<G, false>(S);
+            if (lane < G)
+                reinterpret_cast<float4 *>(grad_log_gates + r0.row * H)[g] = make_float4(S[0], S[1], S[2], S[3]);
+            for (int v0 = lane; v0 < nvec; v0 += 32 * kLwU) {
+                float4 o[kLwU];
+                float w[kLwU];
+#pragma unroll
+                for (int u = 0; u < kLwU; u++)
+                    if (v0 + 32 * u < nvec) {
+                        o[u] = buf[v0 + 32 * u];
+                        w[u] = weight[(v0 + 32 * u) / G];
+                    }
+#pragma unroll
+                for (int u = 0; u < kLwU; u++)
+                    if (v0 + 32 * u < nvec && __float_as_uint(w[u]) != kLwFull) {
+                        float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
+                        ffma2_rn(k.x, k.y, eg[0], eg[1], w[u], w[u]);
+                        ffma2_rn(k.z, k.w, eg[2], eg[3], w[u], w[u]);
+                        fmul2_rn(o[u].x, o[u].y, o[u].x, o[u].y, k.x, k.y);
+                        fmul2_rn(o[u].z, o[u].w, o[u].z, o[u].w, k.z, k.w);
+                        buf[v0 + 32 * u] = o[u];
+                    }
+            }
+            umma::fence_smem_to_async();
+            __syncwarp();
+            unsigned char *const dense = reinterpret_cast<unsigned char *>(grad_content + r0.row * (int64_t)L * H);
+            const int before = (r0.i + 1) * (16 * G), total = L * (16 * G), behind = before + nvec * 16;
+            if (lane == 0 && nvec > 0) lw_bulk_store(dense + before, umma::smem_u32(buf), nvec * 16);
+            // the places of the dense row that no valid successor has
+            for (int at = lane * kLwZeros; at < before; at += 32 * kLwZeros)
+                lw_bulk_store(dense + at, zeros, min(kLwZeros, before - at));
+            for (int at = behind + lane * kLwZeros; at < total; at += 32 * kLwZeros)
+                lw_bulk_store(dense + at, zeros, min(kLwZeros, total - at));
+            lw_bulk_commit();
+        }
+        if (part) {
+            if (lane == 0) row_at[warp] = make_int2((int)(reinterpret_cast<unsigned char *>(buf) - lwsm), nvec);
+            set_sync();
+#pragma unroll
+            for (int w = 0; w < kLwRows; w++) {
+                const int2 at = row_at[set * kLwRows + w];
+                const float4 *const dc = reinterpret_cast<const float4 *>(lwsm + at.x);
+#pragma unroll
+                for (int u = 0; u < UA; u++) {
+                    if (u * (kLwRows * 32) >= at.y) break;
+                    const int v = set_tid + u * (kLwRows * 32);
+                    if (v < at.y) {
+                        const float4 o = dc[v];
+                        fadd2_rn(acc[u].x, acc[u].y, acc[u].x, acc[u].y, o.x, o.y);
+                        fadd2_rn(acc[u].z, acc[u].w, acc[u].z, acc[u].w, o.z, o.w);
+                    }
+                }
+            }
+            set_sync();
+        }
+        if (later) {
+            lw_bulk_read();
+            umma::fence_smem_to_async();
+            __syncwarp();
+            s1.at = 0;
+            lw_issue<G, true>(r1, s1, ring, mbar, content, grad_links, L, K);
+        }
+        r0 = r1;
+        s0 = s1;
+        r1 = r2;
+        lse = lse1;
+        gate = gate1;
+    }
+    lw_bulk_read();
+    if (stalled && lb.status) atomicOr(lb.status, DAT_STATUS_STALLED);
+    if (part) {
+        float4 *p = reinterpret_cast<float4 *>(part + ((size_t)blockIdx.x * NG + set) * K * H);
+#pragma unroll
+        for (int u = 0; u < UA; u++)
+            if (set_tid + u * (kLwRows * 32) < K * G) p[set_tid + u * (kLwRows * 32)] = acc[u];
+    }
+}
+
 // by_distance[x] = sum of part[n][x] over the n CTAs, x = d * H + h: 32 columns per CTA, 16 lanes of rows each
 constexpr int kLbSumCols = 32, kLbSumLanes = 16;
 __global__ void __launch_bounds__(kLbSumCols * kLbSumLanes)
@@ -498,10 +1055,17 @@ static int lb_grid(F kernel, int threads, size_t smem, int64_t rows, const Devic
 
 constexpr int kLbMaxPerSm = 16;   // CTAs per SM that the workspace has room for
 
+// a warp per vertex: by size alone, so that a forward and its backward agree on who fills the spans
+static bool lw_fits(int K, int H, int n, const DeviceInfo &di) {
+    return (int64_t)K * H <= 4 * kLwMaxVec && (int64_t)n * H <= kLwMaxTable &&
+           lw_smem(K, H, n, 3 * kLwRows, lw_one(di)).ring >= lw_row_bytes(K, H);
+}
+
 struct LbArgs {
     const float *grad_links, *content, *log_gates, *head_lse_in;
     LinksMask mk;
     LinksBias lb;
+    int2 *span;
     float *links, *head_lse, *grad_content, *grad_log_gates, *part;
     int B, L, K;
 };
@@ -523,9 +1087,43 @@ static int lb_launch(const LbArgs &a, bool backward, int &grid, cudaStream_t st,
     return check_launch(who);
 }
 
+// CTAs of NG groups, `per_sm` of them to an SM
+template <int G, int NG, typename F, typename... Args>
+static int lw_start(F kernel, int per_sm, const LbArgs &a, int &parts, cudaStream_t st, const DeviceInfo &di,
+                    const char *who, LwSmem &lay, Args... args) {
+    const int64_t groups = (int64_t)a.B * ((a.L + kLwRows - 1) / kLwRows);
+    const int smem = per_sm > 1 ? lw_two(di) : lw_one(di);
+    lay = lw_smem(a.K, 4 * G, a.lb.n, NG * kLwRows, smem);
+    int64_t n = (int64_t)di.sm_count * per_sm;
+    if (n > (groups + NG - 1) / NG) n = (groups + NG - 1) / NG;
+    parts = (int)n * NG;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
+        kernel<<<(unsigned)n, NG * kLwRows * 32, smem, st>>>(args...);
+    return check_launch(who);
+}
+template <int G>
+static int lw_launch(const LbArgs &a, bool backward, int &parts, cudaStream_t st, const DeviceInfo &di, const char *who) {
+    // two CTAs per SM where the rings of both hold more than the longest row, else one
+    const int row = lw_row_bytes(a.K, 4 * G);
+    LwSmem lay;
+    if (!backward) {
+        const bool pair = lw_smem(a.K, 4 * G, a.lb.n, 3 * kLwRows, lw_two(di)).ring >= row + row / 4;
+        return lw_start<G, 3>(lw_fwd_kernel<G, 3>, pair ? 2 : 1, a, parts, st, di, who, lay, a.content, a.log_gates, a.mk,
+                              a.span, a.lb, std::ref(lay), a.links, a.head_lse, a.B, a.L, a.K);
+    }
+    if (a.K * G <= 4 * kLwRows * 32)
+        return lw_start<G, 2>(lw_bwd_kernel<G, 4, 2>, 2, a, parts, st, di, who, lay, a.grad_links, a.content, a.log_gates,
+                              a.head_lse_in, a.mk, a.span, a.lb, std::ref(lay), a.grad_content, a.grad_log_gates, a.part, a.B,
+                              a.L, a.K);
+    return lw_start<G, 3>(lw_bwd_kernel<G, 8, 3>, 1, a, parts, st, di, who, lay, a.grad_links, a.content, a.log_gates,
+                          a.head_lse_in, a.mk, a.span, a.lb, std::ref(lay), a.grad_content, a.grad_log_gates, a.part, a.B, a.L,
+                          a.K);
+}
+
 template <int G>
 static int lb_dispatch(const LbArgs &a, bool backward, int &grid, cudaStream_t st, const DeviceInfo &di, const char *who) {
     const int nvec = a.K * G;
+    if (lw_fits(a.K, 4 * G, a.lb.n, di)) return lw_launch<G>(a, backward, grid, st, di, who);
     if (nvec <= 2 * 128) return lb_launch<G, 128, 2>(a, backward, grid, st, di, who);
     if (nvec <= 4 * 128) return lb_launch<G, 128, 4>(a, backward, grid, st, di, who);
     if (nvec <= 8 * 128) return lb_launch<G, 128, 8>(a, backward, grid, st, di, who);
@@ -564,30 +1162,36 @@ size_t dat_links_bias_workspace_bytes(int bsz, int prelen, int heads, int transl
     DeviceInfo di;
     if (!device_info(&di)) return 0;
     int64_t n = (int64_t)di.sm_count * kLbMaxPerSm;
-    if (n > (int64_t)bsz * prelen) n = (int64_t)bsz * prelen;
+    const int64_t rows = (int64_t)bsz * prelen + 3;   // a CTA per vertex, or groups of up to four in CTAs of three
+    if (n > rows) n = rows;
     return (size_t)translen * heads * (sizeof(double) + (size_t)n * sizeof(float)) + 16;
 }
 
 int dat_links_from_heads_biased(const float *content, const float *log_gates, const float *bias_table,
                                 const int64_t *buckets, int num_buckets, const int64_t *bound_end,
-                                const unsigned char *nonpad, float *links, float *head_lse, int32_t *status, int bsz,
-                                int prelen, int heads, int translen, void *stream) {
+                                const unsigned char *nonpad, float *links, float *head_lse, int32_t *spans,
+                                int32_t *status, int bsz, int prelen, int heads, int translen, void *stream) {
     using namespace dat;
     const char *who = "dat_links_from_heads_biased";
     if (int rc = lb_check(who, bias_table, buckets, num_buckets, bsz, prelen, heads, translen)) return rc;
     if (bsz == 0) return DAT_OK;
-    DAT_REQUIRE(content && log_gates && links, DAT_ERR_BAD_ARG, "%s: null pointer", who);
+    DAT_REQUIRE(content && log_gates && links && (spans || !nonpad), DAT_ERR_BAD_ARG, "%s: null pointer", who);
     DeviceInfo di;
     if (!device_info(&di)) return DAT_ERR_NO_DEVICE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const LinksMask mk{bound_end, nonpad};
     const LinksBias lb{bias_table, buckets, num_buckets, status};
+    if (nonpad && lw_fits(translen, heads, num_buckets, di)) {
+        lw_span_kernel<<<(unsigned)bsz, 128, 0, st>>>(nonpad, reinterpret_cast<int2 *>(spans), prelen);
+        if (int rc = check_launch(who)) return rc;
+    }
     if (lb_vector_form(heads, translen, content, log_gates, head_lse, nullptr)) {
         LbArgs a{};
         a.content = content;
         a.log_gates = log_gates;
         a.mk = mk;
         a.lb = lb;
+        a.span = const_cast<int2 *>(reinterpret_cast<const int2 *>(spans));
         a.links = links;
         a.head_lse = head_lse;
         a.B = bsz;
@@ -602,9 +1206,9 @@ int dat_links_from_heads_biased(const float *content, const float *log_gates, co
 int dat_links_from_heads_biased_backward(const float *grad_links, const float *content, const float *log_gates,
                                          const float *bias_table, const int64_t *buckets, int num_buckets,
                                          const float *links, const float *head_lse, const int64_t *bound_end,
-                                         const unsigned char *nonpad, float *grad_content, float *grad_log_gates,
-                                         float *grad_bias_table, void *workspace, int bsz, int prelen, int heads,
-                                         int translen, void *stream) {
+                                         const unsigned char *nonpad, const int32_t *spans, float *grad_content,
+                                         float *grad_log_gates, float *grad_bias_table, void *workspace, int32_t *status,
+                                         int bsz, int prelen, int heads, int translen, void *stream) {
     using namespace dat;
     const char *who = "dat_links_from_heads_biased_backward";
     if (int rc = lb_check(who, bias_table, buckets, num_buckets, bsz, prelen, heads, translen)) return rc;
@@ -614,12 +1218,12 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
         return check_launch(who);
     }
     DAT_REQUIRE(grad_links && content && log_gates && links && head_lse && grad_content && grad_log_gates &&
-                    (workspace || !grad_bias_table),
+                    (workspace || !grad_bias_table) && (spans || !nonpad),
                 DAT_ERR_BAD_ARG, "%s: null pointer", who);
     DeviceInfo di;
     if (!device_info(&di)) return DAT_ERR_NO_DEVICE;
     const LinksMask mk{bound_end, nonpad};
-    const LinksBias lb{bias_table, buckets, num_buckets, nullptr};
+    const LinksBias lb{bias_table, buckets, num_buckets, status};
     const int KH = translen * heads;
     double *sums = static_cast<double *>(workspace);
     const unsigned sgrid = (unsigned)((KH + kLbSumCols - 1) / kLbSumCols);
@@ -633,6 +1237,7 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
         a.head_lse_in = head_lse;
         a.mk = mk;
         a.lb = lb;
+        a.span = const_cast<int2 *>(reinterpret_cast<const int2 *>(spans));
         a.grad_content = grad_content;
         a.grad_log_gates = grad_log_gates;
         a.part = grad_bias_table ? reinterpret_cast<float *>(sums + (KH + 1) / 2 * 2) : nullptr;

@@ -125,20 +125,21 @@ class DagBiasedLinksFunc(Function):
             buckets = relative_buckets.contiguous()
             nonpad = _mask_bytes(nonpad_mask)
             bound_end = None if bound_end is None else bound_end.contiguous()
+            spans = None if nonpad is None else torch.empty(max(bsz, 1), 2, dtype=torch.int32, device=dev)
             links = torch.empty(bsz, prelen, translen, dtype=torch.float32, device=dev)
             head_lse = torch.empty(bsz, prelen, heads, dtype=torch.float32, device=dev) if need_grad else None
             check(lib().dat_links_from_heads_biased(
                 ptr(content), ptr(gates), ptr(table), ptr(buckets), table.size(0), ptr(bound_end), ptr(nonpad),
-                ptr(links), ptr(head_lse), ptr(_status_word(dev)), bsz, prelen, heads, translen, stream_ptr(dev)),
+                ptr(links), ptr(head_lse), ptr(spans), ptr(_status_word(dev)), bsz, prelen, heads, translen, stream_ptr(dev)),
                 "links_from_heads (biased)")
         if need_grad:
-            ctx.save_for_backward(content, gates, table, buckets, links, head_lse, nonpad, bound_end)
+            ctx.save_for_backward(content, gates, table, buckets, links, head_lse, nonpad, bound_end, spans)
         return links
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_links):
-        content, gates, table, buckets, links, head_lse, nonpad, bound_end = ctx.saved_tensors
+        content, gates, table, buckets, links, head_lse, nonpad, bound_end, spans = ctx.saved_tensors
         bsz, prelen, _, heads = content.shape
         translen = links.size(2)
         dev = content.device
@@ -154,8 +155,8 @@ class DagBiasedLinksFunc(Function):
                                  dtype=torch.uint8, device=dev)
             check(L.dat_links_from_heads_biased_backward(
                 ptr(grad_links), ptr(content), ptr(gates), ptr(table), ptr(buckets), table.size(0), ptr(links),
-                ptr(head_lse), ptr(bound_end), ptr(nonpad), ptr(grad_content), ptr(grad_gates), ptr(grad_table),
-                ptr(ws), bsz, prelen, heads, translen, stream_ptr(dev)), "links_from_heads_backward (biased)")
+                ptr(head_lse), ptr(bound_end), ptr(nonpad), ptr(spans), ptr(grad_content), ptr(grad_gates),
+                ptr(grad_table), ptr(ws), ptr(_status_word(dev)), bsz, prelen, heads, translen, stream_ptr(dev)), "links_from_heads_backward (biased)")
         return grad_content, grad_gates, grad_table, None, None, None, None
 
 

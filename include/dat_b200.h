@@ -57,6 +57,7 @@ enum dat_preference_kind {
 #define DAT_STATUS_BAD_LENGTH 1 /* a sentence had invalid lengths                  */
 #define DAT_STATUS_NO_PATH 2    /* best alignment: a sentence has no finite path   */
 #define DAT_STATUS_BAD_INDEX 4  /* gather: an index outside [0, vocab)             */
+#define DAT_STATUS_STALLED 16  /* a copy did not arrive in time (results not to be used; never seen) */
 #define DAT_STATUS_FAST_FALLBACK 8 /* dat_dag_loss_fast recomputed a sentence exactly (informational) */
 
 int dat_version(void);
@@ -353,12 +354,13 @@ int dat_upload_links(const float *host_links, float *dev_links, int bsz, int pre
  * content[b,i,j,h] + bias_table[buckets[j-i-1], h] takes the place of content[b,i,j,h].
  *   bias_table [num_buckets,heads] fp32, buckets [translen] int64: the bucket of each distance 1..translen.
  * A bucket outside [0, num_buckets) forbids the transitions of its distance (-inf, no gradient) and sets
- * DAT_STATUS_BAD_INDEX.  The other arguments are those of dat_links_from_heads.
+ * DAT_STATUS_BAD_INDEX.  spans ([bsz,2], 8-byte aligned; NULL without nonpad): written here, read by the backward.
+ * The other arguments are those of dat_links_from_heads.
  */
 int dat_links_from_heads_biased(const float *content, const float *log_gates, const float *bias_table,
                                 const int64_t *buckets, int num_buckets, const int64_t *bound_end,
-                                const unsigned char *nonpad, float *links, float *head_lse, int32_t *status,
-                                int bsz, int prelen, int heads, int translen, void *stream);
+                                const unsigned char *nonpad, float *links, float *head_lse, int32_t *spans,
+                                int32_t *status, int bsz, int prelen, int heads, int translen, void *stream);
 
 /*
  * Gradient of dat_links_from_heads_biased.  grad_bias_table [num_buckets,heads] (NULL: not computed) is the sum
@@ -369,9 +371,9 @@ size_t dat_links_bias_workspace_bytes(int bsz, int prelen, int heads, int transl
 int dat_links_from_heads_biased_backward(const float *grad_links, const float *content, const float *log_gates,
                                          const float *bias_table, const int64_t *buckets, int num_buckets,
                                          const float *links, const float *head_lse, const int64_t *bound_end,
-                                         const unsigned char *nonpad, float *grad_content, float *grad_log_gates,
-                                         float *grad_bias_table, void *workspace, int bsz, int prelen, int heads,
-                                         int translen, void *stream);
+                                         const unsigned char *nonpad, const int32_t *spans, float *grad_content,
+                                         float *grad_log_gates, float *grad_bias_table, void *workspace, int32_t *status,
+                                         int bsz, int prelen, int heads, int translen, void *stream);
 
 /*
  * Clipped policy loss with a KL term (no counterpart in the reference).  For the active vertices (mask[b,l] != 0,

@@ -189,7 +189,7 @@ def test_entry_points_refuse_bad_arguments():
     assert lib.dat_preference_loss(*none, None, None, 0.1, 0.0, 0, None, None, None, None, None, 3, None) == 1
     assert lib.dat_policy_loss(*none[:2], 0, *none[:3], 0, 0, *none[:3], 0.0, 0.2, 0.2, None, 1.0, *none, *none, 1, 1, 0,
                                None) == 1 and b"vocab=0" in lib.dat_last_error()
-    assert lib.dat_links_from_heads_biased(*none, 0, None, None, None, None, None, 1, 4, 4, 3, None) == 1
+    assert lib.dat_links_from_heads_biased(*none, 0, *none, None, None, 1, 4, 4, 3, None) == 1
     assert b"num_buckets=0" in lib.dat_last_error()
 
 
