@@ -426,6 +426,10 @@ constexpr int kLwMaxVec = 1024;     // score vectors per vertex
 constexpr int kLwMaxTable = 2048;   // floats of the bias table
 constexpr int kLwZeros = 2048;      // bytes of zeros
 constexpr int kLwU = 4;             // vectors of a lane taken together: loads first, then the arithmetic, then the stores
+template <int N>
+struct LwInt {
+    static constexpr int value = N;
+};
 constexpr int kLwPolls = 1 << 22;   // bound of a wait for a copy (never reached)
 constexpr uint32_t kLwFull = 0x7fc00d1eu;   // weight of a distance whose gradient is in the buffer already (no result of arithmetic)
 
@@ -457,17 +461,37 @@ lw_span_kernel(const unsigned char *__restrict__ nonpad, int2 *__restrict__ span
     }
 }
 
-// The walk: groups of four neighbouring vertices, groups from the two ends of a sentence in turn.
+// The walk: groups of four neighbouring vertices, groups from the two ends of a sentence in turn (which end comes
+// first changes from sentence to sentence: a warp's stride may be even).
 struct LwRow {
     int64_t row;   // b * L + i
     int i, nj;     // vertex, successors up to the last one that the masks allow
     bool exists, holes;
 };
-__device__ __forceinline__ LwRow lw_row(int group, int groups, int L, int K, const LinksMask &mk, const int2 *span) {
+struct LwWalk {
+    int per, step_b, step_q, b, q;
+    __device__ __forceinline__ LwWalk(int group, int step, int L) {
+        per = (L + kLwRows - 1) / kLwRows;
+        step_b = step / per;
+        step_q = step - step_b * per;
+        b = group / per;
+        q = group - b * per;
+    }
+    __device__ __forceinline__ void next() {
+        b += step_b;
+        q += step_q;
+        if (q >= per) {
+            q -= per;
+            b++;
+        }
+    }
+};
+__device__ __forceinline__ LwRow lw_row(LwWalk &walk, int B, int L, int K, const LinksMask &mk, const int2 *span) {
     LwRow r{0, 0, 0, false, false};
-    if (group >= groups) return r;
-    const int per = (L + kLwRows - 1) / kLwRows, b = group / per, q = group - b * per;
-    r.i = ((q & 1) ? per - 1 - (q >> 1) : (q >> 1)) * kLwRows + (threadIdx.x >> 5) % kLwRows;
+    const int per = walk.per, b = walk.b, q = walk.q;
+    if (b >= B) return r;
+    walk.next();
+    r.i = (((q ^ b) & 1) ? per - 1 - (q >> 1) : (q >> 1)) * kLwRows + (threadIdx.x >> 5) % kLwRows;
     if (r.i >= L) return r;
     r.exists = true;
     r.row = (int64_t)b * L + r.i;
@@ -603,6 +627,45 @@ __device__ __forceinline__ void lw_punch(const LwRow &r, float4 *buf, const Link
         if (!np[v / G]) buf[v] = lb_ninf4();
 }
 
+// Runs f(N, partial, v) over a row's vectors: batches of kLwU * 32 without a condition inside, then the rest as one
+// smaller batch in which lanes may lie behind the row's end.  v: the lane's first vector, the others 32 apart.
+template <typename F>
+__device__ __forceinline__ void lw_batches(int nvec, F f) {
+    int v = threadIdx.x & 31;
+    for (; v < (nvec & ~(32 * kLwU - 1)); v += 32 * kLwU) f(LwInt<kLwU>(), LwInt<0>(), v);
+    const int left = nvec & (32 * kLwU - 1);
+    if (left > 96) f(LwInt<4>(), LwInt<1>(), v);
+    else if (left > 64) f(LwInt<3>(), LwInt<1>(), v);
+    else if (left > 32) f(LwInt<2>(), LwInt<1>(), v);
+    else if (left > 0) f(LwInt<1>(), LwInt<1>(), v);
+}
+
+// t = score + bias - r of N vectors, in log2 units (behind the row's end: the last vector's)
+template <int G, int N, bool kPart>
+__device__ __forceinline__ void lw_terms(float4 (&t)[N], const float4 *buf, const float4 *table, const unsigned short *bucket,
+                                         const float (&r)[4], int v, int nvec) {
+    float4 c[N], b[N];
+#pragma unroll
+    for (int u = 0; u < N; u++) {
+        const int x = kPart ? min(v + 32 * u, nvec - 1) : v + 32 * u;
+        c[u] = buf[x];
+        // the head group of the clamped vector is the last one's and may be another: nothing of it is used
+        b[u] = lw_bias<G>(table, bucket, x);
+    }
+    if (kPart) __syncwarp();   // the last vector is read by lanes that do not own it
+#pragma unroll
+    for (int u = 0; u < N; u++) t[u] = lb_shifted(c[u], b[u], r);
+}
+__device__ __forceinline__ float4 lw_exp2(float4 t) { return make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w)); }
+
+// A link that the flush of the exponentials could have touched, from the terms' logarithms (g + z - lse, log2 units)
+template <int G>
+__device__ __noinline__ float lw_tiny_link(float a0, float a1, float a2, float a3) {
+    const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3))), mm = m > -INFINITY ? m : 0.f;
+    const float q = lb_over_heads<G>(ex2(a0 - mm) + ex2(a1 - mm) + ex2(a2 - mm) + ex2(a3 - mm));
+    return m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
+}
+
 // What both kernels begin with: table, barriers, zeros.
 template <int G, int NT>
 __device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, const LinksBias &lb, int K) {
@@ -630,7 +693,8 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
     lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + warp / kLwRows;
-    LwRow r0 = lw_row(group, groups, L, K, mk, span), r1 = lw_row(group + step, groups, L, K, mk, span);
+    LwWalk walk(group, step, L);
+    LwRow r0 = lw_row(walk, B, L, K, mk, span), r1 = lw_row(walk, B, L, K, mk, span);
     LwSlot s0 = lw_slot<G, false>(r0, K, false);
     lw_issue<G, false>(r0, s0, ring, mbar, content, nullptr, L, K);
     const auto gates_of = [&](const LwRow &r) {
@@ -650,7 +714,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
         const bool later = s1.at < 0;
         if (!later) lw_issue<G, false>(r1, s1, ring, mbar, content, nullptr, L, K);
         const float4 gate1 = gates_of(r1);
-        const LwRow r2 = lw_row(group + 2 * step, groups, L, K, mk, span);
+        const LwRow r2 = lw_row(walk, B, L, K, mk, span);
         if (r0.exists) {
             const int nvec = r0.nj * G;
             float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at);
@@ -672,20 +736,21 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 bad = !(fabsf(r[0]) < INFINITY && fabsf(r[1]) < INFINITY && fabsf(r[2]) < INFINITY && fabsf(r[3]) < INFINITY);
                 __syncwarp();   // before the nearest successor's place is written over
             }
-            for (int v0 = lane; v0 < nvec; v0 += 32 * kLwU) {
-                float4 t[kLwU];
+            lw_batches(nvec, [&](auto n, auto part, int v) {
+                constexpr int N = decltype(n)::value;
+                constexpr bool kPart = decltype(part)::value;
+                float4 t[N];
+                lw_terms<G, N, kPart>(t, buf, table, bucket, r, v, nvec);
 #pragma unroll
-                for (int u = 0; u < kLwU; u++)
-                    if (v0 + 32 * u < nvec) t[u] = lb_shifted(buf[v0 + 32 * u], lw_bias<G>(table, bucket, v0 + 32 * u), r);
-#pragma unroll
-                for (int u = 0; u < kLwU; u++)
-                    if (v0 + 32 * u < nvec) {
-                        const float4 e = make_float4(ex2(t[u].x), ex2(t[u].y), ex2(t[u].z), ex2(t[u].w));
-                        buf[v0 + 32 * u] = e;
+                for (int u = 0; u < N; u++) {
+                    const float4 e = lw_exp2(t[u]);
+                    if (!kPart || v + 32 * u < nvec) {
+                        buf[v + 32 * u] = e;
                         fadd2_rn(sum[0], sum[1], sum[0], sum[1], e.x, e.y);
                         fadd2_rn(sum[2], sum[3], sum[2], sum[3], e.z, e.w);
                     }
-            }
+                }
+            });
             bad |= !(fmaxf(fmaxf(sum[0], sum[1]), fmaxf(sum[2], sum[3])) < kLbHuge) ||
                    !(sum[0] + sum[1] + sum[2] + sum[3] < INFINITY);
             if (__any_sync(0xffffffffu, bad)) {   // the exact maximum of each head takes the place of r_h
@@ -734,29 +799,41 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 reinterpret_cast<float4 *>(head_lse + r0.row * H)[g] = o;
             }
             float *const out = links + r0.row * (int64_t)K;
-#pragma unroll 4
-            for (int v0 = 0; v0 < nvec; v0 += 32) {
-                const int v = v0 + lane, d = v / G;
-                const bool in = v < nvec;
-                const float4 e = in ? buf[v] : make_float4(0.f, 0.f, 0.f, 0.f);
-                float q = lb_over_heads<G>(fmaf(e.x, f[0], e.y * f[1]) + fmaf(e.z, f[2], e.w * f[3]));
-                float link = lg2(q) * kLn2;
-                if (__any_sync(0xffffffffu, in && q < kLbTiny)) {
-                    float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    if (in && !(np && !np[d])) {   // log2 of e f without the exponential's flush
-                        const float4 z = lb_shifted(__ldg(src + v), lw_bias<G>(table, bucket, v), r);
-                        if (ls[0] < INFINITY) t[0] = z.x + (g2[0] - ls[0]);
-                        if (ls[1] < INFINITY) t[1] = z.y + (g2[1] - ls[1]);
-                        if (ls[2] < INFINITY) t[2] = z.z + (g2[2] - ls[2]);
-                        if (ls[3] < INFINITY) t[3] = z.w + (g2[3] - ls[3]);
-                    }
-                    const float m = lb_max_over_heads<G>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-                    const float mm = m > -INFINITY ? m : 0.f;
-                    q = lb_over_heads<G>(ex2(t[0] - mm) + ex2(t[1] - mm) + ex2(t[2] - mm) + ex2(t[3] - mm));
-                    link = m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
+            lw_batches(nvec, [&](auto n, auto part, int v) {
+                constexpr int N = decltype(n)::value;
+                constexpr bool kPart = decltype(part)::value;
+                float q[N];
+                float least = 1.f;
+#pragma unroll
+                for (int u = 0; u < N; u++) {
+                    const float4 e = buf[kPart ? min(v + 32 * u, nvec - 1) : v + 32 * u];
+                    q[u] = lb_over_heads<G>(fmaf(e.x, f[0], e.y * f[1]) + fmaf(e.z, f[2], e.w * f[3]));
+                    if (kPart && v + 32 * u >= nvec) q[u] = 1.f;
+                    least = fminf(least, q[u]);
                 }
-                if (g == 0 && in) out[d] = link;
-            }
+                const bool tiny = __any_sync(0xffffffffu, least < kLbTiny);
+#pragma unroll
+                for (int u = 0; u < N; u++) q[u] = lg2(q[u]) * kLn2;
+                if (tiny) {
+                    for (int u = 0; u < N; u++) {
+                        const int x = v + 32 * u;
+                        float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                        if (x < nvec && !(np && !np[x / G])) {   // log2 of e f without the exponential's flush
+                            const float4 z = lb_shifted(__ldg(src + x), lw_bias<G>(table, bucket, x), r);
+                            if (ls[0] < INFINITY) t[0] = z.x + (g2[0] - ls[0]);
+                            if (ls[1] < INFINITY) t[1] = z.y + (g2[1] - ls[1]);
+                            if (ls[2] < INFINITY) t[2] = z.z + (g2[2] - ls[2]);
+                            if (ls[3] < INFINITY) t[3] = z.w + (g2[3] - ls[3]);
+                        }
+                        const float link = lw_tiny_link<G>(t[0], t[1], t[2], t[3]);
+                        if (g == 0 && x < nvec) out[x / G] = link;
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < N; u++)
+                        if (g == 0 && (!kPart || v + 32 * u < nvec)) out[(v + 32 * u) / G] = q[u];
+                }
+            });
             for (int d = r0.nj + lane; d < K; d += 32) out[d] = -INFINITY;
         }
         // this row's place may be copied over from here on
@@ -798,7 +875,8 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + set;
-    LwRow r0 = lw_row(group, groups, L, K, mk, span), r1 = lw_row(group + step, groups, L, K, mk, span);
+    LwWalk walk(group, step, L);
+    LwRow r0 = lw_row(walk, B, L, K, mk, span), r1 = lw_row(walk, B, L, K, mk, span);
     LwSlot s0 = lw_slot<G, true>(r0, K, wide);
     lw_issue<G, true>(r0, s0, ring, mbar, content, grad_links, L, K);
     const auto of_row = [&](const float *p, const LwRow &r) {
@@ -817,7 +895,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         }
         __syncwarp();
         const float4 lse1 = of_row(head_lse, r1), gate1 = of_row(log_gates, r1);
-        const LwRow r2 = lw_row(group + 2 * step, groups, L, K, mk, span);
+        const LwRow r2 = lw_row(walk, B, L, K, mk, span);
         const int nvec = r0.nj * G;
         float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at + s0.window);
         float *const weight = reinterpret_cast<float *>(ring + s0.at) + s0.skip;   // G_d, then w_d
@@ -831,52 +909,67 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         const float g2[4] = {gate.x * kLog2e, gate.y * kLog2e, gate.z * kLog2e, gate.w * kLog2e};
         const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
         float S[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int v0 = lane; v0 - lane < nvec; v0 += 32 * kLwU) {
-            float4 t[kLwU];
-            float gd[kLwU];
+        lw_batches(nvec, [&](auto n, auto part, int v) {
+            constexpr int N = decltype(n)::value;
+            constexpr bool kPart = decltype(part)::value;
+            float4 t[N], q[N];
+            float w[N];
+            lw_terms<G, N, kPart>(t, buf, table, bucket, ls, v, nvec);
+            float least = 1.f;
 #pragma unroll
-            for (int u = 0; u < kLwU; u++) {
-                const int v = v0 + 32 * u;
-                t[u] = lb_ninf4();
-                gd[u] = 0.f;
-                if (v < nvec) {
-                    t[u] = lb_shifted(buf[v], lw_bias<G>(table, bucket, v), ls);
-                    gd[u] = weight[v / G];
-                }
+            for (int u = 0; u < N; u++) {
+                const bool in = !kPart || v + 32 * u < nvec;
+                if (kPart && !in) t[u] = lb_ninf4();
+                w[u] = in ? weight[(v + 32 * u) / G] : 0.f;
             }
 #pragma unroll
-            for (int u = 0; u < kLwU; u++) {
-                const int v = v0 + 32 * u;
-                if (v - lane >= nvec) break;
-                const bool in = v < nvec;
-                float4 keep = make_float4(ex2(t[u].x), ex2(t[u].y), ex2(t[u].z), ex2(t[u].w)), q = keep;
-                fmul2_rn(q.x, q.y, q.x, q.y, eg[0], eg[1]);
-                fmul2_rn(q.z, q.w, q.z, q.w, eg[2], eg[3]);
-                const float tot = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
-                float w = tot >= kLbTiny ? __fdividef(gd[u], tot) : 0.f, mark = w;
-                if (__any_sync(0xffffffffu, in && tot < kLbTiny)) {
+            for (int u = 0; u < N; u++) {
+                const bool in = !kPart || v + 32 * u < nvec;
+                const float4 soft = lw_exp2(t[u]);
+                q[u] = soft;
+                fmul2_rn(q[u].x, q[u].y, q[u].x, q[u].y, eg[0], eg[1]);
+                fmul2_rn(q[u].z, q[u].w, q[u].z, q[u].w, eg[2], eg[3]);
+                const float tot = lb_over_heads<G>((q[u].x + q[u].y) + (q[u].z + q[u].w));
+                if (in) {
+                    buf[v + 32 * u] = soft;
+                    least = fminf(least, tot);
+                }
+                if (tot >= kLbTiny) w[u] = __fdividef(w[u], tot);
+            }
+            if (__any_sync(0xffffffffu, least < kLbTiny)) {
+#pragma unroll
+                for (int u = 0; u < N; u++) {
+                    const bool in = !kPart || v + 32 * u < nvec;
+                    const float tot = lb_over_heads<G>((q[u].x + q[u].y) + (q[u].z + q[u].w));
                     const float a[4] = {t[u].x + g2[0], t[u].y + g2[1], t[u].z + g2[2], t[u].w + g2[3]};
                     const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-                    const bool tiny = tot < kLbTiny;   // the same in all lanes of a distance
+                    const bool tiny = !(tot >= kLbTiny);   // the same in all lanes of a distance
                     const float mm = m > -INFINITY ? m : 0.f;
-                    if (tiny) q = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
-                    const float tot2 = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
+                    float4 p = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
+                    const float tot2 = lb_over_heads<G>((p.x + p.y) + (p.z + p.w));
                     if (tiny) {
                         // p G in full where soft has lost it; soft S_h of such a place is below 2^-80 S_h and is
                         // dropped: the second pass finds the mark and the product in the buffer
-                        w = tot2 > 0.f ? gd[u] / tot2 : 0.f;
-                        keep = tot2 > 0.f ? make_float4(q.x * w, q.y * w, q.z * w, q.w * w) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        mark = __uint_as_float(kLwFull);
+                        const float k = tot2 > 0.f ? w[u] / tot2 : 0.f;   // a link of -inf: whatever its gradient is
+                        p = tot2 > 0.f ? make_float4(p.x * k, p.y * k, p.z * k, p.w * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (in) buf[v + 32 * u] = p;
+                        S[0] += p.x;
+                        S[1] += p.y;
+                        S[2] += p.z;
+                        S[3] += p.w;
+                        q[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        w[u] = __uint_as_float(kLwFull);
                     }
                 }
-                if (in) {
-                    buf[v] = keep;
-                    if (g == 0) weight[v / G] = mark;
-                }
-                ffma2_rn(S[0], S[1], q.x, q.y, w, w);
-                ffma2_rn(S[2], S[3], q.z, q.w, w, w);
             }
-        }
+#pragma unroll
+            for (int u = 0; u < N; u++) {
+                if (g == 0 && (!kPart || v + 32 * u < nvec)) weight[(v + 32 * u) / G] = w[u];
+                const float k = __float_as_uint(w[u]) == kLwFull ? 0.f : w[u];
+                ffma2_rn(S[0], S[1], q[u].x, q[u].y, k, k);
+                ffma2_rn(S[2], S[3], q[u].z, q[u].w, k, k);
+            }
+        });
         __syncwarp();
         // the next row on its way: the gradient of the row before this one has left its place
         LwSlot s1 = lw_slot<G, true>(r1, K, wide);
@@ -891,26 +984,28 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             lw_reduce<G, false>(S);
             if (lane < G)
                 reinterpret_cast<float4 *>(grad_log_gates + r0.row * H)[g] = make_float4(S[0], S[1], S[2], S[3]);
-            for (int v0 = lane; v0 < nvec; v0 += 32 * kLwU) {
-                float4 o[kLwU];
-                float w[kLwU];
+            lw_batches(nvec, [&](auto n, auto part, int v) {
+                constexpr int N = decltype(n)::value;
+                constexpr bool kPart = decltype(part)::value;
+                float4 o[N];
+                float w[N];
 #pragma unroll
-                for (int u = 0; u < kLwU; u++)
-                    if (v0 + 32 * u < nvec) {
-                        o[u] = buf[v0 + 32 * u];
-                        w[u] = weight[(v0 + 32 * u) / G];
-                    }
+                for (int u = 0; u < N; u++) {
+                    const int x = kPart ? min(v + 32 * u, nvec - 1) : v + 32 * u;
+                    o[u] = buf[x];
+                    w[u] = weight[x / G];
+                }
+                if (kPart) __syncwarp();   // the last vector is read by lanes that do not own it
 #pragma unroll
-                for (int u = 0; u < kLwU; u++)
-                    if (v0 + 32 * u < nvec && __float_as_uint(w[u]) != kLwFull) {
-                        float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
-                        ffma2_rn(k.x, k.y, eg[0], eg[1], w[u], w[u]);
-                        ffma2_rn(k.z, k.w, eg[2], eg[3], w[u], w[u]);
-                        fmul2_rn(o[u].x, o[u].y, o[u].x, o[u].y, k.x, k.y);
-                        fmul2_rn(o[u].z, o[u].w, o[u].z, o[u].w, k.z, k.w);
-                        buf[v0 + 32 * u] = o[u];
-                    }
-            }
+                for (int u = 0; u < N; u++) {
+                    float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
+                    ffma2_rn(k.x, k.y, eg[0], eg[1], w[u], w[u]);
+                    ffma2_rn(k.z, k.w, eg[2], eg[3], w[u], w[u]);
+                    fmul2_rn(o[u].x, o[u].y, o[u].x, o[u].y, k.x, k.y);
+                    fmul2_rn(o[u].z, o[u].w, o[u].z, o[u].w, k.z, k.w);
+                    if ((!kPart || v + 32 * u < nvec) && __float_as_uint(w[u]) != kLwFull) buf[v + 32 * u] = o[u];
+                }
+            });
             umma::fence_smem_to_async();
             __syncwarp();
             unsigned char *const dense = reinterpret_cast<unsigned char *>(grad_content + r0.row * (int64_t)L * H);
