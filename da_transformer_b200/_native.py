@@ -146,10 +146,29 @@ def require_cuda(*tensors):
             raise RuntimeError("all tensors of the custom cuda operations must be CUDA tensors")
 
 
-def require_same_device(device, **tensors):
+def require_device(device, **tensors):
+    """All tensors (None is skipped) on the CUDA device ``device``."""
+    if device.type != "cuda":
+        require_cuda()
+        raise RuntimeError("all tensors of the custom cuda operations must be CUDA tensors")
     for name, t in tensors.items():
         if t is not None and t.device != device:
             raise RuntimeError(f"{name} is on {t.device}, expected {device}")
+
+
+def address(t):
+    """Address of a tensor (0 for None) as a number, which ctypes takes for a pointer argument."""
+    return 0 if t is None else t.data_ptr()
+
+
+# torch's own shortcut to the current stream's handle (a Stream object costs 2 us a call); absent, the public way
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def stream_address(device):
+    if _raw_stream is None or device.index is None:
+        return torch.cuda.current_stream(device).cuda_stream
+    return _raw_stream(device.index)
 
 
 def stream_ptr(device):

@@ -12,7 +12,7 @@ import torch
 from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
-from ._native import check, lib, ptr, require_cuda, require_same_device, stream_ptr
+from ._native import address, check, lib, ptr, require_cuda, require_device, stream_address, stream_ptr
 from .dag_loss import _status_word
 
 __all__ = ["DagLinksFromHeadsFunc", "DagBiasedLinksFunc", "dag_links_from_heads", "dag_relative_buckets",
@@ -87,77 +87,90 @@ class DagLinksFromHeadsFunc(Function):
         return grad_content, grad_gates, None, None, None
 
 
+def _check_biased_links(content, gates, table, buckets, nonpad_mask, bound_end, translen):
+    if content.dim() != 4 or content.size(1) != content.size(2):
+        raise RuntimeError("log_multi_content should be [batch, prelen, prelen, heads]")
+    bsz, prelen, _, heads = content.shape
+    if gates.shape != (bsz, prelen, heads):
+        raise RuntimeError("log_gates should be [batch, prelen, heads]")
+    if table.dim() != 2 or table.size(0) < 1 or table.size(1) != heads:
+        raise RuntimeError("relative_bias should be [num_buckets, heads]")
+    for name, t in (("log_multi_content", content), ("log_gates", gates), ("relative_bias", table)):
+        if t.dtype is not torch.float32:
+            raise RuntimeError(f"dag_links_from_heads is implemented for float32 ({name} is {t.dtype})")
+    if translen < 1:
+        raise RuntimeError("max_transition_length must be at least 1 and prelen at least 2")
+    if buckets.dim() != 1 or buckets.dtype is not torch.long or buckets.size(0) < translen:
+        raise RuntimeError(f"relative_buckets should be a long tensor with at least {translen} distances")
+    if nonpad_mask is not None and nonpad_mask.shape != (bsz, prelen):
+        raise RuntimeError("nonpad_mask should be [batch, prelen]")
+    if bound_end is not None and (bound_end.shape != (bsz, prelen) or bound_end.dtype is not torch.long):
+        raise RuntimeError("bound_end should be a long tensor of shape [batch, prelen]")
+    require_device(content.device, log_gates=gates, relative_bias=table, relative_buckets=buckets,
+                   nonpad_mask=nonpad_mask, bound_end=bound_end)
+
+
 class DagBiasedLinksFunc(Function):
-    """``dag_links_from_heads`` with a learned relative position bias."""
+    """``dag_links_from_heads`` with a learned relative position bias.  ``rest``: (relative_buckets, nonpad_mask,
+    bound_end, max_transition_length)."""
 
     @staticmethod
-    def forward(ctx, log_multi_content, log_gates, relative_bias, relative_buckets, nonpad_mask, bound_end,
-                max_transition_length):
-        if log_multi_content.dim() != 4 or log_multi_content.size(1) != log_multi_content.size(2):
-            raise RuntimeError("log_multi_content should be [batch, prelen, prelen, heads]")
+    def forward(ctx, log_multi_content, log_gates, relative_bias, rest):
+        relative_buckets, nonpad_mask, bound_end, max_transition_length = rest
+        translen = min(int(max_transition_length), log_multi_content.size(1) - 1) if log_multi_content.dim() > 1 else 0
+        _check_biased_links(log_multi_content, log_gates, relative_bias, relative_buckets, nonpad_mask, bound_end, translen)
         bsz, prelen, _, heads = log_multi_content.shape
-        if log_gates.shape != (bsz, prelen, heads):
-            raise RuntimeError("log_gates should be [batch, prelen, heads]")
-        if relative_bias.dim() != 2 or relative_bias.size(0) < 1 or relative_bias.size(1) != heads:
-            raise RuntimeError("relative_bias should be [num_buckets, heads]")
-        for name, t in (("log_multi_content", log_multi_content), ("log_gates", log_gates),
-                        ("relative_bias", relative_bias)):
-            if t.dtype != torch.float32:
-                raise RuntimeError(f"dag_links_from_heads is implemented for float32 ({name} is {t.dtype})")
-        translen = min(int(max_transition_length), prelen - 1)
-        if translen < 1:
-            raise RuntimeError("max_transition_length must be at least 1 and prelen at least 2")
-        if relative_buckets.dim() != 1 or relative_buckets.dtype != torch.long or relative_buckets.numel() < translen:
-            raise RuntimeError(f"relative_buckets should be a long tensor with at least {translen} distances")
-        if nonpad_mask is not None and nonpad_mask.shape != (bsz, prelen):
-            raise RuntimeError("nonpad_mask should be [batch, prelen]")
-        if bound_end is not None and (bound_end.shape != (bsz, prelen) or bound_end.dtype != torch.long):
-            raise RuntimeError("bound_end should be a long tensor of shape [batch, prelen]")
-        require_cuda(log_multi_content, log_gates, relative_bias, relative_buckets, nonpad_mask, bound_end)
         dev = log_multi_content.device
-        require_same_device(dev, log_gates=log_gates, relative_bias=relative_bias, relative_buckets=relative_buckets,
-                            nonpad_mask=nonpad_mask, bound_end=bound_end)
-        need_grad = any(ctx.needs_input_grad[:3])
+        need_grad = True in ctx.needs_input_grad
         with torch.cuda.device(dev):
-            content = log_multi_content.contiguous()
-            gates = log_gates.contiguous()
-            table = relative_bias.contiguous()
+            content, gates, table = log_multi_content.contiguous(), log_gates.contiguous(), relative_bias.contiguous()
             buckets = relative_buckets.contiguous()
             nonpad = _mask_bytes(nonpad_mask)
-            bound_end = None if bound_end is None else bound_end.contiguous()
+            if bound_end is not None:
+                bound_end = bound_end.contiguous()
+            links = content.new_empty((bsz, prelen, translen))
+            head_lse = torch.empty_like(gates) if need_grad else None
             spans = None if nonpad is None else torch.empty(max(bsz, 1), 2, dtype=torch.int32, device=dev)
-            links = torch.empty(bsz, prelen, translen, dtype=torch.float32, device=dev)
-            head_lse = torch.empty(bsz, prelen, heads, dtype=torch.float32, device=dev) if need_grad else None
             check(lib().dat_links_from_heads_biased(
-                ptr(content), ptr(gates), ptr(table), ptr(buckets), table.size(0), ptr(bound_end), ptr(nonpad),
-                ptr(links), ptr(head_lse), ptr(spans), ptr(_status_word(dev)), bsz, prelen, heads, translen, stream_ptr(dev)),
+                content.data_ptr(), gates.data_ptr(), table.data_ptr(), buckets.data_ptr(), table.size(0),
+                address(bound_end), address(nonpad), links.data_ptr(), address(head_lse), address(spans),
+                _status_word(dev).data_ptr(), bsz, prelen, heads, translen, stream_address(dev)),
                 "links_from_heads (biased)")
         if need_grad:
             ctx.save_for_backward(content, gates, table, buckets, links, head_lse, nonpad, bound_end, spans)
         return links
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad_links):
-        content, gates, table, buckets, links, head_lse, nonpad, bound_end, spans = ctx.saved_tensors
-        bsz, prelen, _, heads = content.shape
-        translen = links.size(2)
-        dev = content.device
-        L = lib()
-        with torch.cuda.device(dev):
-            grad_links = grad_links.to(torch.float32).contiguous()
-            grad_content = torch.empty_like(content)
-            grad_gates = torch.empty_like(gates)
-            grad_table = ws = None
-            if ctx.needs_input_grad[2]:
-                grad_table = torch.empty_like(table)
-                ws = torch.empty(max(L.dat_links_bias_workspace_bytes(bsz, prelen, heads, translen), 1),
-                                 dtype=torch.uint8, device=dev)
-            check(L.dat_links_from_heads_biased_backward(
-                ptr(grad_links), ptr(content), ptr(gates), ptr(table), ptr(buckets), table.size(0), ptr(links),
-                ptr(head_lse), ptr(bound_end), ptr(nonpad), ptr(spans), ptr(grad_content), ptr(grad_gates),
-                ptr(grad_table), ptr(ws), ptr(_status_word(dev)), bsz, prelen, heads, translen, stream_ptr(dev)), "links_from_heads_backward (biased)")
-        return grad_content, grad_gates, grad_table, None, None, None, None
+        # the wrapper that marks the gradients costs a good part of a small backward and is only wanted by
+        # whoever differentiates again
+        return _biased_links_backward_once(ctx, grad_links) if torch.is_grad_enabled() else _biased_links_backward(ctx, grad_links)
+
+
+def _biased_links_backward(ctx, grad_links):
+    content, gates, table, buckets, links, head_lse, nonpad, bound_end, spans = ctx.saved_tensors
+    bsz, prelen, _, heads = content.shape
+    translen = links.size(2)
+    dev = content.device
+    L = lib()
+    with torch.cuda.device(dev):
+        grad_links = grad_links.to(torch.float32).contiguous()
+        grad_content, grad_gates = torch.empty_like(content), torch.empty_like(gates)
+        grad_table = ws = None
+        if ctx.needs_input_grad[2]:
+            grad_table = torch.empty_like(table)
+            ws = torch.empty(max(L.dat_links_bias_workspace_bytes(bsz, prelen, heads, translen), 1),
+                             dtype=torch.uint8, device=dev)
+        check(L.dat_links_from_heads_biased_backward(
+            grad_links.data_ptr(), content.data_ptr(), gates.data_ptr(), table.data_ptr(), buckets.data_ptr(),
+            table.size(0), links.data_ptr(), head_lse.data_ptr(), address(bound_end), address(nonpad), address(spans),
+            grad_content.data_ptr(), grad_gates.data_ptr(), address(grad_table), address(ws),
+            _status_word(dev).data_ptr(), bsz, prelen, heads, translen, stream_address(dev)),
+            "links_from_heads_backward (biased)")
+    return grad_content, grad_gates, grad_table, None
+
+
+_biased_links_backward_once = once_differentiable(_biased_links_backward)
 
 
 def dag_relative_buckets(num_distances, num_buckets, max_distance=128, device=None):
@@ -207,8 +220,8 @@ def dag_links_from_heads(log_multi_content, log_gates, nonpad_mask=None, bound_e
     if (relative_bias is None) != (relative_buckets is None):
         raise RuntimeError("relative_bias and relative_buckets are given together")
     if relative_bias is not None:
-        return DagBiasedLinksFunc.apply(log_multi_content, log_gates, relative_bias, relative_buckets, nonpad_mask,
-                                        bound_end, max_transition_length)
+        return DagBiasedLinksFunc.apply(log_multi_content, log_gates, relative_bias,
+                                        (relative_buckets, nonpad_mask, bound_end, max_transition_length))
     return DagLinksFromHeadsFunc.apply(log_multi_content, log_gates, nonpad_mask, bound_end,
                                        max_transition_length)
 

@@ -13,7 +13,7 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from ._native import check, lib, ptr, require_cuda, require_same_device, stream_ptr
+from ._native import address, check, lib, require_device, stream_address
 from .dag_loss import _status_word
 from .graph_ops import _mask_bytes
 
@@ -22,46 +22,52 @@ __all__ = ["DagPolicyLossFunc", "dag_policy_loss", "DagPreferenceLossFunc", "dag
 _PREFERENCE_KINDS = {"sigmoid": 0, "hinge": 1, "squared": 2}
 
 
+def _check_policy(word_ins_out, link_logp, tokens, old_logp, advantage, mask, ref_logits, ref_logp, grad_scale):
+    if word_ins_out.dim() != 3:
+        raise RuntimeError("word_ins_out dim != 3")
+    bsz, prelen, vocab = word_ins_out.shape
+    if vocab < 1:
+        raise RuntimeError("word_ins_out has an empty vocabulary")
+    if not word_ins_out.is_contiguous():
+        raise RuntimeError("word_ins_out is not contiguous")
+    shape = (bsz, prelen)
+    if tokens.shape != shape or tokens.dtype is not torch.long:
+        raise RuntimeError("tokens should be a long tensor of shape [batch, prelen]")
+    for name, t in (("old_logp", old_logp), ("link_logp", link_logp), ("ref_logp", ref_logp)):
+        if t is not None and (t.shape != shape or t.dtype is not torch.float32):
+            raise RuntimeError(f"{name} should be a float32 tensor of shape [batch, prelen]")
+    if advantage.dtype is not torch.float32 or (advantage.shape != shape and advantage.shape != (bsz,)):
+        raise RuntimeError("advantage should be a float32 tensor of shape [batch] or [batch, prelen]")
+    if mask is not None and mask.shape != shape:
+        raise RuntimeError("mask should be [batch, prelen]")
+    if ref_logits is not None:
+        if ref_logp is not None:
+            raise RuntimeError("give ref_logits (KL over the vocabulary) or ref_logp (KL estimate), not both")
+        if ref_logits.shape != word_ins_out.shape or ref_logits.dtype is not word_ins_out.dtype:
+            raise RuntimeError("ref_logits should have the shape and dtype of word_ins_out")
+        if not ref_logits.is_contiguous():
+            raise RuntimeError("ref_logits is not contiguous")
+    if grad_scale is not None and (grad_scale.numel() != 1 or grad_scale.dtype is not torch.float32):
+        raise RuntimeError("grad_scale should be a number or a float32 tensor with one element")
+    require_device(word_ins_out.device, link_logp=link_logp, tokens=tokens, old_logp=old_logp, advantage=advantage,
+                   mask=mask, ref_logits=ref_logits, ref_logp=ref_logp, grad_scale=grad_scale)
+
+
 class DagPolicyLossFunc(Function):
+    """``dag_policy_loss``.  ``rest``: its other arguments, in their order."""
+
     @staticmethod
-    def forward(ctx, word_ins_out, link_logp, tokens, old_logp, advantage, mask, ref_logits, ref_logp, kl_coef,
-                clip_low, clip_high, grad_scale):
-        if word_ins_out.dim() != 3:
-            raise RuntimeError("word_ins_out dim != 3")
-        bsz, prelen, vocab = word_ins_out.shape
-        if vocab < 1:
-            raise RuntimeError("word_ins_out has an empty vocabulary")
+    def forward(ctx, word_ins_out, link_logp, rest):
+        (tokens, old_logp, advantage, mask, ref_logits, ref_logp, kl_coef, clip_low, clip_high, grad_scale) = rest
         dt = _native.dtype_code(word_ins_out.dtype)
-        if not word_ins_out.is_contiguous():
-            raise RuntimeError("word_ins_out is not contiguous")
-        if tokens.shape != (bsz, prelen) or tokens.dtype != torch.long:
-            raise RuntimeError("tokens should be a long tensor of shape [batch, prelen]")
-        for name, t in (("old_logp", old_logp), ("link_logp", link_logp), ("ref_logp", ref_logp)):
-            if t is not None and (t.shape != (bsz, prelen) or t.dtype != torch.float32):
-                raise RuntimeError(f"{name} should be a float32 tensor of shape [batch, prelen]")
-        if advantage.dtype != torch.float32 or advantage.shape not in ((bsz,), (bsz, prelen)):
-            raise RuntimeError("advantage should be a float32 tensor of shape [batch] or [batch, prelen]")
-        if mask is not None and mask.shape != (bsz, prelen):
-            raise RuntimeError("mask should be [batch, prelen]")
-        if ref_logits is not None:
-            if ref_logp is not None:
-                raise RuntimeError("give ref_logits (KL over the vocabulary) or ref_logp (KL estimate), not both")
-            if ref_logits.shape != word_ins_out.shape or ref_logits.dtype != word_ins_out.dtype:
-                raise RuntimeError("ref_logits should have the shape and dtype of word_ins_out")
-            if not ref_logits.is_contiguous():
-                raise RuntimeError("ref_logits is not contiguous")
-        clip_low, clip_high = float(clip_low), float(clip_high)
+        clip_low, clip_high, kl_coef = float(clip_low), float(clip_high), float(kl_coef)
         if not (clip_low >= 0 and clip_high >= 0):
             raise RuntimeError("clip_low and clip_high should not be negative")
-        scale_tensor = None
-        if isinstance(grad_scale, torch.Tensor):
-            if grad_scale.numel() != 1 or grad_scale.dtype != torch.float32:
-                raise RuntimeError("grad_scale should be a number or a float32 tensor with one element")
-            scale_tensor = grad_scale
-        require_cuda(word_ins_out, link_logp, tokens, old_logp, advantage, mask, ref_logits, ref_logp, scale_tensor)
+        scale_tensor = grad_scale if isinstance(grad_scale, torch.Tensor) else None
+        _check_policy(word_ins_out, link_logp, tokens, old_logp, advantage, mask, ref_logits, ref_logp, scale_tensor)
+        scale = 1.0 if scale_tensor is not None or grad_scale is None else float(grad_scale)
+        bsz, prelen, vocab = word_ins_out.shape
         dev = word_ins_out.device
-        require_same_device(dev, link_logp=link_logp, tokens=tokens, old_logp=old_logp, advantage=advantage, mask=mask,
-                            ref_logits=ref_logits, ref_logp=ref_logp, grad_scale=scale_tensor)
         L = lib()
         need_logits, need_link = ctx.needs_input_grad[0], link_logp is not None and ctx.needs_input_grad[1]
         with torch.cuda.device(dev):
@@ -72,47 +78,55 @@ class DagPolicyLossFunc(Function):
             refp = None if ref_logp is None else ref_logp.contiguous()
             loss = torch.empty((), dtype=torch.float32, device=dev)
             stats = torch.empty(5, dtype=torch.float64, device=dev)
-            logp = torch.empty(bsz, prelen, dtype=torch.float32, device=dev)
-            kl = torch.empty(bsz, prelen, dtype=torch.float32, device=dev)
-            state = (torch.empty(bsz * prelen, 4, dtype=torch.float32, device=dev)
-                     if need_logits or need_link else None)
+            logp, kl = torch.empty_like(old_logp), torch.empty_like(old_logp)
+            need_grad = need_logits or need_link
             grad = torch.empty_like(word_ins_out) if need_logits and grad_scale is not None else None
-            ws = torch.empty(L.dat_policy_loss_workspace_bytes(bsz, prelen), dtype=torch.uint8, device=dev)
+            # the state of the rows (16 bytes each) for the backward, then the workspace
+            at = bsz * prelen * 16 if need_grad else 0
+            ws = torch.empty(at + L.dat_policy_loss_workspace_bytes(bsz, prelen), dtype=torch.uint8, device=dev)
             check(L.dat_policy_loss(
-                ptr(word_ins_out), ptr(ref_logits), dt, ptr(tokens), ptr(old_logp), ptr(advantage), advantage.stride(0),
-                advantage.stride(1) if advantage.dim() == 2 else 0, ptr(link), ptr(refp), ptr(mask), float(kl_coef),
-                clip_low, clip_high, ptr(scale_tensor), 1.0 if scale_tensor is not None or grad_scale is None else
-                float(grad_scale), ptr(loss), ptr(stats), ptr(logp), ptr(kl), ptr(state), ptr(grad), ptr(ws),
-                ptr(_status_word(dev)), bsz, prelen, vocab, stream_ptr(dev)), "policy_loss")
+                word_ins_out.data_ptr(), address(ref_logits), dt, tokens.data_ptr(), old_logp.data_ptr(),
+                advantage.data_ptr(), advantage.stride(0), advantage.stride(1) if advantage.dim() == 2 else 0,
+                address(link), address(refp), address(mask), kl_coef, clip_low, clip_high, address(scale_tensor), scale,
+                loss.data_ptr(), stats.data_ptr(), logp.data_ptr(), kl.data_ptr(), ws.data_ptr() if at else 0, address(grad),
+                ws.data_ptr() + at, _status_word(dev).data_ptr(), bsz, prelen, vocab, stream_address(dev)), "policy_loss")
         ctx.mark_non_differentiable(logp, kl, stats)
         ctx.set_materialize_grads(False)
-        if state is not None:
-            ctx.save_for_backward(word_ins_out, ref_logits, tokens, mask, state, ws)
-            ctx.grad, ctx.kl_coef = grad, float(kl_coef)
+        if need_grad:
+            ctx.save_for_backward(word_ins_out, ref_logits, tokens, mask)
+            ctx.ws = ws               # the library's own, nobody else holds it
+            ctx.grad, ctx.kl_coef = grad, kl_coef
         return loss, logp, kl, stats
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss, grad_logp, grad_kl, grad_stats):
-        none = (None,) * 12
-        if grad_loss is None:
-            return none
-        word_ins_out, ref_logits, tokens, mask, state, ws = ctx.saved_tensors
-        bsz, prelen, vocab = word_ins_out.shape
-        dev = word_ins_out.device
-        # the buffer that the forward wrote is given away once; a second backward makes its own
-        grad, ctx.grad = ctx.grad, None
-        with torch.cuda.device(dev):
-            grad_loss = grad_loss.to(torch.float32).contiguous()
-            written = grad is not None
-            if not written and ctx.needs_input_grad[0]:
-                grad = torch.empty_like(word_ins_out)
-            link = torch.empty(bsz, prelen, dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
-            check(lib().dat_policy_loss_backward(
-                ptr(word_ins_out), ptr(ref_logits), _native.dtype_code(word_ins_out.dtype), ptr(tokens), ptr(mask),
-                ctx.kl_coef, ptr(state), ptr(ws), ptr(grad_loss), int(written), ptr(grad), ptr(link), bsz, prelen,
-                vocab, stream_ptr(dev)), "policy_loss_backward")
-        return (grad, link) + none[2:]
+    def backward(ctx, grad_loss, *unused):
+        # as for the links: the marking wrapper only for whoever differentiates again
+        return _policy_backward_once(ctx, grad_loss) if torch.is_grad_enabled() else _policy_backward(ctx, grad_loss)
+
+
+def _policy_backward(ctx, grad_loss):
+    if grad_loss is None:
+        return None, None, None
+    word_ins_out, ref_logits, tokens, mask = ctx.saved_tensors
+    ws = ctx.ws.data_ptr()
+    bsz, prelen, vocab = word_ins_out.shape
+    dev = word_ins_out.device
+    # the buffer that the forward wrote is given away once; a second backward makes its own
+    grad, ctx.grad = ctx.grad, None
+    with torch.cuda.device(dev):
+        grad_loss = grad_loss.to(torch.float32).contiguous()
+        written = grad is not None
+        if not written and ctx.needs_input_grad[0]:
+            grad = torch.empty_like(word_ins_out)
+        link = torch.empty(bsz, prelen, dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
+        check(lib().dat_policy_loss_backward(
+            word_ins_out.data_ptr(), address(ref_logits), _native.dtype_code(word_ins_out.dtype), tokens.data_ptr(),
+            address(mask), ctx.kl_coef, ws, ws + bsz * prelen * 16, grad_loss.data_ptr(), int(written),
+            address(grad), address(link), bsz, prelen, vocab, stream_address(dev)), "policy_loss_backward")
+    return grad, link, None
+
+
+_policy_backward_once = once_differentiable(_policy_backward)
 
 
 def dag_policy_loss(word_ins_out, tokens, old_logp, advantage, mask=None, link_logp=None, ref_logits=None,
@@ -140,62 +154,73 @@ def dag_policy_loss(word_ins_out, tokens, old_logp, advantage, mask=None, link_l
     computes it again where another gradient arrives.  ``grad_scale=None`` leaves it to the backward (the
     logits are then read twice, and nothing of their size is held in between).  ``word_ins_out`` is not
     changed.  A token outside the vocabulary makes its row NaN and sets bit 4 of ``last_status()``."""
-    return DagPolicyLossFunc.apply(word_ins_out, link_logp, tokens, old_logp, advantage, mask, ref_logits, ref_logp,
-                                   kl_coef, clip_low, clip_high, grad_scale)
+    return DagPolicyLossFunc.apply(word_ins_out, link_logp, (tokens, old_logp, advantage, mask, ref_logits, ref_logp,
+                                                             kl_coef, clip_low, clip_high, grad_scale))
+
+
+def _check_preference(chosen, rejected, reference_chosen, reference_rejected, chosen_length, rejected_length, kind,
+                      label_smoothing):
+    shape = chosen.shape
+    if len(shape) != 1 or rejected.shape != shape:
+        raise RuntimeError("chosen and rejected must be [pairs]")
+    for name, t in (("chosen", chosen), ("rejected", rejected), ("reference_chosen", reference_chosen),
+                    ("reference_rejected", reference_rejected)):
+        if t is not None and (t.dtype is not torch.float32 or t.shape != shape):
+            raise RuntimeError(f"{name} should be a float32 tensor of shape [pairs]")
+    for name, t in (("chosen_length", chosen_length), ("rejected_length", rejected_length)):
+        if t is not None and (t.dtype is not torch.long or t.shape != shape):
+            raise RuntimeError(f"{name} should be a long tensor of shape [pairs]")
+    if (reference_chosen is None) != (reference_rejected is None):
+        raise RuntimeError("reference_chosen and reference_rejected are given together")
+    if (chosen_length is None) != (rejected_length is None):
+        raise RuntimeError("chosen_length and rejected_length are given together")
+    if kind not in _PREFERENCE_KINDS:
+        raise RuntimeError(f"unknown kind {kind!r} (one of {', '.join(_PREFERENCE_KINDS)})")
+    if not 0.0 <= label_smoothing <= 1.0:
+        raise RuntimeError("label_smoothing should be in [0, 1]")
+    require_device(chosen.device, rejected=rejected, reference_chosen=reference_chosen,
+                   reference_rejected=reference_rejected, chosen_length=chosen_length, rejected_length=rejected_length)
 
 
 class DagPreferenceLossFunc(Function):
+    """``dag_preference_loss``.  ``rest``: its other arguments, in their order."""
+
     @staticmethod
-    def forward(ctx, chosen, rejected, reference_chosen, reference_rejected, chosen_length, rejected_length, beta,
-                kind, label_smoothing):
-        if chosen.dim() != 1 or rejected.shape != chosen.shape:
-            raise RuntimeError("chosen and rejected must be [pairs]")
-        pairs = chosen.numel()
-        for name, t in (("chosen", chosen), ("rejected", rejected), ("reference_chosen", reference_chosen),
-                        ("reference_rejected", reference_rejected)):
-            if t is not None and (t.shape != chosen.shape or t.dtype != torch.float32):
-                raise RuntimeError(f"{name} should be a float32 tensor of shape [pairs]")
-        for name, t in (("chosen_length", chosen_length), ("rejected_length", rejected_length)):
-            if t is not None and (t.shape != chosen.shape or t.dtype != torch.long):
-                raise RuntimeError(f"{name} should be a long tensor of shape [pairs]")
-        if (reference_chosen is None) != (reference_rejected is None):
-            raise RuntimeError("reference_chosen and reference_rejected are given together")
-        if (chosen_length is None) != (rejected_length is None):
-            raise RuntimeError("chosen_length and rejected_length are given together")
-        if kind not in _PREFERENCE_KINDS:
-            raise RuntimeError(f"unknown kind {kind!r} (one of {', '.join(_PREFERENCE_KINDS)})")
-        if not 0.0 <= label_smoothing <= 1.0:
-            raise RuntimeError("label_smoothing should be in [0, 1]")
-        others = dict(rejected=rejected, reference_chosen=reference_chosen, reference_rejected=reference_rejected,
-                      chosen_length=chosen_length, rejected_length=rejected_length)
-        require_cuda(chosen, *others.values())
-        dev = chosen.device
-        require_same_device(dev, **others)
+    def forward(ctx, chosen, rejected, rest):
+        (reference_chosen, reference_rejected, chosen_length, rejected_length, beta, kind, label_smoothing) = rest
+        _check_preference(chosen, rejected, reference_chosen, reference_rejected, chosen_length, rejected_length, kind,
+                          label_smoothing)
+        pairs, dev = chosen.size(0), chosen.device
+        need_grad = True in ctx.needs_input_grad
         with torch.cuda.device(dev):
-            flat = [None if t is None else t.contiguous() for t in (chosen, *others.values())]
+            flat = [None if t is None else t.contiguous() for t in (chosen, rejected, reference_chosen, reference_rejected,
+                                                                    chosen_length, rejected_length)]
             loss = torch.empty((), dtype=torch.float32, device=dev)
             rewards = torch.empty(2, pairs, dtype=torch.float32, device=dev)
             stats = torch.empty(6, dtype=torch.float64, device=dev)
-            need_grad = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-            slope = torch.empty(2, pairs, dtype=torch.float32, device=dev) if need_grad else None
-            check(lib().dat_preference_loss(*(ptr(t) for t in flat), float(beta), float(label_smoothing),
-                                            _PREFERENCE_KINDS[kind], ptr(loss), ptr(rewards), ptr(stats), ptr(slope),
-                                            ptr(_status_word(dev)), pairs, stream_ptr(dev)), "preference_loss")
+            slope = torch.empty_like(rewards) if need_grad else None
+            check(lib().dat_preference_loss(*map(address, flat), float(beta), float(label_smoothing),
+                                            _PREFERENCE_KINDS[kind], loss.data_ptr(), rewards.data_ptr(),
+                                            stats.data_ptr(), address(slope), _status_word(dev).data_ptr(), pairs,
+                                            stream_address(dev)), "preference_loss")
         ctx.mark_non_differentiable(rewards, stats)
         ctx.set_materialize_grads(False)
-        if need_grad:
-            ctx.save_for_backward(slope)
+        ctx.slope = slope     # d loss / d (chosen, rejected): the library's own, nobody else holds it
         return loss, rewards, stats
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_loss, grad_rewards, grad_stats):
-        none = (None,) * 9
-        if grad_loss is None:
-            return none
-        (slope,) = ctx.saved_tensors
-        grads = slope * grad_loss
-        return (grads[0], grads[1]) + none[2:]
+    def backward(ctx, grad_loss, *unused):
+        return _preference_backward_once(ctx, grad_loss) if torch.is_grad_enabled() else _preference_backward(ctx, grad_loss)
+
+
+def _preference_backward(ctx, grad_loss):
+    if grad_loss is None:
+        return None, None, None
+    chosen, rejected = (ctx.slope * grad_loss).unbind()
+    return chosen, rejected, None
+
+
+_preference_backward_once = once_differentiable(_preference_backward)
 
 
 def dag_preference_loss(chosen, rejected, reference_chosen=None, reference_rejected=None, beta=0.1, kind="sigmoid",
@@ -215,5 +240,5 @@ def dag_preference_loss(chosen, rejected, reference_chosen=None, reference_rejec
     sets bit 1 of ``last_status()``).  Returns ``(loss, rewards, stats)``: the scalar, differentiable in
     ``chosen`` and ``rejected``; the rewards [2,B] fp32; the fp64 vector ``[sum of the losses, sum of the chosen
     rewards, of the rejected ones, n with h > 0, n pairs, n invalid]``."""
-    return DagPreferenceLossFunc.apply(chosen, rejected, reference_chosen, reference_rejected, chosen_length,
-                                       rejected_length, beta, kind, label_smoothing)
+    return DagPreferenceLossFunc.apply(chosen, rejected, (reference_chosen, reference_rejected, chosen_length,
+                                                          rejected_length, beta, kind, label_smoothing))
