@@ -430,7 +430,7 @@ template <int N>
 struct LwInt {
     static constexpr int value = N;
 };
-constexpr int kLwPolls = 1 << 22;   // bound of a wait for a copy (never reached)
+constexpr int kLwPolls = 1 << 20;   // bound of a wait for a copy (never reached)
 constexpr uint32_t kLwFull = 0x7fc00d1eu;   // weight of a distance whose gradient is in the buffer already (no result of arithmetic)
 
 // span[b] = (last vertex that the mask allows, whether one between the first and it is not allowed); vertex 0 is
@@ -705,7 +705,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
     bool stalled = false;
     for (; group < groups; group += step) {
         if (r0.nj > 0) {
-            stalled |= !umma::mbar_wait(mbar, phase, kLwPolls);
+            stalled |= !umma::mbar_wait(mbar, phase, stalled ? 1 : kLwPolls);
             phase ^= 1;
         }
         // the next row on its way, where the ring has room for it beside this one
@@ -890,7 +890,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     bool stalled = false;
     for (; group < groups; group += step) {
         if (r0.nj > 0) {
-            stalled |= !umma::mbar_wait(mbar, phase, kLwPolls);
+            stalled |= !umma::mbar_wait(mbar, phase, stalled ? 1 : kLwPolls);
             phase ^= 1;
         }
         __syncwarp();

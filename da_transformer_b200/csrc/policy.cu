@@ -22,6 +22,7 @@
 // in the ratio), sums over rows in 64 bits in a fixed order.  d is taken relative to its value at v = 0, so
 // that a constant between the two models' logits does not cancel.
 #include "dat_common.cuh"
+#include "umma.cuh"
 
 namespace dat {
 
@@ -50,7 +51,7 @@ struct PolicyArgs {
     float *loss;                  // [1]
     double *stats;                // [kPoSums]
     float *logp, *kl;             // [rows]
-    float4 *row_state;            // [rows]: M, 1 / S, c / N, E_p d (for the backward), or null
+    float4 *row_state;            // [rows][2]: r, 1 / S, c / N, E_p d; ry (for the backward), or null
     void *grad;                   // [rows, V] or null
     PolicyHead *head;
     int *done;                    // [chunks]
@@ -144,22 +145,46 @@ __device__ __forceinline__ float policy_offset(const T *x, const T *y) {
     return fabsf(o) < 1e30f ? o : 0.f;
 }
 
-// The gradient of one active row.  a = -c / (N S), w = beta / (N S), each times the loss's gradient; tok_c = c / N
-// times it, added at the token.
+// What the gradient of a row is made of: e (w (d - mean) + a) with e = exp(x - r), d = (x - r) - (y - ry),
+// a = -c / (N S), w = beta / (N S), each times the loss's gradient, and tok_c = c / N times it at the token.
+struct PolicyRow {
+    float r, ry, a, w, mean, tok_c;
+};
+template <bool kRef>
+__device__ __forceinline__ float policy_grad_one(const PolicyRow &p, float x, float y) {
+    const float dx = x - p.r, e = ex2(dx * kLog2e);
+    return e * (kRef ? fmaf(p.w, fmaxf(dx - (y - p.ry), kNegBig) - p.mean, p.a) : p.a);
+}
+
+// the same for several, in two-lane arithmetic (x is written over)
+template <bool kRef, int N>
+__device__ __forceinline__ void policy_grad_vec(const PolicyRow &p, float (&x)[N], const float (&y)[N]) {
+    const float base = kRef ? fmaf(-p.w, p.mean, p.a) : p.a;
+#pragma unroll
+    for (int i = 0; i < N; i += 2) {
+        float a0, a1, l0, l1, c0 = base, c1 = base;
+        fadd2_rn(a0, a1, x[i], x[i + 1], -p.r, -p.r);
+        fmul2_rn(l0, l1, a0, a1, kLog2e, kLog2e);
+        if (kRef) {
+            float b0, b1;
+            fadd2_rn(b0, b1, y[i], y[i + 1], -p.ry, -p.ry);
+            fadd2_rn(a0, a1, a0, a1, -b0, -b1);
+            ffma2_rn(c0, c1, fmaxf(a0, kNegBig), fmaxf(a1, kNegBig), p.w, p.w);
+        }
+        fmul2_rn(x[i], x[i + 1], ex2(l0), ex2(l1), c0, c1);
+    }
+}
+
+// The gradient of one active row.
 template <typename T, bool kRef>
-__device__ __forceinline__ void policy_grad_row(const T *x, const T *y, T *g, bool vec, int V, float M, float a, float w,
-                                                float mean_d, float off, int64_t tok, float tok_c) {
+__device__ __forceinline__ void policy_grad_row(const T *x, const T *y, T *g, bool vec, int V, const PolicyRow &p, int64_t tok) {
     constexpr int kVec = Elem<T>::kVec;
     const int tid = threadIdx.x;
     int head, nvec;
     policy_split(vec, x, V, head, nvec);
     const uint4 *xv = reinterpret_cast<const uint4 *>(x + head), *yv = reinterpret_cast<const uint4 *>(kRef ? y + head : x);
     uint4 *gv = reinterpret_cast<uint4 *>(g + head);
-    const float base = kRef ? fmaf(-w, mean_d, a) : a;
-    auto one = [&](float xe, float ye) {
-        const float e = ex2((xe - M) * kLog2e);
-        return e * (kRef ? fmaf(w, fmaxf((xe - off) - ye, kNegBig), base) : base);
-    };
+    auto one = [&](float xe, float ye) { return policy_grad_one<kRef>(p, xe, ye); };
     constexpr int U = 2;
     for (int v = tid; v < nvec; v += U * kPoThreads) {
         uint4 ux[U], uy[U];
@@ -186,7 +211,7 @@ __device__ __forceinline__ void policy_grad_row(const T *x, const T *y, T *g, bo
         g[e] = Elem<T>::from_float(one(Elem<T>::to_float(x[e]), kRef ? Elem<T>::to_float(y[e]) : 0.f));
     __syncthreads();
     if (tid == 0 && tok >= 0 && tok < V)
-        g[tok] = Elem<T>::from_float(tok_c + one(Elem<T>::to_float(x[tok]), kRef ? Elem<T>::to_float(y[tok]) : 0.f));
+        g[tok] = Elem<T>::from_float(p.tok_c + one(Elem<T>::to_float(x[tok]), kRef ? Elem<T>::to_float(y[tok]) : 0.f));
 }
 
 template <typename T>
@@ -264,7 +289,7 @@ __global__ void __launch_bounds__(kPoThreads)
 policy_fwd_kernel(PolicyArgs a) {
     constexpr int kVec = Elem<T>::kVec;
     __shared__ float red[5][kPoWarps];
-    __shared__ float row_s[4];   // coefficients of the row's gradient
+    __shared__ PolicyRow row_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x;
     const int V = a.V;
@@ -274,7 +299,7 @@ policy_fwd_kernel(PolicyArgs a) {
         if (tid == 0) {
             a.logp[row] = 0.f;
             a.kl[row] = 0.f;
-            if (a.row_state) a.row_state[row] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (a.row_state) a.row_state[2 * row] = a.row_state[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
         policy_sums(a, row);
         return;
@@ -371,15 +396,407 @@ policy_fwd_kernel(PolicyArgs a) {
         a.kl[row] = (float)kl;
         a.row_sums[row] = make_float4((float)term, (float)kl, (float)r, clipped ? 1.f : 0.f);
         const double inv_n = a.head->inv_n, up = inv_n * (double)a.head->scale;
-        if (a.row_state) a.row_state[row] = make_float4(M, (float)(1.0 / S), (float)(c * inv_n), (float)mean_d);
-        row_s[0] = (float)(-c * up / S);
-        row_s[1] = (float)((double)a.beta * up / S);
-        row_s[2] = (float)mean_d;
-        row_s[3] = (float)(c * up);
+        const float ry = M - off;
+        if (a.row_state) {
+            a.row_state[2 * row] = make_float4(M, (float)(1.0 / S), (float)(c * inv_n), (float)mean_d);
+            a.row_state[2 * row + 1] = make_float4(ry, 0.f, 0.f, 0.f);
+        }
+        row_s.r = M;
+        row_s.ry = ry;
+        row_s.a = (float)(-c * up / S);
+        row_s.w = (float)((double)a.beta * up / S);
+        row_s.mean = (float)mean_d;
+        row_s.tok_c = (float)(c * up);
     }
     __syncthreads();
-    if (g) policy_grad_row<T, kRef>(x, y, g, a.vec, V, M, row_s[0], row_s[1], row_s[2], off, tok, row_s[3]);
+    if (g) policy_grad_row<T, kRef>(x, y, g, a.vec, V, row_s, tok);
     policy_sums(a, row);
+}
+
+// ---------------------------------------------------------------------------------------------------
+// Rows of some KB and up that fit the shared memory: a persistent CTA keeps a row (and the reference's) in shared
+// memory between the sum and the gradient, so that HBM sees every logit once.  A producer warp brings the row in
+// chunks by bulk asynchronous copies: the chunk of the next row follows as soon as the gradient of this row's chunk
+// is written, and the next row's sum begins when its first chunk is there.  Another warp writes the zeros of the
+// inactive vertices' rows from a block of zeros by bulk copies.  16 bytes of a chunk belong to one consumer thread.
+// The sums are taken relative to the token's logits r = x[token], ry = y[token] in place of the maxima: they are at
+// least 1, and a row where one overflows (or the token's logit is no number) takes the maxima after all.  One
+// barrier per row; every thread puts the row's numbers together for itself.
+// Bound by the special-function unit next to HBM: three exponentials per logit pair with the full KL, 24 of its
+// cycles per 32 pairs and scheduler against 28 that HBM takes for the 6 bytes of each at 16 bits.
+// ---------------------------------------------------------------------------------------------------
+constexpr int kPpPolls = 1 << 20;      // bound of a wait (never reached)
+constexpr int kPpZeros = 4096;         // bytes of zeros
+constexpr int kPpVecs = 2;             // 16-byte pieces of a chunk that a consumer thread has
+constexpr float kPpHuge = 0x1p100f;
+
+struct PolicyRing {
+    int chunks;        // per row and array
+    int zeros, bars, red, x, y;   // places in the shared memory
+};
+
+// The rows of a CTA, blockIdx.x + k * gridDim.x, 32 at a time through the mask; next() gives those whose bit is set.
+struct PolicyWalk {
+    const unsigned char *mask;
+    int64_t rows;
+    int64_t base;        // row of the block's lane 0
+    unsigned bits, ahead;
+    bool inactive;       // walk the rows that take no part
+    __device__ __forceinline__ unsigned look(int64_t from) const {
+        const int64_t r = from + (int64_t)(threadIdx.x & 31) * gridDim.x;
+        return r < rows ? ((!mask || mask[r] != 0) != inactive ? 1u : 0u) : 0u;
+    }
+    __device__ __forceinline__ PolicyWalk(const unsigned char *m, int64_t n, bool skip) : mask(m), rows(n), inactive(skip) {
+        base = blockIdx.x;
+        bits = __ballot_sync(0xffffffffu, look(base));
+        ahead = look(base + 32 * (int64_t)gridDim.x);
+    }
+    __device__ __forceinline__ int64_t next() {
+        while (!bits) {
+            base += 32 * (int64_t)gridDim.x;
+            if (base >= rows) return -1;
+            bits = __ballot_sync(0xffffffffu, ahead);
+            ahead = look(base + 32 * (int64_t)gridDim.x);
+        }
+        const int j = __ffs(bits) - 1;
+        bits &= bits - 1;
+        return base + (int64_t)j * gridDim.x;
+    }
+};
+
+// A row in the ring: the 16-byte pieces that lie wholly inside it; the elements before and behind them are `head`
+// and `tail` (each fewer than a piece has).
+template <typename T>
+struct PolicySpan {
+    int head, vecs, tail;
+    __device__ __forceinline__ PolicySpan(int64_t row, int V) {
+        constexpr int kVec = Elem<T>::kVec;
+        head = (int)(-(row * V) & (kVec - 1));
+        if (head > V) head = V;
+        vecs = (V - head) / kVec;
+        tail = V - head - vecs * kVec;
+    }
+};
+
+__device__ __forceinline__ void policy_bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t mbar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src), "r"(bytes), "r"(mbar)
+                 : "memory");
+}
+__device__ __forceinline__ void policy_arrive(uint64_t *mbar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(mbar)) : "memory");
+}
+
+// sums of a thread's logits relative to (r, ry)
+template <bool kRef>
+struct PolicyAcc {
+    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f, y0 = 0.f, y1 = 0.f;
+    template <int N>
+    __device__ __forceinline__ void add(const float (&x)[N], const float (&y)[N], float r, float ry) {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) {
+            float a0, a1, l0, l1;
+            fadd2_rn(a0, a1, x[i], x[i + 1], -r, -r);
+            fmul2_rn(l0, l1, a0, a1, kLog2e, kLog2e);
+            const float e0 = ex2(l0), e1 = ex2(l1);
+            fadd2_rn(s0, s1, s0, s1, e0, e1);
+            if (kRef) {
+                float b0, b1, d0, d1;
+                fadd2_rn(b0, b1, y[i], y[i + 1], -ry, -ry);
+                fmul2_rn(l0, l1, b0, b1, kLog2e, kLog2e);
+                fadd2_rn(d0, d1, a0, a1, -b0, -b1);
+                // where p = 0 (a score of -inf) d may be -inf or NaN: a number, times 0
+                ffma2_rn(t0, t1, e0, e1, fmaxf(d0, kNegBig), fmaxf(d1, kNegBig));
+                fadd2_rn(y0, y1, y0, y1, ex2(l0), ex2(l1));
+            }
+        }
+    }
+    __device__ __forceinline__ void add1(float x, float y, float r, float ry) {
+        const float a = x - r, e = ex2(a * kLog2e);
+        s0 += e;
+        if (kRef) {
+            const float b = y - ry;
+            t0 = fmaf(e, fmaxf(a - b, kNegBig), t0);
+            y0 += ex2(b * kLog2e);
+        }
+    }
+};
+
+template <typename T, bool kRef, int NT>
+__global__ void __launch_bounds__(NT + 64, NT == 512 ? 1 : 3)
+policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
+    constexpr int kVec = Elem<T>::kVec, kWarps = NT / 32, kChunk = NT * kPpVecs;
+    extern __shared__ __align__(128) unsigned char posm[];
+    uint64_t *const full = reinterpret_cast<uint64_t *>(posm + ring.bars), *const empty = full + ring.chunks;
+    float4 *const red = reinterpret_cast<float4 *>(posm + ring.red);   // [2][kWarps]: S, T, Sy
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int V = a.V;
+    for (int x = tid; x < kPpZeros / 16; x += NT + 64) reinterpret_cast<uint4 *>(posm + ring.zeros)[x] = make_uint4(0, 0, 0, 0);
+    if (tid < ring.chunks) {
+        umma::mbar_init(full + tid, 1);
+        umma::mbar_init(empty + tid, kWarps);
+    }
+    umma::fence_smem_to_async();
+    __syncthreads();
+    bool stalled = false;
+
+    if (warp == kWarps) {   // ---- producer
+        PolicyWalk walk(a.mask, a.rows, false);
+        uint32_t phase = 1;   // the ring begins empty
+        for (int64_t row = walk.next(); row >= 0 && !stalled; row = walk.next(), phase ^= 1) {
+            const PolicySpan<T> sp(row, V);
+            const int64_t from = row * V + sp.head;
+            for (int c = 0; c < ring.chunks && !stalled; c++) {
+                const int bytes = min(kChunk, sp.vecs - c * kChunk) * 16;
+                if (lane == 0) {
+                    stalled |= !umma::mbar_wait(empty + c, phase, kPpPolls);
+                    if (!stalled) {
+                        const uint32_t mb = umma::smem_u32(full + c);
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mb),
+                                     "r"(bytes > 0 ? bytes * (kRef ? 2 : 1) : 0)
+                                     : "memory");
+                        if (bytes > 0) {
+                            const int64_t at = from + (int64_t)c * kChunk * kVec;
+                            policy_bulk_load(umma::smem_u32(posm + ring.x) + c * kChunk * 16, static_cast<const T *>(a.x) + at, bytes, mb);
+                            if (kRef)
+                                policy_bulk_load(umma::smem_u32(posm + ring.y) + c * kChunk * 16, static_cast<const T *>(a.y) + at, bytes, mb);
+                        }
+                    }
+                }
+                stalled = __any_sync(0xffffffffu, stalled);
+            }
+        }
+    } else if (warp == kWarps + 1) {   // ---- zeros
+        PolicyWalk walk(a.mask, a.rows, true);
+        const uint32_t zeros = umma::smem_u32(posm + ring.zeros);
+        for (int64_t row = a.mask ? walk.next() : -1; row >= 0; row = walk.next()) {
+            if (lane == 0) {
+                a.logp[row] = 0.f;
+                a.kl[row] = 0.f;
+                if (a.row_state) a.row_state[2 * row] = a.row_state[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            if (!a.grad) continue;
+            T *const g = static_cast<T *>(a.grad) + row * V;
+            const PolicySpan<T> sp(row, V);
+            const int bytes = sp.vecs * 16;
+            if (lane < sp.head) g[lane] = Elem<T>::from_float(0.f);
+            if (lane < sp.tail) g[V - sp.tail + lane] = Elem<T>::from_float(0.f);
+            unsigned char *const mid = reinterpret_cast<unsigned char *>(g + sp.head);
+            for (int at = lane * kPpZeros; at < bytes; at += 32 * kPpZeros)
+                asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(mid + at), "r"(zeros),
+                             "r"(min(kPpZeros, bytes - at))
+                             : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group.read 4;" ::: "memory");   // a few rows at a time, beside the active ones
+        }
+        asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    } else {   // ---- consumers
+        const uint4 *const xs = reinterpret_cast<const uint4 *>(posm + ring.x), *const ys = reinterpret_cast<const uint4 *>(posm + ring.y);
+        const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); };
+        const double inv_n = a.head->inv_n;
+        const float up = a.head->scale;
+        PolicyWalk walk(a.mask, a.rows, false);
+        // the next row's token and its logits are on their way while this row is worked on
+        int64_t row = walk.next(), row1 = row >= 0 ? walk.next() : -1;
+        const auto token = [&](int64_t r) { return r >= 0 ? a.tokens[r] : 0; };
+        const auto logit = [&](const void *p, int64_t r, int64_t t) {
+            return r >= 0 ? Elem<T>::to_float(static_cast<const T *>(p)[r * V + (t >= 0 && t < V ? t : 0)]) : 0.f;
+        };
+        int64_t tok = token(row), tok1 = token(row1);
+        float xt = logit(a.x, row, tok), yt = kRef ? logit(a.y, row, tok) : 0.f;
+        double sums[kPoSums] = {};   // of this CTA's rows, in their order (one thread's are used)
+        uint32_t phase = 0;
+        for (; row >= 0; phase ^= 1) {
+            const float xt1 = logit(a.x, row1, tok1), yt1 = kRef ? logit(a.y, row1, tok1) : 0.f;
+            const int64_t row2 = row1 >= 0 ? walk.next() : -1, tok2 = token(row2);
+            const int64_t b = row / a.L, l = row - b * a.L;
+            const float A = a.advantage[b * a.adv_b + l * a.adv_l], old = a.old_logp[row];
+            const float link = a.link_logp ? a.link_logp[row] : 0.f, ref = a.ref_logp ? a.ref_logp[row] : 0.f;
+            const PolicySpan<T> sp(row, V);
+            const T *const x = static_cast<const T *>(a.x) + row * V, *const y = kRef ? static_cast<const T *>(a.y) + row * V : nullptr;
+            // an element before or behind the pieces for the threads 0 .. head-1 and 8 .. 8+tail-1
+            const bool extra = tid < sp.head || (tid >= 8 && tid < 8 + sp.tail);
+            const int te = tid < 8 ? tid : V - sp.tail + tid - 8;
+            const float tx = extra ? Elem<T>::to_float(x[te]) : -INFINITY, ty = extra && kRef ? Elem<T>::to_float(y[te]) : -INFINITY;
+            const auto load = [&](int v, float (&fx)[kVec], float (&fy)[kVec]) {
+                Elem<T>::unpack(xs[v], fx);
+                if (kRef) Elem<T>::unpack(ys[v], fy);
+            };
+            float r = xt, ry = yt;
+            PolicyAcc<kRef> acc;
+            for (int c = 0; c < ring.chunks; c++) {
+                stalled |= !umma::mbar_wait(full + c, phase, stalled ? 1 : kPpPolls);
+                const int v = c * kChunk + tid;
+                if ((c + 1) * kChunk <= sp.vecs) {
+#pragma unroll
+                    for (int q = 0; q < kPpVecs; q++) {
+                        float fx[kVec], fy[kVec];
+                        load(v + q * NT, fx, fy);
+                        acc.add(fx, fy, r, ry);
+                    }
+                } else {
+                    for (int q = 0; q < kPpVecs; q++)
+                        if (v + q * NT < sp.vecs) {
+                            float fx[kVec], fy[kVec];
+                            load(v + q * NT, fx, fy);
+                            acc.add(fx, fy, r, ry);
+                        }
+                }
+            }
+            if (extra) acc.add1(tx, ty, r, ry);
+            float S, Tt, Sy;
+            const auto reduce = [&](float4 *slot) {
+                const float ws = warp_sum(acc.s0 + acc.s1);
+                const float wt = kRef ? warp_sum(acc.t0 + acc.t1) : 0.f, wy = kRef ? warp_sum(acc.y0 + acc.y1) : 0.f;
+                if (lane == 0) slot[warp] = make_float4(ws, wt, wy, 0.f);
+                sync();
+                float4 q = slot[lane & (kWarps - 1)];
+                if (lane >= kWarps) q = make_float4(0.f, 0.f, 0.f, 0.f);
+                S = warp_sum(q.x);
+                if (kRef) {
+                    Tt = warp_sum(q.y);
+                    Sy = warp_sum(q.z);
+                } else {
+                    Tt = 0.f;
+                    Sy = 1.f;
+                }
+            };
+            float4 *const slot = red + (phase ? kWarps : 0);
+            reduce(slot);
+            if (!(S < kPpHuge && fabsf(Tt) < kPpHuge && Sy < kPpHuge)) {   // the same in all threads
+                // the maxima in place of the token's logits
+                float m = -INFINITY, my = -INFINITY;
+                for (int v = tid; v < sp.vecs; v += NT) {
+                    float fx[kVec], fy[kVec];
+                    load(v, fx, fy);
+#pragma unroll
+                    for (int i = 0; i < kVec; i++) {
+                        m = fmaxf(m, fx[i]);
+                        if (kRef) my = fmaxf(my, fy[i]);
+                    }
+                }
+                if (extra) {
+                    m = fmaxf(m, tx);
+                    my = fmaxf(my, ty);
+                }
+                m = warp_max(m);
+                my = warp_max(my);
+                sync();   // the sums have been read
+                if (lane == 0) slot[warp] = make_float4(m, my, 0.f, 0.f);
+                sync();
+                float4 q = slot[lane & (kWarps - 1)];
+                r = warp_max(q.x);
+                ry = kRef ? warp_max(q.y) : 0.f;
+                acc = PolicyAcc<kRef>();
+                for (int v = tid; v < sp.vecs; v += NT) {
+                    float fx[kVec], fy[kVec];
+                    load(v, fx, fy);
+                    acc.add(fx, fy, r, ry);
+                }
+                if (extra) acc.add1(tx, ty, r, ry);
+                sync();
+                reduce(slot);
+            }
+            // the row's numbers: every thread the same
+            const bool ok = tok >= 0 && tok < V;
+            const float lp = ok ? ((xt - r) - logf(S)) + link : __int_as_float(0x7fc00000);
+            const float u = expf(lp - old);
+            const float lo = 1.f - a.clip_low, hi = 1.f + a.clip_high;
+            const float ra = u * A, rc = (u < lo ? lo : u > hi ? hi : u) * A;
+            const bool clipped = (A > 0.f && u > hi) || (A < 0.f && u < lo);
+            float cf = clipped ? 0.f : -ra, kl = 0.f, mean = 0.f;
+            if (kRef) {
+                mean = Tt / S;
+                kl = mean - logf(S / Sy);
+            } else if (a.ref_logp) {
+                const float z = ref - lp, em = expm1f(z);
+                kl = em - z;
+                cf = fmaf(-a.beta, em, cf);
+            }
+            const float n1 = (float)inv_n, inv_s = 1.f / S;
+            if (tid == 0) {
+                if (!ok && a.status) atomicOr(a.status, DAT_STATUS_BAD_INDEX);
+                const float term = -(ra < rc ? ra : rc);
+                a.logp[row] = lp;
+                a.kl[row] = kl;
+                sums[0] += (double)term;
+                sums[1] += (double)kl;
+                sums[2] += (double)u;
+                sums[3] += clipped ? 1.0 : 0.0;
+                sums[4] += 1.0;
+                if (a.row_state) {
+                    a.row_state[2 * row] = make_float4(r, inv_s, cf * n1, mean);
+                    a.row_state[2 * row + 1] = make_float4(ry, 0.f, 0.f, 0.f);
+                }
+            }
+            PolicyRow p;
+            p.r = r;
+            p.ry = ry;
+            p.tok_c = cf * n1 * up;
+            p.a = -p.tok_c * inv_s;
+            p.w = a.beta * n1 * up * inv_s;
+            p.mean = mean;
+            T *const g = a.grad ? static_cast<T *>(a.grad) + row * V : nullptr;
+            uint4 *const gv = reinterpret_cast<uint4 *>(g + sp.head);
+            const auto store = [&](int v) {
+                float fx[kVec], fy[kVec];
+                load(v, fx, fy);
+                policy_grad_vec<kRef>(p, fx, fy);
+                gv[v] = Elem<T>::pack(fx);
+            };
+            for (int c = 0; c < ring.chunks; c++) {
+                const int v = c * kChunk + tid;
+                if (g) {
+                    if ((c + 1) * kChunk <= sp.vecs) {
+#pragma unroll
+                        for (int q = 0; q < kPpVecs; q++) store(v + q * NT);
+                    } else {
+                        for (int q = 0; q < kPpVecs; q++)
+                            if (v + q * NT < sp.vecs) store(v + q * NT);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) policy_arrive(empty + c);
+            }
+            if (g) {
+                if (extra) g[te] = Elem<T>::from_float(policy_grad_one<kRef>(p, tx, ty));
+                // the token's place once more, by the thread that wrote it
+                const int at = (int)tok - sp.head, mine = at < 0 ? (int)tok : at >= sp.vecs * kVec ? (int)tok - (V - sp.tail) + 8 : at / kVec % NT;
+                if (ok && tid == mine) g[tok] = Elem<T>::from_float(policy_grad_one<kRef>(p, xt, yt) + p.tok_c);
+            }
+            row = row1;
+            row1 = row2;
+            tok = tok1;
+            tok1 = tok2;
+            xt = xt1;
+            yt = yt1;
+        }
+        if (stalled)   // copies that may still be on their way, within a bound again
+            for (int c = 0; c < ring.chunks; c++) umma::mbar_wait(full + c, phase, kPpPolls);
+        if (tid == 0)
+            for (int k = 0; k < kPoSums; k++) a.chunk_sums[(int64_t)blockIdx.x * kPoSums + k] = sums[k];
+    }
+    if (stalled && lane == 0 && a.status) atomicOr(a.status, DAT_STATUS_STALLED);
+    // the last CTA adds the CTAs' sums in their order
+    __shared__ int last_s;
+    __syncthreads();
+    if (tid == 0) {
+        __threadfence();
+        last_s = atomicAdd(&a.head->chunks_done, 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last_s || warp > 0) return;
+    __threadfence();
+    double total[2] = {};
+    for (int k = 0; k < kPoSums; k++) {
+        double t = 0.0;
+        for (int c = lane; c < (int)gridDim.x; c += 32) t += __ldcg(a.chunk_sums + (int64_t)c * kPoSums + k);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+        if (k < 2) total[k] = t;
+        if (lane == 0) a.stats[k] = t;
+    }
+    if (lane == 0) *a.loss = (float)((total[0] + (double)a.beta * total[1]) * a.head->inv_n);
 }
 
 struct PolicyBackwardArgs {
@@ -403,7 +820,7 @@ policy_bwd_kernel(PolicyBackwardArgs a) {
     const float up = *a.grad_loss;
     if (a.grad_link)
         for (int64_t r = (int64_t)blockIdx.x * kPoThreads + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * kPoThreads)
-            a.grad_link[r] = a.row_state[r].z * up;
+            a.grad_link[r] = a.row_state[2 * r].z * up;
     if (!a.grad || (a.written && up == a.head->scale)) return;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         T *g = static_cast<T *>(a.grad) + row * a.V;
@@ -412,13 +829,15 @@ policy_bwd_kernel(PolicyBackwardArgs a) {
             continue;
         }
         const T *x = static_cast<const T *>(a.x) + row * a.V, *y = kRef ? static_cast<const T *>(a.y) + row * a.V : nullptr;
-        const float4 st = a.row_state[row];
+        const float4 st = a.row_state[2 * row];
         const float c = st.z * up;
-        policy_grad_row<T, kRef>(x, y, g, a.vec, a.V, st.x, -c * st.y, (float)((double)a.beta * a.head->inv_n * up * st.y),
-                                 st.w, kRef ? policy_offset(x, y) : 0.f, a.tokens[row], c);
+        const PolicyRow p{st.x, a.row_state[2 * row + 1].x, -c * st.y, (float)((double)a.beta * a.head->inv_n * up * st.y),
+                          st.w, c};
+        policy_grad_row<T, kRef>(x, y, g, a.vec, a.V, p, a.tokens[row]);
     }
 }
 
+constexpr int kPoMaxCtas = 1024;   // persistent CTAs of a launch
 static int64_t policy_chunks(int64_t rows) { return (rows + kPoChunk - 1) / kPoChunk; }
 
 struct PolicyWorkspace {
@@ -428,7 +847,9 @@ struct PolicyWorkspace {
         done = up(sizeof(PolicyHead));
         sums = up(done + (size_t)policy_chunks(rows) * sizeof(int));
         chunk = up(sums + (size_t)rows * sizeof(float4));
-        total = up(chunk + (size_t)policy_chunks(rows) * kPoSums * sizeof(double));
+        // one line of sums per chunk of rows, or per persistent CTA (at most one per row)
+        const int64_t lines = rows < kPoMaxCtas ? rows : kPoMaxCtas;
+        total = up(chunk + (size_t)(policy_chunks(rows) > lines ? policy_chunks(rows) : lines) * kPoSums * sizeof(double));
     }
 };
 
@@ -436,8 +857,46 @@ static bool aligned16(const void *a, const void *b, const void *c) {
     return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
 }
 
+// The ring of a CTA with nt consumer threads: how many of them fit an SM (0: none).
+static int policy_ring(int nt, int V, int size, bool ref, const DeviceInfo &di, PolicyRing &ring, int &smem) {
+    const auto up = [](int n) { return (n + 127) / 128 * 128; };
+    const int64_t pieces = ((int64_t)V * size) / 16;   // 16-byte pieces inside a row
+    if (pieces < 1 || pieces > (1 << 16)) return 0;
+    ring.chunks = (int)((pieces + nt * kPpVecs - 1) / (nt * kPpVecs));
+    ring.zeros = 0;
+    ring.bars = kPpZeros;
+    ring.red = up(ring.bars + ring.chunks * 16);
+    ring.x = up(ring.red + 2 * (nt / 32) * 16);
+    ring.y = ring.x + up((int)pieces * 16);
+    smem = ref ? ring.y + up((int)pieces * 16) : ring.y;
+    if (ring.chunks > nt || smem > di.max_smem_optin - 256) return 0;
+    return (di.max_smem_optin + 1024) / (smem + 1024 + 256);
+}
+
+template <typename T, bool kRef, int NT>
+static int policy_ring_launch(const PolicyArgs &a, const PolicyRing &ring, int smem, int per_sm, const DeviceInfo &di,
+                              cudaStream_t st, const char *who) {
+    int64_t grid = (int64_t)di.sm_count * per_sm;
+    if (grid > a.rows) grid = a.rows;
+    if (grid > kPoMaxCtas) grid = kPoMaxCtas;
+    if (cudaFuncSetAttribute(policy_ring_kernel<T, kRef, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
+        policy_ring_kernel<T, kRef, NT><<<(unsigned)grid, NT + 64, smem, st>>>(a, ring);
+    return check_launch(who);
+}
+
 template <typename T>
-static int policy_fwd_t(const PolicyArgs &a, cudaStream_t st, const char *who) {
+static int policy_fwd_t(const PolicyArgs &a, const DeviceInfo &di, cudaStream_t st, const char *who) {
+    // Rows of 8 KB and up that fit: the ring, with 256 consumers per CTA where three CTAs fit an SM, else with 512.
+    if (a.vec && (int64_t)a.V * sizeof(T) >= 8192) {
+        PolicyRing ring;
+        int smem;
+        if (policy_ring(256, a.V, sizeof(T), a.y != nullptr, di, ring, smem) >= 3)
+            return a.y ? policy_ring_launch<T, true, 256>(a, ring, smem, 3, di, st, who)
+                       : policy_ring_launch<T, false, 256>(a, ring, smem, 3, di, st, who);
+        if (policy_ring(512, a.V, sizeof(T), a.y != nullptr, di, ring, smem) >= 1)
+            return a.y ? policy_ring_launch<T, true, 512>(a, ring, smem, 1, di, st, who)
+                       : policy_ring_launch<T, false, 512>(a, ring, smem, 1, di, st, who);
+    }
     if (a.y)
         policy_fwd_kernel<T, true><<<(unsigned)a.rows, kPoThreads, 0, st>>>(a);
     else
@@ -489,6 +948,8 @@ int dat_policy_loss(const void *word_ins_out, const void *ref_logits, int dtype,
         return check_launch(who);
     }
     DAT_REQUIRE(word_ins_out && tokens && old_logp && advantage && logp && kl, DAT_ERR_BAD_ARG, "%s: null pointer", who);
+    DeviceInfo di;
+    if (!device_info(&di)) return DAT_ERR_NO_DEVICE;
     const PolicyWorkspace lay(rows);
     unsigned char *ws = static_cast<unsigned char *>(workspace);
     PolicyArgs a{};
@@ -523,9 +984,9 @@ int dat_policy_loss(const void *word_ins_out, const void *ref_logits, int dtype,
     policy_prep_kernel<<<1, 1024, 0, st>>>(mask, rows, a.head, a.done, (int)policy_chunks(rows), grad_scale_ptr, grad_scale);
     if (int rc = check_launch(who)) return rc;
     switch (dtype) {
-        case DAT_F32: return policy_fwd_t<float>(a, st, who);
-        case DAT_F16: return policy_fwd_t<__half>(a, st, who);
-        default: return policy_fwd_t<__nv_bfloat16>(a, st, who);
+        case DAT_F32: return policy_fwd_t<float>(a, di, st, who);
+        case DAT_F16: return policy_fwd_t<__half>(a, di, st, who);
+        default: return policy_fwd_t<__nv_bfloat16>(a, di, st, who);
     }
 }
 

@@ -81,8 +81,8 @@ class DagPolicyLossFunc(Function):
             logp, kl = torch.empty_like(old_logp), torch.empty_like(old_logp)
             need_grad = need_logits or need_link
             grad = torch.empty_like(word_ins_out) if need_logits and grad_scale is not None else None
-            # the state of the rows (16 bytes each) for the backward, then the workspace
-            at = bsz * prelen * 16 if need_grad else 0
+            # the state of the rows (32 bytes each) for the backward, then the workspace
+            at = bsz * prelen * 32 if need_grad else 0
             ws = torch.empty(at + L.dat_policy_loss_workspace_bytes(bsz, prelen), dtype=torch.uint8, device=dev)
             check(L.dat_policy_loss(
                 word_ins_out.data_ptr(), address(ref_logits), dt, tokens.data_ptr(), old_logp.data_ptr(),
@@ -121,7 +121,7 @@ def _policy_backward(ctx, grad_loss):
         link = torch.empty(bsz, prelen, dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
         check(lib().dat_policy_loss_backward(
             word_ins_out.data_ptr(), address(ref_logits), _native.dtype_code(word_ins_out.dtype), tokens.data_ptr(),
-            address(mask), ctx.kl_coef, ws, ws + bsz * prelen * 16, grad_loss.data_ptr(), int(written),
+            address(mask), ctx.kl_coef, ws, ws + bsz * prelen * 32, grad_loss.data_ptr(), int(written),
             address(grad), address(link), bsz, prelen, vocab, stream_address(dev)), "policy_loss_backward")
     return grad, link, None
 

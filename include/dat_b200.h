@@ -389,7 +389,7 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
  * inactive vertex is read.  A token outside [0, vocab) makes its log-probability NaN and sets DAT_STATUS_BAD_INDEX.
  * Outputs: loss (one fp32), stats [5] fp64 = sums over the active vertices of term, kl and r, the number of clipped
  * and of active vertices; logp, kl [bsz,prelen] fp32 (0 where inactive).
- * For the backward: row_state [bsz*prelen,4] fp32, and grad_logits (optional, like word_ins_out): d loss /
+ * For the backward: row_state [bsz*prelen,8] fp32 (16-byte aligned), and grad_logits (optional, like word_ins_out): d loss /
  * d word_ins_out times *grad_scale_ptr (a device float) or, when that is NULL, times grad_scale, rounded once.
  * workspace: dat_policy_loss_workspace_bytes(...) bytes, 16-byte aligned; the backward reads it.
  */
