@@ -415,24 +415,42 @@ policy_fwd_kernel(PolicyArgs a) {
 
 // ---------------------------------------------------------------------------------------------------
 // Rows of some KB and up that fit the shared memory: a persistent CTA keeps a row (and the reference's) in shared
-// memory between the sum and the gradient, so that HBM sees every logit once.  A producer warp brings the row in
-// chunks by bulk asynchronous copies: the chunk of the next row follows as soon as the gradient of this row's chunk
-// is written, and the next row's sum begins when its first chunk is there.  Another warp writes the zeros of the
-// inactive vertices' rows from a block of zeros by bulk copies.  16 bytes of a chunk belong to one consumer thread.
+// memory between the sum and the gradient, so that HBM sees every logit once.  Its warps share the work as a
+// pipeline over rows: a producer brings chunks of rows by bulk asynchronous copies into a ring of slots, one half of
+// the others sums row n + 1 while the other half writes the gradient of row n and frees its slots, and one warp
+// writes the zeros of the inactive vertices' rows from a block of zeros by bulk copies.  (With all warps on one row
+// the SM waits for the row's last sum, its numbers and the first chunk of the next: 1.42 against ... ms.)
 // The sums are taken relative to the token's logits r = x[token], ry = y[token] in place of the maxima: they are at
 // least 1, and a row where one overflows (or the token's logit is no number) takes the maxima after all.  One
 // barrier per row; every thread puts the row's numbers together for itself.
-// Bound by the special-function unit next to HBM: three exponentials per logit pair with the full KL, 24 of its
-// cycles per 32 pairs and scheduler against 28 that HBM takes for the 6 bytes of each at 16 bits.
+// Next to HBM the special-function unit bounds it: three exponentials per logit pair with the full KL, 24 of its
+// cycles per 32 pairs and scheduler against 33 that HBM takes for the 6 bytes of each at 16 bits.
 // ---------------------------------------------------------------------------------------------------
 constexpr int kPpPolls = 1 << 20;      // bound of a wait (never reached)
 constexpr int kPpZeros = 4096;         // bytes of zeros
-constexpr int kPpVecs = 2;             // 16-byte pieces of a chunk that a consumer thread has
+constexpr int kPpVecs = 2;             // 16-byte pieces of a chunk that a thread of either half has
 constexpr float kPpHuge = 0x1p100f;
 
 struct PolicyRing {
-    int chunks;        // per row and array
+    int chunks, slots;            // chunks of a row (and array), slots of the ring: chunks <= slots <= 2 * chunks
     int zeros, bars, red, x, y;   // places in the shared memory
+};
+// what the summing half hands to the writing half
+struct PolicyHand {
+    PolicyRow row;
+    float xt, yt;   // the token's logits
+    int tok;        // -1: outside the vocabulary
+};
+// position of a row's chunk in the ring: slot and the parity of the phase in which it is full
+struct PolicyTurn {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ void next(int slots) {
+        if (++slot == slots) {
+            slot = 0;
+            phase ^= 1;
+        }
+    }
 };
 
 // The rows of a CTA, blockIdx.x + k * gridDim.x, 32 at a time through the mask; next() gives those whose bit is set.
@@ -522,51 +540,60 @@ struct PolicyAcc {
     }
 };
 
+// NT threads in each half, two warps beside them
 template <typename T, bool kRef, int NT>
-__global__ void __launch_bounds__(NT + 64, NT == 512 ? 1 : 3)
+__global__ void __launch_bounds__(2 * NT + 64, NT == 256 ? 1 : 3)
 policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
     constexpr int kVec = Elem<T>::kVec, kWarps = NT / 32, kChunk = NT * kPpVecs;
     extern __shared__ __align__(128) unsigned char posm[];
-    uint64_t *const full = reinterpret_cast<uint64_t *>(posm + ring.bars), *const empty = full + ring.chunks;
+    __shared__ PolicyHand hand_s[2];
+    __shared__ __align__(8) uint64_t hand_bar[2];
+    uint64_t *const full = reinterpret_cast<uint64_t *>(posm + ring.bars), *const empty = full + ring.slots;
     float4 *const red = reinterpret_cast<float4 *>(posm + ring.red);   // [2][kWarps]: S, T, Sy
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int V = a.V;
-    for (int x = tid; x < kPpZeros / 16; x += NT + 64) reinterpret_cast<uint4 *>(posm + ring.zeros)[x] = make_uint4(0, 0, 0, 0);
-    if (tid < ring.chunks) {
+    for (int x = tid; x < kPpZeros / 16; x += 2 * NT + 64) reinterpret_cast<uint4 *>(posm + ring.zeros)[x] = make_uint4(0, 0, 0, 0);
+    if (tid < ring.slots) {
         umma::mbar_init(full + tid, 1);
         umma::mbar_init(empty + tid, kWarps);
     }
+    if (tid < 2) umma::mbar_init(hand_bar + tid, 1);
     umma::fence_smem_to_async();
     __syncthreads();
     bool stalled = false;
+    const uint4 *const xs = reinterpret_cast<const uint4 *>(posm + ring.x), *const ys = reinterpret_cast<const uint4 *>(posm + ring.y);
+    const auto load = [&](int v, float (&fx)[kVec], float (&fy)[kVec]) {   // v: piece of the ring
+        Elem<T>::unpack(xs[v], fx);
+        if (kRef) Elem<T>::unpack(ys[v], fy);
+    };
+    PolicyTurn turn;
 
-    if (warp == kWarps) {   // ---- producer
+    if (warp == 2 * kWarps) {   // ---- producer
         PolicyWalk walk(a.mask, a.rows, false);
-        uint32_t phase = 1;   // the ring begins empty
-        for (int64_t row = walk.next(); row >= 0 && !stalled; row = walk.next(), phase ^= 1) {
+        for (int64_t row = walk.next(); row >= 0 && !stalled; row = walk.next()) {
             const PolicySpan<T> sp(row, V);
             const int64_t from = row * V + sp.head;
-            for (int c = 0; c < ring.chunks && !stalled; c++) {
+            for (int c = 0; c < ring.chunks && !stalled; c++, turn.next(ring.slots)) {
                 const int bytes = min(kChunk, sp.vecs - c * kChunk) * 16;
                 if (lane == 0) {
-                    stalled |= !umma::mbar_wait(empty + c, phase, kPpPolls);
+                    stalled |= !umma::mbar_wait(empty + turn.slot, turn.phase ^ 1, kPpPolls);   // the ring begins empty
                     if (!stalled) {
-                        const uint32_t mb = umma::smem_u32(full + c);
+                        const uint32_t mb = umma::smem_u32(full + turn.slot);
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mb),
                                      "r"(bytes > 0 ? bytes * (kRef ? 2 : 1) : 0)
                                      : "memory");
                         if (bytes > 0) {
                             const int64_t at = from + (int64_t)c * kChunk * kVec;
-                            policy_bulk_load(umma::smem_u32(posm + ring.x) + c * kChunk * 16, static_cast<const T *>(a.x) + at, bytes, mb);
-                            if (kRef)
-                                policy_bulk_load(umma::smem_u32(posm + ring.y) + c * kChunk * 16, static_cast<const T *>(a.y) + at, bytes, mb);
+                            const uint32_t to = turn.slot * (kChunk * 16);
+                            policy_bulk_load(umma::smem_u32(posm + ring.x) + to, static_cast<const T *>(a.x) + at, bytes, mb);
+                            if (kRef) policy_bulk_load(umma::smem_u32(posm + ring.y) + to, static_cast<const T *>(a.y) + at, bytes, mb);
                         }
                     }
                 }
                 stalled = __any_sync(0xffffffffu, stalled);
             }
         }
-    } else if (warp == kWarps + 1) {   // ---- zeros
+    } else if (warp == 2 * kWarps + 1) {   // ---- zeros
         PolicyWalk walk(a.mask, a.rows, true);
         const uint32_t zeros = umma::smem_u32(posm + ring.zeros);
         for (int64_t row = a.mask ? walk.next() : -1; row >= 0; row = walk.next()) {
@@ -590,11 +617,9 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             asm volatile("cp.async.bulk.wait_group.read 4;" ::: "memory");   // a few rows at a time, beside the active ones
         }
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-    } else {   // ---- consumers
-        const uint4 *const xs = reinterpret_cast<const uint4 *>(posm + ring.x), *const ys = reinterpret_cast<const uint4 *>(posm + ring.y);
+    } else if (warp < kWarps) {   // ---- the summing half
         const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); };
-        const double inv_n = a.head->inv_n;
-        const float up = a.head->scale;
+        const float n1 = (float)a.head->inv_n, up = a.head->scale;
         PolicyWalk walk(a.mask, a.rows, false);
         // the next row's token and its logits are on their way while this row is worked on
         int64_t row = walk.next(), row1 = row >= 0 ? walk.next() : -1;
@@ -605,8 +630,8 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
         int64_t tok = token(row), tok1 = token(row1);
         float xt = logit(a.x, row, tok), yt = kRef ? logit(a.y, row, tok) : 0.f;
         double sums[kPoSums] = {};   // of this CTA's rows, in their order (one thread's are used)
-        uint32_t phase = 0;
-        for (; row >= 0; phase ^= 1) {
+        int par = 0;
+        for (; row >= 0; par ^= 1) {
             const float xt1 = logit(a.x, row1, tok1), yt1 = kRef ? logit(a.y, row1, tok1) : 0.f;
             const int64_t row2 = row1 >= 0 ? walk.next() : -1, tok2 = token(row2);
             const int64_t b = row / a.L, l = row - b * a.L;
@@ -618,16 +643,13 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             const bool extra = tid < sp.head || (tid >= 8 && tid < 8 + sp.tail);
             const int te = tid < 8 ? tid : V - sp.tail + tid - 8;
             const float tx = extra ? Elem<T>::to_float(x[te]) : -INFINITY, ty = extra && kRef ? Elem<T>::to_float(y[te]) : -INFINITY;
-            const auto load = [&](int v, float (&fx)[kVec], float (&fy)[kVec]) {
-                Elem<T>::unpack(xs[v], fx);
-                if (kRef) Elem<T>::unpack(ys[v], fy);
-            };
+            const int first = turn.slot;
             float r = xt, ry = yt;
             PolicyAcc<kRef> acc;
-            for (int c = 0; c < ring.chunks; c++) {
-                stalled |= !umma::mbar_wait(full + c, phase, stalled ? 1 : kPpPolls);
-                const int v = c * kChunk + tid;
-                if ((c + 1) * kChunk <= sp.vecs) {
+            for (int c = 0; c < ring.chunks; c++, turn.next(ring.slots)) {
+                stalled |= !umma::mbar_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
+                const int v = turn.slot * kChunk + tid, left = sp.vecs - c * kChunk;
+                if (left >= kChunk) {
 #pragma unroll
                     for (int q = 0; q < kPpVecs; q++) {
                         float fx[kVec], fy[kVec];
@@ -636,7 +658,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                     }
                 } else {
                     for (int q = 0; q < kPpVecs; q++)
-                        if (v + q * NT < sp.vecs) {
+                        if (tid + q * NT < left) {
                             float fx[kVec], fy[kVec];
                             load(v + q * NT, fx, fy);
                             acc.add(fx, fy, r, ry);
@@ -661,20 +683,30 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                     Sy = 1.f;
                 }
             };
-            float4 *const slot = red + (phase ? kWarps : 0);
+            float4 *const slot = red + (par ? kWarps : 0);
             reduce(slot);
             if (!(S < kPpHuge && fabsf(Tt) < kPpHuge && Sy < kPpHuge)) {   // the same in all threads
-                // the maxima in place of the token's logits
+                // the maxima in place of the token's logits; the row's slots are not freed before its gradient
+                const auto again = [&](auto f) {
+                    int at = first;
+                    for (int c = 0; c < ring.chunks; c++) {
+                        for (int q = 0; q < kPpVecs; q++)
+                            if (c * kChunk + tid + q * NT < sp.vecs) {
+                                float fx[kVec], fy[kVec];
+                                load(at * kChunk + tid + q * NT, fx, fy);
+                                f(fx, fy);
+                            }
+                        if (++at == ring.slots) at = 0;
+                    }
+                };
                 float m = -INFINITY, my = -INFINITY;
-                for (int v = tid; v < sp.vecs; v += NT) {
-                    float fx[kVec], fy[kVec];
-                    load(v, fx, fy);
+                again([&](const float (&fx)[kVec], const float (&fy)[kVec]) {
 #pragma unroll
                     for (int i = 0; i < kVec; i++) {
                         m = fmaxf(m, fx[i]);
                         if (kRef) my = fmaxf(my, fy[i]);
                     }
-                }
+                });
                 if (extra) {
                     m = fmaxf(m, tx);
                     my = fmaxf(my, ty);
@@ -684,42 +716,48 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 sync();   // the sums have been read
                 if (lane == 0) slot[warp] = make_float4(m, my, 0.f, 0.f);
                 sync();
-                float4 q = slot[lane & (kWarps - 1)];
+                const float4 q = slot[lane & (kWarps - 1)];
                 r = warp_max(q.x);
                 ry = kRef ? warp_max(q.y) : 0.f;
                 acc = PolicyAcc<kRef>();
-                for (int v = tid; v < sp.vecs; v += NT) {
-                    float fx[kVec], fy[kVec];
-                    load(v, fx, fy);
-                    acc.add(fx, fy, r, ry);
-                }
+                again([&](const float (&fx)[kVec], const float (&fy)[kVec]) { acc.add(fx, fy, r, ry); });
                 if (extra) acc.add1(tx, ty, r, ry);
                 sync();
                 reduce(slot);
             }
-            // the row's numbers: every thread the same
-            const bool ok = tok >= 0 && tok < V;
-            const float lp = ok ? ((xt - r) - logf(S)) + link : __int_as_float(0x7fc00000);
-            const float u = expf(lp - old);
-            const float lo = 1.f - a.clip_low, hi = 1.f + a.clip_high;
-            const float ra = u * A, rc = (u < lo ? lo : u > hi ? hi : u) * A;
-            const bool clipped = (A > 0.f && u > hi) || (A < 0.f && u < lo);
-            float cf = clipped ? 0.f : -ra, kl = 0.f, mean = 0.f;
-            if (kRef) {
-                mean = Tt / S;
-                kl = mean - logf(S / Sy);
-            } else if (a.ref_logp) {
-                const float z = ref - lp, em = expm1f(z);
-                kl = em - z;
-                cf = fmaf(-a.beta, em, cf);
-            }
-            const float n1 = (float)inv_n, inv_s = 1.f / S;
+            // the row's numbers
             if (tid == 0) {
+                const bool ok = tok >= 0 && tok < V;
+                const float lp = ok ? ((xt - r) - logf(S)) + link : __int_as_float(0x7fc00000);
+                const float u = expf(lp - old);
+                const float lo = 1.f - a.clip_low, hi = 1.f + a.clip_high;
+                const float ra = u * A, rc = (u < lo ? lo : u > hi ? hi : u) * A;
+                const bool clipped = (A > 0.f && u > hi) || (A < 0.f && u < lo);
+                float cf = clipped ? 0.f : -ra, kl = 0.f, mean = 0.f;
+                if (kRef) {
+                    mean = Tt / S;
+                    kl = mean - logf(S / Sy);
+                } else if (a.ref_logp) {
+                    const float z = ref - lp, em = expm1f(z);
+                    kl = em - z;
+                    cf = fmaf(-a.beta, em, cf);
+                }
+                const float inv_s = 1.f / S;
+                PolicyHand &h = hand_s[par];
+                h.row.r = r;
+                h.row.ry = ry;
+                h.row.tok_c = cf * n1 * up;
+                h.row.a = -h.row.tok_c * inv_s;
+                h.row.w = a.beta * n1 * up * inv_s;
+                h.row.mean = mean;
+                h.xt = xt;
+                h.yt = yt;
+                h.tok = ok ? (int)tok : -1;
+                policy_arrive(hand_bar + par);
                 if (!ok && a.status) atomicOr(a.status, DAT_STATUS_BAD_INDEX);
-                const float term = -(ra < rc ? ra : rc);
                 a.logp[row] = lp;
                 a.kl[row] = kl;
-                sums[0] += (double)term;
+                sums[0] += (double)-(ra < rc ? ra : rc);
                 sums[1] += (double)kl;
                 sums[2] += (double)u;
                 sums[3] += clipped ? 1.0 : 0.0;
@@ -729,41 +767,6 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                     a.row_state[2 * row + 1] = make_float4(ry, 0.f, 0.f, 0.f);
                 }
             }
-            PolicyRow p;
-            p.r = r;
-            p.ry = ry;
-            p.tok_c = cf * n1 * up;
-            p.a = -p.tok_c * inv_s;
-            p.w = a.beta * n1 * up * inv_s;
-            p.mean = mean;
-            T *const g = a.grad ? static_cast<T *>(a.grad) + row * V : nullptr;
-            uint4 *const gv = reinterpret_cast<uint4 *>(g + sp.head);
-            const auto store = [&](int v) {
-                float fx[kVec], fy[kVec];
-                load(v, fx, fy);
-                policy_grad_vec<kRef>(p, fx, fy);
-                gv[v] = Elem<T>::pack(fx);
-            };
-            for (int c = 0; c < ring.chunks; c++) {
-                const int v = c * kChunk + tid;
-                if (g) {
-                    if ((c + 1) * kChunk <= sp.vecs) {
-#pragma unroll
-                        for (int q = 0; q < kPpVecs; q++) store(v + q * NT);
-                    } else {
-                        for (int q = 0; q < kPpVecs; q++)
-                            if (v + q * NT < sp.vecs) store(v + q * NT);
-                    }
-                }
-                __syncwarp();
-                if (lane == 0) policy_arrive(empty + c);
-            }
-            if (g) {
-                if (extra) g[te] = Elem<T>::from_float(policy_grad_one<kRef>(p, tx, ty));
-                // the token's place once more, by the thread that wrote it
-                const int at = (int)tok - sp.head, mine = at < 0 ? (int)tok : at >= sp.vecs * kVec ? (int)tok - (V - sp.tail) + 8 : at / kVec % NT;
-                if (ok && tid == mine) g[tok] = Elem<T>::from_float(policy_grad_one<kRef>(p, xt, yt) + p.tok_c);
-            }
             row = row1;
             row1 = row2;
             tok = tok1;
@@ -772,9 +775,56 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             yt = yt1;
         }
         if (stalled)   // copies that may still be on their way, within a bound again
-            for (int c = 0; c < ring.chunks; c++) umma::mbar_wait(full + c, phase, kPpPolls);
+            for (int c = 0; c < ring.slots; c++) umma::mbar_wait(full + c, turn.phase, kPpPolls);
         if (tid == 0)
             for (int k = 0; k < kPoSums; k++) a.chunk_sums[(int64_t)blockIdx.x * kPoSums + k] = sums[k];
+    } else {   // ---- the writing half
+        const int wt = tid - NT;
+        PolicyWalk walk(a.mask, a.rows, false);
+        uint32_t par = 0, hand_phase = 0;
+        for (int64_t row = walk.next(); row >= 0; row = walk.next()) {
+            stalled |= !umma::mbar_wait(hand_bar + par, hand_phase, stalled ? 1 : kPpPolls);
+            const PolicyHand h = hand_s[par];
+            par ^= 1;
+            hand_phase ^= par ^ 1;
+            const PolicyRow p = h.row;
+            const PolicySpan<T> sp(row, V);
+            T *const g = a.grad ? static_cast<T *>(a.grad) + row * V : nullptr;
+            uint4 *const gv = reinterpret_cast<uint4 *>(g + sp.head);
+            for (int c = 0; c < ring.chunks; c++, turn.next(ring.slots)) {
+                // full since the row was summed: the wait only makes the copy's bytes this thread's too
+                stalled |= !umma::mbar_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
+                const int v = turn.slot * kChunk + wt, to = c * kChunk + wt;
+                const auto store = [&](int q) {
+                    float fx[kVec], fy[kVec];
+                    load(v + q * NT, fx, fy);
+                    policy_grad_vec<kRef>(p, fx, fy);
+                    gv[to + q * NT] = Elem<T>::pack(fx);
+                };
+                if (g) {
+                    if ((c + 1) * kChunk <= sp.vecs) {
+#pragma unroll
+                        for (int q = 0; q < kPpVecs; q++) store(q);
+                    } else {
+                        for (int q = 0; q < kPpVecs; q++)
+                            if (to + q * NT < sp.vecs) store(q);
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) policy_arrive(empty + turn.slot);
+            }
+            if (g) {
+                if (wt < sp.head || (wt >= 8 && wt < 8 + sp.tail)) {
+                    const int te = wt < 8 ? wt : V - sp.tail + wt - 8;
+                    const float ty = kRef ? Elem<T>::to_float(static_cast<const T *>(a.y)[row * V + te]) : 0.f;
+                    g[te] = Elem<T>::from_float(policy_grad_one<kRef>(p, Elem<T>::to_float(static_cast<const T *>(a.x)[row * V + te]), ty));
+                }
+                // the token's place once more, by the thread that wrote it
+                const int at = h.tok - sp.head;
+                const int mine = at < 0 ? h.tok : at >= sp.vecs * kVec ? h.tok - (V - sp.tail) + 8 : at / kVec % NT;
+                if (h.tok >= 0 && wt == mine) g[h.tok] = Elem<T>::from_float(policy_grad_one<kRef>(p, h.xt, h.yt) + p.tok_c);
+            }
+        }
     }
     if (stalled && lane == 0 && a.status) atomicOr(a.status, DAT_STATUS_STALLED);
     // the last CTA adds the CTAs' sums in their order
@@ -857,20 +907,25 @@ static bool aligned16(const void *a, const void *b, const void *c) {
     return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
 }
 
-// The ring of a CTA with nt consumer threads: how many of them fit an SM (0: none).
-static int policy_ring(int nt, int V, int size, bool ref, const DeviceInfo &di, PolicyRing &ring, int &smem) {
+// The ring of a CTA with nt threads in each half, `per_sm` of them on an SM; false: a row does not fit.
+static bool policy_ring(int nt, int per_sm, int V, int size, bool ref, const DeviceInfo &di, PolicyRing &ring, int &smem) {
     const auto up = [](int n) { return (n + 127) / 128 * 128; };
-    const int64_t pieces = ((int64_t)V * size) / 16;   // 16-byte pieces inside a row
-    if (pieces < 1 || pieces > (1 << 16)) return 0;
-    ring.chunks = (int)((pieces + nt * kPpVecs - 1) / (nt * kPpVecs));
+    const int64_t pieces = (int64_t)V * size / 16;   // 16-byte pieces inside a row
+    const int chunk = nt * kPpVecs, slot = chunk * 16 * (ref ? 2 : 1);
+    if (pieces < 1 || pieces > (1 << 16)) return false;
+    ring.chunks = (int)((pieces + chunk - 1) / chunk);
+    const int avail = (di.max_smem_optin + 1024) / per_sm - 1024 - 512;   // what the kernel declares itself is below 512
+    const int fixed = up(kPpZeros + 4 * ring.chunks * 8) + up(2 * (nt / 32) * 16);
+    ring.slots = (avail - fixed) / slot;
+    if (ring.slots > 2 * ring.chunks) ring.slots = 2 * ring.chunks;
+    if (ring.slots < ring.chunks || ring.slots > 2 * nt) return false;
     ring.zeros = 0;
     ring.bars = kPpZeros;
-    ring.red = up(ring.bars + ring.chunks * 16);
+    ring.red = up(ring.bars + 2 * ring.slots * 8);
     ring.x = up(ring.red + 2 * (nt / 32) * 16);
-    ring.y = ring.x + up((int)pieces * 16);
-    smem = ref ? ring.y + up((int)pieces * 16) : ring.y;
-    if (ring.chunks > nt || smem > di.max_smem_optin - 256) return 0;
-    return (di.max_smem_optin + 1024) / (smem + 1024 + 256);
+    ring.y = ring.x + ring.slots * chunk * 16;
+    smem = ref ? ring.y + ring.slots * chunk * 16 : ring.y;
+    return true;
 }
 
 template <typename T, bool kRef, int NT>
@@ -880,22 +935,23 @@ static int policy_ring_launch(const PolicyArgs &a, const PolicyRing &ring, int s
     if (grid > a.rows) grid = a.rows;
     if (grid > kPoMaxCtas) grid = kPoMaxCtas;
     if (cudaFuncSetAttribute(policy_ring_kernel<T, kRef, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
-        policy_ring_kernel<T, kRef, NT><<<(unsigned)grid, NT + 64, smem, st>>>(a, ring);
+        policy_ring_kernel<T, kRef, NT><<<(unsigned)grid, 2 * NT + 64, smem, st>>>(a, ring);
     return check_launch(who);
 }
 
 template <typename T>
 static int policy_fwd_t(const PolicyArgs &a, const DeviceInfo &di, cudaStream_t st, const char *who) {
-    // Rows of 8 KB and up that fit: the ring, with 256 consumers per CTA where three CTAs fit an SM, else with 512.
+    // Rows of 8 KB and up that fit: the ring, with 128 threads in each half where three CTAs fit an SM, else with 256.
     if (a.vec && (int64_t)a.V * sizeof(T) >= 8192) {
         PolicyRing ring;
         int smem;
-        if (policy_ring(256, a.V, sizeof(T), a.y != nullptr, di, ring, smem) >= 3)
-            return a.y ? policy_ring_launch<T, true, 256>(a, ring, smem, 3, di, st, who)
-                       : policy_ring_launch<T, false, 256>(a, ring, smem, 3, di, st, who);
-        if (policy_ring(512, a.V, sizeof(T), a.y != nullptr, di, ring, smem) >= 1)
-            return a.y ? policy_ring_launch<T, true, 512>(a, ring, smem, 1, di, st, who)
-                       : policy_ring_launch<T, false, 512>(a, ring, smem, 1, di, st, who);
+        const bool ref = a.y != nullptr;
+        if (policy_ring(128, 3, a.V, sizeof(T), ref, di, ring, smem))
+            return ref ? policy_ring_launch<T, true, 128>(a, ring, smem, 3, di, st, who)
+                       : policy_ring_launch<T, false, 128>(a, ring, smem, 3, di, st, who);
+        if (policy_ring(256, 1, a.V, sizeof(T), ref, di, ring, smem))
+            return ref ? policy_ring_launch<T, true, 256>(a, ring, smem, 1, di, st, who)
+                       : policy_ring_launch<T, false, 256>(a, ring, smem, 1, di, st, who);
     }
     if (a.y)
         policy_fwd_kernel<T, true><<<(unsigned)a.rows, kPoThreads, 0, st>>>(a);
