@@ -156,25 +156,6 @@ __device__ __forceinline__ float policy_grad_one(const PolicyRow &p, float x, fl
     return e * (kRef ? fmaf(p.w, fmaxf(dx - (y - p.ry), kNegBig) - p.mean, p.a) : p.a);
 }
 
-// the same for several, in two-lane arithmetic (x is written over)
-template <bool kRef, int N>
-__device__ __forceinline__ void policy_grad_vec(const PolicyRow &p, float (&x)[N], const float (&y)[N]) {
-    const float base = kRef ? fmaf(-p.w, p.mean, p.a) : p.a;
-#pragma unroll
-    for (int i = 0; i < N; i += 2) {
-        float a0, a1, l0, l1, c0 = base, c1 = base;
-        fadd2_rn(a0, a1, x[i], x[i + 1], -p.r, -p.r);
-        fmul2_rn(l0, l1, a0, a1, kLog2e, kLog2e);
-        if (kRef) {
-            float b0, b1;
-            fadd2_rn(b0, b1, y[i], y[i + 1], -p.ry, -p.ry);
-            fadd2_rn(a0, a1, a0, a1, -b0, -b1);
-            ffma2_rn(c0, c1, fmaxf(a0, kNegBig), fmaxf(a1, kNegBig), p.w, p.w);
-        }
-        fmul2_rn(x[i], x[i + 1], ex2(l0), ex2(l1), c0, c1);
-    }
-}
-
 // The gradient of one active row.
 template <typename T, bool kRef>
 __device__ __forceinline__ void policy_grad_row(const T *x, const T *y, T *g, bool vec, int V, const PolicyRow &p, int64_t tok) {
@@ -426,7 +407,7 @@ policy_fwd_kernel(PolicyArgs a) {
 // Next to HBM the special-function unit bounds it: three exponentials per logit pair with the full KL, 24 of its
 // cycles per 32 pairs and scheduler against 33 that HBM takes for the 6 bytes of each at 16 bits.
 // ---------------------------------------------------------------------------------------------------
-constexpr int kPpPolls = 1 << 20;      // bound of a wait (never reached)
+constexpr int kPpPolls = 1 << 14;      // bound of a wait (never reached)
 constexpr int kPpZeros = 4096;         // bytes of zeros
 constexpr int kPpVecs = 2;             // 16-byte pieces of a chunk that a thread of either half has
 constexpr float kPpHuge = 0x1p100f;
@@ -440,6 +421,11 @@ struct PolicyHand {
     PolicyRow row;
     float xt, yt;   // the token's logits
     int tok;        // -1: outside the vocabulary
+    bool careful;   // the row has logits of -inf
+};
+template <bool B>
+struct PolicyBool {
+    static constexpr bool value = B;
 };
 // position of a row's chunk in the ring: slot and the parity of the phase in which it is full
 struct PolicyTurn {
@@ -452,6 +438,56 @@ struct PolicyTurn {
         }
     }
 };
+
+// A pair of fp32 numbers in one 64-bit register, so that the two-lane instructions need no moves between them.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_get(F2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 f2_ex2(F2 v) {
+    float a, b;
+    f2_get(v, a, b);
+    return f2(ex2(a), ex2(b));
+}
+__device__ __forceinline__ F2 f2_floor(F2 v) {   // what is below -1e30, or NaN, becomes -1e30
+    float a, b;
+    f2_get(v, a, b);
+    return f2(fmaxf(a, kNegBig), fmaxf(b, kNegBig));
+}
+
+// Waits for a phase of a barrier; the hardware suspends the warp for up to the hint (in ns) per poll, so that waiting
+// warps take no issue slots (polling without it took a quarter of them).  false: gave up.
+__device__ __forceinline__ bool policy_wait(uint64_t *mbar, uint32_t parity, int polls) {
+    const uint32_t a = umma::smem_u32(mbar);
+    for (int i = 0; i < polls; i++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(a), "r"(parity), "r"(1000000)
+            : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
 
 // The rows of a CTA, blockIdx.x + k * gridDim.x, 32 at a time through the mask; next() gives those whose bit is set.
 struct PolicyWalk {
@@ -505,40 +541,80 @@ __device__ __forceinline__ void policy_arrive(uint64_t *mbar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(umma::smem_u32(mbar)) : "memory");
 }
 
-// sums of a thread's logits relative to (r, ry)
+// Sums of a thread's logits relative to (r, ry).  kCareful: a logit of -inf in x makes d = (x-r) - (y-ry) -inf or NaN
+// where p is 0; it is made a number there.  Without, such a row shows as a sum that is NaN.
 template <bool kRef>
 struct PolicyAcc {
-    float s0 = 0.f, s1 = 0.f, t0 = 0.f, t1 = 0.f, y0 = 0.f, y1 = 0.f;
-    template <int N>
-    __device__ __forceinline__ void add(const float (&x)[N], const float (&y)[N], float r, float ry) {
+    F2 s = 0, t = 0, sy = 0;   // (0, 0)
+    template <bool kCareful, int N>
+    __device__ __forceinline__ void add(const F2 (&x)[N], const F2 (&y)[N], F2 minus_r, F2 minus_ry) {
+        const F2 l2e = f2(kLog2e, kLog2e), neg = f2(-1.f, -1.f);
 #pragma unroll
-        for (int i = 0; i < N; i += 2) {
-            float a0, a1, l0, l1;
-            fadd2_rn(a0, a1, x[i], x[i + 1], -r, -r);
-            fmul2_rn(l0, l1, a0, a1, kLog2e, kLog2e);
-            const float e0 = ex2(l0), e1 = ex2(l1);
-            fadd2_rn(s0, s1, s0, s1, e0, e1);
+        for (int i = 0; i < N; i++) {
+            const F2 a = f2_add(x[i], minus_r), e = f2_ex2(f2_mul(a, l2e));
+            s = f2_add(s, e);
             if (kRef) {
-                float b0, b1, d0, d1;
-                fadd2_rn(b0, b1, y[i], y[i + 1], -ry, -ry);
-                fmul2_rn(l0, l1, b0, b1, kLog2e, kLog2e);
-                fadd2_rn(d0, d1, a0, a1, -b0, -b1);
-                // where p = 0 (a score of -inf) d may be -inf or NaN: a number, times 0
-                ffma2_rn(t0, t1, e0, e1, fmaxf(d0, kNegBig), fmaxf(d1, kNegBig));
-                fadd2_rn(y0, y1, y0, y1, ex2(l0), ex2(l1));
+                const F2 b = f2_add(y[i], minus_ry);
+                F2 d = f2_fma(b, neg, a);
+                if (kCareful) d = f2_floor(d);
+                t = f2_fma(e, d, t);
+                sy = f2_add(sy, f2_ex2(f2_mul(b, l2e)));
             }
         }
     }
     __device__ __forceinline__ void add1(float x, float y, float r, float ry) {
         const float a = x - r, e = ex2(a * kLog2e);
-        s0 += e;
+        s = f2_add(s, f2(e, 0.f));
         if (kRef) {
             const float b = y - ry;
-            t0 = fmaf(e, fmaxf(a - b, kNegBig), t0);
-            y0 += ex2(b * kLog2e);
+            t = f2_add(t, f2(e * fmaxf(a - b, kNegBig), 0.f));
+            sy = f2_add(sy, f2(ex2(b * kLog2e), 0.f));
         }
     }
+    static __device__ __forceinline__ float both(F2 v) {
+        float a, b;
+        f2_get(v, a, b);
+        return a + b;
+    }
 };
+
+// 16 bytes of logits as pairs
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[2], const float *) {
+    p[0] = f2(__uint_as_float(u.x), __uint_as_float(u.y));
+    p[1] = f2(__uint_as_float(u.z), __uint_as_float(u.w));
+}
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], const __nv_bfloat16 *) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = f2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+}
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], const __half *) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        p[i] = f2(v.x, v.y);
+    }
+}
+
+// the gradient of pairs of logits
+template <bool kRef, bool kCareful, int N>
+__device__ __forceinline__ void policy_grad_pairs(const PolicyRow &p, const F2 (&x)[N], const F2 (&y)[N], float (&out)[2 * N]) {
+    const float base = kRef ? fmaf(-p.w, p.mean, p.a) : p.a;
+    const F2 l2e = f2(kLog2e, kLog2e), neg = f2(-1.f, -1.f), mr = f2(-p.r, -p.r), mry = f2(-p.ry, -p.ry), w = f2(p.w, p.w),
+             bb = f2(base, base);
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const F2 a = f2_add(x[i], mr), e = f2_ex2(f2_mul(a, l2e));
+        F2 k = bb;
+        if (kRef) {
+            F2 d = f2_fma(f2_add(y[i], mry), neg, a);
+            if (kCareful) d = f2_floor(d);
+            k = f2_fma(d, w, bb);
+        }
+        f2_get(f2_mul(e, k), out[2 * i], out[2 * i + 1]);
+    }
+}
 
 // NT threads in each half, two warps beside them
 template <typename T, bool kRef, int NT>
@@ -562,9 +638,9 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
     __syncthreads();
     bool stalled = false;
     const uint4 *const xs = reinterpret_cast<const uint4 *>(posm + ring.x), *const ys = reinterpret_cast<const uint4 *>(posm + ring.y);
-    const auto load = [&](int v, float (&fx)[kVec], float (&fy)[kVec]) {   // v: piece of the ring
-        Elem<T>::unpack(xs[v], fx);
-        if (kRef) Elem<T>::unpack(ys[v], fy);
+    const auto load = [&](int v, F2 (&px)[kVec / 2], F2 (&py)[kVec / 2]) {   // v: piece of the ring
+        policy_pairs(xs[v], px, static_cast<const T *>(nullptr));
+        if (kRef) policy_pairs(ys[v], py, static_cast<const T *>(nullptr));
     };
     PolicyTurn turn;
 
@@ -576,7 +652,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             for (int c = 0; c < ring.chunks && !stalled; c++, turn.next(ring.slots)) {
                 const int bytes = min(kChunk, sp.vecs - c * kChunk) * 16;
                 if (lane == 0) {
-                    stalled |= !umma::mbar_wait(empty + turn.slot, turn.phase ^ 1, kPpPolls);   // the ring begins empty
+                    stalled |= !policy_wait(empty + turn.slot, turn.phase ^ 1, kPpPolls);   // the ring begins empty
                     if (!stalled) {
                         const uint32_t mb = umma::smem_u32(full + turn.slot);
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mb),
@@ -631,6 +707,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
         float xt = logit(a.x, row, tok), yt = kRef ? logit(a.y, row, tok) : 0.f;
         double sums[kPoSums] = {};   // of this CTA's rows, in their order (one thread's are used)
         int par = 0;
+        bool careful = false;
         for (; row >= 0; par ^= 1) {
             const float xt1 = logit(a.x, row1, tok1), yt1 = kRef ? logit(a.y, row1, tok1) : 0.f;
             const int64_t row2 = row1 >= 0 ? walk.next() : -1, tok2 = token(row2);
@@ -645,31 +722,35 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             const float tx = extra ? Elem<T>::to_float(x[te]) : -INFINITY, ty = extra && kRef ? Elem<T>::to_float(y[te]) : -INFINITY;
             const int first = turn.slot;
             float r = xt, ry = yt;
+            F2 mr = f2(-r, -r), mry = f2(-ry, -ry);
             PolicyAcc<kRef> acc;
-            for (int c = 0; c < ring.chunks; c++, turn.next(ring.slots)) {
-                stalled |= !umma::mbar_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
-                const int v = turn.slot * kChunk + tid, left = sp.vecs - c * kChunk;
-                if (left >= kChunk) {
+            const auto sum = [&](auto care) {
+                for (int c = 0; c < ring.chunks; c++, turn.next(ring.slots)) {
+                    stalled |= !policy_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
+                    const int v = turn.slot * kChunk + tid, left = sp.vecs - c * kChunk;
+                    if (left >= kChunk) {
+                        F2 px[kPpVecs][kVec / 2], py[kPpVecs][kVec / 2];
 #pragma unroll
-                    for (int q = 0; q < kPpVecs; q++) {
-                        float fx[kVec], fy[kVec];
-                        load(v + q * NT, fx, fy);
-                        acc.add(fx, fy, r, ry);
+                        for (int q = 0; q < kPpVecs; q++) load(v + q * NT, px[q], py[q]);
+#pragma unroll
+                        for (int q = 0; q < kPpVecs; q++) acc.template add<decltype(care)::value>(px[q], py[q], mr, mry);
+                    } else {
+                        for (int q = 0; q < kPpVecs; q++)
+                            if (tid + q * NT < left) {
+                                F2 px[kVec / 2], py[kVec / 2];
+                                load(v + q * NT, px, py);
+                                acc.template add<decltype(care)::value>(px, py, mr, mry);
+                            }
                     }
-                } else {
-                    for (int q = 0; q < kPpVecs; q++)
-                        if (tid + q * NT < left) {
-                            float fx[kVec], fy[kVec];
-                            load(v + q * NT, fx, fy);
-                            acc.add(fx, fy, r, ry);
-                        }
                 }
-            }
+            };
+            if (careful) sum(PolicyBool<true>());
+            else sum(PolicyBool<false>());
             if (extra) acc.add1(tx, ty, r, ry);
             float S, Tt, Sy;
             const auto reduce = [&](float4 *slot) {
-                const float ws = warp_sum(acc.s0 + acc.s1);
-                const float wt = kRef ? warp_sum(acc.t0 + acc.t1) : 0.f, wy = kRef ? warp_sum(acc.y0 + acc.y1) : 0.f;
+                const float ws = warp_sum(acc.both(acc.s));
+                const float wt = kRef ? warp_sum(acc.both(acc.t)) : 0.f, wy = kRef ? warp_sum(acc.both(acc.sy)) : 0.f;
                 if (lane == 0) slot[warp] = make_float4(ws, wt, wy, 0.f);
                 sync();
                 float4 q = slot[lane & (kWarps - 1)];
@@ -687,24 +768,30 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             reduce(slot);
             if (!(S < kPpHuge && fabsf(Tt) < kPpHuge && Sy < kPpHuge)) {   // the same in all threads
                 // the maxima in place of the token's logits; the row's slots are not freed before its gradient
+                careful = kRef;   // and from here on: rows of one batch share their forbidden tokens
                 const auto again = [&](auto f) {
                     int at = first;
                     for (int c = 0; c < ring.chunks; c++) {
                         for (int q = 0; q < kPpVecs; q++)
                             if (c * kChunk + tid + q * NT < sp.vecs) {
-                                float fx[kVec], fy[kVec];
-                                load(at * kChunk + tid + q * NT, fx, fy);
-                                f(fx, fy);
+                                F2 px[kVec / 2], py[kVec / 2];
+                                load(at * kChunk + tid + q * NT, px, py);
+                                f(px, py);
                             }
                         if (++at == ring.slots) at = 0;
                     }
                 };
                 float m = -INFINITY, my = -INFINITY;
-                again([&](const float (&fx)[kVec], const float (&fy)[kVec]) {
+                again([&](const F2 (&px)[kVec / 2], const F2 (&py)[kVec / 2]) {
 #pragma unroll
-                    for (int i = 0; i < kVec; i++) {
-                        m = fmaxf(m, fx[i]);
-                        if (kRef) my = fmaxf(my, fy[i]);
+                    for (int i = 0; i < kVec / 2; i++) {
+                        float u, w;
+                        f2_get(px[i], u, w);
+                        m = fmaxf(m, fmaxf(u, w));
+                        if (kRef) {
+                            f2_get(py[i], u, w);
+                            my = fmaxf(my, fmaxf(u, w));
+                        }
                     }
                 });
                 if (extra) {
@@ -719,8 +806,10 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 const float4 q = slot[lane & (kWarps - 1)];
                 r = warp_max(q.x);
                 ry = kRef ? warp_max(q.y) : 0.f;
+                mr = f2(-r, -r);
+                mry = f2(-ry, -ry);
                 acc = PolicyAcc<kRef>();
-                again([&](const float (&fx)[kVec], const float (&fy)[kVec]) { acc.add(fx, fy, r, ry); });
+                again([&](const F2 (&px)[kVec / 2], const F2 (&py)[kVec / 2]) { acc.template add<kRef>(px, py, mr, mry); });
                 if (extra) acc.add1(tx, ty, r, ry);
                 sync();
                 reduce(slot);
@@ -753,6 +842,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 h.xt = xt;
                 h.yt = yt;
                 h.tok = ok ? (int)tok : -1;
+                h.careful = careful;
                 policy_arrive(hand_bar + par);
                 if (!ok && a.status) atomicOr(a.status, DAT_STATUS_BAD_INDEX);
                 a.logp[row] = lp;
@@ -775,7 +865,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             yt = yt1;
         }
         if (stalled)   // copies that may still be on their way, within a bound again
-            for (int c = 0; c < ring.slots; c++) umma::mbar_wait(full + c, turn.phase, kPpPolls);
+            for (int c = 0; c < ring.slots; c++) policy_wait(full + c, turn.phase, kPpPolls);
         if (tid == 0)
             for (int k = 0; k < kPoSums; k++) a.chunk_sums[(int64_t)blockIdx.x * kPoSums + k] = sums[k];
     } else {   // ---- the writing half
@@ -783,7 +873,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
         PolicyWalk walk(a.mask, a.rows, false);
         uint32_t par = 0, hand_phase = 0;
         for (int64_t row = walk.next(); row >= 0; row = walk.next()) {
-            stalled |= !umma::mbar_wait(hand_bar + par, hand_phase, stalled ? 1 : kPpPolls);
+            stalled |= !policy_wait(hand_bar + par, hand_phase, stalled ? 1 : kPpPolls);
             const PolicyHand h = hand_s[par];
             par ^= 1;
             hand_phase ^= par ^ 1;
@@ -793,21 +883,22 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             uint4 *const gv = reinterpret_cast<uint4 *>(g + sp.head);
             for (int c = 0; c < ring.chunks; c++, turn.next(ring.slots)) {
                 // full since the row was summed: the wait only makes the copy's bytes this thread's too
-                stalled |= !umma::mbar_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
+                stalled |= !policy_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
                 const int v = turn.slot * kChunk + wt, to = c * kChunk + wt;
-                const auto store = [&](int q) {
-                    float fx[kVec], fy[kVec];
-                    load(v + q * NT, fx, fy);
-                    policy_grad_vec<kRef>(p, fx, fy);
-                    gv[to + q * NT] = Elem<T>::pack(fx);
+                const auto store = [&](auto care, int q) {
+                    F2 px[kVec / 2], py[kVec / 2];
+                    float out[kVec];
+                    load(v + q * NT, px, py);
+                    policy_grad_pairs<kRef, decltype(care)::value>(p, px, py, out);
+                    gv[to + q * NT] = Elem<T>::pack(out);
                 };
                 if (g) {
-                    if ((c + 1) * kChunk <= sp.vecs) {
+                    if ((c + 1) * kChunk <= sp.vecs && !h.careful) {
 #pragma unroll
-                        for (int q = 0; q < kPpVecs; q++) store(q);
+                        for (int q = 0; q < kPpVecs; q++) store(PolicyBool<false>(), q);
                     } else {
                         for (int q = 0; q < kPpVecs; q++)
-                            if (to + q * NT < sp.vecs) store(q);
+                            if (to + q * NT < sp.vecs) store(PolicyBool<kRef>(), q);
                     }
                 }
                 __syncwarp();
