@@ -465,8 +465,11 @@ lw_span_kernel(const unsigned char *__restrict__ nonpad, int2 *__restrict__ span
 // first changes from sentence to sentence: a warp's stride may be even).
 struct LwRow {
     int64_t row;   // b * L + i
-    int i, nj;     // vertex, successors up to the last one that the masks allow
+    int i, nj;     // vertex, successors up to the last one that the masks allow (after lw_resolve)
     bool exists, holes;
+    // as they lie in memory: looked at a row later, when they have arrived
+    int2 sp;
+    int64_t bound;
 };
 struct LwWalk {
     int per, step_b, step_q, b, q;
@@ -486,8 +489,8 @@ struct LwWalk {
         }
     }
 };
-__device__ __forceinline__ LwRow lw_row(LwWalk &walk, int B, int L, int K, const LinksMask &mk, const int2 *span) {
-    LwRow r{0, 0, 0, false, false};
+__device__ __forceinline__ LwRow lw_row(LwWalk &walk, int B, int L, const LinksMask &mk, const int2 *span) {
+    LwRow r{0, 0, 0, false, false, {0, 0}, 0};
     const int per = walk.per, b = walk.b, q = walk.q;
     if (b >= B) return r;
     walk.next();
@@ -495,14 +498,19 @@ __device__ __forceinline__ LwRow lw_row(LwWalk &walk, int B, int L, int K, const
     if (r.i >= L) return r;
     r.exists = true;
     r.row = (int64_t)b * L + r.i;
-    int jhi = links_jhi(r.i, L, K, mk, r.row);
-    if (mk.nonpad) {
-        const int2 sp = __ldg(span + b);
-        jhi = min(jhi, sp.x);
-        r.holes = sp.y != 0;
-    }
-    r.nj = jhi - r.i > 0 ? jhi - r.i : 0;
+    if (mk.nonpad) r.sp = __ldg(span + b);
+    if (mk.bound_end) r.bound = __ldg(mk.bound_end + r.row);
     return r;
+}
+__device__ __forceinline__ void lw_resolve(LwRow &r, int L, int K, const LinksMask &mk) {
+    if (!r.exists) return;
+    int jhi = min(r.i + K, L - 1);
+    if (mk.nonpad) {
+        jhi = min(jhi, r.sp.x);
+        r.holes = r.sp.y != 0;
+    }
+    if (mk.bound_end && r.bound < jhi) jhi = r.bound < 0 ? -1 : (int)r.bound;
+    r.nj = jhi - r.i > 0 ? jhi - r.i : 0;
 }
 
 // bias of vector v in log2 units, from the table in shared memory (its last row: -inf, for buckets outside)
@@ -694,7 +702,8 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + warp / kLwRows;
     LwWalk walk(group, step, L);
-    LwRow r0 = lw_row(walk, B, L, K, mk, span), r1 = lw_row(walk, B, L, K, mk, span);
+    LwRow r0 = lw_row(walk, B, L, mk, span), r1 = lw_row(walk, B, L, mk, span);
+    lw_resolve(r0, L, K, mk);
     LwSlot s0 = lw_slot<G, false>(r0, K, false);
     lw_issue<G, false>(r0, s0, ring, mbar, content, nullptr, L, K);
     const auto gates_of = [&](const LwRow &r) {
@@ -709,12 +718,13 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             phase ^= 1;
         }
         // the next row on its way, where the ring has room for it beside this one
+        lw_resolve(r1, L, K, mk);
         LwSlot s1 = lw_slot<G, false>(r1, K, false);
         s1.at = lw_place(s0, s1.bytes, lay.ring);
         const bool later = s1.at < 0;
         if (!later) lw_issue<G, false>(r1, s1, ring, mbar, content, nullptr, L, K);
         const float4 gate1 = gates_of(r1);
-        const LwRow r2 = lw_row(walk, B, L, K, mk, span);
+        const LwRow r2 = lw_row(walk, B, L, mk, span);
         if (r0.exists) {
             const int nvec = r0.nj * G;
             float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at);
@@ -876,7 +886,8 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + set;
     LwWalk walk(group, step, L);
-    LwRow r0 = lw_row(walk, B, L, K, mk, span), r1 = lw_row(walk, B, L, K, mk, span);
+    LwRow r0 = lw_row(walk, B, L, mk, span), r1 = lw_row(walk, B, L, mk, span);
+    lw_resolve(r0, L, K, mk);
     LwSlot s0 = lw_slot<G, true>(r0, K, wide);
     lw_issue<G, true>(r0, s0, ring, mbar, content, grad_links, L, K);
     const auto of_row = [&](const float *p, const LwRow &r) {
@@ -895,7 +906,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         }
         __syncwarp();
         const float4 lse1 = of_row(head_lse, r1), gate1 = of_row(log_gates, r1);
-        const LwRow r2 = lw_row(walk, B, L, K, mk, span);
+        const LwRow r2 = lw_row(walk, B, L, mk, span);
         const int nvec = r0.nj * G;
         float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at + s0.window);
         float *const weight = reinterpret_cast<float *>(ring + s0.at) + s0.skip;   // G_d, then w_d
@@ -972,6 +983,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         });
         __syncwarp();
         // the next row on its way: the gradient of the row before this one has left its place
+        lw_resolve(r1, L, K, mk);
         LwSlot s1 = lw_slot<G, true>(r1, K, wide);
         s1.at = lw_place(s0, s1.bytes, lay.ring);
         const bool later = s1.at < 0;

@@ -21,6 +21,7 @@
 // are put together in 64 bits by one thread (a 32-bit log-probability near -10 carries 5e-7, which would show
 // in the ratio), sums over rows in 64 bits in a fixed order.  d is taken relative to its value at v = 0, so
 // that a constant between the two models' logits does not cancel.
+#include "cluster_util.cuh"
 #include "dat_common.cuh"
 #include "umma.cuh"
 
@@ -407,21 +408,29 @@ policy_fwd_kernel(PolicyArgs a) {
 // Next to HBM the special-function unit bounds it: three exponentials per logit pair with the full KL, 24 of its
 // cycles per 32 pairs and scheduler against 33 that HBM takes for the 6 bytes of each at 16 bits.
 // ---------------------------------------------------------------------------------------------------
-constexpr int kPpPolls = 1 << 14;      // bound of a wait (never reached)
+constexpr int kPpPolls = 1 << 20;      // bound of a wait (never reached)
 constexpr int kPpZeros = 4096;         // bytes of zeros
-constexpr int kPpVecs = 2;             // 16-byte pieces of a chunk that a thread of either half has
 constexpr float kPpHuge = 0x1p100f;
 
+constexpr int kPpDepth = 4;            // rows under way in a CTA
+constexpr int kPpRanks = 8;            // CTAs that share a row at most
+
 struct PolicyRing {
-    int chunks, slots;            // chunks of a row (and array), slots of the ring: chunks <= slots <= 2 * chunks
+    int ranks;                    // CTAs (of a cluster) that share a row, its chunks dealt to them in turn
+    int chunks, slots;            // chunks of a row that a CTA has, slots of the ring: chunks <= slots <= kPpDepth * chunks
     int zeros, bars, red, x, y;   // places in the shared memory
 };
-// what the summing half hands to the writing half
+// a CTA's sums of a row, relative to (r, ry)
+struct PolicyPart {
+    float r, ry, S, T, Sy;
+    uint32_t careful;   // the row has logits of -inf
+};
+// what the writing half needs of a row
 struct PolicyHand {
     PolicyRow row;
     float xt, yt;   // the token's logits
     int tok;        // -1: outside the vocabulary
-    bool careful;   // the row has logits of -inf
+    uint32_t careful;
 };
 template <bool B>
 struct PolicyBool {
@@ -473,48 +482,39 @@ __device__ __forceinline__ F2 f2_floor(F2 v) {   // what is below -1e30, or NaN,
     return f2(fmaxf(a, kNegBig), fmaxf(b, kNegBig));
 }
 
-// Waits for a phase of a barrier; the hardware suspends the warp for up to the hint (in ns) per poll, so that waiting
-// warps take no issue slots (polling without it took a quarter of them).  false: gave up.
+// Waits for a phase of a barrier.  false: gave up.
 __device__ __forceinline__ bool policy_wait(uint64_t *mbar, uint32_t parity, int polls) {
-    const uint32_t a = umma::smem_u32(mbar);
-    for (int i = 0; i < polls; i++) {
-        uint32_t ok;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\tselp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(ok)
-            : "r"(a), "r"(parity), "r"(1000000)
-            : "memory");
-        if (ok) return true;
-    }
-    return false;
+    return umma::mbar_wait(mbar, parity, polls);
 }
 
-// The rows of a CTA, blockIdx.x + k * gridDim.x, 32 at a time through the mask; next() gives those whose bit is set.
+// The rows of a cluster, its number + k * clusters, 32 at a time through the mask; next() gives those whose bit is set.
 struct PolicyWalk {
     const unsigned char *mask;
     int64_t rows;
+    int step;            // clusters of the grid
     int64_t base;        // row of the block's lane 0
     unsigned bits, ahead;
     bool inactive;       // walk the rows that take no part
     __device__ __forceinline__ unsigned look(int64_t from) const {
-        const int64_t r = from + (int64_t)(threadIdx.x & 31) * gridDim.x;
+        const int64_t r = from + (int64_t)(threadIdx.x & 31) * step;
         return r < rows ? ((!mask || mask[r] != 0) != inactive ? 1u : 0u) : 0u;
     }
-    __device__ __forceinline__ PolicyWalk(const unsigned char *m, int64_t n, bool skip) : mask(m), rows(n), inactive(skip) {
-        base = blockIdx.x;
+    __device__ __forceinline__ PolicyWalk(const unsigned char *m, int64_t n, int ranks, bool skip)
+        : mask(m), rows(n), step(gridDim.x / ranks), inactive(skip) {
+        base = blockIdx.x / ranks;
         bits = __ballot_sync(0xffffffffu, look(base));
-        ahead = look(base + 32 * (int64_t)gridDim.x);
+        ahead = look(base + 32 * (int64_t)step);
     }
     __device__ __forceinline__ int64_t next() {
         while (!bits) {
-            base += 32 * (int64_t)gridDim.x;
+            base += 32 * (int64_t)step;
             if (base >= rows) return -1;
             bits = __ballot_sync(0xffffffffu, ahead);
-            ahead = look(base + 32 * (int64_t)gridDim.x);
+            ahead = look(base + 32 * (int64_t)step);
         }
         const int j = __ffs(bits) - 1;
         bits &= bits - 1;
-        return base + (int64_t)j * gridDim.x;
+        return base + (int64_t)j * step;
     }
 };
 
@@ -616,41 +616,78 @@ __device__ __forceinline__ void policy_grad_pairs(const PolicyRow &p, const F2 (
     }
 }
 
-// NT threads in each half, two warps beside them
-template <typename T, bool kRef, int NT>
-__global__ void __launch_bounds__(2 * NT + 64, NT == 256 ? 1 : 3)
+// the loss's numbers of a row from its sums
+struct PolicyNumbers {
+    float lp, u, term, kl, mean, cf, inv_s;
+    bool clipped;
+};
+template <bool kRef>
+__device__ __forceinline__ PolicyNumbers policy_numbers(const PolicyArgs &a, const PolicyPart &p, bool ok, float xt, float A,
+                                                        float old, float link, float ref) {
+    PolicyNumbers n;
+    n.lp = ok ? ((xt - p.r) - logf(p.S)) + link : __int_as_float(0x7fc00000);
+    n.u = expf(n.lp - old);
+    const float lo = 1.f - a.clip_low, hi = 1.f + a.clip_high;
+    const float ra = n.u * A, rc = (n.u < lo ? lo : n.u > hi ? hi : n.u) * A;
+    n.term = -(ra < rc ? ra : rc);
+    n.clipped = (A > 0.f && n.u > hi) || (A < 0.f && n.u < lo);
+    n.cf = n.clipped ? 0.f : -ra;
+    n.kl = n.mean = 0.f;
+    n.inv_s = 1.f / p.S;
+    if (kRef) {
+        n.mean = p.T / p.S;
+        n.kl = n.mean - logf(p.S / p.Sy);
+    } else if (a.ref_logp) {
+        const float z = ref - n.lp, em = expm1f(z);
+        n.kl = em - z;
+        n.cf = fmaf(-a.beta, em, n.cf);
+    }
+    return n;
+}
+
+// NT threads in each half, kPpVecs pieces of a chunk to each, three warps beside them
+template <typename T, bool kRef, int NT, int kPpVecs>
+__global__ void __launch_bounds__(2 * NT + 96, NT == 256 ? 1 : 3)
 policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
-    constexpr int kVec = Elem<T>::kVec, kWarps = NT / 32, kChunk = NT * kPpVecs;
+    constexpr int kVec = Elem<T>::kVec, kWarps = NT / 32, kChunk = NT * kPpVecs, kAll = 2 * NT + 96;
     extern __shared__ __align__(128) unsigned char posm[];
-    __shared__ PolicyHand hand_s[2];
-    __shared__ __align__(8) uint64_t hand_bar[2];
+    __shared__ PolicyPart part_s[kPpDepth];               // a row's sums on their way to its numbers
+    __shared__ PolicyHand hand_s[kPpDepth];               // and those on their way to the gradient
+    __shared__ PolicyPart cluster_s[2][kPpRanks];         // the sums of all CTAs that share a row
+    __shared__ __align__(8) uint64_t part_bar[kPpDepth], hand_bar[kPpDepth], cluster_bar[2];
     uint64_t *const full = reinterpret_cast<uint64_t *>(posm + ring.bars), *const empty = full + ring.slots;
     float4 *const red = reinterpret_cast<float4 *>(posm + ring.red);   // [2][kWarps]: S, T, Sy
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int V = a.V;
-    for (int x = tid; x < kPpZeros / 16; x += 2 * NT + 64) reinterpret_cast<uint4 *>(posm + ring.zeros)[x] = make_uint4(0, 0, 0, 0);
-    if (tid < ring.slots) {
-        umma::mbar_init(full + tid, 1);
-        umma::mbar_init(empty + tid, kWarps);
+    const int V = a.V, ranks = ring.ranks, rank = blockIdx.x % ranks;
+    for (int x = tid; x < kPpZeros / 16; x += kAll) reinterpret_cast<uint4 *>(posm + ring.zeros)[x] = make_uint4(0, 0, 0, 0);
+    for (int x = tid; x < ring.slots; x += kAll) {
+        umma::mbar_init(full + x, 1);
+        umma::mbar_init(empty + x, kWarps);
     }
-    if (tid < 2) umma::mbar_init(hand_bar + tid, 1);
+    if (tid < kPpDepth) {
+        umma::mbar_init(part_bar + tid, 1);
+        umma::mbar_init(hand_bar + tid, 1);
+    }
+    if (tid < 2) umma::mbar_init(cluster_bar + tid, 1);
     umma::fence_smem_to_async();
     __syncthreads();
+    if (ranks > 1) cluster_barrier();   // every CTA's barriers stand before a neighbour's sums arrive on them
     bool stalled = false;
     const uint4 *const xs = reinterpret_cast<const uint4 *>(posm + ring.x), *const ys = reinterpret_cast<const uint4 *>(posm + ring.y);
     const auto load = [&](int v, F2 (&px)[kVec / 2], F2 (&py)[kVec / 2]) {   // v: piece of the ring
         policy_pairs(xs[v], px, static_cast<const T *>(nullptr));
         if (kRef) policy_pairs(ys[v], py, static_cast<const T *>(nullptr));
     };
+    const auto polls = [&] { return stalled ? 1 : kPpPolls; };
     PolicyTurn turn;
 
     if (warp == 2 * kWarps) {   // ---- producer
-        PolicyWalk walk(a.mask, a.rows, false);
+        PolicyWalk walk(a.mask, a.rows, ranks, false);
         for (int64_t row = walk.next(); row >= 0 && !stalled; row = walk.next()) {
             const PolicySpan<T> sp(row, V);
             const int64_t from = row * V + sp.head;
-            for (int c = 0; c < ring.chunks && !stalled; c++, turn.next(ring.slots)) {
-                const int bytes = min(kChunk, sp.vecs - c * kChunk) * 16;
+            for (int j = 0; j < ring.chunks && !stalled; j++, turn.next(ring.slots)) {
+                const int c = j * ranks + rank, bytes = min(kChunk, sp.vecs - c * kChunk) * 16;
                 if (lane == 0) {
                     stalled |= !policy_wait(empty + turn.slot, turn.phase ^ 1, kPpPolls);   // the ring begins empty
                     if (!stalled) {
@@ -670,10 +707,10 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             }
         }
     } else if (warp == 2 * kWarps + 1) {   // ---- zeros
-        PolicyWalk walk(a.mask, a.rows, true);
+        PolicyWalk walk(a.mask, a.rows, ranks, true);
         const uint32_t zeros = umma::smem_u32(posm + ring.zeros);
         for (int64_t row = a.mask ? walk.next() : -1; row >= 0; row = walk.next()) {
-            if (lane == 0) {
+            if (lane == 0 && rank == 0) {
                 a.logp[row] = 0.f;
                 a.kl[row] = 0.f;
                 if (a.row_state) a.row_state[2 * row] = a.row_state[2 * row + 1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -682,10 +719,10 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             T *const g = static_cast<T *>(a.grad) + row * V;
             const PolicySpan<T> sp(row, V);
             const int bytes = sp.vecs * 16;
-            if (lane < sp.head) g[lane] = Elem<T>::from_float(0.f);
-            if (lane < sp.tail) g[V - sp.tail + lane] = Elem<T>::from_float(0.f);
+            if (rank == 0 && lane < sp.head) g[lane] = Elem<T>::from_float(0.f);
+            if (rank == 0 && lane < sp.tail) g[V - sp.tail + lane] = Elem<T>::from_float(0.f);
             unsigned char *const mid = reinterpret_cast<unsigned char *>(g + sp.head);
-            for (int at = lane * kPpZeros; at < bytes; at += 32 * kPpZeros)
+            for (int at = (lane * ranks + rank) * kPpZeros; at < bytes; at += 32 * ranks * kPpZeros)
                 asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(mid + at), "r"(zeros),
                              "r"(min(kPpZeros, bytes - at))
                              : "memory");
@@ -693,47 +730,136 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             asm volatile("cp.async.bulk.wait_group.read 4;" ::: "memory");   // a few rows at a time, beside the active ones
         }
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    } else if (warp == 2 * kWarps + 2) {   // ---- numbers
+        const double inv_n = a.head->inv_n;
+        const float n1 = (float)inv_n, up = a.head->scale;
+        PolicyWalk walk(a.mask, a.rows, ranks, false);
+        double sums[kPoSums] = {};   // of this cluster's rows, in their order
+        uint32_t n = 0;
+        for (int64_t row = walk.next(); row >= 0; row = walk.next(), n++) {
+            const int64_t b = row / a.L, l = row - b * a.L, tok = a.tokens[row];
+            const bool ok = tok >= 0 && tok < V;
+            const int64_t at = row * V + (ok ? tok : 0);
+            const float xt = Elem<T>::to_float(static_cast<const T *>(a.x)[at]), yt = kRef ? Elem<T>::to_float(static_cast<const T *>(a.y)[at]) : 0.f;
+            const float A = a.advantage[b * a.adv_b + l * a.adv_l], old = a.old_logp[row];
+            const float link = a.link_logp ? a.link_logp[row] : 0.f, ref = a.ref_logp ? a.ref_logp[row] : 0.f;
+            stalled |= !policy_wait(part_bar + n % kPpDepth, n / kPpDepth & 1, polls());
+            PolicyPart p = part_s[n % kPpDepth];
+            if (ranks > 1) {
+                // to the neighbours, and theirs.  Two buffers do: a neighbour sends row n + 2 only after it has this
+                // CTA's row n + 1, which is sent below once row n has been read.
+                PolicyPart *const all = cluster_s[n & 1];
+                uint64_t *const bar = cluster_bar + (n & 1);
+                if (lane == 0) {
+                    all[rank] = p;
+                    cluster_mbar_expect(bar, (ranks - 1) * (uint32_t)sizeof(PolicyPart));
+                }
+                if (lane < ranks && lane != rank) {
+                    const uint32_t to = cluster_map(all + rank, lane), rbar = cluster_map(bar, lane);
+                    const uint32_t w[6] = {__float_as_uint(p.r), __float_as_uint(p.ry), __float_as_uint(p.S), __float_as_uint(p.T),
+                                           __float_as_uint(p.Sy), p.careful};
+#pragma unroll
+                    for (int k = 0; k < 6; k++) cluster_st_async_b32(to + 4 * k, w[k], rbar);
+                }
+                __syncwarp();
+                stalled |= !policy_wait(bar, n / 2 & 1, polls());
+                // in the order of the ranks, relative to the largest reference (they differ only where a CTA took its
+                // maximum)
+                float r = -INFINITY, ry = -INFINITY;
+                for (int q = 0; q < ranks; q++) {
+                    if (all[q].S != 0.f) r = fmaxf(r, all[q].r);
+                    if (all[q].Sy != 0.f) ry = fmaxf(ry, all[q].ry);
+                }
+                float S = 0.f, Tt = 0.f, Sy = 0.f;
+                uint32_t careful = 0;
+                for (int q = 0; q < ranks; q++) {
+                    const PolicyPart o = all[q];
+                    careful |= o.careful;
+                    if (o.S != 0.f) {
+                        const float f = o.r == r ? 1.f : ex2((o.r - r) * kLog2e), move = (o.r - r) - (o.ry - ry);
+                        S = fmaf(o.S, f, S);
+                        if (kRef) Tt = fmaf(move == 0.f ? o.T : fmaf(move, o.S, o.T), f, Tt);
+                    }
+                    if (kRef && o.Sy != 0.f) Sy = fmaf(o.Sy, o.ry == ry ? 1.f : ex2((o.ry - ry) * kLog2e), Sy);
+                }
+                p.r = r;
+                p.ry = kRef ? ry : 0.f;
+                p.S = S;
+                p.T = Tt;
+                p.Sy = kRef ? Sy : 1.f;
+                p.careful = careful;
+                __syncwarp();   // everybody has read the buffer
+            }
+            if (lane == 0) {
+                const PolicyNumbers m = policy_numbers<kRef>(a, p, ok, xt, A, old, link, ref);
+                PolicyHand &h = hand_s[n % kPpDepth];
+                h.row.r = p.r;
+                h.row.ry = p.ry;
+                h.row.tok_c = m.cf * n1 * up;
+                h.row.a = -h.row.tok_c * m.inv_s;
+                h.row.w = a.beta * n1 * up * m.inv_s;
+                h.row.mean = m.mean;
+                h.xt = xt;
+                h.yt = yt;
+                h.tok = ok ? (int)tok : -1;
+                h.careful = p.careful;
+                policy_arrive(hand_bar + n % kPpDepth);
+                if (rank == 0) {
+                    if (!ok && a.status) atomicOr(a.status, DAT_STATUS_BAD_INDEX);
+                    a.logp[row] = m.lp;
+                    a.kl[row] = m.kl;
+                    sums[0] += (double)m.term;
+                    sums[1] += (double)m.kl;
+                    sums[2] += (double)m.u;
+                    sums[3] += m.clipped ? 1.0 : 0.0;
+                    sums[4] += 1.0;
+                    if (a.row_state) {
+                        a.row_state[2 * row] = make_float4(p.r, m.inv_s, m.cf * n1, m.mean);
+                        a.row_state[2 * row + 1] = make_float4(p.ry, 0.f, 0.f, 0.f);
+                    }
+                }
+            }
+        }
+        if (lane == 0 && rank == 0)
+            for (int k = 0; k < kPoSums; k++) a.chunk_sums[(int64_t)(blockIdx.x / ranks) * kPoSums + k] = sums[k];
     } else if (warp < kWarps) {   // ---- the summing half
         const auto sync = [] { asm volatile("bar.sync 1, %0;" ::"n"(NT) : "memory"); };
-        const float n1 = (float)a.head->inv_n, up = a.head->scale;
-        PolicyWalk walk(a.mask, a.rows, false);
+        PolicyWalk walk(a.mask, a.rows, ranks, false);
         // the next row's token and its logits are on their way while this row is worked on
         int64_t row = walk.next(), row1 = row >= 0 ? walk.next() : -1;
         const auto token = [&](int64_t r) { return r >= 0 ? a.tokens[r] : 0; };
+        // as it lies in memory: a conversion here would wait for the load
         const auto logit = [&](const void *p, int64_t r, int64_t t) {
-            return r >= 0 ? Elem<T>::to_float(static_cast<const T *>(p)[r * V + (t >= 0 && t < V ? t : 0)]) : 0.f;
+            return static_cast<const T *>(p)[r >= 0 ? r * V + (t >= 0 && t < V ? t : 0) : 0];
         };
-        int64_t tok = token(row), tok1 = token(row1);
-        float xt = logit(a.x, row, tok), yt = kRef ? logit(a.y, row, tok) : 0.f;
-        double sums[kPoSums] = {};   // of this CTA's rows, in their order (one thread's are used)
-        int par = 0;
+        int64_t tok1 = token(row1);
+        T xt = logit(a.x, row, token(row)), yt = kRef ? logit(a.y, row, token(row)) : xt;
+        uint32_t n = 0;
         bool careful = false;
-        for (; row >= 0; par ^= 1) {
-            const float xt1 = logit(a.x, row1, tok1), yt1 = kRef ? logit(a.y, row1, tok1) : 0.f;
+        for (; row >= 0; n++) {
+            const T xt1 = logit(a.x, row1, tok1), yt1 = kRef ? logit(a.y, row1, tok1) : xt1;
             const int64_t row2 = row1 >= 0 ? walk.next() : -1, tok2 = token(row2);
-            const int64_t b = row / a.L, l = row - b * a.L;
-            const float A = a.advantage[b * a.adv_b + l * a.adv_l], old = a.old_logp[row];
-            const float link = a.link_logp ? a.link_logp[row] : 0.f, ref = a.ref_logp ? a.ref_logp[row] : 0.f;
             const PolicySpan<T> sp(row, V);
             const T *const x = static_cast<const T *>(a.x) + row * V, *const y = kRef ? static_cast<const T *>(a.y) + row * V : nullptr;
-            // an element before or behind the pieces for the threads 0 .. head-1 and 8 .. 8+tail-1
-            const bool extra = tid < sp.head || (tid >= 8 && tid < 8 + sp.tail);
+            // an element before or behind the pieces for the threads 0 .. head-1 and 8 .. 8+tail-1 of the first CTA
+            const bool extra = rank == 0 && (tid < sp.head || (tid >= 8 && tid < 8 + sp.tail));
             const int te = tid < 8 ? tid : V - sp.tail + tid - 8;
-            const float tx = extra ? Elem<T>::to_float(x[te]) : -INFINITY, ty = extra && kRef ? Elem<T>::to_float(y[te]) : -INFINITY;
+            const T tx_raw = x[extra ? te : 0], ty_raw = kRef ? y[extra ? te : 0] : tx_raw;
             const int first = turn.slot;
-            float r = xt, ry = yt;
+            float r = Elem<T>::to_float(xt), ry = kRef ? Elem<T>::to_float(yt) : 0.f;
             F2 mr = f2(-r, -r), mry = f2(-ry, -ry);
             PolicyAcc<kRef> acc;
             const auto sum = [&](auto care) {
-                for (int c = 0; c < ring.chunks; c++, turn.next(ring.slots)) {
-                    stalled |= !policy_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
-                    const int v = turn.slot * kChunk + tid, left = sp.vecs - c * kChunk;
+                for (int j = 0; j < ring.chunks; j++, turn.next(ring.slots)) {
+                    stalled |= !policy_wait(full + turn.slot, turn.phase, polls());
+                    const int v = turn.slot * kChunk + tid, left = sp.vecs - (j * ranks + rank) * kChunk;
                     if (left >= kChunk) {
-                        F2 px[kPpVecs][kVec / 2], py[kPpVecs][kVec / 2];
 #pragma unroll
-                        for (int q = 0; q < kPpVecs; q++) load(v + q * NT, px[q], py[q]);
-#pragma unroll
-                        for (int q = 0; q < kPpVecs; q++) acc.template add<decltype(care)::value>(px[q], py[q], mr, mry);
+                        for (int q = 0; q < kPpVecs; q++) {
+                            F2 px[kVec / 2], py[kVec / 2];
+                            load(v + q * NT, px, py);
+                            acc.template add<decltype(care)::value>(px, py, mr, mry);
+                        }
                     } else {
                         for (int q = 0; q < kPpVecs; q++)
                             if (tid + q * NT < left) {
@@ -746,6 +872,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             };
             if (careful) sum(PolicyBool<true>());
             else sum(PolicyBool<false>());
+            const float tx = Elem<T>::to_float(tx_raw), ty = Elem<T>::to_float(ty_raw);
             if (extra) acc.add1(tx, ty, r, ry);
             float S, Tt, Sy;
             const auto reduce = [&](float4 *slot) {
@@ -764,16 +891,16 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                     Sy = 1.f;
                 }
             };
-            float4 *const slot = red + (par ? kWarps : 0);
+            float4 *const slot = red + (n & 1 ? kWarps : 0);
             reduce(slot);
             if (!(S < kPpHuge && fabsf(Tt) < kPpHuge && Sy < kPpHuge)) {   // the same in all threads
                 // the maxima in place of the token's logits; the row's slots are not freed before its gradient
                 careful = kRef;   // and from here on: rows of one batch share their forbidden tokens
                 const auto again = [&](auto f) {
                     int at = first;
-                    for (int c = 0; c < ring.chunks; c++) {
+                    for (int j = 0; j < ring.chunks; j++) {
                         for (int q = 0; q < kPpVecs; q++)
-                            if (c * kChunk + tid + q * NT < sp.vecs) {
+                            if ((j * ranks + rank) * kChunk + tid + q * NT < sp.vecs) {
                                 F2 px[kVec / 2], py[kVec / 2];
                                 load(at * kChunk + tid + q * NT, px, py);
                                 f(px, py);
@@ -806,6 +933,9 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 const float4 q = slot[lane & (kWarps - 1)];
                 r = warp_max(q.x);
                 ry = kRef ? warp_max(q.y) : 0.f;
+                // nothing but -inf in this CTA's share: any reference gives the sum 0
+                r = r > -INFINITY ? r : 0.f;
+                ry = ry > -INFINITY ? ry : 0.f;
                 mr = f2(-r, -r);
                 mry = f2(-ry, -ry);
                 acc = PolicyAcc<kRef>();
@@ -814,77 +944,32 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 sync();
                 reduce(slot);
             }
-            // the row's numbers
             if (tid == 0) {
-                const bool ok = tok >= 0 && tok < V;
-                const float lp = ok ? ((xt - r) - logf(S)) + link : __int_as_float(0x7fc00000);
-                const float u = expf(lp - old);
-                const float lo = 1.f - a.clip_low, hi = 1.f + a.clip_high;
-                const float ra = u * A, rc = (u < lo ? lo : u > hi ? hi : u) * A;
-                const bool clipped = (A > 0.f && u > hi) || (A < 0.f && u < lo);
-                float cf = clipped ? 0.f : -ra, kl = 0.f, mean = 0.f;
-                if (kRef) {
-                    mean = Tt / S;
-                    kl = mean - logf(S / Sy);
-                } else if (a.ref_logp) {
-                    const float z = ref - lp, em = expm1f(z);
-                    kl = em - z;
-                    cf = fmaf(-a.beta, em, cf);
-                }
-                const float inv_s = 1.f / S;
-                PolicyHand &h = hand_s[par];
-                h.row.r = r;
-                h.row.ry = ry;
-                h.row.tok_c = cf * n1 * up;
-                h.row.a = -h.row.tok_c * inv_s;
-                h.row.w = a.beta * n1 * up * inv_s;
-                h.row.mean = mean;
-                h.xt = xt;
-                h.yt = yt;
-                h.tok = ok ? (int)tok : -1;
-                h.careful = careful;
-                policy_arrive(hand_bar + par);
-                if (!ok && a.status) atomicOr(a.status, DAT_STATUS_BAD_INDEX);
-                a.logp[row] = lp;
-                a.kl[row] = kl;
-                sums[0] += (double)-(ra < rc ? ra : rc);
-                sums[1] += (double)kl;
-                sums[2] += (double)u;
-                sums[3] += clipped ? 1.0 : 0.0;
-                sums[4] += 1.0;
-                if (a.row_state) {
-                    a.row_state[2 * row] = make_float4(r, inv_s, cf * n1, mean);
-                    a.row_state[2 * row + 1] = make_float4(ry, 0.f, 0.f, 0.f);
-                }
+                part_s[n % kPpDepth] = PolicyPart{r, ry, S, Tt, Sy, careful ? 1u : 0u};
+                policy_arrive(part_bar + n % kPpDepth);
             }
             row = row1;
             row1 = row2;
-            tok = tok1;
             tok1 = tok2;
             xt = xt1;
             yt = yt1;
         }
         if (stalled)   // copies that may still be on their way, within a bound again
             for (int c = 0; c < ring.slots; c++) policy_wait(full + c, turn.phase, kPpPolls);
-        if (tid == 0)
-            for (int k = 0; k < kPoSums; k++) a.chunk_sums[(int64_t)blockIdx.x * kPoSums + k] = sums[k];
     } else {   // ---- the writing half
         const int wt = tid - NT;
-        PolicyWalk walk(a.mask, a.rows, false);
-        uint32_t par = 0, hand_phase = 0;
-        for (int64_t row = walk.next(); row >= 0; row = walk.next()) {
-            stalled |= !policy_wait(hand_bar + par, hand_phase, stalled ? 1 : kPpPolls);
-            const PolicyHand h = hand_s[par];
-            par ^= 1;
-            hand_phase ^= par ^ 1;
+        PolicyWalk walk(a.mask, a.rows, ranks, false);
+        uint32_t n = 0;
+        for (int64_t row = walk.next(); row >= 0; row = walk.next(), n++) {
+            stalled |= !policy_wait(hand_bar + n % kPpDepth, n / kPpDepth & 1, polls());
+            const PolicyHand h = hand_s[n % kPpDepth];
             const PolicyRow p = h.row;
             const PolicySpan<T> sp(row, V);
             T *const g = a.grad ? static_cast<T *>(a.grad) + row * V : nullptr;
             uint4 *const gv = reinterpret_cast<uint4 *>(g + sp.head);
-            for (int c = 0; c < ring.chunks; c++, turn.next(ring.slots)) {
-                // full since the row was summed: the wait only makes the copy's bytes this thread's too
-                stalled |= !policy_wait(full + turn.slot, turn.phase, stalled ? 1 : kPpPolls);
-                const int v = turn.slot * kChunk + wt, to = c * kChunk + wt;
+            for (int j = 0; j < ring.chunks; j++, turn.next(ring.slots)) {
+                // (full since the row was summed, which the hand-over above makes known here)
+                const int v = turn.slot * kChunk + wt, to = (j * ranks + rank) * kChunk + wt;
                 const auto store = [&](auto care, int q) {
                     F2 px[kVec / 2], py[kVec / 2];
                     float out[kVec];
@@ -893,7 +978,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                     gv[to + q * NT] = Elem<T>::pack(out);
                 };
                 if (g) {
-                    if ((c + 1) * kChunk <= sp.vecs && !h.careful) {
+                    if (to - wt + kChunk <= sp.vecs && !h.careful) {
 #pragma unroll
                         for (int q = 0; q < kPpVecs; q++) store(PolicyBool<false>(), q);
                     } else {
@@ -905,17 +990,24 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 if (lane == 0) policy_arrive(empty + turn.slot);
             }
             if (g) {
-                if (wt < sp.head || (wt >= 8 && wt < 8 + sp.tail)) {
+                if (rank == 0 && (wt < sp.head || (wt >= 8 && wt < 8 + sp.tail))) {
                     const int te = wt < 8 ? wt : V - sp.tail + wt - 8;
                     const float ty = kRef ? Elem<T>::to_float(static_cast<const T *>(a.y)[row * V + te]) : 0.f;
                     g[te] = Elem<T>::from_float(policy_grad_one<kRef>(p, Elem<T>::to_float(static_cast<const T *>(a.x)[row * V + te]), ty));
                 }
                 // the token's place once more, by the thread that wrote it
-                const int at = h.tok - sp.head;
-                const int mine = at < 0 ? h.tok : at >= sp.vecs * kVec ? h.tok - (V - sp.tail) + 8 : at / kVec % NT;
-                if (h.tok >= 0 && wt == mine) g[h.tok] = Elem<T>::from_float(policy_grad_one<kRef>(p, h.xt, h.yt) + p.tok_c);
+                const int at = h.tok - sp.head, piece = at / kVec;
+                const bool inside = at >= 0 && piece < sp.vecs;
+                const int mine = inside ? piece % NT : at < 0 ? h.tok : h.tok - (V - sp.tail) + 8;
+                const int owner = inside ? piece / kChunk % ranks : 0;
+                if (h.tok >= 0 && rank == owner && wt == mine)
+                    g[h.tok] = Elem<T>::from_float(policy_grad_one<kRef>(p, h.xt, h.yt) + p.tok_c);
             }
         }
+    }
+    if (ranks > 1) {   // nobody leaves while a neighbour may still send to it
+        __syncwarp();
+        cluster_barrier();
     }
     if (stalled && lane == 0 && a.status) atomicOr(a.status, DAT_STATUS_STALLED);
     // the last CTA adds the CTAs' sums in their order
@@ -931,7 +1023,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
     double total[2] = {};
     for (int k = 0; k < kPoSums; k++) {
         double t = 0.0;
-        for (int c = lane; c < (int)gridDim.x; c += 32) t += __ldcg(a.chunk_sums + (int64_t)c * kPoSums + k);
+        for (int c = lane; c < (int)gridDim.x / ranks; c += 32) t += __ldcg(a.chunk_sums + (int64_t)c * kPoSums + k);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
         if (k < 2) total[k] = t;
@@ -998,18 +1090,21 @@ static bool aligned16(const void *a, const void *b, const void *c) {
     return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c)) & 15) == 0;
 }
 
-// The ring of a CTA with nt threads in each half, `per_sm` of them on an SM; false: a row does not fit.
-static bool policy_ring(int nt, int per_sm, int V, int size, bool ref, const DeviceInfo &di, PolicyRing &ring, int &smem) {
+// The ring of a CTA with nt threads in each half and chunks of nt * vecs pieces, `per_sm` of them on an SM and `ranks`
+// to a row; false: a row does not fit.
+static bool policy_ring(int nt, int vecs, int per_sm, int ranks, int V, int size, bool ref, const DeviceInfo &di, PolicyRing &ring,
+                        int &smem) {
     const auto up = [](int n) { return (n + 127) / 128 * 128; };
     const int64_t pieces = (int64_t)V * size / 16;   // 16-byte pieces inside a row
-    const int chunk = nt * kPpVecs, slot = chunk * 16 * (ref ? 2 : 1);
-    if (pieces < 1 || pieces > (1 << 16)) return false;
-    ring.chunks = (int)((pieces + chunk - 1) / chunk);
-    const int avail = (di.max_smem_optin + 1024) / per_sm - 1024 - 512;   // what the kernel declares itself is below 512
-    const int fixed = up(kPpZeros + 4 * ring.chunks * 8) + up(2 * (nt / 32) * 16);
+    const int chunk = nt * vecs, slot = chunk * 16 * (ref ? 2 : 1);
+    if (pieces < 1 || pieces > (1 << 20)) return false;
+    ring.ranks = ranks;
+    ring.chunks = (int)((pieces + (int64_t)chunk * ranks - 1) / (chunk * ranks));
+    const int avail = (di.max_smem_optin + 1024) / per_sm - 1024 - 1024;   // what the kernel declares itself is below 1024
+    const int fixed = up(kPpZeros + 2 * kPpDepth * ring.chunks * 8) + up(2 * (nt / 32) * 16);
     ring.slots = (avail - fixed) / slot;
-    if (ring.slots > 2 * ring.chunks) ring.slots = 2 * ring.chunks;
-    if (ring.slots < ring.chunks || ring.slots > 2 * nt) return false;
+    if (ring.slots > kPpDepth * ring.chunks) ring.slots = kPpDepth * ring.chunks;
+    if (ring.slots < ring.chunks) return false;
     ring.zeros = 0;
     ring.bars = kPpZeros;
     ring.red = up(ring.bars + 2 * ring.slots * 8);
@@ -1019,30 +1114,63 @@ static bool policy_ring(int nt, int per_sm, int V, int size, bool ref, const Dev
     return true;
 }
 
-template <typename T, bool kRef, int NT>
+template <typename T, bool kRef, int NT, int kPpVecs>
 static int policy_ring_launch(const PolicyArgs &a, const PolicyRing &ring, int smem, int per_sm, const DeviceInfo &di,
                               cudaStream_t st, const char *who) {
-    int64_t grid = (int64_t)di.sm_count * per_sm;
-    if (grid > a.rows) grid = a.rows;
-    if (grid > kPoMaxCtas) grid = kPoMaxCtas;
-    if (cudaFuncSetAttribute(policy_ring_kernel<T, kRef, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
-        policy_ring_kernel<T, kRef, NT><<<(unsigned)grid, 2 * NT + 64, smem, st>>>(a, ring);
+    int64_t n = (int64_t)di.sm_count * per_sm / ring.ranks;   // clusters
+    if (n > a.rows) n = a.rows;
+    if (n > kPoMaxCtas) n = kPoMaxCtas;
+    if (cudaFuncSetAttribute(policy_ring_kernel<T, kRef, NT, kPpVecs>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return check_launch(who);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)n * ring.ranks);
+    cfg.blockDim = dim3(2 * NT + 96);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim = {(unsigned)ring.ranks, 1, 1};
+    cfg.attrs = at;
+    cfg.numAttrs = ring.ranks > 1 ? 1 : 0;
+    cudaLaunchKernelEx(&cfg, policy_ring_kernel<T, kRef, NT, kPpVecs>, a, ring);
     return check_launch(who);
 }
 
 template <typename T>
 static int policy_fwd_t(const PolicyArgs &a, const DeviceInfo &di, cudaStream_t st, const char *who) {
-    // Rows of 8 KB and up that fit: the ring, with 128 threads in each half where three CTAs fit an SM, else with 256.
+    // Rows of 8 KB and up: the ring, with 128 threads in each half where three CTAs with two rows each fit an SM, else
+    // with 256 and as few CTAs to a row as it takes for more than one row in a ring.  Chunks are as large as that allows:
+    // a chunk of four pieces a thread keeps more arithmetic in flight than one of two (32x1024x32000 with the full KL
+    // 1308 against 1390 us, 1623 with one), a ring without a spare chunk lets the halves wait for each other.
+    // Fewer rows than SMs: more CTAs to a row, as long as each has a chunk of it.
     if (a.vec && (int64_t)a.V * sizeof(T) >= 8192) {
-        PolicyRing ring;
-        int smem;
+        PolicyRing ring, more;
+        int smem, smem2;
         const bool ref = a.y != nullptr;
-        if (policy_ring(128, 3, a.V, sizeof(T), ref, di, ring, smem))
-            return ref ? policy_ring_launch<T, true, 128>(a, ring, smem, 3, di, st, who)
-                       : policy_ring_launch<T, false, 128>(a, ring, smem, 3, di, st, who);
-        if (policy_ring(256, 1, a.V, sizeof(T), ref, di, ring, smem))
-            return ref ? policy_ring_launch<T, true, 256>(a, ring, smem, 1, di, st, who)
-                       : policy_ring_launch<T, false, 256>(a, ring, smem, 1, di, st, who);
+        const auto spread = [&](int nt, int vecs, int per_sm) {
+            while (ring.ranks < kPpRanks && a.rows * ring.ranks * 2 <= di.sm_count && ring.chunks > 1 &&
+                   policy_ring(nt, vecs, per_sm, ring.ranks * 2, a.V, sizeof(T), ref, di, more, smem2)) {
+                ring = more;
+                smem = smem2;
+            }
+        };
+        if (policy_ring(128, 2, 3, 1, a.V, sizeof(T), ref, di, ring, smem) && ring.slots >= 2 * ring.chunks) {
+            spread(128, 2, 3);
+            return ref ? policy_ring_launch<T, true, 128, 2>(a, ring, smem, 3, di, st, who)
+                       : policy_ring_launch<T, false, 128, 2>(a, ring, smem, 3, di, st, who);
+        }
+        for (int ranks = 1; ranks <= kPpRanks; ranks *= 2) {
+            if (policy_ring(256, 4, 1, ranks, a.V, sizeof(T), ref, di, ring, smem) && ring.slots > ring.chunks) {
+                spread(256, 4, 1);
+                return ref ? policy_ring_launch<T, true, 256, 4>(a, ring, smem, 1, di, st, who)
+                           : policy_ring_launch<T, false, 256, 4>(a, ring, smem, 1, di, st, who);
+            }
+            if (policy_ring(256, 2, 1, ranks, a.V, sizeof(T), ref, di, ring, smem) && ring.slots > ring.chunks) {
+                spread(256, 2, 1);
+                return ref ? policy_ring_launch<T, true, 256, 2>(a, ring, smem, 1, di, st, who)
+                           : policy_ring_launch<T, false, 256, 2>(a, ring, smem, 1, di, st, who);
+            }
+        }
     }
     if (a.y)
         policy_fwd_kernel<T, true><<<(unsigned)a.rows, kPoThreads, 0, st>>>(a);
