@@ -191,6 +191,28 @@ struct Elem<__nv_bfloat16> {
     }
 };
 
+// Programmatic dependent launch: a kernel launched with launch_after may begin before the kernel before it on the
+// stream has ended, and sees that kernel's results after pdl_wait; the kernel before lets it begin with pdl_trigger.
+__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+template <typename... P, typename... A>
+void launch_after(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, unsigned cluster,
+                  A... args) {
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim = {cluster, 1, 1};
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = at;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 struct DeviceInfo {
     int device;
     int sm_count;

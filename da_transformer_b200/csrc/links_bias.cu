@@ -438,6 +438,7 @@ constexpr uint32_t kLwFull = 0x7fc00d1eu;   // weight of a distance whose gradie
 __global__ void __launch_bounds__(128)
 lw_span_kernel(const unsigned char *__restrict__ nonpad, int2 *__restrict__ span, int L) {
     __shared__ int last_s[4], n_s[4];
+    pdl_trigger();
     const unsigned char *np = nonpad + (int64_t)blockIdx.x * L;
     int last = -1, n = 0;
     for (int j = 1 + threadIdx.x; j < L; j += 128)
@@ -687,7 +688,7 @@ __device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, c
 
 // NG groups of four vertices at work in a CTA
 template <int G, int NG>
-__global__ void __launch_bounds__(NG * kLwRows * 32, 2)
+__global__ void __launch_bounds__(NG * kLwRows * 32, NG == 2 ? 2 : 1)
 lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk,
               const int2 *__restrict__ span, LinksBias lb, LwSmem lay, float *__restrict__ links,
               float *__restrict__ head_lse, int B, int L, int K) {
@@ -699,6 +700,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
     unsigned char *const ring = lwsm + lay.rings + warp * lay.ring;
     uint64_t *const mbar = reinterpret_cast<uint64_t *>(lwsm + lay.mbar) + warp;
     lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
+    pdl_wait();   // the spans
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + warp / kLwRows;
     LwWalk walk(group, step, L);
@@ -883,6 +885,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     const int set = warp / kLwRows, set_tid = tid - set * (kLwRows * 32);
     const auto set_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(set + 1), "n"(kLwRows * 32) : "memory"); };
     lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
+    pdl_trigger();
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + set;
     LwWalk walk(group, step, L);
@@ -1066,10 +1069,33 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     lw_bulk_read();
     if (stalled && lb.status) atomicOr(lb.status, DAT_STATUS_STALLED);
     if (part) {
-        float4 *p = reinterpret_cast<float4 *>(part + ((size_t)blockIdx.x * NG + set) * K * H);
+        // the groups' sums together, through the rings, whose copies have all come and gone
+        float4 *const sums = reinterpret_cast<float4 *>(lwsm + lay.rings);
+        __syncthreads();
 #pragma unroll
-        for (int u = 0; u < UA; u++)
-            if (set_tid + u * (kLwRows * 32) < K * G) p[set_tid + u * (kLwRows * 32)] = acc[u];
+        for (int u = 0; u < UA; u++) {
+            const int v = set_tid + u * (kLwRows * 32);
+            if (set > 0 && v < K * G) sums[(set - 1) * K * G + v] = acc[u];
+        }
+        __syncthreads();
+        if (set == 0) {
+            float4 *p = reinterpret_cast<float4 *>(part + (size_t)blockIdx.x * K * H);
+#pragma unroll
+            for (int u = 0; u < UA; u++) {
+                const int v = set_tid + u * (kLwRows * 32);
+                if (v < K * G) {
+#pragma unroll
+                    for (int q = 0; q < NG - 1; q++) {
+                        const float4 o = sums[q * K * G + v];
+                        acc[u].x += o.x;
+                        acc[u].y += o.y;
+                        acc[u].z += o.z;
+                        acc[u].w += o.w;
+                    }
+                    p[v] = acc[u];
+                }
+            }
+        }
     }
 }
 
@@ -1080,6 +1106,8 @@ lb_sum_kernel(const float *__restrict__ part, double *__restrict__ by_distance, 
     __shared__ double lane_s[kLbSumLanes][kLbSumCols];
     const int c = threadIdx.x % kLbSumCols, q = threadIdx.x / kLbSumCols, x = blockIdx.x * kLbSumCols + c;
     double acc = 0.0;
+    pdl_trigger();
+    pdl_wait();
     if (x < KH) {
 #pragma unroll 8
         for (int k = q; k < n; k += kLbSumLanes) acc += (double)part[(size_t)k * KH + x];
@@ -1099,6 +1127,8 @@ lb_diag_kernel(const float *__restrict__ grad_content, double *__restrict__ by_d
     __shared__ double lane_s[kLbSumLanes][kLbSumCols];
     const int c = threadIdx.x % kLbSumCols, q = threadIdx.x / kLbSumCols, x = blockIdx.x * kLbSumCols + c;
     double acc = 0.0;
+    pdl_trigger();
+    pdl_wait();
     if (x < K * H) {
         const int n = L - 1 - x / H;   // vertices that have a successor at this distance
         for (int b = 0; b < B; b++) {
@@ -1124,6 +1154,7 @@ lb_join_kernel(const double *__restrict__ by_distance, const int64_t *__restrict
     __shared__ double lane_s[kLbJoinThreads];
     const int k = blockIdx.x, P = kLbJoinThreads / H, h = threadIdx.x % H, p = threadIdx.x / H;
     double acc = 0.0;
+    pdl_wait();
     if (p < P) {
 #pragma unroll 8
         for (int d = p; d < K; d += P) {
@@ -1173,6 +1204,7 @@ struct LbArgs {
     LinksMask mk;
     LinksBias lb;
     int2 *span;
+    bool after;   // the kernel that fills the spans has just been launched
     float *links, *head_lse, *grad_content, *grad_log_gates, *part;
     int B, L, K;
 };
@@ -1203,19 +1235,23 @@ static int lw_start(F kernel, int per_sm, const LbArgs &a, int &parts, cudaStrea
     lay = lw_smem(a.K, 4 * G, a.lb.n, NG * kLwRows, smem);
     int64_t n = (int64_t)di.sm_count * per_sm;
     if (n > (groups + NG - 1) / NG) n = (groups + NG - 1) / NG;
-    parts = (int)n * NG;
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess)
-        kernel<<<(unsigned)n, NG * kLwRows * 32, smem, st>>>(args...);
+    parts = (int)n;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) == cudaSuccess) {
+        if (a.after) launch_after(kernel, (unsigned)n, NG * kLwRows * 32, smem, st, 1, args...);
+        else kernel<<<(unsigned)n, NG * kLwRows * 32, smem, st>>>(args...);
+    }
     return check_launch(who);
 }
 template <int G>
 static int lw_launch(const LbArgs &a, bool backward, int &parts, cudaStream_t st, const DeviceInfo &di, const char *who) {
-    // two CTAs per SM where the rings of both hold more than the longest row, else one
+    // two CTAs per SM, of eight warps, where the rings of both hold more than the longest row, else one of twelve
     const int row = lw_row_bytes(a.K, 4 * G);
     LwSmem lay;
     if (!backward) {
-        const bool pair = lw_smem(a.K, 4 * G, a.lb.n, 3 * kLwRows, lw_two(di)).ring >= row + row / 4;
-        return lw_start<G, 3>(lw_fwd_kernel<G, 3>, pair ? 2 : 1, a, parts, st, di, who, lay, a.content, a.log_gates, a.mk,
+        if (lw_smem(a.K, 4 * G, a.lb.n, 2 * kLwRows, lw_two(di)).ring >= row + row / 4)
+            return lw_start<G, 2>(lw_fwd_kernel<G, 2>, 2, a, parts, st, di, who, lay, a.content, a.log_gates, a.mk, a.span,
+                                  a.lb, std::ref(lay), a.links, a.head_lse, a.B, a.L, a.K);
+        return lw_start<G, 3>(lw_fwd_kernel<G, 3>, 1, a, parts, st, di, who, lay, a.content, a.log_gates, a.mk,
                               a.span, a.lb, std::ref(lay), a.links, a.head_lse, a.B, a.L, a.K);
     }
     if (a.K * G <= 4 * kLwRows * 32)
@@ -1288,7 +1324,8 @@ int dat_links_from_heads_biased(const float *content, const float *log_gates, co
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const LinksMask mk{bound_end, nonpad};
     const LinksBias lb{bias_table, buckets, num_buckets, status};
-    if (nonpad && lw_fits(translen, heads, num_buckets, di)) {
+    const bool after = nonpad && lw_fits(translen, heads, num_buckets, di);
+    if (after) {
         lw_span_kernel<<<(unsigned)bsz, 128, 0, st>>>(nonpad, reinterpret_cast<int2 *>(spans), prelen);
         if (int rc = check_launch(who)) return rc;
     }
@@ -1301,6 +1338,7 @@ int dat_links_from_heads_biased(const float *content, const float *log_gates, co
         a.span = const_cast<int2 *>(reinterpret_cast<const int2 *>(spans));
         a.links = links;
         a.head_lse = head_lse;
+        a.after = after;
         a.B = bsz;
         a.L = prelen;
         a.K = translen;
@@ -1354,16 +1392,16 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
         int grid;
         if (int rc = lb_run(a, heads, true, grid, st, di, who)) return rc;
         if (!grad_bias_table) return DAT_OK;
-        lb_sum_kernel<<<sgrid, kSum, 0, st>>>(a.part, sums, grid, KH);
+        launch_after(lb_sum_kernel, sgrid, kSum, 0, st, 1, a.part, sums, grid, KH);
     } else {
         if (int rc = links_bwd_rows<true>(grad_links, content, log_gates, links, head_lse, mk, lb, grad_content,
                                           grad_log_gates, bsz, prelen, heads, translen, st, di, who))
             return rc;
         if (!grad_bias_table) return DAT_OK;
-        lb_diag_kernel<<<sgrid, kSum, 0, st>>>(grad_content, sums, bsz, prelen, heads, translen);
+        launch_after(lb_diag_kernel, sgrid, kSum, 0, st, 1, grad_content, sums, bsz, prelen, heads, translen);
     }
     if (int rc = check_launch(who)) return rc;
-    lb_join_kernel<<<(unsigned)num_buckets, kLbJoinThreads, 0, st>>>(sums, buckets, grad_bias_table, heads, translen);
+    launch_after(lb_join_kernel, (unsigned)num_buckets, kLbJoinThreads, 0, st, 1, sums, buckets, grad_bias_table, heads, translen);
     return check_launch(who);
 }
 

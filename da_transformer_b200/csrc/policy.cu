@@ -71,6 +71,7 @@ policy_prep_kernel(const unsigned char *__restrict__ mask, int64_t rows, PolicyH
     __shared__ long long part[32];
     const int tid = threadIdx.x;
     long long n = 0;
+    pdl_trigger();
     if (mask)
         for (int64_t r = tid; r < rows; r += 1024) n += mask[r] != 0;
     for (int c = tid; c < chunks; c += 1024) done[c] = 0;
@@ -731,6 +732,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
         }
         asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
     } else if (warp == 2 * kWarps + 2) {   // ---- numbers
+        pdl_wait();   // the count of the active rows
         const double inv_n = a.head->inv_n;
         const float n1 = (float)inv_n, up = a.head->scale;
         PolicyWalk walk(a.mask, a.rows, ranks, false);
@@ -1012,6 +1014,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
     if (stalled && lane == 0 && a.status) atomicOr(a.status, DAT_STATUS_STALLED);
     // the last CTA adds the CTAs' sums in their order
     __shared__ int last_s;
+    pdl_wait();
     __syncthreads();
     if (tid == 0) {
         __threadfence();
@@ -1122,17 +1125,7 @@ static int policy_ring_launch(const PolicyArgs &a, const PolicyRing &ring, int s
     if (n > kPoMaxCtas) n = kPoMaxCtas;
     if (cudaFuncSetAttribute(policy_ring_kernel<T, kRef, NT, kPpVecs>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return check_launch(who);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3((unsigned)n * ring.ranks);
-    cfg.blockDim = dim3(2 * NT + 96);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim = {(unsigned)ring.ranks, 1, 1};
-    cfg.attrs = at;
-    cfg.numAttrs = ring.ranks > 1 ? 1 : 0;
-    cudaLaunchKernelEx(&cfg, policy_ring_kernel<T, kRef, NT, kPpVecs>, a, ring);
+    launch_after(policy_ring_kernel<T, kRef, NT, kPpVecs>, (unsigned)n * ring.ranks, 2 * NT + 96, smem, st, ring.ranks, a, ring);
     return check_launch(who);
 }
 
