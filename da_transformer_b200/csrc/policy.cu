@@ -548,14 +548,14 @@ template <bool kRef>
 struct PolicyAcc {
     F2 s = 0, t = 0, sy = 0;   // (0, 0)
     template <bool kCareful, int N>
-    __device__ __forceinline__ void add(const F2 (&x)[N], const F2 (&y)[N], F2 minus_r, F2 minus_ry) {
+    __device__ __forceinline__ void add(const F2 (&x)[N], const F2 (&y)[N]) {
         const F2 l2e = f2(kLog2e, kLog2e), neg = f2(-1.f, -1.f);
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const F2 a = f2_add(x[i], minus_r), e = f2_ex2(f2_mul(a, l2e));
+            const F2 a = x[i], e = f2_ex2(f2_mul(a, l2e));
             s = f2_add(s, e);
             if (kRef) {
-                const F2 b = f2_add(y[i], minus_ry);
+                const F2 b = y[i];
                 F2 d = f2_fma(b, neg, a);
                 if (kCareful) d = f2_floor(d);
                 t = f2_fma(e, d, t);
@@ -579,22 +579,28 @@ struct PolicyAcc {
     }
 };
 
-// 16 bytes of logits as pairs
-__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[2], const float *) {
-    p[0] = f2(__uint_as_float(u.x), __uint_as_float(u.y));
-    p[1] = f2(__uint_as_float(u.z), __uint_as_float(u.w));
+// 16 bytes of logits less a reference, as pairs (sm_100 subtracts an fp32 number from a 16-bit one in one instruction,
+// rounded once)
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[2], float r, const float *) {
+    p[0] = f2_add(f2(__uint_as_float(u.x), __uint_as_float(u.y)), f2(-r, -r));
+    p[1] = f2_add(f2(__uint_as_float(u.z), __uint_as_float(u.w)), f2(-r, -r));
 }
-__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], const __nv_bfloat16 *) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) p[i] = f2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
-}
-__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], const __half *) {
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], float r, const __nv_bfloat16 *) {
     const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const float2 v = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        p[i] = f2(v.x, v.y);
+        float a, b;
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.bf16 %0, l, %3;\n\tsub.rn.f32.bf16 %1, h, %3;\n\t}" : "=f"(a), "=f"(b) : "r"(w[i]), "f"(r));
+        p[i] = f2(a, b);
+    }
+}
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], float r, const __half *) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a, b;
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %3;\n\t}" : "=f"(a), "=f"(b) : "r"(w[i]), "f"(r));
+        p[i] = f2(a, b);
     }
 }
 
@@ -602,14 +608,14 @@ __device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], const _
 template <bool kRef, bool kCareful, int N>
 __device__ __forceinline__ void policy_grad_pairs(const PolicyRow &p, const F2 (&x)[N], const F2 (&y)[N], float (&out)[2 * N]) {
     const float base = kRef ? fmaf(-p.w, p.mean, p.a) : p.a;
-    const F2 l2e = f2(kLog2e, kLog2e), neg = f2(-1.f, -1.f), mr = f2(-p.r, -p.r), mry = f2(-p.ry, -p.ry), w = f2(p.w, p.w),
+    const F2 l2e = f2(kLog2e, kLog2e), neg = f2(-1.f, -1.f), w = f2(p.w, p.w),
              bb = f2(base, base);
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const F2 a = f2_add(x[i], mr), e = f2_ex2(f2_mul(a, l2e));
+        const F2 a = x[i], e = f2_ex2(f2_mul(a, l2e));
         F2 k = bb;
         if (kRef) {
-            F2 d = f2_fma(f2_add(y[i], mry), neg, a);
+            F2 d = f2_fma(y[i], neg, a);
             if (kCareful) d = f2_floor(d);
             k = f2_fma(d, w, bb);
         }
@@ -675,9 +681,10 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
     if (ranks > 1) cluster_barrier();   // every CTA's barriers stand before a neighbour's sums arrive on them
     bool stalled = false;
     const uint4 *const xs = reinterpret_cast<const uint4 *>(posm + ring.x), *const ys = reinterpret_cast<const uint4 *>(posm + ring.y);
-    const auto load = [&](int v, F2 (&px)[kVec / 2], F2 (&py)[kVec / 2]) {   // v: piece of the ring
-        policy_pairs(xs[v], px, static_cast<const T *>(nullptr));
-        if (kRef) policy_pairs(ys[v], py, static_cast<const T *>(nullptr));
+    // x - r and y - ry of a piece of the ring
+    const auto load = [&](int v, float r, float ry, F2 (&px)[kVec / 2], F2 (&py)[kVec / 2]) {
+        policy_pairs(xs[v], px, r, static_cast<const T *>(nullptr));
+        if (kRef) policy_pairs(ys[v], py, ry, static_cast<const T *>(nullptr));
     };
     const auto polls = [&] { return stalled ? 1 : kPpPolls; };
     PolicyTurn turn;
@@ -849,7 +856,6 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
             const T tx_raw = x[extra ? te : 0], ty_raw = kRef ? y[extra ? te : 0] : tx_raw;
             const int first = turn.slot;
             float r = Elem<T>::to_float(xt), ry = kRef ? Elem<T>::to_float(yt) : 0.f;
-            F2 mr = f2(-r, -r), mry = f2(-ry, -ry);
             PolicyAcc<kRef> acc;
             const auto sum = [&](auto care) {
                 for (int j = 0; j < ring.chunks; j++, turn.next(ring.slots)) {
@@ -859,15 +865,15 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
 #pragma unroll
                         for (int q = 0; q < kPpVecs; q++) {
                             F2 px[kVec / 2], py[kVec / 2];
-                            load(v + q * NT, px, py);
-                            acc.template add<decltype(care)::value>(px, py, mr, mry);
+                            load(v + q * NT, r, ry, px, py);
+                            acc.template add<decltype(care)::value>(px, py);
                         }
                     } else {
                         for (int q = 0; q < kPpVecs; q++)
                             if (tid + q * NT < left) {
                                 F2 px[kVec / 2], py[kVec / 2];
-                                load(v + q * NT, px, py);
-                                acc.template add<decltype(care)::value>(px, py, mr, mry);
+                                load(v + q * NT, r, ry, px, py);
+                                acc.template add<decltype(care)::value>(px, py);
                             }
                     }
                 }
@@ -904,12 +910,13 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                         for (int q = 0; q < kPpVecs; q++)
                             if ((j * ranks + rank) * kChunk + tid + q * NT < sp.vecs) {
                                 F2 px[kVec / 2], py[kVec / 2];
-                                load(at * kChunk + tid + q * NT, px, py);
+                                load(at * kChunk + tid + q * NT, r, ry, px, py);
                                 f(px, py);
                             }
                         if (++at == ring.slots) at = 0;
                     }
                 };
+                r = ry = 0.f;   // the logits themselves
                 float m = -INFINITY, my = -INFINITY;
                 again([&](const F2 (&px)[kVec / 2], const F2 (&py)[kVec / 2]) {
 #pragma unroll
@@ -938,10 +945,8 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 // nothing but -inf in this CTA's share: any reference gives the sum 0
                 r = r > -INFINITY ? r : 0.f;
                 ry = ry > -INFINITY ? ry : 0.f;
-                mr = f2(-r, -r);
-                mry = f2(-ry, -ry);
                 acc = PolicyAcc<kRef>();
-                again([&](const F2 (&px)[kVec / 2], const F2 (&py)[kVec / 2]) { acc.template add<kRef>(px, py, mr, mry); });
+                again([&](const F2 (&px)[kVec / 2], const F2 (&py)[kVec / 2]) { acc.template add<kRef>(px, py); });
                 if (extra) acc.add1(tx, ty, r, ry);
                 sync();
                 reduce(slot);
@@ -975,7 +980,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 const auto store = [&](auto care, int q) {
                     F2 px[kVec / 2], py[kVec / 2];
                     float out[kVec];
-                    load(v + q * NT, px, py);
+                    load(v + q * NT, p.r, p.ry, px, py);
                     policy_grad_pairs<kRef, decltype(care)::value>(p, px, py, out);
                     gv[to + q * NT] = Elem<T>::pack(out);
                 };
@@ -1137,8 +1142,8 @@ static int policy_fwd_t(const PolicyArgs &a, const DeviceInfo &di, cudaStream_t 
     // 1308 against 1390 us, 1623 with one), a ring without a spare chunk lets the halves wait for each other.
     // Fewer rows than SMs: more CTAs to a row, as long as each has a chunk of it.
     if (a.vec && (int64_t)a.V * sizeof(T) >= 8192) {
-        PolicyRing ring, more;
-        int smem, smem2;
+        PolicyRing ring{}, more{};
+        int smem = 0, smem2 = 0;
         const bool ref = a.y != nullptr;
         const auto spread = [&](int nt, int vecs, int per_sm) {
             while (ring.ranks < kPpRanks && a.rows * ring.ranks * 2 <= di.sm_count && ring.chunks > 1 &&
