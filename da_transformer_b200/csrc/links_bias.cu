@@ -431,7 +431,7 @@ struct LwInt {
     static constexpr int value = N;
 };
 constexpr int kLwPolls = 1 << 20;   // bound of a wait for a copy (never reached)
-constexpr uint32_t kLwFull = 0x7fc00d1eu;   // weight of a distance whose gradient is in the buffer already (no result of arithmetic)
+constexpr uint32_t kLwFull = 0x7fc00d1eu;   // weight of a distance whose shares are taken in full (no result of arithmetic)
 
 // span[b] = (last vertex that the mask allows, whether one between the first and it is not allowed); vertex 0 is
 // nobody's successor
@@ -675,6 +675,17 @@ __device__ __noinline__ float lw_tiny_link(float a0, float a1, float a2, float a
     return m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
 }
 
+// G_d p_h of a distance whose sum over the heads the 32-bit exponent has flushed: relative to its largest term (t, g2 in
+// log2 units).  A link of -inf has no share, whatever its gradient is.
+template <int G>
+__device__ __noinline__ float4 lw_full_share(float4 t, const float (&g2)[4], float gd) {
+    const float a[4] = {t.x + g2[0], t.y + g2[1], t.z + g2[2], t.w + g2[3]};
+    const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]))), mm = m > -INFINITY ? m : 0.f;
+    const float4 p = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
+    const float tot = lb_over_heads<G>((p.x + p.y) + (p.z + p.w)), k = gd / tot;
+    return tot > 0.f ? make_float4(p.x * k, p.y * k, p.z * k, p.w * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+}
+
 // What both kernels begin with: table, barriers, zeros.
 template <int G, int NT>
 __device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, const LinksBias &lb, int K) {
@@ -912,6 +923,8 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         const LwRow r2 = lw_row(walk, B, L, mk, span);
         const int nvec = r0.nj * G;
         float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at + s0.window);
+        const float4 *const src = reinterpret_cast<const float4 *>(content + (r0.row * L + r0.i + 1) * (int64_t)H);
+        const unsigned char *const np = r0.holes ? mk.nonpad + r0.row + 1 : nullptr;
         float *const weight = reinterpret_cast<float *>(ring + s0.at) + s0.skip;   // G_d, then w_d
         if (r0.holes) {
             lw_punch<G>(r0, buf, mk);
@@ -953,26 +966,16 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             if (__any_sync(0xffffffffu, least < kLbTiny)) {
 #pragma unroll
                 for (int u = 0; u < N; u++) {
-                    const bool in = !kPart || v + 32 * u < nvec;
                     const float tot = lb_over_heads<G>((q[u].x + q[u].y) + (q[u].z + q[u].w));
-                    const float a[4] = {t[u].x + g2[0], t[u].y + g2[1], t[u].z + g2[2], t[u].w + g2[3]};
-                    const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
                     const bool tiny = !(tot >= kLbTiny);   // the same in all lanes of a distance
-                    const float mm = m > -INFINITY ? m : 0.f;
-                    float4 p = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
-                    const float tot2 = lb_over_heads<G>((p.x + p.y) + (p.z + p.w));
+                    const float4 p = lw_full_share<G>(t[u], g2, w[u]);
                     if (tiny) {
-                        // p G in full where soft has lost it; soft S_h of such a place is below 2^-80 S_h and is
-                        // dropped: the second pass finds the mark and the product in the buffer
-                        const float k = tot2 > 0.f ? w[u] / tot2 : 0.f;   // a link of -inf: whatever its gradient is
-                        p = tot2 > 0.f ? make_float4(p.x * k, p.y * k, p.z * k, p.w * k) : make_float4(0.f, 0.f, 0.f, 0.f);
-                        if (in) buf[v + 32 * u] = p;
                         S[0] += p.x;
                         S[1] += p.y;
                         S[2] += p.z;
                         S[3] += p.w;
                         q[u] = make_float4(0.f, 0.f, 0.f, 0.f);
-                        w[u] = __uint_as_float(kLwFull);
+                        w[u] = __uint_as_float(kLwFull);   // the second pass takes the share in full again
                     }
                 }
             }
@@ -1011,14 +1014,34 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
                     w[u] = weight[x / G];
                 }
                 if (kPart) __syncwarp();   // the last vector is read by lanes that do not own it
+bool full = false;
 #pragma unroll
-                for (int u = 0; u < N; u++) {
-                    float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
-                    ffma2_rn(k.x, k.y, eg[0], eg[1], w[u], w[u]);
-                    ffma2_rn(k.z, k.w, eg[2], eg[3], w[u], w[u]);
-                    fmul2_rn(o[u].x, o[u].y, o[u].x, o[u].y, k.x, k.y);
-                    fmul2_rn(o[u].z, o[u].w, o[u].z, o[u].w, k.z, k.w);
-                    if ((!kPart || v + 32 * u < nvec) && __float_as_uint(w[u]) != kLwFull) buf[v + 32 * u] = o[u];
+                for (int u = 0; u < N; u++) full |= __float_as_uint(w[u]) == kLwFull;
+                if (__any_sync(0xffffffffu, full)) {   // see the first pass
+                    for (int u = 0; u < N; u++) {
+                        const int x = min(v + 32 * u, nvec - 1);
+                        const bool dead = np && !np[x / G];
+                        const float4 t = dead ? lb_ninf4() : lb_shifted(__ldg(src + x), lw_bias<G>(table, bucket, x), ls);
+                        const float4 p = lw_full_share<G>(t, g2, __ldg(grad_links + r0.row * (int64_t)K + x / G));
+                        float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
+                        if (__float_as_uint(w[u]) == kLwFull) {
+                            k = make_float4(fmaf(k.x, o[u].x, p.x), fmaf(k.y, o[u].y, p.y), fmaf(k.z, o[u].z, p.z), fmaf(k.w, o[u].w, p.w));
+                        } else {
+                            k = make_float4(o[u].x * fmaf(eg[0], w[u], k.x), o[u].y * fmaf(eg[1], w[u], k.y),
+                                            o[u].z * fmaf(eg[2], w[u], k.z), o[u].w * fmaf(eg[3], w[u], k.w));
+                        }
+                        if (v + 32 * u < nvec) buf[v + 32 * u] = k;
+                    }
+                } else {
+#pragma unroll
+                    for (int u = 0; u < N; u++) {
+                        float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
+                        ffma2_rn(k.x, k.y, eg[0], eg[1], w[u], w[u]);
+                        ffma2_rn(k.z, k.w, eg[2], eg[3], w[u], w[u]);
+                        fmul2_rn(o[u].x, o[u].y, o[u].x, o[u].y, k.x, k.y);
+                        fmul2_rn(o[u].z, o[u].w, o[u].z, o[u].w, k.z, k.w);
+                        if (!kPart || v + 32 * u < nvec) buf[v + 32 * u] = o[u];
+                    }
                 }
             });
             umma::fence_smem_to_async();

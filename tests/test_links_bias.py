@@ -132,7 +132,8 @@ def test_refusals_come_before_any_device_work():
 
 # ------------------------------------------------------------------------------------------------ GPU
 
-SHAPES = [(1, 2, 1, 1), (2, 5, 8, 4), (3, 33, 8, 32), (2, 64, 4, 63), (2, 70, 16, 20), (1, 40, 32, 39), (3, 37, 6, 36),
+SHAPES = [(2, 400, 8, 399), (1, 514, 8, 512), (1, 513, 8, 512), (1, 1026, 4, 1025), (1, 1025, 4, 1024), (3, 140, 32, 128),
+          (2, 131, 32, 130), (7, 4, 4, 3), (150, 5, 8, 4), (9, 61, 16, 60), (1, 2, 1, 1), (2, 5, 8, 4), (3, 33, 8, 32), (2, 64, 4, 63), (2, 70, 16, 20), (1, 40, 32, 39), (3, 37, 6, 36),
           (2, 50, 3, 7), (1, 129, 12, 128), (2, 300, 8, 299), (1, 520, 4, 519), (1, 600, 16, 450), (2, 30, 128, 29),
           (5, 18, 2, 1), (1, 9, 5, 8), (1, 260, 32, 259), (1, 1100, 4, 1099)]
 
@@ -152,6 +153,96 @@ def test_against_64_bits_without_mask_and_with_bound(B, L, H, K):
     gen = torch.Generator().manual_seed(1)
     bound = torch.randint(-1, L + 3, (B, L), generator=gen).to(DEV)   # also past the graph and before the vertex
     check(content, gates, table, grad, bk, K, bound_end=bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,L,K", [(8, 90, 89), (4, 200, 60), (16, 65, 64), (3, 40, 39), (8, 700, 699)])
+def test_masks_with_holes(H, L, K):
+    """Padding inside a sentence and before it, a sentence without a vertex, one with a single one."""
+    B = 6
+    content, gates, table, grad, bk, _ = make(B, L, H, K, seed=H * L)
+    gen = torch.Generator().manual_seed(7)
+    mask = torch.rand(B, L, generator=gen) < 0.6
+    mask[1, :L // 2] = False
+    mask[2] = False
+    mask[3] = False
+    mask[3, L - 2] = True
+    mask[4] = True
+    mask[4, 1] = False            # the nearest successor of vertex 0 alone
+    for form in (mask.to(DEV), mask.to(DEV).to(torch.uint8) * 5):
+        check(content, gates, table, grad, bk, K, nonpad_mask=form)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,L", [(8, 50), (6, 50), (16, 40), (8, 600)])
+@pytest.mark.parametrize("scale", [30.0, 200.0])
+def test_scores_far_apart(H, L, scale):
+    """Scores hundreds apart: the nearest successor's is far below the largest, and links reach -1000, which 32-bit
+    probabilities do not.  Against the log-domain oracle; the values are rounded where scores and bias are added
+    (2^-24 of the score) and where the exponent is taken apart, a few 2^-24 of 1500."""
+    K = L - 1
+    content, gates, table, grad, bk, nonpad = make(2, L, H, K, seed=3)
+    content = content * scale
+    leaves = [t.detach().clone().requires_grad_() for t in (content, gates, table)]
+    links = dat.dag_links_from_heads(leaves[0], leaves[1], nonpad_mask=nonpad, relative_bias=leaves[2], relative_buckets=bk)
+    got = torch.autograd.grad(links, leaves, grad)
+    want = oracle(content, gates, table, bk, K, nonpad_mask=nonpad, grad=grad)
+    fin = np.isfinite(want[0])
+    a = links.detach().cpu().numpy()
+    assert np.array_equal(np.isfinite(a), fin)
+    top = float(content.abs().max()) * 1.5
+    assert np.abs(a[fin] - want[0][fin]).max() <= 8 * 2.0 ** -24 * top + 2e-6
+    # a probability off by as much as its logarithm
+    for name, u, v in zip(("content", "gates"), got, want[1:3]):
+        assert np.abs(u.cpu().numpy() - v).max() <= 3 * 8 * 2.0 ** -24 * top * float(grad.abs().max()) + 4e-6, name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,L", [(8, 60), (4, 33), (16, 50), (5, 40), (8, 640)])
+def test_gates_far_apart(H, L):
+    """Heads that a vertex all but never takes (gates of -70 to -300) are the only ones to reach some successors: there
+    their share is 1 however small their probability, and what they lose through the softmax is as large."""
+    K = L - 1
+    content, gates, table, grad, bk, nonpad = make(2, L, H, K, seed=L)
+    gates[:, ::2, 1] = -70
+    gates[:, ::3, 2] = -300
+    content[:, :, 3::4] -= 500                  # no head reaches these ...
+    content[:, :, 3::4, 1:3] += 500             # ... but the rare ones
+    leaves = [t.detach().clone().requires_grad_() for t in (content, gates, table)]
+    links = dat.dag_links_from_heads(leaves[0], leaves[1], nonpad_mask=nonpad, relative_bias=leaves[2], relative_buckets=bk)
+    got = torch.autograd.grad(links, leaves, grad)
+    want = oracle(content, gates, table, bk, K, nonpad_mask=nonpad, grad=grad)
+    fin = np.isfinite(want[0])
+    a = links.detach().cpu().numpy()
+    # a score of 500 is rounded by 2^-24 of it, a few times over
+    assert np.abs(a[fin] - want[0][fin]).max() <= 8 * 2.0 ** -24 * 800
+    for name, u, v in zip(("content", "gates"), got, want[1:3]):
+        top = np.abs(v).max()
+        assert np.abs(u.cpu().numpy() - v).max() <= 3 * 8 * 2.0 ** -24 * 800 * max(top, float(grad.abs().max())), name
+
+
+@pytest.mark.gpu
+def test_large_tables_take_the_other_kernels():
+    """A table that does not fit beside the rows (more than 2048 numbers)."""
+    content, gates, table, grad, _, nonpad = make(2, 40, 8, 39, buckets=300, seed=5)
+    gen = torch.Generator().manual_seed(3)
+    bk = torch.randint(0, 300, (39,), generator=gen).to(DEV)
+    check(content, gates, table, grad, bk, 39, nonpad_mask=nonpad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [37, 38, 39])
+def test_band_gradient_on_any_address(K):
+    """The band's gradient is copied in 16-byte pieces: rows that start anywhere, and a tensor that does."""
+    content, gates, table, grad, bk, nonpad = make(5, 40, 8, K, seed=K)
+    want = check(content, gates, table, grad, bk, K, nonpad_mask=nonpad)[1]
+    for shift in (1, 2, 3):
+        moved = torch.empty(grad.numel() + shift, device=DEV)[shift:].view(grad.shape).copy_(grad)
+        leaves = [t.detach().clone().requires_grad_() for t in (content, gates, table)]
+        links = dat.dag_links_from_heads(leaves[0], leaves[1], nonpad_mask=nonpad, max_transition_length=K,
+                                         relative_bias=leaves[2], relative_buckets=bk)
+        for a, b in zip(torch.autograd.grad(links, leaves, moved), want):
+            assert torch.equal(a, b)
 
 
 @pytest.mark.gpu

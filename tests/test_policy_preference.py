@@ -195,7 +195,7 @@ def test_entry_points_refuse_bad_arguments():
 
 # ------------------------------------------------------------------------------------------------ GPU: policy
 
-SIZES = [(1, 1, 1), (1, 1, 2), (2, 3, 7), (1, 2, 255), (3, 5, 1000), (2, 130, 513), (1, 4, 4099), (1, 3, 32000), (2, 2, 30523),
+SIZES = [(1, 20, 9001), (40, 5, 8192), (1, 2, 128000), (2, 90, 20011), (1, 1, 1), (1, 1, 2), (2, 3, 7), (1, 2, 255), (3, 5, 1000), (2, 130, 513), (1, 4, 4099), (1, 3, 32000), (2, 2, 30523),
          (5, 60, 64), (1, 2, 64001)]
 
 
@@ -212,10 +212,11 @@ def test_policy_against_64_bits(B, L, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [777, 9001])
 @pytest.mark.parametrize("ref", [None, "estimate", "full"])
-def test_policy_scales_of_the_loss(ref):
+def test_policy_scales_of_the_loss(ref, V):
     """Whatever gradient reaches the loss, expected or not, the logits' gradient is rounded once."""
-    x, kw = policy_inputs(2, 9, 777, torch.float16, seed=4, link=True, ref=ref, mask=0.7)
+    x, kw = policy_inputs(2, 9, V, torch.float16, seed=4, link=True, ref=ref, mask=0.7)
     base = policy_oracle(x, kl_coef=0.1, **kw)
     for expected, scale in ((1.0, None), (1.0, 1024.0), (1024.0, 1024.0), (None, 1.0), (None, 1024.0), (2.0, None),
                             (torch.tensor(1024.0, device=DEV), 1024.0), (torch.tensor([8.0], device=DEV), 0.5)):
@@ -249,9 +250,106 @@ def test_policy_second_backward_has_its_own_buffer():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [700, 9001, 40000])
+@pytest.mark.parametrize("ref", [None, "full"])
+def test_policy_logits_far_apart(V, ref):
+    """The token's logit 200 below the largest in both models (a ratio of probabilities that 32 bits do not hold), a
+    row of which a single logit carries all, and logits of +-1e4."""
+    x, kw = policy_inputs(2, 6, V, torch.float32, seed=V, ref=ref)
+    b, l = torch.arange(2, device=DEV).view(2, 1), torch.arange(6, device=DEV).view(1, 6)
+    tok = kw["tokens"]
+    x[b, l, (tok + 1) % V] += torch.tensor([0., 60., 100., 200., 1000., 1e4], device=DEV)
+    x[1, 5] *= 100
+    if ref:
+        kw["ref_logits"] = x * 0.9 + 0.5 * torch.randn(2, 6, V, generator=torch.Generator().manual_seed(1)).to(DEV)
+    lp = torch.log_softmax(x.double(), -1).gather(-1, tok.unsqueeze(-1)).squeeze(-1)
+    kw["old"] = (lp - 0.05).float()
+    got = run_policy(x, kw, kl_coef=0.1)
+    want = policy_oracle(x, kl_coef=0.1, **kw)
+    # log-probabilities near -1e4 carry 5e-4 in 32 bits, and the ratio with them; the gradient is as far off as the
+    # ratio, and the exponents of the logits that count are below 16
+    a, w = got[1].cpu().numpy().astype(np.float64), want[1]
+    tol = row_tolerance(V) + 4 * U * np.abs(w)
+    assert (np.abs(a - w) <= tol).all()
+    d = d_range(x, kw)
+    assert (np.abs(got[2].cpu().numpy() - want[2]) <= 4 * row_tolerance(V) * (1 + d)).all()
+    off = np.abs(got[4].cpu().numpy() - want[4])
+    assert (off <= (3 * tol.max() + 4 * row_tolerance(V) * (1 + d)) / 12 * 3).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V", [9001, 33000, 70001])
+def test_policy_forbidden_tokens_in_long_rows(V, dtype):
+    """-inf in both models, in every row and in the first rows only; a reference that has them alone; a token that is
+    forbidden itself (its log-probability is -inf, and no number of its row but the loss's is asked for)."""
+    x, kw = policy_inputs(1, 12, V, dtype, seed=V, ref="full", link=True)
+    gen = torch.Generator().manual_seed(2)
+    ban = (torch.rand(V, generator=gen) < 0.2).to(DEV)
+    ban[kw["tokens"].unique()] = False
+    for rows in (slice(0, 12), slice(0, 3), slice(7, 8)):
+        xx, k = x.clone(), {n: t.clone() for n, t in kw.items()}
+        xx[:, rows, ban] = NEG_INF
+        k["ref_logits"][:, rows, ban] = NEG_INF
+        lp = torch.log_softmax(xx.double(), -1).gather(-1, k["tokens"].unsqueeze(-1)).squeeze(-1) + k["link"].double()
+        k["old"] = (lp - 0.1).float()
+        got = run_policy(xx, k, kl_coef=0.2)
+        check_policy(got, policy_oracle(xx, kl_coef=0.2, **k), dtype, V, k, kl_coef=0.2, d_max=d_range(xx, k))
+    # every second logit of the policy forbidden, the reference free: finite
+    xx = x.clone()
+    keep = torch.zeros(V, dtype=torch.bool, device=DEV)
+    keep[::2] = True
+    keep[kw["tokens"].unique()] = True
+    xx[..., ~keep] = NEG_INF
+    lp = torch.log_softmax(xx.double(), -1).gather(-1, kw["tokens"].unsqueeze(-1)).squeeze(-1) + kw["link"].double()
+    k = {**kw, "old": (lp - 0.1).float()}
+    check_policy(run_policy(xx, k, kl_coef=0.2), policy_oracle(xx, kl_coef=0.2, **k), dtype, V, k, kl_coef=0.2,
+                 d_max=d_range(xx, k))
+    # the token itself forbidden
+    xx = x.clone()
+    xx[0, 4, kw["tokens"][0, 4]] = NEG_INF
+    loss, logp, kl, stats, gx, gl = run_policy(xx, {**kw, "old": kw["old"].clone()}, kl_coef=0.2)
+    assert float(logp[0, 4]) == NEG_INF and logp[0, 5:].isfinite().all() and logp[0, :4].isfinite().all()
+    rest = [n for n in range(12) if n != 4]
+    want = policy_oracle(x, kl_coef=0.2, **kw)
+    assert_rel(logp[0, rest].cpu().numpy(), want[1][0, rest], 1e-5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("V", [5000, 9003, 30000, 64000])
+def test_policy_rows_of_a_long_batch(V, dtype):
+    """More rows than CTAs, a mask that leaves some CTAs nothing, every kind of KL: each row by itself as in a call
+    of its own rows (one thread's order of sums apart)."""
+    B, L = 3, 200
+    for ref in (None, "estimate", "full"):
+        x, kw = policy_inputs(B, L, V, dtype, seed=V, ref=ref, mask=0.3)
+        kw["mask"][1] = False
+        got = run_policy(x, kw, kl_coef=0.1)
+        rows = kw["mask"].nonzero()[::7]
+        pick = lambda t: t[rows[:, 0], rows[:, 1]].unsqueeze(0).contiguous()  # noqa: E731
+        small = {n: pick(t) for n, t in kw.items() if n != "mask"}
+        want = policy_oracle(pick(x), kl_coef=0.1, **small)
+        share = len(rows) / int(kw["mask"].sum())       # the mean is over more rows here
+        sub = (got[0], pick(got[1]), pick(got[2]), got[3], pick(got[4]), None)
+        tol = row_tolerance(V)
+        assert (np.abs(sub[1].cpu().numpy() - want[1]) <= tol + 2 * U * np.abs(want[1])).all()
+        g, w = sub[4].float().cpu().numpy(), want[4] * share
+        if dtype == torch.float32:
+            assert_rel(g, w, 1e-4)
+        else:
+            assert_rel_quantized(g, w, 1e-4, str(dtype).split(".")[1])
+        assert not got[4][~kw["mask"]].any() and float(got[3][4]) == int(kw["mask"].sum())
+        again = run_policy(x, kw, kl_coef=0.1)
+        for a, b in zip(got[:5], again[:5]):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [130, 10001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_policy_masked_vertices_may_hold_anything(dtype):
-    x, kw = policy_inputs(3, 90, 130, dtype, seed=7, link=True, ref="full", mask=0.5)
+def test_policy_masked_vertices_may_hold_anything(dtype, V):
+    x, kw = policy_inputs(3, 90, V, dtype, seed=7, link=True, ref="full", mask=0.5)
     want = run_policy(x, kw, kl_coef=0.1)
     off = ~kw["mask"]
     for value in (NAN, float("inf"), NEG_INF, torch.finfo(dtype).min):
@@ -303,9 +401,10 @@ def test_policy_forbidden_tokens_and_shifted_references(dtype):
 
 
 @pytest.mark.gpu
-def test_policy_token_outside_the_vocabulary():
-    x, kw = policy_inputs(2, 3, 40, torch.float32, seed=10)
-    kw["tokens"][0, 1], kw["tokens"][1, 2] = 40, -1
+@pytest.mark.parametrize("V", [40, 9001])
+def test_policy_token_outside_the_vocabulary(V):
+    x, kw = policy_inputs(2, 3, V, torch.float32, seed=10)
+    kw["tokens"][0, 1], kw["tokens"][1, 2] = V, -1
     dat.last_status(DEV)
     loss, logp, _, _, gx, _ = run_policy(x, kw)
     assert dat.last_status(DEV) & 4
@@ -315,7 +414,7 @@ def test_policy_token_outside_the_vocabulary():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
-@pytest.mark.parametrize("V", [64, 333])
+@pytest.mark.parametrize("V", [64, 333, 9001])
 def test_policy_strides_and_alignment(dtype, V):
     x, kw = policy_inputs(3, 4, V, dtype, seed=11, link=True, ref="full", adv_rows=True)
     kw["mask"] = torch.tensor([1, 0, 1, 1], device=DEV, dtype=torch.bool).expand(3, 4)
@@ -393,8 +492,9 @@ def test_policy_many_rows_repeat_and_sum_in_a_fixed_order():
 
 
 @pytest.mark.gpu
-def test_policy_on_streams_and_in_graphs():
-    x, kw = policy_inputs(2, 40, 500, torch.bfloat16, seed=14, link=True, ref="full", mask=0.5)
+@pytest.mark.parametrize("V", [500, 20000])
+def test_policy_on_streams_and_in_graphs(V):
+    x, kw = policy_inputs(2, 40, V, torch.bfloat16, seed=14, link=True, ref="full", mask=0.5)
     want = run_policy(x, kw, kl_coef=0.1)
     side = torch.cuda.Stream(DEV)
     side.wait_stream(torch.cuda.current_stream())
@@ -427,7 +527,7 @@ def test_policy_on_streams_and_in_graphs():
         graph.replay()
         for a, b in zip(out, want):
             assert torch.equal(a, b)
-    other = policy_inputs(2, 40, 500, torch.bfloat16, seed=15, link=True, ref="full", mask=0.5)
+    other = policy_inputs(2, 40, V, torch.bfloat16, seed=15, link=True, ref="full", mask=0.5)
     with torch.no_grad():
         xs.copy_(other[0])
         for n, t in other[1].items():
