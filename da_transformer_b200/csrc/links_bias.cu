@@ -19,8 +19,9 @@
 //   backward  soft = exp(z - lse_h), q_h = soft exp(g_h), p_h = q_h / sum q.
 // Where sum q is below 2^-80 (a link below -55) it is taken again relative to its largest term, so that what
 // the 32-bit exponent flushes stays below 2^-40 of what it is added to.
-// Head counts of 4, 8, 16, 32 and up to 4096 score vectors per vertex; others take the kernels of links.cu (one
-// CTA per vertex, scores in shared memory) and a pass over the gradient's diagonals.
+// Two forms, a warp or a CTA per vertex (below): the first up to 32 heads and rows of 2048 vectors that fit its rings,
+// the second 4, 8, 16 and 32 heads up to 4096 vectors.  What neither takes goes to the kernels of links.cu (one CTA per
+// vertex, scores in shared memory) and a pass over the gradient's diagonals.
 #include <functional>
 
 #include "links_common.cuh"
@@ -419,10 +420,17 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
 // the warp works on the vertex before, the exponentials and then the gradient take the scores' place, and a bulk
 // copy writes the gradient back (the zeros around it come from a block of zeros).  Rows are triangular, so a ring
 // little larger than the longest row holds two ordinary ones.
-// Used where a row has at most kLwMaxVec vectors and the bias table a few KB.
+// A lane holds four heads of a distance, G lanes (a power of two) a distance.  kExact: H = 4 G, so that a row is an array
+// of 16-byte vectors; other head counts up to 32 leave places empty (-inf, no part in anything) and read and write the
+// row's numbers one by one, and where H is no multiple of four a row begins at any address: the copy takes the 16-byte
+// pieces up to its end, the up to three numbers behind them are loaded singly, and the gradient is stored by the lanes.
+// Used where a row has at most kLwMaxVec vectors, fits a ring, and the bias table takes a few KB.
+// Forward and backward, called from Python, against the kernels of links.cu with the pass over the diagonals: 16 graphs of
+// 512 vertices and 12 heads 76 + 147 us against 140 + 515, 32 and 6 heads 79 + 146 against 135 + 740, 64 and 3 heads
+// 77 + 185 against 185 + 1265, 64 and one head 64 + 165 against 166 + 927.
 // ---------------------------------------------------------------------------------------------------
 constexpr int kLwRows = 4;          // vertices of a group, a warp each
-constexpr int kLwMaxVec = 1024;     // score vectors per vertex
+constexpr int kLwMaxVec = 2048;     // score vectors per vertex (places of empty heads included)
 constexpr int kLwMaxTable = 2048;   // floats of the bias table
 constexpr int kLwZeros = 2048;      // bytes of zeros
 constexpr int kLwU = 4;             // vectors of a lane taken together: loads first, then the arithmetic, then the stores
@@ -514,17 +522,54 @@ __device__ __forceinline__ void lw_resolve(LwRow &r, int L, int K, const LinksMa
     r.nj = jhi - r.i > 0 ? jhi - r.i : 0;
 }
 
-// bias of vector v in log2 units, from the table in shared memory (its last row: -inf, for buckets outside)
+// Vector v of a row (distance v / G, heads 4 (v % G) ..) from and to memory; `fill` stands for heads that are not there.
+template <int G, bool kExact>
+__device__ __forceinline__ float4 lw_get(const float *row, int v, int H, float fill) {
+    if (kExact) return reinterpret_cast<const float4 *>(row)[v];
+    const int h = (v & (G - 1)) * 4;
+    const float *p = row + (v / G) * H + h;
+    float4 r = make_float4(fill, fill, fill, fill);
+    if ((H & 3) == 0) {
+        if (h < H) r = *reinterpret_cast<const float4 *>(p);
+    } else {
+        if (h < H) r.x = p[0];
+        if (h + 1 < H) r.y = p[1];
+        if (h + 2 < H) r.z = p[2];
+        if (h + 3 < H) r.w = p[3];
+    }
+    return r;
+}
+template <int G, bool kExact>
+__device__ __forceinline__ void lw_put(float *row, int v, int H, float4 x) {
+    if (kExact) {
+        reinterpret_cast<float4 *>(row)[v] = x;
+        return;
+    }
+    const int h = (v & (G - 1)) * 4;
+    float *p = row + (v / G) * H + h;
+    if ((H & 3) == 0) {
+        if (h < H) *reinterpret_cast<float4 *>(p) = x;
+    } else {
+        if (h < H) p[0] = x.x;
+        if (h + 1 < H) p[1] = x.y;
+        if (h + 2 < H) p[2] = x.z;
+        if (h + 3 < H) p[3] = x.w;
+    }
+}
+
+// bias of vector v in log2 units, from the table in shared memory (rows of 4 G; its last row: -inf, for buckets outside)
 template <int G>
 __device__ __forceinline__ float4 lw_bias(const float4 *table, const unsigned short *bucket, int v) {
     return table[bucket[v / G] * G + (v & (G - 1))];
 }
 template <int G, int NT>
-__device__ __forceinline__ void lw_load_table(const LinksBias &lb, float *table, unsigned short *bucket, int K) {
-    constexpr int H = 4 * G;
+__device__ __forceinline__ void lw_load_table(const LinksBias &lb, float *table, unsigned short *bucket, int H, int K) {
     bool bad = false;
-    for (int x = threadIdx.x; x < lb.n * H; x += NT) table[x] = __ldg(lb.table + x) * kLog2e;
-    for (int x = threadIdx.x; x < H; x += NT) table[lb.n * H + x] = -INFINITY;
+    for (int x = threadIdx.x; x < lb.n * (4 * G); x += NT) {
+        const int k = x / (4 * G), h = x - k * (4 * G);
+        table[x] = h < H ? __ldg(lb.table + k * H + h) * kLog2e : 0.f;
+    }
+    for (int x = threadIdx.x; x < 4 * G; x += NT) table[lb.n * (4 * G) + x] = -INFINITY;
     for (int d = threadIdx.x; d < K; d += NT) {
         const int64_t k = __ldg(lb.bucket + d);
         const bool ok = k >= 0 && k < lb.n;
@@ -541,10 +586,13 @@ struct LwSmem {
 // dynamic shared memory of one CTA per SM (a little is left for what the kernels declare themselves) and of two
 static int lw_one(const DeviceInfo &di) { return di.max_smem_optin - 256; }
 static int lw_two(const DeviceInfo &di) { return (di.max_smem_optin + 1024) / 2 - 1024 - 256; }
-static int lw_row_bytes(int K, int H) { return K * H * 4 + (K + 8) * 4 / 16 * 16; }   // scores and the band's gradient
+// lanes of a distance
+static int lw_lanes(int H) { return H <= 4 ? 1 : H <= 8 ? 2 : H <= 16 ? 4 : 8; }
+// scores and the band's gradient, each with room for a beginning inside a 16-byte piece
+static int lw_row_bytes(int K, int H) { return (K * H + 8) * 4 / 16 * 16 + (K + 8) * 4 / 16 * 16; }
 static LwSmem lw_smem(int K, int H, int n, int warps, int avail) {
     LwSmem m;
-    m.bucket = (n + 1) * H * 4;
+    m.bucket = (n + 1) * (4 * lw_lanes(H)) * 4;
     m.zeros = (m.bucket + K * 2 + 15) / 16 * 16;
     m.mbar = m.zeros + kLwZeros;
     m.rings = m.mbar + (warps * 8 + 15) / 16 * 16;
@@ -561,28 +609,47 @@ __device__ __forceinline__ void lw_bulk_store(void *dst, uint32_t src, uint32_t 
     asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void lw_bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// n zeros from p on: whole 16-byte pieces by the lanes' copies of the block of zeros, those around them (kEdges) singly
+template <bool kEdges>
+__device__ __forceinline__ void lw_zero(float *p, int n, uint32_t zeros) {
+    const int lane = threadIdx.x & 31;
+    if (kEdges) {
+        const int head = min((int)(-(reinterpret_cast<uintptr_t>(p) >> 2) & 3), n), tail = (n - head) & 3;
+        if (lane < head) p[lane] = 0.f;
+        if (lane < tail) p[n - tail + lane] = 0.f;
+        p += head;
+        n -= head + tail;
+    }
+    for (int at = lane * (kLwZeros / 4); at < n; at += 32 * (kLwZeros / 4))
+        lw_bulk_store(p + at, zeros, min(kLwZeros / 4, n - at) * 4);
+}
 // all bulk stores of this thread have read their shared memory
 __device__ __forceinline__ void lw_bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 
-// A row in the ring: [window of the band's gradient (backward)][scores].  The window is the 16-byte pieces of
-// grad_links that lie before the row's end; the up to three values behind them are loaded singly (all of them where
-// grad_links does not start on a 16-byte boundary: wide = false).
+// A row in the ring: [window of the band's gradient (backward)][scores].  A window is the 16-byte pieces of an array
+// that reach up to the row's end; the up to three numbers behind them are loaded singly (all of them where the array
+// does not start on a 16-byte boundary: wide = false).
+__device__ __forceinline__ int lw_skip(int64_t first) { return (int)(first & 3); }   // numbers of the first piece before the row
+__device__ __forceinline__ int lw_whole(int skip, int n, bool wide) {                // numbers of the row that the pieces hold
+    const int to = (skip + n) & ~3;
+    return wide && to > 0 ? to - skip : 0;
+}
 struct LwSlot {
-    int at, bytes;    // place in the ring
-    int window;       // bytes of the window
-    int skip;         // values of the window before the row's first
-    int whole;        // values of the row that the window holds
+    int at, bytes;       // place in the ring
+    int window, skip;    // of the band's gradient: bytes, numbers before the row
+    int front;           // numbers before the row's scores
 };
-template <int G, bool kBackward>
-__device__ __forceinline__ LwSlot lw_slot(const LwRow &r, int K, bool wide) {
+template <int G, bool kExact, bool kBackward>
+__device__ __forceinline__ LwSlot lw_slot(const LwRow &r, int L, int H, int K) {
     LwSlot s{0, 0, 0, 0, 0};
-    if (kBackward && r.nj > 0) {
-        const int64_t first = r.row * (int64_t)K, from = first & ~(int64_t)3, to = (first + r.nj) & ~(int64_t)3;
-        s.skip = (int)(first - from);
-        s.window = (s.skip + r.nj + 3) / 4 * 16;   // room for the single values too
-        s.whole = wide && to > first ? (int)(to - first) : 0;
+    if (r.nj > 0) {
+        if (kBackward) {
+            s.skip = lw_skip(r.row * (int64_t)K);
+            s.window = (s.skip + r.nj + 3) / 4 * 16;
+        }
+        if (!kExact) s.front = lw_skip((r.row * L + r.i + 1) * (int64_t)H);
+        s.bytes = s.window + (kExact ? r.nj * (16 * G) : (s.front + r.nj * H + 3) / 4 * 16);
     }
-    s.bytes = s.window + r.nj * (16 * G);
     return s;
 }
 // the place after `at + bytes` in the ring that keeps clear of [at, at + bytes), or -1
@@ -591,23 +658,31 @@ __device__ __forceinline__ int lw_place(const LwSlot &cur, int need, int ring) {
     return need <= cur.at ? 0 : -1;
 }
 
-// Lane 0: starts the copies of a row into its slot; the other lanes fetch the single values of the window.
-template <int G, bool kBackward>
+// Lane 0: starts the copies of a row into its slot; all lanes fetch the single numbers behind the windows.
+template <int G, bool kExact, bool kBackward>
 __device__ __forceinline__ void lw_issue(const LwRow &r, const LwSlot &s, unsigned char *ring, uint64_t *mbar,
-                                         const float *content, const float *grad_links, int L, int K) {
+                                         const float *content, const float *grad_links, int L, int H, int K, bool wide) {
     if (r.nj <= 0) return;
     const int lane = threadIdx.x & 31;
+    const float *const scores = content + (r.row * L + r.i + 1) * (int64_t)H;
+    const float *const grad = kBackward ? grad_links + r.row * (int64_t)K : nullptr;
+    const int n = r.nj * H, sc_whole = kExact ? n : lw_whole(s.front, n, true);
+    const int grad_whole = kBackward ? lw_whole(s.skip, r.nj, wide) : 0;
     if (lane == 0) {
         const uint32_t mb = umma::smem_u32(mbar), base = umma::smem_u32(ring) + s.at;
-        const uint32_t scores = r.nj * (16 * G);
-        const uint32_t win = kBackward && s.whole > 0 ? (s.skip + s.whole) * 4 : 0;
-        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mb), "r"(scores + win) : "memory");
-        lw_bulk_load(base + s.window, content + (r.row * L + r.i + 1) * (int64_t)(4 * G), scores, mb);
-        if (win) lw_bulk_load(base, grad_links + (r.row * (int64_t)K - s.skip), win, mb);
+        const uint32_t sc = sc_whole > 0 ? (s.front + sc_whole) * 4 : 0;
+        const uint32_t win = kBackward && grad_whole > 0 ? (s.skip + grad_whole) * 4 : 0;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(mb), "r"(sc + win) : "memory");
+        if (sc) lw_bulk_load(base + s.window, scores - s.front, sc, mb);
+        if (win) lw_bulk_load(base, grad - s.skip, win, mb);
     }
     if (kBackward) {
         float *w = reinterpret_cast<float *>(ring + s.at) + s.skip;
-        for (int d = s.whole + lane; d < r.nj; d += 32) w[d] = __ldg(grad_links + r.row * (int64_t)K + d);
+        for (int d = grad_whole + lane; d < r.nj; d += 32) w[d] = __ldg(grad + d);
+    }
+    if (!kExact) {
+        float *w = reinterpret_cast<float *>(ring + s.at + s.window) + s.front;
+        for (int x = sc_whole + lane; x < n; x += 32) w[x] = __ldg(scores + x);
     }
 }
 
@@ -629,11 +704,17 @@ __device__ __forceinline__ void lw_reduce(float (&v)[4]) {
 }
 
 // scores of masked places inside the span to -inf (each lane its own places)
-template <int G>
-__device__ __forceinline__ void lw_punch(const LwRow &r, float4 *buf, const LinksMask &mk) {
+template <int G, bool kExact>
+__device__ __forceinline__ void lw_punch(const LwRow &r, float *buf, int H, const LinksMask &mk) {
     const unsigned char *np = mk.nonpad + r.row + 1;   // b * L + i + 1
     for (int v = threadIdx.x & 31; v < r.nj * G; v += 32)
-        if (!np[v / G]) buf[v] = lb_ninf4();
+        if (!np[v / G]) lw_put<G, kExact>(buf, v, H, lb_ninf4());
+}
+
+// the four heads of lane group g of a row of [.., H], -inf for those that are not there
+template <int G, bool kExact>
+__device__ __forceinline__ float4 lw_heads(const float *p, int64_t row, int H, int g) {
+    return lw_get<G, kExact>(p + row * H, g, H, -INFINITY);
 }
 
 // Runs f(N, partial, v) over a row's vectors: batches of kLwU * 32 without a condition inside, then the rest as one
@@ -650,14 +731,14 @@ __device__ __forceinline__ void lw_batches(int nvec, F f) {
 }
 
 // t = score + bias - r of N vectors, in log2 units (behind the row's end: the last vector's)
-template <int G, int N, bool kPart>
-__device__ __forceinline__ void lw_terms(float4 (&t)[N], const float4 *buf, const float4 *table, const unsigned short *bucket,
-                                         const float (&r)[4], int v, int nvec) {
+template <int G, bool kExact, int N, bool kPart>
+__device__ __forceinline__ void lw_terms(float4 (&t)[N], const float *buf, int H, const float4 *table,
+                                         const unsigned short *bucket, const float (&r)[4], int v, int nvec) {
     float4 c[N], b[N];
 #pragma unroll
     for (int u = 0; u < N; u++) {
         const int x = kPart ? min(v + 32 * u, nvec - 1) : v + 32 * u;
-        c[u] = buf[x];
+        c[u] = lw_get<G, kExact>(buf, x, H, -INFINITY);
         // the head group of the clamped vector is the last one's and may be another: nothing of it is used
         b[u] = lw_bias<G>(table, bucket, x);
     }
@@ -688,8 +769,8 @@ __device__ __noinline__ float4 lw_full_share(float4 t, const float (&g2)[4], flo
 
 // What both kernels begin with: table, barriers, zeros.
 template <int G, int NT>
-__device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, const LinksBias &lb, int K) {
-    lw_load_table<G, NT>(lb, reinterpret_cast<float *>(sm), reinterpret_cast<unsigned short *>(sm + lay.bucket), K);
+__device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, const LinksBias &lb, int H, int K) {
+    lw_load_table<G, NT>(lb, reinterpret_cast<float *>(sm), reinterpret_cast<unsigned short *>(sm + lay.bucket), H, K);
     for (int x = threadIdx.x; x < kLwZeros / 16; x += NT)
         reinterpret_cast<float4 *>(sm + lay.zeros)[x] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (threadIdx.x < NT / 32) umma::mbar_init(reinterpret_cast<uint64_t *>(sm + lay.mbar) + threadIdx.x, 1);
@@ -698,29 +779,29 @@ __device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, c
 }
 
 // NG groups of four vertices at work in a CTA
-template <int G, int NG>
+template <int G, bool kExact, int NG>
 __global__ void __launch_bounds__(NG * kLwRows * 32, NG == 2 ? 2 : 1)
 lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk,
               const int2 *__restrict__ span, LinksBias lb, LwSmem lay, float *__restrict__ links,
-              float *__restrict__ head_lse, int B, int L, int K) {
-    constexpr int H = 4 * G;
+              float *__restrict__ head_lse, int B, int L, int heads, int K) {
+    const int H = kExact ? 4 * G : heads;
     extern __shared__ __align__(16) unsigned char lwsm[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane & (G - 1);
     const float4 *const table = reinterpret_cast<const float4 *>(lwsm);
     const unsigned short *const bucket = reinterpret_cast<const unsigned short *>(lwsm + lay.bucket);
     unsigned char *const ring = lwsm + lay.rings + warp * lay.ring;
     uint64_t *const mbar = reinterpret_cast<uint64_t *>(lwsm + lay.mbar) + warp;
-    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
+    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, H, K);
     pdl_wait();   // the spans
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + warp / kLwRows;
     LwWalk walk(group, step, L);
     LwRow r0 = lw_row(walk, B, L, mk, span), r1 = lw_row(walk, B, L, mk, span);
     lw_resolve(r0, L, K, mk);
-    LwSlot s0 = lw_slot<G, false>(r0, K, false);
-    lw_issue<G, false>(r0, s0, ring, mbar, content, nullptr, L, K);
+    LwSlot s0 = lw_slot<G, kExact, false>(r0, L, H, K);
+    lw_issue<G, kExact, false>(r0, s0, ring, mbar, content, nullptr, L, H, K, false);
     const auto gates_of = [&](const LwRow &r) {
-        return r.exists ? __ldg(reinterpret_cast<const float4 *>(log_gates + r.row * H) + g) : lb_ninf4();
+        return r.exists ? lw_heads<G, kExact>(log_gates, r.row, H, g) : lb_ninf4();
     };
     float4 gate = gates_of(r0);
     uint32_t phase = 0;
@@ -730,28 +811,29 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             stalled |= !umma::mbar_wait(mbar, phase, stalled ? 1 : kLwPolls);
             phase ^= 1;
         }
+        if (!kExact) __syncwarp();   // the numbers that came singly
         // the next row on its way, where the ring has room for it beside this one
         lw_resolve(r1, L, K, mk);
-        LwSlot s1 = lw_slot<G, false>(r1, K, false);
+        LwSlot s1 = lw_slot<G, kExact, false>(r1, L, H, K);
         s1.at = lw_place(s0, s1.bytes, lay.ring);
         const bool later = s1.at < 0;
-        if (!later) lw_issue<G, false>(r1, s1, ring, mbar, content, nullptr, L, K);
+        if (!later) lw_issue<G, kExact, false>(r1, s1, ring, mbar, content, nullptr, L, H, K, false);
         const float4 gate1 = gates_of(r1);
         const LwRow r2 = lw_row(walk, B, L, mk, span);
         if (r0.exists) {
             const int nvec = r0.nj * G;
-            float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at);
-            const float4 *const src = reinterpret_cast<const float4 *>(content + (r0.row * L + r0.i + 1) * (int64_t)H);
+            float *const buf = reinterpret_cast<float *>(ring + s0.at) + s0.front;
+            const float *const src = content + (r0.row * L + r0.i + 1) * (int64_t)H;
             const unsigned char *const np = r0.holes ? mk.nonpad + r0.row + 1 : nullptr;
             if (r0.holes) {
-                lw_punch<G>(r0, buf, mk);
+                lw_punch<G, kExact>(r0, buf, H, mk);
                 __syncwarp();
             }
             // r_h in log2 units
             float r[4] = {0.f, 0.f, 0.f, 0.f}, sum[4] = {0.f, 0.f, 0.f, 0.f};
             bool bad = false;
             if (nvec > 0) {
-                const float4 c = buf[g], b0 = lw_bias<G>(table, bucket, g);
+                const float4 c = lw_get<G, kExact>(buf, g, H, 0.f), b0 = lw_bias<G>(table, bucket, g);
                 r[0] = fmaf(c.x, kLog2e, b0.x);
                 r[1] = fmaf(c.y, kLog2e, b0.y);
                 r[2] = fmaf(c.z, kLog2e, b0.z);
@@ -763,12 +845,12 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 constexpr int N = decltype(n)::value;
                 constexpr bool kPart = decltype(part)::value;
                 float4 t[N];
-                lw_terms<G, N, kPart>(t, buf, table, bucket, r, v, nvec);
+                lw_terms<G, kExact, N, kPart>(t, buf, H, table, bucket, r, v, nvec);
 #pragma unroll
                 for (int u = 0; u < N; u++) {
                     const float4 e = lw_exp2(t[u]);
                     if (!kPart || v + 32 * u < nvec) {
-                        buf[v + 32 * u] = e;
+                        lw_put<G, kExact>(buf, v + 32 * u, H, e);
                         fadd2_rn(sum[0], sum[1], sum[0], sum[1], e.x, e.y);
                         fadd2_rn(sum[2], sum[3], sum[2], sum[3], e.z, e.w);
                     }
@@ -780,7 +862,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 for (int v = lane; v < nvec; v += 32)
                     if (!(np && !np[v / G])) {
-                        const float4 c = __ldg(src + v), t = lw_bias<G>(table, bucket, v);
+                        const float4 c = lw_get<G, kExact>(src, v, H, -INFINITY), t = lw_bias<G>(table, bucket, v);
                         m[0] = fmaxf(m[0], fmaf(c.x, kLog2e, t.x));
                         m[1] = fmaxf(m[1], fmaf(c.y, kLog2e, t.y));
                         m[2] = fmaxf(m[2], fmaf(c.z, kLog2e, t.z));
@@ -794,12 +876,12 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 for (int v = lane; v < nvec; v += 32) {
                     float4 e = make_float4(0.f, 0.f, 0.f, 0.f);
                     if (!(np && !np[v / G])) {
-                        const float4 t = lb_shifted(__ldg(src + v), lw_bias<G>(table, bucket, v), r);
+                        const float4 t = lb_shifted(lw_get<G, kExact>(src, v, H, -INFINITY), lw_bias<G>(table, bucket, v), r);
                         e = make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w));
                         fadd2_rn(sum[0], sum[1], sum[0], sum[1], e.x, e.y);
                         fadd2_rn(sum[2], sum[3], sum[2], sum[3], e.z, e.w);
                     }
-                    buf[v] = e;
+                    lw_put<G, kExact>(buf, v, H, e);
                 }
                 __syncwarp();
             }
@@ -819,7 +901,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 o.y = ls[1] < INFINITY ? (r[1] + ls[1]) * kLn2 : -INFINITY;
                 o.z = ls[2] < INFINITY ? (r[2] + ls[2]) * kLn2 : -INFINITY;
                 o.w = ls[3] < INFINITY ? (r[3] + ls[3]) * kLn2 : -INFINITY;
-                reinterpret_cast<float4 *>(head_lse + r0.row * H)[g] = o;
+                lw_put<G, kExact>(head_lse + r0.row * H, g, H, o);
             }
             float *const out = links + r0.row * (int64_t)K;
             lw_batches(nvec, [&](auto n, auto part, int v) {
@@ -829,7 +911,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 float least = 1.f;
 #pragma unroll
                 for (int u = 0; u < N; u++) {
-                    const float4 e = buf[kPart ? min(v + 32 * u, nvec - 1) : v + 32 * u];
+                    const float4 e = lw_get<G, kExact>(buf, kPart ? min(v + 32 * u, nvec - 1) : v + 32 * u, H, 0.f);
                     q[u] = lb_over_heads<G>(fmaf(e.x, f[0], e.y * f[1]) + fmaf(e.z, f[2], e.w * f[3]));
                     if (kPart && v + 32 * u >= nvec) q[u] = 1.f;
                     least = fminf(least, q[u]);
@@ -842,7 +924,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                         const int x = v + 32 * u;
                         float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                         if (x < nvec && !(np && !np[x / G])) {   // log2 of e f without the exponential's flush
-                            const float4 z = lb_shifted(__ldg(src + x), lw_bias<G>(table, bucket, x), r);
+                            const float4 z = lb_shifted(lw_get<G, kExact>(src, x, H, -INFINITY), lw_bias<G>(table, bucket, x), r);
                             if (ls[0] < INFINITY) t[0] = z.x + (g2[0] - ls[0]);
                             if (ls[1] < INFINITY) t[1] = z.y + (g2[1] - ls[1]);
                             if (ls[2] < INFINITY) t[2] = z.z + (g2[2] - ls[2]);
@@ -864,7 +946,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
         __syncwarp();
         if (later) {
             s1.at = 0;
-            lw_issue<G, false>(r1, s1, ring, mbar, content, nullptr, L, K);
+            lw_issue<G, kExact, false>(r1, s1, ring, mbar, content, nullptr, L, H, K, false);
         }
         r0 = r1;
         s0 = s1;
@@ -877,13 +959,14 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
 // Backward.  With w_d = G_d / sum_h q the gradient of a score is soft_h (exp(g_h) w_d - S_h): the scores' place holds
 // soft and then the gradient itself, which the four rows' warps add to their sums by distance (registers of the 128
 // threads, UA vectors each).
-template <int G, int UA, int NG>
+template <int G, bool kExact, int UA, int NG>
 __global__ void __launch_bounds__(NG * kLwRows * 32, UA <= 4 ? 2 : 1)
 lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ content,
               const float *__restrict__ log_gates, const float *__restrict__ head_lse, LinksMask mk,
               const int2 *__restrict__ span, LinksBias lb, LwSmem lay, float *__restrict__ grad_content,
-              float *__restrict__ grad_log_gates, float *__restrict__ part, int B, int L, int K) {
-    constexpr int H = 4 * G;
+              float *__restrict__ grad_log_gates, float *__restrict__ part, int B, int L, int heads, int K) {
+    const int H = kExact ? 4 * G : heads;
+    const bool whole = kExact || (H & 3) == 0;   // rows of 16-byte pieces
     extern __shared__ __align__(16) unsigned char lwsm[];
     __shared__ int2 row_at[NG * kLwRows];   // where a row's gradient lies (bytes from lwsm), its vectors
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane & (G - 1);
@@ -895,17 +978,17 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     const bool wide = (reinterpret_cast<uintptr_t>(grad_links) & 15) == 0;
     const int set = warp / kLwRows, set_tid = tid - set * (kLwRows * 32);
     const auto set_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(set + 1), "n"(kLwRows * 32) : "memory"); };
-    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, K);
+    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, H, K);
     pdl_trigger();
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + set;
     LwWalk walk(group, step, L);
     LwRow r0 = lw_row(walk, B, L, mk, span), r1 = lw_row(walk, B, L, mk, span);
     lw_resolve(r0, L, K, mk);
-    LwSlot s0 = lw_slot<G, true>(r0, K, wide);
-    lw_issue<G, true>(r0, s0, ring, mbar, content, grad_links, L, K);
+    LwSlot s0 = lw_slot<G, kExact, true>(r0, L, H, K);
+    lw_issue<G, kExact, true>(r0, s0, ring, mbar, content, grad_links, L, H, K, wide);
     const auto of_row = [&](const float *p, const LwRow &r) {
-        return r.exists ? __ldg(reinterpret_cast<const float4 *>(p + r.row * H) + g) : lb_ninf4();
+        return r.exists ? lw_heads<G, kExact>(p, r.row, H, g) : lb_ninf4();
     };
     float4 lse = of_row(head_lse, r0), gate = of_row(log_gates, r0);
     float4 acc[UA];
@@ -922,12 +1005,12 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         const float4 lse1 = of_row(head_lse, r1), gate1 = of_row(log_gates, r1);
         const LwRow r2 = lw_row(walk, B, L, mk, span);
         const int nvec = r0.nj * G;
-        float4 *const buf = reinterpret_cast<float4 *>(ring + s0.at + s0.window);
-        const float4 *const src = reinterpret_cast<const float4 *>(content + (r0.row * L + r0.i + 1) * (int64_t)H);
+        float *const buf = reinterpret_cast<float *>(ring + s0.at + s0.window) + s0.front;
+        const float *const src = content + (r0.row * L + r0.i + 1) * (int64_t)H;
         const unsigned char *const np = r0.holes ? mk.nonpad + r0.row + 1 : nullptr;
         float *const weight = reinterpret_cast<float *>(ring + s0.at) + s0.skip;   // G_d, then w_d
         if (r0.holes) {
-            lw_punch<G>(r0, buf, mk);
+            lw_punch<G, kExact>(r0, buf, H, mk);
             __syncwarp();
         }
         // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
@@ -941,7 +1024,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             constexpr bool kPart = decltype(part)::value;
             float4 t[N], q[N];
             float w[N];
-            lw_terms<G, N, kPart>(t, buf, table, bucket, ls, v, nvec);
+            lw_terms<G, kExact, N, kPart>(t, buf, H, table, bucket, ls, v, nvec);
             float least = 1.f;
 #pragma unroll
             for (int u = 0; u < N; u++) {
@@ -958,7 +1041,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
                 fmul2_rn(q[u].z, q[u].w, q[u].z, q[u].w, eg[2], eg[3]);
                 const float tot = lb_over_heads<G>((q[u].x + q[u].y) + (q[u].z + q[u].w));
                 if (in) {
-                    buf[v + 32 * u] = soft;
+                    lw_put<G, kExact>(buf, v + 32 * u, H, soft);
                     least = fminf(least, tot);
                 }
                 if (tot >= kLbTiny) w[u] = __fdividef(w[u], tot);
@@ -990,18 +1073,18 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         __syncwarp();
         // the next row on its way: the gradient of the row before this one has left its place
         lw_resolve(r1, L, K, mk);
-        LwSlot s1 = lw_slot<G, true>(r1, K, wide);
+        LwSlot s1 = lw_slot<G, kExact, true>(r1, L, H, K);
         s1.at = lw_place(s0, s1.bytes, lay.ring);
         const bool later = s1.at < 0;
         if (!later) {
             lw_bulk_read();
             __syncwarp();
-            lw_issue<G, true>(r1, s1, ring, mbar, content, grad_links, L, K);
+            lw_issue<G, kExact, true>(r1, s1, ring, mbar, content, grad_links, L, H, K, wide);
         }
         if (r0.exists) {
             lw_reduce<G, false>(S);
             if (lane < G)
-                reinterpret_cast<float4 *>(grad_log_gates + r0.row * H)[g] = make_float4(S[0], S[1], S[2], S[3]);
+                lw_put<G, kExact>(grad_log_gates + r0.row * H, g, H, make_float4(S[0], S[1], S[2], S[3]));
             lw_batches(nvec, [&](auto n, auto part, int v) {
                 constexpr int N = decltype(n)::value;
                 constexpr bool kPart = decltype(part)::value;
@@ -1010,18 +1093,18 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
 #pragma unroll
                 for (int u = 0; u < N; u++) {
                     const int x = kPart ? min(v + 32 * u, nvec - 1) : v + 32 * u;
-                    o[u] = buf[x];
+                    o[u] = lw_get<G, kExact>(buf, x, H, 0.f);
                     w[u] = weight[x / G];
                 }
                 if (kPart) __syncwarp();   // the last vector is read by lanes that do not own it
-bool full = false;
+                bool full = false;
 #pragma unroll
                 for (int u = 0; u < N; u++) full |= __float_as_uint(w[u]) == kLwFull;
                 if (__any_sync(0xffffffffu, full)) {   // see the first pass
                     for (int u = 0; u < N; u++) {
                         const int x = min(v + 32 * u, nvec - 1);
                         const bool dead = np && !np[x / G];
-                        const float4 t = dead ? lb_ninf4() : lb_shifted(__ldg(src + x), lw_bias<G>(table, bucket, x), ls);
+                        const float4 t = dead ? lb_ninf4() : lb_shifted(lw_get<G, kExact>(src, x, H, -INFINITY), lw_bias<G>(table, bucket, x), ls);
                         const float4 p = lw_full_share<G>(t, g2, __ldg(grad_links + r0.row * (int64_t)K + x / G));
                         float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
                         if (__float_as_uint(w[u]) == kLwFull) {
@@ -1030,7 +1113,7 @@ bool full = false;
                             k = make_float4(o[u].x * fmaf(eg[0], w[u], k.x), o[u].y * fmaf(eg[1], w[u], k.y),
                                             o[u].z * fmaf(eg[2], w[u], k.z), o[u].w * fmaf(eg[3], w[u], k.w));
                         }
-                        if (v + 32 * u < nvec) buf[v + 32 * u] = k;
+                        if (v + 32 * u < nvec) lw_put<G, kExact>(buf, v + 32 * u, H, k);
                     }
                 } else {
 #pragma unroll
@@ -1040,20 +1123,22 @@ bool full = false;
                         ffma2_rn(k.z, k.w, eg[2], eg[3], w[u], w[u]);
                         fmul2_rn(o[u].x, o[u].y, o[u].x, o[u].y, k.x, k.y);
                         fmul2_rn(o[u].z, o[u].w, o[u].z, o[u].w, k.z, k.w);
-                        if (!kPart || v + 32 * u < nvec) buf[v + 32 * u] = o[u];
+                        if (!kPart || v + 32 * u < nvec) lw_put<G, kExact>(buf, v + 32 * u, H, o[u]);
                     }
                 }
             });
             umma::fence_smem_to_async();
             __syncwarp();
-            unsigned char *const dense = reinterpret_cast<unsigned char *>(grad_content + r0.row * (int64_t)L * H);
-            const int before = (r0.i + 1) * (16 * G), total = L * (16 * G), behind = before + nvec * 16;
-            if (lane == 0 && nvec > 0) lw_bulk_store(dense + before, umma::smem_u32(buf), nvec * 16);
+            float *const dense = grad_content + r0.row * (int64_t)L * H;
+            const int before = (r0.i + 1) * H, total = L * H, behind = before + r0.nj * H;
+            if (whole) {
+                if (lane == 0 && nvec > 0) lw_bulk_store(dense + before, umma::smem_u32(buf), (behind - before) * 4);
+            } else {
+                for (int x = lane; x < behind - before; x += 32) dense[before + x] = buf[x];
+            }
             // the places of the dense row that no valid successor has
-            for (int at = lane * kLwZeros; at < before; at += 32 * kLwZeros)
-                lw_bulk_store(dense + at, zeros, min(kLwZeros, before - at));
-            for (int at = behind + lane * kLwZeros; at < total; at += 32 * kLwZeros)
-                lw_bulk_store(dense + at, zeros, min(kLwZeros, total - at));
+            lw_zero<!kExact>(dense, before, zeros);
+            lw_zero<!kExact>(dense + behind, total - behind, zeros);
             lw_bulk_commit();
         }
         if (part) {
@@ -1062,13 +1147,13 @@ bool full = false;
 #pragma unroll
             for (int w = 0; w < kLwRows; w++) {
                 const int2 at = row_at[set * kLwRows + w];
-                const float4 *const dc = reinterpret_cast<const float4 *>(lwsm + at.x);
+                const float *const dc = reinterpret_cast<const float *>(lwsm + at.x);
 #pragma unroll
                 for (int u = 0; u < UA; u++) {
                     if (u * (kLwRows * 32) >= at.y) break;
                     const int v = set_tid + u * (kLwRows * 32);
                     if (v < at.y) {
-                        const float4 o = dc[v];
+                        const float4 o = lw_get<G, kExact>(dc, v, H, 0.f);
                         fadd2_rn(acc[u].x, acc[u].y, acc[u].x, acc[u].y, o.x, o.y);
                         fadd2_rn(acc[u].z, acc[u].w, acc[u].z, acc[u].w, o.z, o.w);
                     }
@@ -1081,7 +1166,7 @@ bool full = false;
             umma::fence_smem_to_async();
             __syncwarp();
             s1.at = 0;
-            lw_issue<G, true>(r1, s1, ring, mbar, content, grad_links, L, K);
+            lw_issue<G, kExact, true>(r1, s1, ring, mbar, content, grad_links, L, H, K, wide);
         }
         r0 = r1;
         s0 = s1;
@@ -1102,7 +1187,7 @@ bool full = false;
         }
         __syncthreads();
         if (set == 0) {
-            float4 *p = reinterpret_cast<float4 *>(part + (size_t)blockIdx.x * K * H);
+            float *const p = part + (size_t)blockIdx.x * K * H;
 #pragma unroll
             for (int u = 0; u < UA; u++) {
                 const int v = set_tid + u * (kLwRows * 32);
@@ -1115,7 +1200,7 @@ bool full = false;
                         acc[u].z += o.z;
                         acc[u].w += o.w;
                     }
-                    p[v] = acc[u];
+                    lw_put<G, kExact>(p, v, H, acc[u]);
                 }
             }
         }
@@ -1193,9 +1278,18 @@ lb_join_kernel(const double *__restrict__ by_distance, const int64_t *__restrict
     }
 }
 
-static bool lb_vector_form(int heads, int translen, const void *a, const void *b, const void *c, const void *d) {
+// a warp per vertex: by size alone, so that a forward and its backward agree on who fills the spans
+static bool lw_fits(int K, int H, int n, const DeviceInfo &di) {
+    return H <= 32 && (int64_t)K * lw_lanes(H) <= kLwMaxVec && (int64_t)n * 4 * lw_lanes(H) <= kLwMaxTable &&
+           lw_smem(K, H, n, 2 * kLwRows, lw_one(di)).ring >= lw_row_bytes(K, H);
+}
+
+// the kernels of this file: a warp or a CTA per vertex, by size, on 16-byte boundaries
+static bool lb_own_form(int heads, int translen, int n, const DeviceInfo &di, const void *a, const void *b, const void *c,
+                        const void *d) {
     const int G = heads / 4;
-    return heads % 4 == 0 && (G == 1 || G == 2 || G == 4 || G == 8) && (int64_t)translen * G <= kLbMaxVec &&
+    const bool vectors = heads % 4 == 0 && (G == 1 || G == 2 || G == 4 || G == 8) && (int64_t)translen * G <= kLbMaxVec;
+    return (lw_fits(translen, heads, n, di) || vectors) &&
            ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
              reinterpret_cast<uintptr_t>(d)) & 15) == 0;
 }
@@ -1216,12 +1310,6 @@ static int lb_grid(F kernel, int threads, size_t smem, int64_t rows, const Devic
 
 constexpr int kLbMaxPerSm = 16;   // CTAs per SM that the workspace has room for
 
-// a warp per vertex: by size alone, so that a forward and its backward agree on who fills the spans
-static bool lw_fits(int K, int H, int n, const DeviceInfo &di) {
-    return (int64_t)K * H <= 4 * kLwMaxVec && (int64_t)n * H <= kLwMaxTable &&
-           lw_smem(K, H, n, 3 * kLwRows, lw_one(di)).ring >= lw_row_bytes(K, H);
-}
-
 struct LbArgs {
     const float *grad_links, *content, *log_gates, *head_lse_in;
     LinksMask mk;
@@ -1229,7 +1317,7 @@ struct LbArgs {
     int2 *span;
     bool after;   // the kernel that fills the spans has just been launched
     float *links, *head_lse, *grad_content, *grad_log_gates, *part;
-    int B, L, K;
+    int B, L, H, K;
 };
 
 template <int G, int NT, int U>
@@ -1250,12 +1338,12 @@ static int lb_launch(const LbArgs &a, bool backward, int &grid, cudaStream_t st,
 }
 
 // CTAs of NG groups, `per_sm` of them to an SM
-template <int G, int NG, typename F, typename... Args>
+template <int NG, typename F, typename... Args>
 static int lw_start(F kernel, int per_sm, const LbArgs &a, int &parts, cudaStream_t st, const DeviceInfo &di,
                     const char *who, LwSmem &lay, Args... args) {
     const int64_t groups = (int64_t)a.B * ((a.L + kLwRows - 1) / kLwRows);
     const int smem = per_sm > 1 ? lw_two(di) : lw_one(di);
-    lay = lw_smem(a.K, 4 * G, a.lb.n, NG * kLwRows, smem);
+    lay = lw_smem(a.K, a.H, a.lb.n, NG * kLwRows, smem);
     int64_t n = (int64_t)di.sm_count * per_sm;
     if (n > (groups + NG - 1) / NG) n = (groups + NG - 1) / NG;
     parts = (int)n;
@@ -1265,31 +1353,44 @@ static int lw_start(F kernel, int per_sm, const LbArgs &a, int &parts, cudaStrea
     }
     return check_launch(who);
 }
-template <int G>
+template <int G, bool kExact>
 static int lw_launch(const LbArgs &a, bool backward, int &parts, cudaStream_t st, const DeviceInfo &di, const char *who) {
-    // two CTAs per SM, of eight warps, where the rings of both hold more than the longest row, else one of twelve
-    const int row = lw_row_bytes(a.K, 4 * G);
+    const int row = lw_row_bytes(a.K, a.H), nvec = a.K * G;
+    const int two = lw_smem(a.K, a.H, a.lb.n, 2 * kLwRows, lw_two(di)).ring;     // rings of eight warps, two CTAs per SM
+    const int one = lw_smem(a.K, a.H, a.lb.n, 3 * kLwRows, lw_one(di)).ring;     // of twelve, one CTA
     LwSmem lay;
+    const auto fwd = [&](auto kernel, auto ng, int per_sm) {
+        return lw_start<decltype(ng)::value>(kernel, per_sm, a, parts, st, di, who, lay, a.content, a.log_gates, a.mk, a.span,
+                                             a.lb, std::ref(lay), a.links, a.head_lse, a.B, a.L, a.H, a.K);
+    };
+    const auto bwd = [&](auto kernel, auto ng, int per_sm) {
+        return lw_start<decltype(ng)::value>(kernel, per_sm, a, parts, st, di, who, lay, a.grad_links, a.content, a.log_gates,
+                                             a.head_lse_in, a.mk, a.span, a.lb, std::ref(lay), a.grad_content,
+                                             a.grad_log_gates, a.part, a.B, a.L, a.H, a.K);
+    };
+    // Two CTAs per SM, of eight warps, where their rings hold more than the longest row; else one of twelve; longer rows
+    // leave room for eight.  (16 graphs of 1024 vertices, band of 256, forward: 30 us with 16 warps per SM, 43 with 12.)
     if (!backward) {
-        if (lw_smem(a.K, 4 * G, a.lb.n, 2 * kLwRows, lw_two(di)).ring >= row + row / 4)
-            return lw_start<G, 2>(lw_fwd_kernel<G, 2>, 2, a, parts, st, di, who, lay, a.content, a.log_gates, a.mk, a.span,
-                                  a.lb, std::ref(lay), a.links, a.head_lse, a.B, a.L, a.K);
-        return lw_start<G, 3>(lw_fwd_kernel<G, 3>, 1, a, parts, st, di, who, lay, a.content, a.log_gates, a.mk,
-                              a.span, a.lb, std::ref(lay), a.links, a.head_lse, a.B, a.L, a.K);
+        if (two >= row + row / 4) return fwd(lw_fwd_kernel<G, kExact, 2>, LwInt<2>(), 2);
+        if (one >= row) return fwd(lw_fwd_kernel<G, kExact, 3>, LwInt<3>(), 1);
+        return fwd(lw_fwd_kernel<G, kExact, 2>, LwInt<2>(), 1);
     }
-    if (a.K * G <= 4 * kLwRows * 32)
-        return lw_start<G, 2>(lw_bwd_kernel<G, 4, 2>, 2, a, parts, st, di, who, lay, a.grad_links, a.content, a.log_gates,
-                              a.head_lse_in, a.mk, a.span, a.lb, std::ref(lay), a.grad_content, a.grad_log_gates, a.part, a.B,
-                              a.L, a.K);
-    return lw_start<G, 3>(lw_bwd_kernel<G, 8, 3>, 1, a, parts, st, di, who, lay, a.grad_links, a.content, a.log_gates,
-                          a.head_lse_in, a.mk, a.span, a.lb, std::ref(lay), a.grad_content, a.grad_log_gates, a.part, a.B, a.L,
-                          a.K);
+    if (nvec <= 4 * kLwRows * 32 && two >= row) return bwd(lw_bwd_kernel<G, kExact, 4, 2>, LwInt<2>(), 2);
+    if (nvec <= 8 * kLwRows * 32 && one >= row) return bwd(lw_bwd_kernel<G, kExact, 8, 3>, LwInt<3>(), 1);
+    return bwd(lw_bwd_kernel<G, kExact, 16, 2>, LwInt<2>(), 1);
+}
+static int lw_run(const LbArgs &a, bool backward, int &parts, cudaStream_t st, const DeviceInfo &di, const char *who) {
+    switch (lw_lanes(a.H)) {
+        case 1: return a.H == 4 ? lw_launch<1, true>(a, backward, parts, st, di, who) : lw_launch<1, false>(a, backward, parts, st, di, who);
+        case 2: return a.H == 8 ? lw_launch<2, true>(a, backward, parts, st, di, who) : lw_launch<2, false>(a, backward, parts, st, di, who);
+        case 4: return a.H == 16 ? lw_launch<4, true>(a, backward, parts, st, di, who) : lw_launch<4, false>(a, backward, parts, st, di, who);
+        default: return a.H == 32 ? lw_launch<8, true>(a, backward, parts, st, di, who) : lw_launch<8, false>(a, backward, parts, st, di, who);
+    }
 }
 
 template <int G>
 static int lb_dispatch(const LbArgs &a, bool backward, int &grid, cudaStream_t st, const DeviceInfo &di, const char *who) {
     const int nvec = a.K * G;
-    if (lw_fits(a.K, 4 * G, a.lb.n, di)) return lw_launch<G>(a, backward, grid, st, di, who);
     if (nvec <= 2 * 128) return lb_launch<G, 128, 2>(a, backward, grid, st, di, who);
     if (nvec <= 4 * 128) return lb_launch<G, 128, 4>(a, backward, grid, st, di, who);
     if (nvec <= 8 * 128) return lb_launch<G, 128, 8>(a, backward, grid, st, di, who);
@@ -1297,9 +1398,9 @@ static int lb_dispatch(const LbArgs &a, bool backward, int &grid, cudaStream_t s
     return lb_launch<G, 512, 8>(a, backward, grid, st, di, who);
 }
 
-static int lb_run(const LbArgs &a, int heads, bool backward, int &grid, cudaStream_t st, const DeviceInfo &di,
-                  const char *who) {
-    switch (heads / 4) {
+static int lb_run(const LbArgs &a, bool backward, int &grid, cudaStream_t st, const DeviceInfo &di, const char *who) {
+    if (lw_fits(a.K, a.H, a.lb.n, di)) return lw_run(a, backward, grid, st, di, who);
+    switch (a.H / 4) {
         case 1: return lb_dispatch<1>(a, backward, grid, st, di, who);
         case 2: return lb_dispatch<2>(a, backward, grid, st, di, who);
         case 4: return lb_dispatch<4>(a, backward, grid, st, di, who);
@@ -1352,7 +1453,7 @@ int dat_links_from_heads_biased(const float *content, const float *log_gates, co
         lw_span_kernel<<<(unsigned)bsz, 128, 0, st>>>(nonpad, reinterpret_cast<int2 *>(spans), prelen);
         if (int rc = check_launch(who)) return rc;
     }
-    if (lb_vector_form(heads, translen, content, log_gates, head_lse, nullptr)) {
+    if (lb_own_form(heads, translen, num_buckets, di, content, log_gates, head_lse, nullptr)) {
         LbArgs a{};
         a.content = content;
         a.log_gates = log_gates;
@@ -1364,9 +1465,10 @@ int dat_links_from_heads_biased(const float *content, const float *log_gates, co
         a.after = after;
         a.B = bsz;
         a.L = prelen;
+        a.H = heads;
         a.K = translen;
         int grid;
-        return lb_run(a, heads, false, grid, st, di, who);
+        return lb_run(a, false, grid, st, di, who);
     }
     return links_fwd_rows<true>(content, log_gates, mk, lb, links, head_lse, bsz, prelen, heads, translen, st, di, who);
 }
@@ -1396,7 +1498,7 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
     double *sums = static_cast<double *>(workspace);
     const unsigned sgrid = (unsigned)((KH + kLbSumCols - 1) / kLbSumCols);
     constexpr int kSum = kLbSumCols * kLbSumLanes;
-    if (lb_vector_form(heads, translen, content, log_gates, head_lse, grad_content) &&
+    if (lb_own_form(heads, translen, num_buckets, di, content, log_gates, head_lse, grad_content) &&
         (reinterpret_cast<uintptr_t>(grad_log_gates) & 15) == 0) {
         LbArgs a{};
         a.grad_links = grad_links;
@@ -1411,9 +1513,10 @@ int dat_links_from_heads_biased_backward(const float *grad_links, const float *c
         a.part = grad_bias_table ? reinterpret_cast<float *>(sums + (KH + 1) / 2 * 2) : nullptr;
         a.B = bsz;
         a.L = prelen;
+        a.H = heads;
         a.K = translen;
         int grid;
-        if (int rc = lb_run(a, heads, true, grid, st, di, who)) return rc;
+        if (int rc = lb_run(a, true, grid, st, di, who)) return rc;
         if (!grad_bias_table) return DAT_OK;
         launch_after(lb_sum_kernel, sgrid, kSum, 0, st, 1, a.part, sums, grid, KH);
     } else {

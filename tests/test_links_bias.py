@@ -135,7 +135,10 @@ def test_refusals_come_before_any_device_work():
 SHAPES = [(2, 400, 8, 399), (1, 514, 8, 512), (1, 513, 8, 512), (1, 1026, 4, 1025), (1, 1025, 4, 1024), (3, 140, 32, 128),
           (2, 131, 32, 130), (7, 4, 4, 3), (150, 5, 8, 4), (9, 61, 16, 60), (1, 2, 1, 1), (2, 5, 8, 4), (3, 33, 8, 32), (2, 64, 4, 63), (2, 70, 16, 20), (1, 40, 32, 39), (3, 37, 6, 36),
           (2, 50, 3, 7), (1, 129, 12, 128), (2, 300, 8, 299), (1, 520, 4, 519), (1, 600, 16, 450), (2, 30, 128, 29),
-          (5, 18, 2, 1), (1, 9, 5, 8), (1, 260, 32, 259), (1, 1100, 4, 1099)]
+          (5, 18, 2, 1), (1, 9, 5, 8), (1, 260, 32, 259), (1, 1100, 4, 1099),
+          (3, 71, 1, 70), (1, 700, 1, 699), (1, 1100, 2, 1030), (1, 400, 3, 390), (2, 90, 7, 89), (1, 512, 12, 511),
+          (1, 300, 10, 257), (2, 40, 20, 39), (1, 150, 29, 149), (1, 410, 16, 390), (1, 1030, 6, 1029), (2, 9, 31, 2),
+          (1, 140, 24, 130), (1, 300, 18, 256)]
 
 
 @pytest.mark.gpu
@@ -156,7 +159,7 @@ def test_against_64_bits_without_mask_and_with_bound(B, L, H, K):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H,L,K", [(8, 90, 89), (4, 200, 60), (16, 65, 64), (3, 40, 39), (8, 700, 699)])
+@pytest.mark.parametrize("H,L,K", [(8, 90, 89), (4, 200, 60), (16, 65, 64), (3, 40, 39), (8, 700, 699), (12, 90, 89), (5, 50, 30)])
 def test_masks_with_holes(H, L, K):
     """Padding inside a sentence and before it, a sentence without a vertex, one with a single one."""
     B = 6
@@ -174,7 +177,7 @@ def test_masks_with_holes(H, L, K):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("H,L", [(8, 50), (6, 50), (16, 40), (8, 600)])
+@pytest.mark.parametrize("H,L", [(8, 50), (6, 50), (16, 40), (8, 600), (12, 40), (3, 300)])
 @pytest.mark.parametrize("scale", [30.0, 200.0])
 def test_scores_far_apart(H, L, scale):
     """Scores hundreds apart: the nearest successor's is far below the largest, and links reach -1000, which 32-bit
