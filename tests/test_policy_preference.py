@@ -785,3 +785,23 @@ def test_training_step_of_links_likelihoods_and_both_losses():
     assert pstats[4] == P and pstats[5] == 0 and int(stats[4]) == int(mask.sum())
     for name, u, v in zip(("logits", "scores", "gates", "bias"), got, want):
         assert_rel(u.cpu().numpy(), v.numpy(), 1e-4, name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [500, 30000])
+@pytest.mark.parametrize("step", [0.004, -0.02, 0.3, -0.45])
+def test_estimated_kl_of_small_steps_near_a_far_log_probability(V, step):
+    """Equal logits: every exponential is 1 and the sum V, without a rounding, so that the log-probability is -log V and
+    all that is left is how the row's numbers are put together.  The logarithm of V's mantissa (below 0.7) may be off by
+    two units of its last place, 2^-23, and u is rounded once, 2^-25 of 1: less than 2^-22 that the KL takes times
+    e^u - 1; the KL itself is a product of about ten rounded
+    factors, each 2^-24 of it, and u enters it twice.  (A log-probability rounded to 32 bits is off by 2^-22 and more.)"""
+    logits = torch.full((1, 4, V), 0.75, dtype=torch.bfloat16, device=DEV)
+    ref = torch.full((1, 4), -math.log(V) + step, dtype=torch.float32, device=DEV)
+    old = torch.full((1, 4), -math.log(V), dtype=torch.float32, device=DEV)
+    tokens = torch.tensor([[0, 1, V // 2, V - 1]], device=DEV)
+    _, logp, kl, _ = dat.dag_policy_loss(logits, tokens, old, torch.ones(1, 4, device=DEV), ref_logp=ref, kl_coef=0.1)
+    u = ref.double() + math.log(V)
+    want = torch.expm1(u) - u
+    assert ((logp.double() + math.log(V)).abs() <= 2.0 ** -23 + 2.0 ** -24 * math.log(V)).all()
+    assert ((kl.double() - want).abs() <= torch.expm1(u).abs() * 2.0 ** -22 + 16 * 2.0 ** -24 * want).all()
