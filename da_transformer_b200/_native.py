@@ -28,6 +28,7 @@ EXPORTS = (
     "dat_upload_links", "dat_upload_links_bytes", "dat_upload_links_head_rows",
     "dat_links_from_heads_biased", "dat_links_from_heads_biased_backward", "dat_links_bias_workspace_bytes",
     "dat_policy_loss", "dat_policy_loss_backward", "dat_policy_loss_workspace_bytes", "dat_preference_loss",
+    "dat_stream_capture_id",
 )
 
 _lib = None
@@ -98,6 +99,8 @@ def _declare(lib):
     lib.dat_links_bias_workspace_bytes.argtypes = [_i32] * 4
     lib.dat_links_from_heads_biased_backward.restype = _i32
     lib.dat_links_from_heads_biased_backward.argtypes = [_vp] * 5 + [_i32] + [_vp] * 10 + [_i32] * 4 + [_vp]
+    lib.dat_stream_capture_id.restype = ctypes.c_uint64
+    lib.dat_stream_capture_id.argtypes = [_vp]
     lib.dat_policy_loss_workspace_bytes.restype = ctypes.c_size_t
     lib.dat_policy_loss_workspace_bytes.argtypes = [_i32] * 2
     lib.dat_policy_loss.restype = _i32

@@ -1082,7 +1082,7 @@ policy_bwd_kernel(PolicyBackwardArgs a) {
     const float up = *a.grad_loss;
     if (a.grad_link)
         for (int64_t r = (int64_t)blockIdx.x * kPoThreads + threadIdx.x; r < a.rows; r += (int64_t)gridDim.x * kPoThreads)
-            a.grad_link[r] = a.row_state[2 * r].z * up;
+            a.grad_link[r] = a.mask && !a.mask[r] ? 0.f : a.row_state[2 * r].z * up;
     if (!a.grad || (a.written && up == a.head->scale)) return;
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         T *g = static_cast<T *>(a.grad) + row * a.V;
@@ -1231,6 +1231,7 @@ int dat_policy_loss(const void *word_ins_out, const void *ref_logits, int dtype,
     DAT_REQUIRE(loss && stats && workspace, DAT_ERR_BAD_ARG, "%s: null pointer", who);
     DAT_REQUIRE(!(ref_logits && ref_logp), DAT_ERR_BAD_ARG, "%s: ref_logits and ref_logp exclude each other", who);
     DAT_REQUIRE(clip_low >= 0.f && clip_high >= 0.f, DAT_ERR_BAD_ARG, "%s: negative clip range", who);
+    DAT_REQUIRE(vocab <= 0x3fffffff, DAT_ERR_UNSUPPORTED, "%s: vocab = %d exceeds 2^30-1", who, vocab);
     const int64_t rows = (int64_t)bsz * prelen;
     DAT_REQUIRE(rows <= 0x7fffffff, DAT_ERR_UNSUPPORTED, "%s: bsz*prelen = %lld exceeds 2^31-1", who, (long long)rows);
     DAT_REQUIRE(dtype == DAT_F32 || dtype == DAT_F16 || dtype == DAT_BF16, DAT_ERR_UNSUPPORTED,
@@ -1282,6 +1283,16 @@ int dat_policy_loss(const void *word_ins_out, const void *ref_logits, int dtype,
         case DAT_F16: return policy_fwd_t<__half>(a, di, st, who);
         default: return policy_fwd_t<__nv_bfloat16>(a, di, st, who);
     }
+}
+
+unsigned long long dat_stream_capture_id(void *stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &status, &id) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusActive ? id : 0;
 }
 
 int dat_policy_loss_backward(const void *word_ins_out, const void *ref_logits, int dtype, const int64_t *tokens,

@@ -28,6 +28,8 @@ def _check_policy(word_ins_out, link_logp, tokens, old_logp, advantage, mask, re
     bsz, prelen, vocab = word_ins_out.shape
     if vocab < 1:
         raise RuntimeError("word_ins_out has an empty vocabulary")
+    if vocab >= 2 ** 30 or bsz * prelen >= 2 ** 31:
+        raise RuntimeError("dag_policy_loss takes vocabularies below 2^30 and less than 2^31 vertices")
     if not word_ins_out.is_contiguous():
         raise RuntimeError("word_ins_out is not contiguous")
     shape = (bsz, prelen)
@@ -71,6 +73,7 @@ class DagPolicyLossFunc(Function):
         L = lib()
         need_logits, need_link = ctx.needs_input_grad[0], link_logp is not None and ctx.needs_input_grad[1]
         with torch.cuda.device(dev):
+            stream = stream_address(dev)
             tokens = tokens.contiguous()
             mask = _mask_bytes(mask)
             old_logp = old_logp.contiguous()
@@ -89,13 +92,15 @@ class DagPolicyLossFunc(Function):
                 advantage.data_ptr(), advantage.stride(0), advantage.stride(1) if advantage.dim() == 2 else 0,
                 address(link), address(refp), address(mask), kl_coef, clip_low, clip_high, address(scale_tensor), scale,
                 loss.data_ptr(), stats.data_ptr(), logp.data_ptr(), kl.data_ptr(), ws.data_ptr() if at else 0, address(grad),
-                ws.data_ptr() + at, _status_word(dev).data_ptr(), bsz, prelen, vocab, stream_address(dev)), "policy_loss")
+                ws.data_ptr() + at, _status_word(dev).data_ptr(), bsz, prelen, vocab, stream), "policy_loss")
         ctx.mark_non_differentiable(logp, kl, stats)
         ctx.set_materialize_grads(False)
         if need_grad:
             ctx.save_for_backward(word_ins_out, ref_logits, tokens, mask)
             ctx.ws = ws               # the library's own, nobody else holds it
             ctx.grad, ctx.kl_coef = grad, kl_coef
+            # a graph that holds the backward alone would find the buffer as it was left after the last replay
+            ctx.capture = 0 if grad is None else L.dat_stream_capture_id(stream)
         return loss, logp, kl, stats
 
     @staticmethod
@@ -115,14 +120,17 @@ def _policy_backward(ctx, grad_loss):
     grad, ctx.grad = ctx.grad, None
     with torch.cuda.device(dev):
         grad_loss = grad_loss.to(torch.float32).contiguous()
-        written = grad is not None
+        stream = stream_address(dev)
+        written = grad is not None and lib().dat_stream_capture_id(stream) == ctx.capture
+        if not written:
+            grad = None
         if not written and ctx.needs_input_grad[0]:
             grad = torch.empty_like(word_ins_out)
         link = torch.empty(bsz, prelen, dtype=torch.float32, device=dev) if ctx.needs_input_grad[1] else None
         check(lib().dat_policy_loss_backward(
             word_ins_out.data_ptr(), address(ref_logits), _native.dtype_code(word_ins_out.dtype), tokens.data_ptr(),
             address(mask), ctx.kl_coef, ws, ws + bsz * prelen * 32, grad_loss.data_ptr(), int(written),
-            address(grad), address(link), bsz, prelen, vocab, stream_address(dev)), "policy_loss_backward")
+            address(grad), address(link), bsz, prelen, vocab, stream), "policy_loss_backward")
     return grad, link, None
 
 

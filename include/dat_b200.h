@@ -405,7 +405,11 @@ int dat_policy_loss(const void *word_ins_out, const void *ref_logits, int dtype,
  * Gradient of dat_policy_loss's loss times *grad_loss (device).  grad_written != 0: grad_logits is what
  * dat_policy_loss wrote; it is left as it is when *grad_loss equals the scale it was written for and written
  * again otherwise.  grad_logits or grad_link ([bsz,prelen] fp32) may be NULL.
+ * A CUDA graph that holds this call with grad_written != 0 has to hold the dat_policy_loss that writes grad_logits too,
+ * before it: a replay finds the buffer as the last one's reader left it.  dat_stream_capture_id names the capture that a
+ * stream is in, 0 outside one.
  */
+unsigned long long dat_stream_capture_id(void *stream);
 int dat_policy_loss_backward(const void *word_ins_out, const void *ref_logits, int dtype, const int64_t *tokens,
                              const unsigned char *mask, float kl_coef, const float *row_state, const void *workspace,
                              const float *grad_loss, int grad_written, void *grad_logits, float *grad_link, int bsz,

@@ -805,3 +805,37 @@ def test_estimated_kl_of_small_steps_near_a_far_log_probability(V, step):
     want = torch.expm1(u) - u
     assert ((logp.double() + math.log(V)).abs() <= 2.0 ** -23 + 2.0 ** -24 * math.log(V)).all()
     assert ((kl.double() - want).abs() <= torch.expm1(u).abs() * 2.0 ** -22 + 16 * 2.0 ** -24 * want).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [300, 9000])
+def test_policy_backward_in_a_graph_of_its_own(V):
+    """The forward runs once, its backward is captured alone and replayed with changing gradients of the loss; in
+    between the gradient is written over, as an optimiser's zeroing does."""
+    x, kw = policy_inputs(2, 20, V, torch.bfloat16, seed=21, link=True, ref="full", mask=0.5)
+    up = torch.ones((), device=DEV)
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        leaf = x.clone().requires_grad_()
+        loss = policy_call(leaf, kl_coef=0.1, **kw)[0]
+        graph = torch.cuda.CUDAGraph()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            grad, = torch.autograd.grad(loss, leaf, up)
+    torch.cuda.current_stream().wait_stream(side)
+    for scale in (1.0, 4.0, 1.0, 1.0, 0.5):
+        up.fill_(scale)
+        graph.replay()
+        want = run_policy(x, kw, kl_coef=0.1, scale=scale, grad_scale=None)[4]   # the same kernel, in the backward
+        assert torch.equal(grad, want), scale
+        grad.zero_()
+
+
+@pytest.mark.gpu
+def test_policy_link_gradient_of_masked_vertices_stays_zero():
+    x, kw = policy_inputs(2, 20, 300, torch.float32, seed=22, link=True, mask=0.5)
+    link = kw.pop("link").clone().requires_grad_()
+    loss = policy_call(x, link=link, **kw)[0]
+    grad, = torch.autograd.grad(loss, link, torch.full((), math.inf, device=DEV))
+    assert (grad[~kw["mask"]] == 0).all()
