@@ -54,8 +54,9 @@ def _status_word(device):
 def last_status(device=None, reset=True):
     """Status bits accumulated on ``device`` since the last reset (synchronises):
     1 = a sentence had invalid lengths, 2 = a sentence had no finite alignment,
-    4 = a gather index was outside the vocabulary, 8 = the fast dag_loss path handed at least
-    one sentence to the exact kernels (informational)."""
+    4 = a gather index was outside the vocabulary (or a bucket outside the table of relative biases),
+    8 = the fast dag_loss path handed at least one sentence to the exact kernels (informational),
+    16 = a bounded wait inside a kernel ran out (never expected; the results of that call are not valid)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     buf = _status_word(device)
     value = int(buf.item())
