@@ -21,7 +21,8 @@ namespace dat {
 
 constexpr int kLinksThreads = 128;   // 256 and 64 threads per vertex row were slower (0.25 / 0.26 against 0.22 ms forward)
 
-// Stages content[b,i,j,:] (+ bias) for j in [i+1, jhi] into sm[(j-i-1)*H + h]; masked columns become -inf.
+// Stages content[b,i,j,:] for j in [i+1, jhi] into sm[(j-i-1)*H + h]; masked columns become -inf.  kBias: content +
+// bias, in log2 units, in which everything is put together then: each score is rounded once, so that it less itself is 0.
 template <bool kBias>
 __device__ __forceinline__ void links_stage_row(const float *__restrict__ crow, float *sm, int i, int jhi,
                                                 int H, const unsigned char *np_row, const LinksBias &lb) {
@@ -33,7 +34,7 @@ __device__ __forceinline__ void links_stage_row(const float *__restrict__ crow, 
             const int d = x / H;
             const float t = links_bias1(lb, d, x - d * H, H, bad);
             const bool dead = (np_row && !np_row[i + 1 + d]) || t == -INFINITY;   // also where the score is +inf or NaN
-            sm[x] = dead ? -INFINITY : __ldg(src + x) + t;
+            sm[x] = dead ? -INFINITY : fmaf(__ldg(src + x), kLog2e, t * kLog2e);
         }
         if (bad && lb.status) atomicOr(lb.status, DAT_STATUS_BAD_INDEX);
     } else if ((H & 3) == 0) {
@@ -53,9 +54,10 @@ __device__ __forceinline__ void links_stage_row(const float *__restrict__ crow, 
     }
 }
 
-// Per-head log-sum-exp (natural log) over the staged successors.  Thread (h = tid % H, part = tid / H)
+// Per-head log-sum-exp (natural log; kBias: log2) over the staged successors.  Thread (h = tid % H, part = tid / H)
 // walks the successors part, part + P, ...; partial (max, sum) pairs meet in shared memory.
 // Result in lse_s[h] (-inf when the head sees no finite score).  Needs H <= kLinksThreads.
+template <bool kBias>
 __device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, float *part_m, float *part_s,
                                                float *lse_s) {
     const int tid = threadIdx.x;
@@ -64,7 +66,7 @@ __device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, f
     float m = kNegBig, s = 0.f;
     if (part < P) {
         for (int j = part; j < nj; j += P) {
-            const float v = sm[j * H + h] * kLog2e;
+            const float v = kBias ? sm[j * H + h] : sm[j * H + h] * kLog2e;
             if (v > m) {
                 s *= ex2(m - v);
                 m = v;
@@ -78,7 +80,7 @@ __device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, f
     if (tid < H) {
         float M = kNegBig, S = 0.f;
         for (int p = 0; p < P; p++) lse_merge(M, S, part_m[p * H + tid], part_s[p * H + tid]);
-        lse_s[tid] = (S > 0.f && M > 0.5f * kNegBig) ? (M + lg2(S)) * kLn2 : -INFINITY;
+        lse_s[tid] = (S > 0.f && M > 0.5f * kNegBig) ? (M + lg2(S)) * (kBias ? 1.f : kLn2) : -INFINITY;
     }
     __syncthreads();
 }
@@ -103,22 +105,29 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
     links_stage_row<kBias>(content + row * (size_t)L * H, sm, i, jhi, H, np_row, lb);
     if (tid < H) gate_s[tid] = log_gates[row * H + tid];
     __syncthreads();
-    links_head_lse(sm, nj, H, part_m, part_s, lse_s);
+    links_head_lse<kBias>(sm, nj, H, part_m, part_s, lse_s);
     if (head_lse && tid < H) head_lse[row * H + tid] = lse_s[tid];
-    // per head, what is added to a score: (gate - lse) in log2 units; a head whose every score is -inf
-    // (lse = -inf) takes no part
-    if (tid < H) gate_s[tid] = lse_s[tid] > -INFINITY ? (gate_s[tid] - lse_s[tid]) * kLog2e : -INFINITY;
+    // per head, what is added to a score: (gate - lse) in log2 units (kBias: the gate, after the lse); a head whose every
+    // score is -inf (lse = -inf) takes no part
+    if (tid < H) {
+        const float gate = (kBias ? gate_s[tid] : gate_s[tid] - lse_s[tid]) * kLog2e;
+        gate_s[tid] = lse_s[tid] > -INFINITY ? gate : -INFINITY;
+        if (kBias && !(lse_s[tid] > -INFINITY)) lse_s[tid] = 0.f;
+    }
     __syncthreads();
+    const auto term = [&](int d, int h) {
+        return kBias ? (sm[d * H + h] - lse_s[h]) + gate_s[h] : fmaf(sm[d * H + h], kLog2e, gate_s[h]);
+    };
     float *out = links + row * (size_t)K;
     for (int d = tid; d < K; d += kLinksThreads) {
         float v = -INFINITY;
         if (d < nj) {
             // max over the heads first, then the sum: no rescaling and no branches inside the loops
             float m = -INFINITY;
-            for (int h = 0; h < H; h++) m = fmaxf(m, fmaf(sm[d * H + h], kLog2e, gate_s[h]));
+            for (int h = 0; h < H; h++) m = fmaxf(m, term(d, h));
             if (m > -INFINITY) {
                 float s = 0.f;
-                for (int h = 0; h < H; h++) s += ex2(fmaf(sm[d * H + h], kLog2e, gate_s[h]) - m);
+                for (int h = 0; h < H; h++) s += ex2(term(d, h) - m);
                 v = (m + lg2(s)) * kLn2;
             }
         }
@@ -131,7 +140,8 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
 //     S_h          = sum_j G[j] p[j,h]                          = d / d log_gates[h]
 //     d / d c[j,h] = G[j] p[j,h] - exp(c[j,h] - lse_h) * S_h
 // grad_content is written for the whole [L,H] row (zeros outside the valid successors); it may alias
-// content (a CTA has its row in shared memory before it writes).
+// content (a CTA has its row in shared memory before it writes).  kBias: G p is rounded the same way in the sum and in
+// the difference, so that a vertex with one successor (p the same, soft = 1) has the gradient 0.
 template <bool kBias>
 __global__ void __launch_bounds__(kLinksThreads)
 links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
@@ -172,7 +182,9 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
         if (lse_s[h] > -INFINITY)
             for (int j = pt; j < nj; j += P) {
                 const float lk = lk_s[j];
-                if (lk > -INFINITY) acc += gl_s[j] * ex2(fmaf(sm[j * H + h], kLog2e, k) - lk * kLog2e);
+                if (!(lk > -INFINITY)) continue;
+                if (kBias) acc = __fadd_rn(acc, __fmul_rn(gl_s[j], ex2((sm[j * H + h] - lse_s[h]) + (gate_s[h] - lk) * kLog2e)));
+                else acc += gl_s[j] * ex2(fmaf(sm[j * H + h], kLog2e, k) - lk * kLog2e);
             }
         part[pt * H + h] = acc;
     }
@@ -194,10 +206,15 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
         if (d >= 0 && d < nj) {
             const float c = sm[d * H + hh], lse = lse_s[hh], lk = lk_s[d];
             if (c > -INFINITY && lse > -INFINITY) {
-                const float soft = ex2((c - lse) * kLog2e);
                 float pg = 0.f;
-                if (lk > -INFINITY) pg = gl_s[d] * ex2(((c - lse) + gate_s[hh] - lk) * kLog2e);
-                v = pg - soft * S_s[hh];
+                if (kBias) {
+                    if (lk > -INFINITY) pg = __fmul_rn(gl_s[d], ex2((c - lse) + (gate_s[hh] - lk) * kLog2e));
+                    v = __fmaf_rn(-ex2(c - lse), S_s[hh], pg);
+                } else {
+                    const float soft = ex2((c - lse) * kLog2e);
+                    if (lk > -INFINITY) pg = gl_s[d] * ex2(((c - lse) + gate_s[hh] - lk) * kLog2e);
+                    v = pg - soft * S_s[hh];
+                }
             }
         }
         grow[x] = v;

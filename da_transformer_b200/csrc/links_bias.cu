@@ -142,13 +142,22 @@ __device__ __forceinline__ float lb_max_over_heads(float v) {
     for (int o = 1; o < G; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
-// t = c log2e + (b - r)
+// t = z - r with z = c log2e + b rounded as the reference r was, so that t is 0 where z is the reference
 __device__ __forceinline__ float4 lb_shifted(float4 c, float4 b, const float (&r)[4]) {
-    fadd2_rn(b.x, b.y, b.x, b.y, -r[0], -r[1]);
-    fadd2_rn(b.z, b.w, b.z, b.w, -r[2], -r[3]);
     ffma2_rn(b.x, b.y, c.x, c.y, kLog2e, kLog2e);
     ffma2_rn(b.z, b.w, c.z, c.w, kLog2e, kLog2e);
+    fadd2_rn(b.x, b.y, b.x, b.y, -r[0], -r[1]);
+    fadd2_rn(b.z, b.w, b.z, b.w, -r[2], -r[3]);
     return b;
+}
+// Gradient of four scores, q w - soft S: the product is rounded as its sum S was, so that a vertex with one successor
+// (soft = 1, S that product) has the gradient 0 that it has by definition
+__device__ __forceinline__ float4 lb_grad(float4 soft, float4 q, float w, const float (&S)[4]) {
+    fmul2_rn(q.x, q.y, q.x, q.y, w, w);
+    fmul2_rn(q.z, q.w, q.z, q.w, w, w);
+    ffma2_rn(q.x, q.y, soft.x, soft.y, -S[0], -S[1]);
+    ffma2_rn(q.z, q.w, soft.z, soft.w, -S[2], -S[3]);
+    return q;
 }
 
 // Shared memory of both kernels: the bias by distance [K * H], two rows of scores [K * H], red [2][NT / 32][H].
@@ -258,7 +267,7 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
         if (head_lse && tid < G) {
 #pragma unroll
             for (int k = 0; k < 4; k++)
-                head_lse[r0.row * H + 4 * g + k] = some[k] ? (r[k] + lg2(sum[k])) * kLn2 : -INFINITY;
+                head_lse[r0.row * H + 4 * g + k] = some[k] ? r[k] + lg2(sum[k]) : -INFINITY;
         }
         float *out = links + r0.row * (int64_t)K;
 #pragma unroll
@@ -337,8 +346,8 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         const LbRow r2 = lb_row(slot + 2 * step, rows, L, K, mk);
         const unsigned live2 = lb_live<G, NT, U>(r2, L, mk);
         // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
-        const float ls[4] = {lse0.x > -INFINITY ? lse0.x * kLog2e : INFINITY, lse0.y > -INFINITY ? lse0.y * kLog2e : INFINITY,
-                             lse0.z > -INFINITY ? lse0.z * kLog2e : INFINITY, lse0.w > -INFINITY ? lse0.w * kLog2e : INFINITY};
+        const float ls[4] = {lse0.x > -INFINITY ? lse0.x : INFINITY, lse0.y > -INFINITY ? lse0.y : INFINITY,
+                             lse0.z > -INFINITY ? lse0.z : INFINITY, lse0.w > -INFINITY ? lse0.w : INFINITY};
         const float g2[4] = {gate0.x * kLog2e, gate0.y * kLog2e, gate0.z * kLog2e, gate0.w * kLog2e};
         const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
         lb_copy_wait<1>();
@@ -772,12 +781,35 @@ __device__ __forceinline__ void lw_terms(float4 (&t)[N], const float *buf, int H
 }
 __device__ __forceinline__ float4 lw_exp2(float4 t) { return make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w)); }
 
+// q_h = soft_h exp(g_h)
+__device__ __forceinline__ float4 lw_gated(float4 soft, const float (&eg)[4]) {
+    fmul2_rn(soft.x, soft.y, soft.x, soft.y, eg[0], eg[1]);
+    fmul2_rn(soft.z, soft.w, soft.z, soft.w, eg[2], eg[3]);
+    return soft;
+}
+
 // A link that the flush of the exponentials could have touched, from the terms' logarithms (g + z - lse, log2 units)
 template <int G>
 __device__ __noinline__ float lw_tiny_link(float a0, float a1, float a2, float a3) {
     const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3))), mm = m > -INFINITY ? m : 0.f;
     const float q = lb_over_heads<G>(ex2(a0 - mm) + ex2(a1 - mm) + ex2(a2 - mm) + ex2(a3 - mm));
     return m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
+}
+
+// The link to an only successor: the log-sum-exp of the gates of the heads that have a sum, near 0 where the gates are
+// log-probabilities, so that the 2^-22 of lg2 would be all of it.  Heads on lanes.
+template <int G>
+__device__ __noinline__ float lw_only_link(float4 gate, const float (&sum)[4], int H) {
+    const int lane = threadIdx.x & 31;
+    const float gates[4] = {gate.x, gate.y, gate.z, gate.w};
+    float g = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const float o = __shfl_sync(0xffffffffu, sum[k] > 0.f && sum[k] < INFINITY ? gates[k] : -INFINITY, lane / 4);
+        if ((lane & 3) == k && lane < H) g = o;
+    }
+    const float m = warp_max(g), mm = m > -INFINITY ? m : 0.f;
+    return mm + logf(warp_sum(expf(g - mm)));
 }
 
 // G_d p_h of a distance whose sum over the heads the 32-bit exponent has flushed: relative to its largest term (t, g2 in
@@ -921,14 +953,18 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             }
             if (head_lse && lane < G) {
                 float4 o;
-                o.x = ls[0] < INFINITY ? (r[0] + ls[0]) * kLn2 : -INFINITY;
-                o.y = ls[1] < INFINITY ? (r[1] + ls[1]) * kLn2 : -INFINITY;
-                o.z = ls[2] < INFINITY ? (r[2] + ls[2]) * kLn2 : -INFINITY;
-                o.w = ls[3] < INFINITY ? (r[3] + ls[3]) * kLn2 : -INFINITY;
+                o.x = ls[0] < INFINITY ? r[0] + ls[0] : -INFINITY;
+                o.y = ls[1] < INFINITY ? r[1] + ls[1] : -INFINITY;
+                o.z = ls[2] < INFINITY ? r[2] + ls[2] : -INFINITY;
+                o.w = ls[3] < INFINITY ? r[3] + ls[3] : -INFINITY;
                 lw_put<G, kExact>(head_lse + r0.row * H, g, H, o);
             }
             float *const out = links + r0.row * (int64_t)K;
-            lw_batches(nvec, [&](auto n, auto part, int v) {
+            if (r0.nj == 1) {
+                const float link = lw_only_link<G>(gate, sum, H);
+                if (lane == 0) out[0] = link;
+            }
+            lw_batches(r0.nj == 1 ? 0 : nvec, [&](auto n, auto part, int v) {
                 constexpr int N = decltype(n)::value;
                 constexpr bool kPart = decltype(part)::value;
                 float q[N];
@@ -980,8 +1016,8 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
     if (stalled && lb.status) atomicOr(lb.status, DAT_STATUS_STALLED);
 }
 
-// Backward.  With w_d = G_d / sum_h q the gradient of a score is soft_h (exp(g_h) w_d - S_h): the scores' place holds
-// soft and then the gradient itself, which the four rows' warps add to their sums by distance (registers of the 128
+// Backward.  With q_h = soft_h exp(g_h) and w_d = G_d / sum_h q_h the gradient of a score is q_h w_d - soft_h S_h: the
+// scores' place holds soft and then the gradient itself, which the four rows' warps add to their sums by distance (registers of the 128
 // threads, UA vectors each).
 template <int G, bool kExact, int UA, int NG>
 __global__ void __launch_bounds__(NG * kLwRows * 32, UA <= 4 ? 2 : 1)
@@ -1038,8 +1074,8 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             __syncwarp();
         }
         // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
-        const float ls[4] = {lse.x > -INFINITY ? lse.x * kLog2e : INFINITY, lse.y > -INFINITY ? lse.y * kLog2e : INFINITY,
-                             lse.z > -INFINITY ? lse.z * kLog2e : INFINITY, lse.w > -INFINITY ? lse.w * kLog2e : INFINITY};
+        const float ls[4] = {lse.x > -INFINITY ? lse.x : INFINITY, lse.y > -INFINITY ? lse.y : INFINITY,
+                             lse.z > -INFINITY ? lse.z : INFINITY, lse.w > -INFINITY ? lse.w : INFINITY};
         const float g2[4] = {gate.x * kLog2e, gate.y * kLog2e, gate.z * kLog2e, gate.w * kLog2e};
         const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
         float S[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1060,9 +1096,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             for (int u = 0; u < N; u++) {
                 const bool in = !kPart || v + 32 * u < nvec;
                 const float4 soft = lw_exp2(t[u]);
-                q[u] = soft;
-                fmul2_rn(q[u].x, q[u].y, q[u].x, q[u].y, eg[0], eg[1]);
-                fmul2_rn(q[u].z, q[u].w, q[u].z, q[u].w, eg[2], eg[3]);
+                q[u] = lw_gated(soft, eg);
                 const float tot = lb_over_heads<G>((q[u].x + q[u].y) + (q[u].z + q[u].w));
                 if (in) {
                     lw_put<G, kExact>(buf, v + 32 * u, H, soft);
@@ -1130,23 +1164,16 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
                         const bool dead = np && !np[x / G];
                         const float4 t = dead ? lb_ninf4() : lb_shifted(lw_get<G, kExact>(src, x, H, -INFINITY), lw_bias<G>(table, bucket, x), ls);
                         const float4 p = lw_full_share<G>(t, g2, __ldg(grad_links + r0.row * (int64_t)K + x / G));
-                        float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
-                        if (__float_as_uint(w[u]) == kLwFull) {
-                            k = make_float4(fmaf(k.x, o[u].x, p.x), fmaf(k.y, o[u].y, p.y), fmaf(k.z, o[u].z, p.z), fmaf(k.w, o[u].w, p.w));
-                        } else {
-                            k = make_float4(o[u].x * fmaf(eg[0], w[u], k.x), o[u].y * fmaf(eg[1], w[u], k.y),
-                                            o[u].z * fmaf(eg[2], w[u], k.z), o[u].w * fmaf(eg[3], w[u], k.w));
-                        }
+                        float4 k = lb_grad(o[u], lw_gated(o[u], eg), w[u], S);
+                        if (__float_as_uint(w[u]) == kLwFull)
+                            k = make_float4(fmaf(-S[0], o[u].x, p.x), fmaf(-S[1], o[u].y, p.y), fmaf(-S[2], o[u].z, p.z),
+                                            fmaf(-S[3], o[u].w, p.w));
                         if (v + 32 * u < nvec) lw_put<G, kExact>(buf, v + 32 * u, H, k);
                     }
                 } else {
 #pragma unroll
                     for (int u = 0; u < N; u++) {
-                        float4 k = make_float4(-S[0], -S[1], -S[2], -S[3]);
-                        ffma2_rn(k.x, k.y, eg[0], eg[1], w[u], w[u]);
-                        ffma2_rn(k.z, k.w, eg[2], eg[3], w[u], w[u]);
-                        fmul2_rn(o[u].x, o[u].y, o[u].x, o[u].y, k.x, k.y);
-                        fmul2_rn(o[u].z, o[u].w, o[u].z, o[u].w, k.z, k.w);
+                        o[u] = lb_grad(o[u], lw_gated(o[u], eg), w[u], S);
                         if (!kPart || v + 32 * u < nvec) lw_put<G, kExact>(buf, v + 32 * u, H, o[u]);
                     }
                 }

@@ -355,7 +355,7 @@ int dat_upload_links(const float *host_links, float *dev_links, int bsz, int pre
  *   bias_table [num_buckets,heads] fp32, buckets [translen] int64: the bucket of each distance 1..translen.
  * A bucket outside [0, num_buckets) forbids the transitions of its distance (-inf, no gradient) and sets
  * DAT_STATUS_BAD_INDEX.  spans ([bsz,2], 8-byte aligned; NULL without nonpad): written here, read by the backward.
- * The other arguments are those of dat_links_from_heads.
+ * head_lse (for the backward alone) is in log2 units.  The other arguments are those of dat_links_from_heads.
  */
 int dat_links_from_heads_biased(const float *content, const float *log_gates, const float *bias_table,
                                 const int64_t *buckets, int num_buckets, const int64_t *bound_end,

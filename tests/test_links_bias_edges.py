@@ -1,0 +1,80 @@
+"""Biased links (``dag_links_from_heads(..., relative_bias=...)``) at the edges of their definition: vertices with one
+successor, gates of any size, values that are no numbers, and sizes that leave the shared memory.
+
+Every test runs the three forms of the kernels: a warp per vertex (the ordinary sizes), a CTA per vertex (here by a table
+of more than 2048 numbers) and the kernels of the links without a bias (here by more than 32 heads, or by such a table
+and a head count that is no multiple of four)."""
+import numpy as np
+import pytest
+import torch
+
+import da_transformer_b200 as dat
+from test_links_bias import make, oracle
+
+DEV = "cuda:0"
+NEG_INF = float("-inf")
+NAN = float("nan")
+U = 2.0 ** -24          # half a step of fp32 relative to the value
+
+# heads, buckets of the table: a warp per vertex (exact and filled-up groups of heads), a CTA per vertex, the others
+FORMS = [(1, 8), (2, 8), (4, 8), (5, 8), (6, 8), (8, 8), (12, 8), (16, 8), (32, 8), (4, 600), (8, 300), (16, 200), (32, 100),
+         (1, 600), (5, 300), (12, 200), (40, 8), (128, 8)]
+
+
+def run(content, gates, table, bk, K, grad, **mask):
+    """links and the gradients of scores, gates and table, on the CPU in 64 bits."""
+    leaves = [t.detach().clone().requires_grad_() for t in (content, gates, table)]
+    links = dat.dag_links_from_heads(leaves[0], leaves[1], max_transition_length=K, relative_bias=leaves[2],
+                                     relative_buckets=bk, **mask)
+    grads = torch.autograd.grad(links, leaves, grad)
+    return [t.detach().double().cpu().numpy() for t in (links, *grads)]
+
+
+def some_buckets(K, n, seed=1):
+    return torch.randint(0, n, (K,), generator=torch.Generator().manual_seed(seed)).to(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0.0, 50.0, 1000.0])
+@pytest.mark.parametrize("H,buckets", FORMS)
+def test_one_successor(H, buckets, offset):
+    """A softmax over one element is 1 whatever the score: the gradient of the scores and of the table is 0, the link the
+    log-sum-exp of the gates, and with one head whose gate is 0 the link is 0.
+
+    The log-sum-exp: each exponential is off by 2^-22 of itself, their sum by 2^-24 in each of its log2(H) + 2 steps
+    (2^-20 for all at most), its logarithm by 2^-22, the result by half a step."""
+    B, L = 3, 20
+    content, gates, table, grad, _, _ = make(B, L, H, L - 1, buckets=buckets, seed=H)
+    if H == 1:
+        gates.zero_()
+    content += offset
+    ar = torch.arange(L, device=DEV)
+    last = (ar == L - 1).expand(B, L)                                   # all vertices reach the last one alone
+    two = ar.view(1, L) < torch.tensor([2, 1, L], device=DEV).view(B, 1)   # graphs of two, one and L vertices
+    cases = [(1, {}), (1, dict(nonpad_mask=two)), (L - 1, dict(bound_end=(ar + 1).expand(B, L).contiguous())),
+             (L - 1, dict(nonpad_mask=last)), (3, dict(nonpad_mask=last))]
+    if H <= 8:
+        cases.append((1, dict(bound_end=(ar + 1).expand(B, L).contiguous())))
+    for K, mask in cases:
+        bk, g = some_buckets(K, buckets), grad[..., :K].contiguous()
+        links, gc, gg, gt = run(content, gates, table, bk, K, g, **mask)
+        fin = np.isfinite(links)
+        assert fin.sum(2).max() == 1 and fin.any()
+        assert not gc.any() and not gt.any(), (K, list(mask), np.abs(gc).max(), np.abs(gt).max())
+        want = torch.logsumexp(gates.double(), -1).cpu().numpy()[..., None] * np.ones_like(links)
+        assert (np.abs(links - want)[fin] <= (0 if H == 1 else 2.0 ** -20 + U * np.abs(want[fin]))).all()
+        assert (links[~fin] == NEG_INF).all()
+        share = torch.softmax(gates.double(), -1).cpu().numpy()
+        at = np.where(fin, g.double().cpu().numpy(), 0).sum(2)[..., None]
+        assert (np.abs(gg - at * share) <= 2.0 ** -19 * np.abs(at)).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,buckets", [(1, 8), (6, 8), (8, 8), (8, 300), (5, 300), (40, 8)])
+def test_last_but_one_vertex_of_a_training_graph(H, buckets):
+    """Padded graphs: the last but one vertex of each has a single successor, scores near 1000."""
+    B, L = 4, 30
+    content, gates, table, grad, _, nonpad = make(B, L, H, L - 1, buckets=buckets, seed=2)
+    _, gc, _, _ = run(content + 1000, gates, table, some_buckets(L - 1, buckets), L - 1, grad, nonpad_mask=nonpad)
+    for b, n in enumerate(nonpad.sum(1).tolist()):
+        assert not gc[b, n - 2].any() and gc[b, n - 3].any()
