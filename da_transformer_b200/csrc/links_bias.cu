@@ -15,7 +15,8 @@
 // bit).  One exponential per score and direction:
 //   forward   e = exp(z - r_h), r_h the score of the nearest successor in place of the maximum over all of them:
 //             the sum is at least 1, and a vertex where it overflows (a score 60 above r_h) or whose nearest
-//             successor is masked takes the maximum after all.  links = log sum_h e_h exp(g_h) / S_h.
+//             successor is masked takes the maximum after all.  links = log sum_h e_h exp(g_h) / S_h,
+//             the gates relative to the vertex's largest.
 //   backward  soft = exp(z - lse_h), q_h = soft exp(g_h), p_h = q_h / sum q.
 // Where sum q is below 2^-80 (a link below -55) it is taken again relative to its largest term, so that what
 // the 32-bit exponent flushes stays below 2^-40 of what it is added to.
@@ -142,6 +143,17 @@ __device__ __forceinline__ float lb_max_over_heads(float v) {
     for (int o = 1; o < G; o <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
+// The gates of a vertex less its largest, in log2 units, so that their exponentials are at most 1 whatever the gates are;
+// returns what was taken away (it is added to the link; the shares of the heads do not change with it)
+template <int G>
+__device__ __forceinline__ float lb_gates(float4 gate, float (&g2)[4]) {
+    const float top = lb_max_over_heads<G>(fmaxf(fmaxf(gate.x, gate.y), fmaxf(gate.z, gate.w))), m = top > -INFINITY ? top : 0.f;
+    g2[0] = (gate.x - m) * kLog2e;
+    g2[1] = (gate.y - m) * kLog2e;
+    g2[2] = (gate.z - m) * kLog2e;
+    g2[3] = (gate.w - m) * kLog2e;
+    return m;
+}
 // t = z - r with z = c log2e + b rounded as the reference r was, so that t is 0 where z is the reference
 __device__ __forceinline__ float4 lb_shifted(float4 c, float4 b, const float (&r)[4]) {
     ffma2_rn(b.x, b.y, c.x, c.y, kLog2e, kLog2e);
@@ -256,8 +268,8 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
         }
         lb_collect<G, NT, false>(sum, rd);
         // f_h = exp(g_h) / S_h; a head without a finite score takes no part
-        const float g2[4] = {gate0.x * kLog2e, gate0.y * kLog2e, gate0.z * kLog2e, gate0.w * kLog2e};
-        float f[4];
+        float g2[4], f[4];
+        const float top = lb_gates<G>(gate0, g2);
         bool some[4];
 #pragma unroll
         for (int k = 0; k < 4; k++) {
@@ -278,7 +290,7 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             float link = -INFINITY;
             if (u * NT + (tid & ~31) < nvec) {
                 float q = lb_over_heads<G>(fmaf(e4[u].x, f[0], e4[u].y * f[1]) + fmaf(e4[u].z, f[2], e4[u].w * f[3]));
-                link = ok ? lg2(q) * kLn2 : -INFINITY;
+                link = ok ? fmaf(lg2(q), kLn2, top) : -INFINITY;
                 if (__any_sync(0xffffffffu, ok && q < kLbTiny)) {
                     float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (ok) {   // log2 of e f without the exponential's flush
@@ -291,7 +303,7 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                     const float m = lb_max_over_heads<G>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
                     const float mm = m > -INFINITY ? m : 0.f;
                     q = lb_over_heads<G>(ex2(t[0] - mm) + ex2(t[1] - mm) + ex2(t[2] - mm) + ex2(t[3] - mm));
-                    link = m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
+                    link = m > -INFINITY ? fmaf(m + lg2(q), kLn2, top) : -INFINITY;
                 }
             }
             if (g == 0 && d < K) out[d] = link;
@@ -348,7 +360,8 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
         const float ls[4] = {lse0.x > -INFINITY ? lse0.x : INFINITY, lse0.y > -INFINITY ? lse0.y : INFINITY,
                              lse0.z > -INFINITY ? lse0.z : INFINITY, lse0.w > -INFINITY ? lse0.w : INFINITY};
-        const float g2[4] = {gate0.x * kLog2e, gate0.y * kLog2e, gate0.z * kLog2e, gate0.w * kLog2e};
+        float g2[4];
+        lb_gates<G>(gate0, g2);
         const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
         lb_copy_wait<1>();
         float4 p4[U];
@@ -788,12 +801,13 @@ __device__ __forceinline__ float4 lw_gated(float4 soft, const float (&eg)[4]) {
     return soft;
 }
 
-// A link that the flush of the exponentials could have touched, from the terms' logarithms (g + z - lse, log2 units)
+// A link that the flush of the exponentials could have touched, from the terms' logarithms (g + z - lse, log2 units); top:
+// what was taken from the gates
 template <int G>
-__device__ __noinline__ float lw_tiny_link(float a0, float a1, float a2, float a3) {
+__device__ __noinline__ float lw_tiny_link(float a0, float a1, float a2, float a3, float top) {
     const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3))), mm = m > -INFINITY ? m : 0.f;
     const float q = lb_over_heads<G>(ex2(a0 - mm) + ex2(a1 - mm) + ex2(a2 - mm) + ex2(a3 - mm));
-    return m > -INFINITY ? (m + lg2(q)) * kLn2 : -INFINITY;
+    return m > -INFINITY ? fmaf(m + lg2(q), kLn2, top) : -INFINITY;
 }
 
 // The link to an only successor: the log-sum-exp of the gates of the heads that have a sum, near 0 where the gates are
@@ -943,8 +957,8 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             }
             lw_reduce<G, false>(sum);
             // f_h = exp(g_h) / S_h; a head without a finite score takes no part
-            const float g2[4] = {gate.x * kLog2e, gate.y * kLog2e, gate.z * kLog2e, gate.w * kLog2e};
-            float f[4], ls[4];
+            float g2[4], f[4], ls[4];
+            const float top = lb_gates<G>(gate, g2);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const bool some = sum[k] > 0.f && sum[k] < INFINITY;
@@ -978,7 +992,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 }
                 const bool tiny = __any_sync(0xffffffffu, least < kLbTiny);
 #pragma unroll
-                for (int u = 0; u < N; u++) q[u] = lg2(q[u]) * kLn2;
+                for (int u = 0; u < N; u++) q[u] = fmaf(lg2(q[u]), kLn2, top);
                 if (tiny) {
                     for (int u = 0; u < N; u++) {
                         const int x = v + 32 * u;
@@ -990,7 +1004,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                             if (ls[2] < INFINITY) t[2] = z.z + (g2[2] - ls[2]);
                             if (ls[3] < INFINITY) t[3] = z.w + (g2[3] - ls[3]);
                         }
-                        const float link = lw_tiny_link<G>(t[0], t[1], t[2], t[3]);
+                        const float link = lw_tiny_link<G>(t[0], t[1], t[2], t[3], top);
                         if (g == 0 && x < nvec) out[x / G] = link;
                     }
                 } else {
@@ -1076,7 +1090,8 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
         const float ls[4] = {lse.x > -INFINITY ? lse.x : INFINITY, lse.y > -INFINITY ? lse.y : INFINITY,
                              lse.z > -INFINITY ? lse.z : INFINITY, lse.w > -INFINITY ? lse.w : INFINITY};
-        const float g2[4] = {gate.x * kLog2e, gate.y * kLog2e, gate.z * kLog2e, gate.w * kLog2e};
+        float g2[4];
+        lb_gates<G>(gate, g2);
         const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
         float S[4] = {0.f, 0.f, 0.f, 0.f};
         lw_batches(nvec, [&](auto n, auto part, int v) {

@@ -78,3 +78,39 @@ def test_last_but_one_vertex_of_a_training_graph(H, buckets):
     _, gc, _, _ = run(content + 1000, gates, table, some_buckets(L - 1, buckets), L - 1, grad, nonpad_mask=nonpad)
     for b, n in enumerate(nonpad.sum(1).tolist()):
         assert not gc[b, n - 2].any() and gc[b, n - 3].any()
+
+
+def against_64_bits(content, gates, table, bk, K, grad, size, links_off=0.0, **mask):
+    """size: the largest number that scores, gates and links are put together from; each is rounded a few times in 32
+    bits, which a probability carries as a factor."""
+    got = run(content, gates, table, bk, K, grad, **mask)
+    want = oracle(content, gates, table, bk, K, grad=grad, **mask)
+    fin = np.isfinite(want[0])
+    assert np.array_equal(got[0][~fin], want[0][~fin])
+    tol = 8 * U * size + 2e-6
+    assert np.abs(got[0][fin] - want[0][fin]).max() <= tol + links_off
+    rows = content.shape[0] * content.shape[1]
+    for name, a, b, terms in zip(("scores", "gates", "table"), got[1:], want[1:], (1, rows ** 0.5, rows)):
+        off = np.abs(a - b).max()
+        assert off <= 4 * tol * float(grad.abs().max()) * terms + 1e-4 * np.abs(b).max(), (name, off)
+    return got
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,buckets", FORMS)
+@pytest.mark.parametrize("kind", ["all", "one", "far"])
+def test_gates_above_zero(H, buckets, kind):
+    """log_gates may be any numbers: +100 for all heads of a vertex, for one of them, +3000 and -3000."""
+    B, L = 2, 24
+    content, gates, table, grad, _, nonpad = make(B, L, H, L - 1, buckets=buckets, seed=H + 1)
+    if kind == "all":
+        gates[:, ::2] += 100
+    elif kind == "one":
+        gates[:, ::2, 0] = 100
+        gates[:, 1::2, -1] = 100
+    else:
+        gates[:, ::2, 0] = 3000
+        gates[:, 1::3] = -3000
+    got = against_64_bits(content, gates, table, some_buckets(L - 1, buckets), L - 1, grad, float(gates.abs().max()) + 10,
+                          nonpad_mask=nonpad)
+    assert np.isfinite(got[1]).all() and np.isfinite(got[2]).all() and np.isfinite(got[3]).all()
