@@ -19,7 +19,9 @@
 //             the gates relative to the vertex's largest.
 //   backward  soft = exp(z - lse_h), q_h = soft exp(g_h), p_h = q_h / sum q.
 // Where sum q is below 2^-80 (a link below -55) it is taken again relative to its largest term, so that what
-// the 32-bit exponent flushes stays below 2^-40 of what it is added to.
+// the 32-bit exponent flushes stays below 2^-40 of what it is added to: below 2^-126 in the backward, where soft and exp(g)
+// are at most 1, and in the forward as long as exp(g_h) / S_h is a normal number (S_h may reach 2^86).  A vertex with a
+// head whose factor is below 2^-100 takes all its links that way.
 // Two forms, a warp or a CTA per vertex (below): the first up to 32 heads and rows of 2048 vectors that fit its rings,
 // the second 4, 8, 16 and 32 heads up to 4096 vectors.  What neither takes goes to the kernels of links.cu (one CTA per
 // vertex, scores in shared memory) and a pass over the gradient's diagonals.
@@ -32,6 +34,7 @@ namespace dat {
 
 constexpr float kLbTiny = 0x1p-80f;
 constexpr float kLbHuge = 0x1p+86f;
+constexpr float kLbRare = 0x1p-100f;    // a head's factor below this may lose terms that count: the logarithms are taken
 constexpr int kLbMaxVec = 4096;         // score vectors per vertex: 512 threads with eight each
 
 // bias by distance in log2 units into shared memory; -inf for a bucket outside the table
@@ -270,12 +273,14 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
         // f_h = exp(g_h) / S_h; a head without a finite score takes no part
         float g2[4], f[4];
         const float top = lb_gates<G>(gate0, g2);
-        bool some[4];
+        bool some[4], rare = false;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
             some[k] = sum[k] > 0.f && sum[k] < INFINITY;
             f[k] = some[k] ? __fdividef(ex2(g2[k]), sum[k]) : 0.f;
+            rare |= some[k] && f[k] < kLbRare && g2[k] > -INFINITY;
         }
+        rare = __any_sync(0xffffffffu, rare);
         if (head_lse && tid < G) {
 #pragma unroll
             for (int k = 0; k < 4; k++)
@@ -291,7 +296,7 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             if (u * NT + (tid & ~31) < nvec) {
                 float q = lb_over_heads<G>(fmaf(e4[u].x, f[0], e4[u].y * f[1]) + fmaf(e4[u].z, f[2], e4[u].w * f[3]));
                 link = ok ? fmaf(lg2(q), kLn2, top) : -INFINITY;
-                if (__any_sync(0xffffffffu, ok && q < kLbTiny)) {
+                if (rare || __any_sync(0xffffffffu, ok && q < kLbTiny)) {
                     float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (ok) {   // log2 of e f without the exponential's flush
                         const float4 z = lb_shifted(stage[v], bl4[v], r);
@@ -959,12 +964,15 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             // f_h = exp(g_h) / S_h; a head without a finite score takes no part
             float g2[4], f[4], ls[4];
             const float top = lb_gates<G>(gate, g2);
+            float least = 1.f;   // of the factors of the heads that take part
 #pragma unroll
             for (int k = 0; k < 4; k++) {
                 const bool some = sum[k] > 0.f && sum[k] < INFINITY;
                 ls[k] = some ? lg2(sum[k]) : INFINITY;
                 f[k] = some ? __fdividef(ex2(g2[k]), sum[k]) : 0.f;
+                if (some && g2[k] > -INFINITY) least = fminf(least, f[k]);
             }
+            const float enough = __any_sync(0xffffffffu, least < kLbRare) ? INFINITY : kLbTiny;   // of the links' sums
             if (head_lse && lane < G) {
                 float4 o;
                 o.x = ls[0] < INFINITY ? r[0] + ls[0] : -INFINITY;
@@ -990,7 +998,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                     if (kPart && v + 32 * u >= nvec) q[u] = 1.f;
                     least = fminf(least, q[u]);
                 }
-                const bool tiny = __any_sync(0xffffffffu, least < kLbTiny);
+                const bool tiny = __any_sync(0xffffffffu, least < enough);
 #pragma unroll
                 for (int u = 0; u < N; u++) q[u] = fmaf(lg2(q[u]), kLn2, top);
                 if (tiny) {

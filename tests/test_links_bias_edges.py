@@ -114,3 +114,22 @@ def test_gates_above_zero(H, buckets, kind):
     got = against_64_bits(content, gates, table, some_buckets(L - 1, buckets), L - 1, grad, float(gates.abs().max()) + 10,
                           nonpad_mask=nonpad)
     assert np.isfinite(got[1]).all() and np.isfinite(got[2]).all() and np.isfinite(got[3]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,buckets", [f for f in FORMS if f[0] >= 2])
+@pytest.mark.parametrize("gap,gate,other", [(55, -45, -70), (58, -48, -54), (59, -35, -60), (50, -50, -69), (59, -66, -90)])
+def test_rare_head_far_above_its_nearest_score(H, buckets, gap, gate, other):
+    """A head that is rarely taken, whose score of one successor is far above the nearest successor's, while the other
+    heads all but exclude that successor: the rare head's share is nearly all of the link."""
+    B, L = 2, 9
+    content, gates, table, grad, _, _ = make(B, L, H, L - 1, buckets=buckets, seed=H + 2)
+    gates = torch.log_softmax(gates, -1)
+    content *= 0.1
+    table *= 0.1
+    gates[:, :, H // 2] = gate
+    far = 4                                         # successor 5 of the vertices before it
+    content[:, :far, far + 1] += other
+    content[:, :far, far + 1, H // 2] += gap - other
+    got = against_64_bits(content, gates, table, some_buckets(L - 1, buckets), L - 1, grad, 100.0)
+    assert (np.abs(got[0][:, 0, far] - gate) < 3).all() or other > gate - 4
