@@ -80,7 +80,8 @@ __device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, f
     if (tid < H) {
         float M = kNegBig, S = 0.f;
         for (int p = 0; p < P; p++) lse_merge(M, S, part_m[p * H + tid], part_s[p * H + tid]);
-        lse_s[tid] = (S > 0.f && M > 0.5f * kNegBig) ? (M + lg2(S)) * (kBias ? 1.f : kLn2) : -INFINITY;
+        if (kBias) lse_s[tid] = S != 0.f ? M + lg2(S) : -INFINITY;   // NaN where a score is NaN or +inf
+        else lse_s[tid] = (S > 0.f && M > 0.5f * kNegBig) ? (M + lg2(S)) * kLn2 : -INFINITY;
     }
     __syncthreads();
 }
@@ -110,9 +111,12 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
     // per head, what is added to a score: (gate - lse) in log2 units (kBias: the gate, after the lse); a head whose every
     // score is -inf (lse = -inf) takes no part
     if (tid < H) {
-        const float gate = (kBias ? gate_s[tid] : gate_s[tid] - lse_s[tid]) * kLog2e;
-        gate_s[tid] = lse_s[tid] > -INFINITY ? gate : -INFINITY;
-        if (kBias && !(lse_s[tid] > -INFINITY)) lse_s[tid] = 0.f;
+        if (kBias) {
+            gate_s[tid] = lse_s[tid] == -INFINITY ? -INFINITY : gate_s[tid] * kLog2e;
+            if (lse_s[tid] == -INFINITY) lse_s[tid] = 0.f;
+        } else {
+            gate_s[tid] = lse_s[tid] > -INFINITY ? (gate_s[tid] - lse_s[tid]) * kLog2e : -INFINITY;
+        }
     }
     __syncthreads();
     const auto term = [&](int d, int h) {
@@ -121,10 +125,11 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
     float *out = links + row * (size_t)K;
     for (int d = tid; d < K; d += kLinksThreads) {
         float v = -INFINITY;
-        if (d < nj) {
+        if (d < nj && !(kBias && np_row && !np_row[i + 1 + d])) {
             // max over the heads first, then the sum: no rescaling and no branches inside the loops
             float m = -INFINITY;
             for (int h = 0; h < H; h++) m = fmaxf(m, term(d, h));
+            if (kBias && !(m > -INFINITY)) m = 0.f;   // nothing but -inf and NaN: one or the other comes of it below
             if (m > -INFINITY) {
                 float s = 0.f;
                 for (int h = 0; h < H; h++) s += ex2(term(d, h) - m);
@@ -179,10 +184,10 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
     float acc = 0.f;
     if (pt < P) {
         const float k = (gate_s[h] - lse_s[h]) * kLog2e;
-        if (lse_s[h] > -INFINITY)
+        if (kBias ? lse_s[h] != -INFINITY : lse_s[h] > -INFINITY)
             for (int j = pt; j < nj; j += P) {
                 const float lk = lk_s[j];
-                if (!(lk > -INFINITY)) continue;
+                if (kBias ? lk == -INFINITY : !(lk > -INFINITY)) continue;
                 if (kBias) acc = __fadd_rn(acc, __fmul_rn(gl_s[j], ex2((sm[j * H + h] - lse_s[h]) + (gate_s[h] - lk) * kLog2e)));
                 else acc += gl_s[j] * ex2(fmaf(sm[j * H + h], kLog2e, k) - lk * kLog2e);
             }
@@ -205,16 +210,15 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
         const int d = j - i - 1;
         if (d >= 0 && d < nj) {
             const float c = sm[d * H + hh], lse = lse_s[hh], lk = lk_s[d];
-            if (c > -INFINITY && lse > -INFINITY) {
+            if (kBias) {
+                // (a link of -inf: masked, or no head with a gate above -inf reaches it, and what the others lose, S, is 0)
+                if (lk != -INFINITY && lse != -INFINITY)
+                    v = __fmaf_rn(-ex2(c - lse), S_s[hh], __fmul_rn(gl_s[d], ex2((c - lse) + (gate_s[hh] - lk) * kLog2e)));
+            } else if (c > -INFINITY && lse > -INFINITY) {
+                const float soft = ex2((c - lse) * kLog2e);
                 float pg = 0.f;
-                if (kBias) {
-                    if (lk > -INFINITY) pg = __fmul_rn(gl_s[d], ex2((c - lse) + (gate_s[hh] - lk) * kLog2e));
-                    v = __fmaf_rn(-ex2(c - lse), S_s[hh], pg);
-                } else {
-                    const float soft = ex2((c - lse) * kLog2e);
-                    if (lk > -INFINITY) pg = gl_s[d] * ex2(((c - lse) + gate_s[hh] - lk) * kLog2e);
-                    v = pg - soft * S_s[hh];
-                }
+                if (lk > -INFINITY) pg = gl_s[d] * ex2(((c - lse) + gate_s[hh] - lk) * kLog2e);
+                v = pg - soft * S_s[hh];
             }
         }
         grow[x] = v;

@@ -21,7 +21,8 @@
 // Where sum q is below 2^-80 (a link below -55) it is taken again relative to its largest term, so that what
 // the 32-bit exponent flushes stays below 2^-40 of what it is added to: below 2^-126 in the backward, where soft and exp(g)
 // are at most 1, and in the forward as long as exp(g_h) / S_h is a normal number (S_h may reach 2^86).  A vertex with a
-// head whose factor is below 2^-100 takes all its links that way.
+// head whose factor is below 2^-100 takes all its links that way.  A valid score of NaN or +inf makes the sum of its head
+// NaN, and with it every link and gradient of the vertex, as it does by definition.
 // Two forms, a warp or a CTA per vertex (below): the first up to 32 heads and rows of 2048 vectors that fit its rings,
 // the second 4, 8, 16 and 32 heads up to 4096 vectors.  What neither takes goes to the kernels of links.cu (one CTA per
 // vertex, scores in shared memory) and a pass over the gradient's diagonals.
@@ -34,7 +35,7 @@ namespace dat {
 
 constexpr float kLbTiny = 0x1p-80f;
 constexpr float kLbHuge = 0x1p+86f;
-constexpr float kLbRare = 0x1p-100f;    // a head's factor below this may lose terms that count: the logarithms are taken
+constexpr float kLbRare = 0x1p-100f;
 constexpr int kLbMaxVec = 4096;         // score vectors per vertex: 512 threads with eight each
 
 // bias by distance in log2 units into shared memory; -inf for a bucket outside the table
@@ -157,6 +158,11 @@ __device__ __forceinline__ float lb_gates(float4 gate, float (&g2)[4]) {
     g2[3] = (gate.w - m) * kLog2e;
     return m;
 }
+// A head's factor f = exp(g) / S may lose terms that count, or is NaN: the links are taken from the logarithms (which also
+// keep NaN from the masked places).  A gate of -inf leaves nothing to lose.
+__device__ __forceinline__ bool lb_rare(float f, float g2) { return !(f >= kLbRare || (f == 0.f && g2 == -INFINITY)); }
+// A head's log-sum in the backward; that of one without a finite score is +inf: soft = exp(-inf) = 0
+__device__ __forceinline__ float lb_lse(float lse) { return lse == -INFINITY ? INFINITY : lse; }
 // t = z - r with z = c log2e + b rounded as the reference r was, so that t is 0 where z is the reference
 __device__ __forceinline__ float4 lb_shifted(float4 c, float4 b, const float (&r)[4]) {
     ffma2_rn(b.x, b.y, c.x, c.y, kLog2e, kLog2e);
@@ -276,9 +282,9 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
         bool some[4], rare = false;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            some[k] = sum[k] > 0.f && sum[k] < INFINITY;
+            some[k] = sum[k] != 0.f;
             f[k] = some[k] ? __fdividef(ex2(g2[k]), sum[k]) : 0.f;
-            rare |= some[k] && f[k] < kLbRare && g2[k] > -INFINITY;
+            rare |= some[k] && lb_rare(f[k], g2[k]);
         }
         rare = __any_sync(0xffffffffu, rare);
         if (head_lse && tid < G) {
@@ -296,7 +302,7 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             if (u * NT + (tid & ~31) < nvec) {
                 float q = lb_over_heads<G>(fmaf(e4[u].x, f[0], e4[u].y * f[1]) + fmaf(e4[u].z, f[2], e4[u].w * f[3]));
                 link = ok ? fmaf(lg2(q), kLn2, top) : -INFINITY;
-                if (rare || __any_sync(0xffffffffu, ok && q < kLbTiny)) {
+                if (rare || __any_sync(0xffffffffu, ok && !(q >= kLbTiny))) {
                     float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                     if (ok) {   // log2 of e f without the exponential's flush
                         const float4 z = lb_shifted(stage[v], bl4[v], r);
@@ -308,7 +314,7 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                     const float m = lb_max_over_heads<G>(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
                     const float mm = m > -INFINITY ? m : 0.f;
                     q = lb_over_heads<G>(ex2(t[0] - mm) + ex2(t[1] - mm) + ex2(t[2] - mm) + ex2(t[3] - mm));
-                    link = m > -INFINITY ? fmaf(m + lg2(q), kLn2, top) : -INFINITY;
+                    link = ok ? fmaf(mm + lg2(q), kLn2, top) : -INFINITY;
                 }
             }
             if (g == 0 && d < K) out[d] = link;
@@ -362,9 +368,7 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         const float4 lse1 = of_row(head_lse, r1), gate1 = of_row(log_gates, r1);
         const LbRow r2 = lb_row(slot + 2 * step, rows, L, K, mk);
         const unsigned live2 = lb_live<G, NT, U>(r2, L, mk);
-        // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
-        const float ls[4] = {lse0.x > -INFINITY ? lse0.x : INFINITY, lse0.y > -INFINITY ? lse0.y : INFINITY,
-                             lse0.z > -INFINITY ? lse0.z : INFINITY, lse0.w > -INFINITY ? lse0.w : INFINITY};
+        const float ls[4] = {lb_lse(lse0.x), lb_lse(lse0.y), lb_lse(lse0.z), lb_lse(lse0.w)};
         float g2[4];
         lb_gates<G>(gate0, g2);
         const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
@@ -384,15 +388,15 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             float4 q = make_float4(soft.x * eg[0], soft.y * eg[1], soft.z * eg[2], soft.w * eg[3]);
             const float tot = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
             float w = tot >= kLbTiny ? __fdividef(gd[u], tot) : 0.f;
-            if (__any_sync(0xffffffffu, ok && tot < kLbTiny)) {
+            if (__any_sync(0xffffffffu, ok && !(tot >= kLbTiny))) {
                 const float a[4] = {t.x + g2[0], t.y + g2[1], t.z + g2[2], t.w + g2[3]};
                 const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3])));
-                if (tot < kLbTiny) {   // the same in all lanes of a distance
+                if (!(tot >= kLbTiny)) {   // the same in all lanes of a distance
                     const float mm = m > -INFINITY ? m : 0.f;
                     q = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
                 }
                 const float tot2 = lb_over_heads<G>((q.x + q.y) + (q.z + q.w));
-                w = tot2 > 0.f ? gd[u] / tot2 : 0.f;
+                w = ok && tot2 != 0.f ? gd[u] / tot2 : 0.f;
             }
             // a link of -inf has w = 0 times a gradient that may be anything
             p4[u] = w != 0.f ? make_float4(q.x * w, q.y * w, q.z * w, q.w * w) : p4[u];
@@ -412,6 +416,7 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         if (tid < G)
             reinterpret_cast<float4 *>(grad_log_gates + r0.row * H)[g] = make_float4(S[0], S[1], S[2], S[3]);
         float4 *dst = rowv + (r0.i + 1) * G;
+        const bool odd = !(fabsf(S[0] + S[1] + S[2] + S[3]) < INFINITY);
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int v = tid + u * NT;
@@ -420,6 +425,7 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             float4 o = p4[u];
             ffma2_rn(o.x, o.y, soft.x, soft.y, -S[0], -S[1]);
             ffma2_rn(o.z, o.w, soft.z, soft.w, -S[2], -S[3]);
+            if (odd && !(live0 >> u & 1)) o = make_float4(0.f, 0.f, 0.f, 0.f);   // a masked place beside NaN
             dst[v] = o;
             fadd2_rn(acc[u].x, acc[u].y, acc[u].x, acc[u].y, o.x, o.y);
             fadd2_rn(acc[u].z, acc[u].w, acc[u].z, acc[u].w, o.z, o.w);
@@ -812,7 +818,7 @@ template <int G>
 __device__ __noinline__ float lw_tiny_link(float a0, float a1, float a2, float a3, float top) {
     const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a0, a1), fmaxf(a2, a3))), mm = m > -INFINITY ? m : 0.f;
     const float q = lb_over_heads<G>(ex2(a0 - mm) + ex2(a1 - mm) + ex2(a2 - mm) + ex2(a3 - mm));
-    return m > -INFINITY ? fmaf(m + lg2(q), kLn2, top) : -INFINITY;
+    return fmaf(mm + lg2(q), kLn2, top);
 }
 
 // The link to an only successor: the log-sum-exp of the gates of the heads that have a sum, near 0 where the gates are
@@ -824,7 +830,7 @@ __device__ __noinline__ float lw_only_link(float4 gate, const float (&sum)[4], i
     float g = -INFINITY;
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        const float o = __shfl_sync(0xffffffffu, sum[k] > 0.f && sum[k] < INFINITY ? gates[k] : -INFINITY, lane / 4);
+        const float o = __shfl_sync(0xffffffffu, sum[k] == 0.f ? -INFINITY : sum[k] > 0.f ? gates[k] : sum[k], lane / 4);
         if ((lane & 3) == k && lane < H) g = o;
     }
     const float m = warp_max(g), mm = m > -INFINITY ? m : 0.f;
@@ -839,7 +845,7 @@ __device__ __noinline__ float4 lw_full_share(float4 t, const float (&g2)[4], flo
     const float m = lb_max_over_heads<G>(fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]))), mm = m > -INFINITY ? m : 0.f;
     const float4 p = make_float4(ex2(a[0] - mm), ex2(a[1] - mm), ex2(a[2] - mm), ex2(a[3] - mm));
     const float tot = lb_over_heads<G>((p.x + p.y) + (p.z + p.w)), k = gd / tot;
-    return tot > 0.f ? make_float4(p.x * k, p.y * k, p.z * k, p.w * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+    return tot != 0.f ? make_float4(p.x * k, p.y * k, p.z * k, p.w * k) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
 // What both kernels begin with: table, barriers, zeros.
@@ -964,21 +970,21 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             // f_h = exp(g_h) / S_h; a head without a finite score takes no part
             float g2[4], f[4], ls[4];
             const float top = lb_gates<G>(gate, g2);
-            float least = 1.f;   // of the factors of the heads that take part
+            bool rare = false;
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                const bool some = sum[k] > 0.f && sum[k] < INFINITY;
+                const bool some = sum[k] != 0.f;
                 ls[k] = some ? lg2(sum[k]) : INFINITY;
                 f[k] = some ? __fdividef(ex2(g2[k]), sum[k]) : 0.f;
-                if (some && g2[k] > -INFINITY) least = fminf(least, f[k]);
+                rare |= some && lb_rare(f[k], g2[k]);
             }
-            const float enough = __any_sync(0xffffffffu, least < kLbRare) ? INFINITY : kLbTiny;   // of the links' sums
+            const float enough = __any_sync(0xffffffffu, rare) ? INFINITY : kLbTiny;   // of the links' sums
             if (head_lse && lane < G) {
                 float4 o;
-                o.x = ls[0] < INFINITY ? r[0] + ls[0] : -INFINITY;
-                o.y = ls[1] < INFINITY ? r[1] + ls[1] : -INFINITY;
-                o.z = ls[2] < INFINITY ? r[2] + ls[2] : -INFINITY;
-                o.w = ls[3] < INFINITY ? r[3] + ls[3] : -INFINITY;
+                o.x = ls[0] == INFINITY ? -INFINITY : r[0] + ls[0];
+                o.y = ls[1] == INFINITY ? -INFINITY : r[1] + ls[1];
+                o.z = ls[2] == INFINITY ? -INFINITY : r[2] + ls[2];
+                o.w = ls[3] == INFINITY ? -INFINITY : r[3] + ls[3];
                 lw_put<G, kExact>(head_lse + r0.row * H, g, H, o);
             }
             float *const out = links + r0.row * (int64_t)K;
@@ -1007,10 +1013,10 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                         float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                         if (x < nvec && !(np && !np[x / G])) {   // log2 of e f without the exponential's flush
                             const float4 z = lb_shifted(lw_get<G, kExact>(src, x, H, -INFINITY), lw_bias<G>(table, bucket, x), r);
-                            if (ls[0] < INFINITY) t[0] = z.x + (g2[0] - ls[0]);
-                            if (ls[1] < INFINITY) t[1] = z.y + (g2[1] - ls[1]);
-                            if (ls[2] < INFINITY) t[2] = z.z + (g2[2] - ls[2]);
-                            if (ls[3] < INFINITY) t[3] = z.w + (g2[3] - ls[3]);
+                            if (ls[0] != INFINITY) t[0] = z.x + (g2[0] - ls[0]);
+                            if (ls[1] != INFINITY) t[1] = z.y + (g2[1] - ls[1]);
+                            if (ls[2] != INFINITY) t[2] = z.z + (g2[2] - ls[2]);
+                            if (ls[3] != INFINITY) t[3] = z.w + (g2[3] - ls[3]);
                         }
                         const float link = lw_tiny_link<G>(t[0], t[1], t[2], t[3], top);
                         if (g == 0 && x < nvec) out[x / G] = link;
@@ -1095,9 +1101,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             lw_punch<G, kExact>(r0, buf, H, mk);
             __syncwarp();
         }
-        // a head that takes no part (lse = -inf): soft = exp(-inf) = 0
-        const float ls[4] = {lse.x > -INFINITY ? lse.x : INFINITY, lse.y > -INFINITY ? lse.y : INFINITY,
-                             lse.z > -INFINITY ? lse.z : INFINITY, lse.w > -INFINITY ? lse.w : INFINITY};
+        const float ls[4] = {lb_lse(lse.x), lb_lse(lse.y), lb_lse(lse.z), lb_lse(lse.w)};
         float g2[4];
         lb_gates<G>(gate, g2);
         const float eg[4] = {ex2(g2[0]), ex2(g2[1]), ex2(g2[2]), ex2(g2[3])};
@@ -1108,7 +1112,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
             float4 t[N], q[N];
             float w[N];
             lw_terms<G, kExact, N, kPart>(t, buf, H, table, bucket, ls, v, nvec);
-            float least = 1.f;
+            bool tiny = false;
 #pragma unroll
             for (int u = 0; u < N; u++) {
                 const bool in = !kPart || v + 32 * u < nvec;
@@ -1123,17 +1127,16 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
                 const float tot = lb_over_heads<G>((q[u].x + q[u].y) + (q[u].z + q[u].w));
                 if (in) {
                     lw_put<G, kExact>(buf, v + 32 * u, H, soft);
-                    least = fminf(least, tot);
+                    tiny |= !(tot >= kLbTiny);
                 }
                 if (tot >= kLbTiny) w[u] = __fdividef(w[u], tot);
             }
-            if (__any_sync(0xffffffffu, least < kLbTiny)) {
+            if (__any_sync(0xffffffffu, tiny)) {
 #pragma unroll
                 for (int u = 0; u < N; u++) {
                     const float tot = lb_over_heads<G>((q[u].x + q[u].y) + (q[u].z + q[u].w));
-                    const bool tiny = !(tot >= kLbTiny);   // the same in all lanes of a distance
                     const float4 p = lw_full_share<G>(t[u], g2, w[u]);
-                    if (tiny) {
+                    if (!(tot >= kLbTiny)) {   // the same in all lanes of a distance
                         S[0] += p.x;
                         S[1] += p.y;
                         S[2] += p.z;
@@ -1191,6 +1194,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
                         if (__float_as_uint(w[u]) == kLwFull)
                             k = make_float4(fmaf(-S[0], o[u].x, p.x), fmaf(-S[1], o[u].y, p.y), fmaf(-S[2], o[u].z, p.z),
                                             fmaf(-S[3], o[u].w, p.w));
+                        if (dead) k = make_float4(0.f, 0.f, 0.f, 0.f);   // also beside NaN
                         if (v + 32 * u < nvec) lw_put<G, kExact>(buf, v + 32 * u, H, k);
                     }
                 } else {

@@ -216,7 +216,8 @@ def dag_links_from_heads(log_multi_content, log_gates, nonpad_mask=None, bound_e
     ``relative_bias[relative_buckets[j-i-1]]`` is added to the scores of the transition i -> j
     (``relative_buckets``: int64, one bucket for each distance 1..K or more, see ``dag_relative_buckets``).
     Differentiable in it too; the gradient is summed in a fixed order.  A bucket outside the table forbids
-    the transitions of its distance and sets bit 4 of ``last_status()``."""
+    the transitions of its distance and sets bit 4 of ``last_status()``.  With a bias, NaN or +inf at a valid
+    successor makes the links and gradients of its vertex NaN; masked places may hold anything."""
     if (relative_bias is None) != (relative_buckets is None):
         raise RuntimeError("relative_bias and relative_buckets are given together")
     if relative_bias is not None:

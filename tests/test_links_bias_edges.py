@@ -133,3 +133,39 @@ def test_rare_head_far_above_its_nearest_score(H, buckets, gap, gate, other):
     content[:, :far, far + 1, H // 2] += gap - other
     got = against_64_bits(content, gates, table, some_buckets(L - 1, buckets), L - 1, grad, 100.0)
     assert (np.abs(got[0][:, 0, far] - gate) < 3).all() or other > gate - 4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,buckets", FORMS)
+@pytest.mark.parametrize("value", [NAN, float("inf")])
+def test_valid_scores_that_are_no_numbers_show(H, buckets, value):
+    """A score of NaN or +inf at a valid successor makes the softmax of its head NaN, and with it every link of the vertex;
+    nothing of another vertex changes.  A sentence with holes, one without a mask, one with a single vertex left."""
+    B, L = 3, 33
+    content, gates, table, grad, _, _ = make(B, L, H, L - 1, buckets=buckets, seed=H + 3)
+    nonpad = torch.rand(B, L, generator=torch.Generator().manual_seed(5)).to(DEV) < 0.6
+    nonpad[1] = True
+    nonpad[0, 1], nonpad[0, 3], nonpad[0, 9], nonpad[0, 12], nonpad[0, 20] = True, False, False, True, True
+    bk = some_buckets(L - 1, buckets)
+    bad = ((0, 2, 12, 0), (0, 5, 20, H - 1), (1, 0, 1, H // 2), (1, 7, L - 1, 0))
+    clean = run(content, gates, table, bk, L - 1, grad, nonpad_mask=nonpad)
+    for at in bad:
+        content[at] = value
+    content[0, 2, 3], content[0, 5, 9] = NAN, value                        # masked ones, of no account
+    links, gc, gg, gt = run(content, gates, table, bk, L - 1, grad, nonpad_mask=nonpad)
+    hit = np.zeros((B, L), bool)
+    for b, i, _, _ in bad:
+        hit[b, i] = True
+    ok = np.isfinite(clean[0])
+    assert np.isnan(links[hit][ok[hit]]).all() and (links[hit][~ok[hit]] == NEG_INF).all()
+    assert np.array_equal(links[~hit], clean[0][~hit])
+    dense = np.zeros((B, L, L), bool)
+    b, i, d = np.nonzero(ok)
+    dense[b, i, i + d + 1] = True
+    assert np.isnan(gc[hit][dense[hit]]).all() and not gc[hit][~dense[hit]].any()
+    assert np.array_equal(gc[~hit], clean[1][~hit]) and np.array_equal(gg[~hit], clean[2][~hit])
+    assert np.isnan(gg[hit]).all()
+    reached = np.unique(bk.cpu().numpy()[(ok & hit[..., None]).any((0, 1))])
+    assert np.isnan(gt[reached]).all()
+    others = np.setdiff1d(np.arange(buckets), reached)
+    assert np.array_equal(gt[others], clean[3][others])
