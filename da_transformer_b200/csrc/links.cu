@@ -29,12 +29,22 @@ __device__ __forceinline__ void links_stage_row(const float *__restrict__ crow, 
     const int n = (jhi - i) * H;   // may be <= 0
     const float *src = crow + (size_t)(i + 1) * H;
     if (kBias) {
+        // (no branch in the loop: a score waits for its bucket and that for its place in the table, four of them at a time)
         bool bad = false;
+#pragma unroll 4
         for (int x = threadIdx.x; x < n; x += kLinksThreads) {
             const int d = x / H;
-            const float t = links_bias1(lb, d, x - d * H, H, bad);
-            const bool dead = (np_row && !np_row[i + 1 + d]) || t == -INFINITY;   // also where the score is +inf or NaN
-            sm[x] = dead ? -INFINITY : fmaf(__ldg(src + x), kLog2e, t * kLog2e);
+            const int64_t k = __ldg(lb.bucket + d);
+            const bool in = (uint64_t)k < (uint64_t)lb.n;
+            const float c = __ldg(src + x), t = __ldg(lb.table + (in ? (int)k : 0) * H + (x - d * H));
+            sm[x] = in ? fmaf(c, kLog2e, t * kLog2e) : -INFINITY;
+            bad |= !in;
+        }
+        if (np_row) {
+            __syncthreads();
+            for (int d = threadIdx.x; d < jhi - i; d += kLinksThreads)
+                if (!np_row[i + 1 + d])
+                    for (int h = 0; h < H; h++) sm[d * H + h] = -INFINITY;
         }
         if (bad && lb.status) atomicOr(lb.status, DAT_STATUS_BAD_INDEX);
     } else if ((H & 3) == 0) {
@@ -125,7 +135,7 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
     float *out = links + row * (size_t)K;
     for (int d = tid; d < K; d += kLinksThreads) {
         float v = -INFINITY;
-        if (d < nj && !(kBias && np_row && !np_row[i + 1 + d])) {
+        if (d < nj) {
             // max over the heads first, then the sum: no rescaling and no branches inside the loops
             float m = -INFINITY;
             for (int h = 0; h < H; h++) m = fmaxf(m, term(d, h));
@@ -135,6 +145,8 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
                 for (int h = 0; h < H; h++) s += ex2(term(d, h) - m);
                 v = (m + lg2(s)) * kLn2;
             }
+            // a vertex with NaN: the places that are not allowed are -inf all the same
+            if (kBias && v != v && ((np_row && !np_row[i + 1 + d]) || !links_bucket_ok(lb, d))) v = -INFINITY;
         }
         out[d] = v;
     }

@@ -83,6 +83,17 @@ __device__ __forceinline__ unsigned lb_live(const LbRow &r, int L, const LinksMa
     }
     return np[0] ? live | 0x80000000u : live;
 }
+// the bits of lb_live whose distance has a bucket; the scores of the others are not looked at
+template <int G, int NT, int U>
+__device__ __forceinline__ unsigned lb_in_table(const LinksBias &lb, int K) {
+    unsigned in = links_bucket_ok(lb, 0) ? 0x80000000u : 0;
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+        const int v = threadIdx.x + u * NT;
+        if (v < K * G && links_bucket_ok(lb, v / G)) in |= 1u << u;
+    }
+    return in;
+}
 __device__ __forceinline__ void lb_copy16(float4 *dst, const float4 *src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
@@ -196,7 +207,8 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
     const int rows = B * L, step = gridDim.x;
     int slot = blockIdx.x;
     LbRow r0 = lb_row(slot, rows, L, K, mk), r1 = lb_row(slot + step, rows, L, K, mk);
-    unsigned live0 = lb_live<G, NT, U>(r0, L, mk), live1 = lb_live<G, NT, U>(r1, L, mk);
+    const unsigned in_table = lb_in_table<G, NT, U>(lb, K);
+    unsigned live0 = lb_live<G, NT, U>(r0, L, mk) & in_table, live1 = lb_live<G, NT, U>(r1, L, mk) & in_table;
     const auto nearest = [&](const LbRow &r) {
         return r.nj > 0 ? __ldg(reinterpret_cast<const float4 *>(content + (r.row * L + r.i + 1) * (int64_t)H) + g) : lb_ninf4();
     };
@@ -213,7 +225,7 @@ lb_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
         lb_fetch<G, NT, U>(r1, live1, content, L, bl4 + (size_t)(2 - par) * K * G);
         const float4 near1 = nearest(r1), gate1 = gates_of(r1);
         const LbRow r2 = lb_row(slot + 2 * step, rows, L, K, mk);
-        const unsigned live2 = lb_live<G, NT, U>(r2, L, mk);
+        const unsigned live2 = lb_live<G, NT, U>(r2, L, mk) & in_table;
         lb_copy_wait<1>();
         // r_h in log2 units
         const float4 b0 = bl4[g];
@@ -343,7 +355,8 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     const int rows = B * L, step = gridDim.x;
     int slot = blockIdx.x;
     LbRow r0 = lb_row(slot, rows, L, K, mk), r1 = lb_row(slot + step, rows, L, K, mk);
-    unsigned live0 = lb_live<G, NT, U>(r0, L, mk), live1 = lb_live<G, NT, U>(r1, L, mk);
+    const unsigned in_table = lb_in_table<G, NT, U>(lb, K);
+    unsigned live0 = lb_live<G, NT, U>(r0, L, mk) & in_table, live1 = lb_live<G, NT, U>(r1, L, mk) & in_table;
     const auto of_row = [&](const float *p, const LbRow &r) {
         return r.nj >= 0 ? __ldg(reinterpret_cast<const float4 *>(p + r.row * H) + g) : lb_ninf4();
     };
@@ -367,7 +380,7 @@ lb_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         lb_fetch<G, NT, U>(r1, live1, content, L, bl4 + (size_t)(2 - par) * K * G);
         const float4 lse1 = of_row(head_lse, r1), gate1 = of_row(log_gates, r1);
         const LbRow r2 = lb_row(slot + 2 * step, rows, L, K, mk);
-        const unsigned live2 = lb_live<G, NT, U>(r2, L, mk);
+        const unsigned live2 = lb_live<G, NT, U>(r2, L, mk) & in_table;
         const float ls[4] = {lb_lse(lse0.x), lb_lse(lse0.y), lb_lse(lse0.z), lb_lse(lse0.w)};
         float g2[4];
         lb_gates<G>(gate0, g2);
@@ -620,7 +633,7 @@ __device__ __forceinline__ float4 lw_bias(const float4 *table, const unsigned sh
     return table[bucket[v / G] * G + (v & (G - 1))];
 }
 template <int G, int NT>
-__device__ __forceinline__ void lw_load_table(const LinksBias &lb, float *table, unsigned short *bucket, int H, int K) {
+__device__ __forceinline__ bool lw_load_table(const LinksBias &lb, float *table, unsigned short *bucket, int H, int K) {
     bool bad = false;
     for (int x = threadIdx.x; x < lb.n * (4 * G); x += NT) {
         const int k = x / (4 * G), h = x - k * (4 * G);
@@ -634,7 +647,18 @@ __device__ __forceinline__ void lw_load_table(const LinksBias &lb, float *table,
         bucket[d] = (unsigned short)(ok ? k : lb.n);
     }
     if (bad && lb.status) atomicOr(lb.status, DAT_STATUS_BAD_INDEX);
+    return bad;
 }
+
+// The distances of a row whose transitions are not allowed although they lie inside its span: a hole in the mask, or a
+// bucket outside the table.  Their scores may be anything.
+struct LwDead {
+    const unsigned char *np;       // mask of the row's successors, or null: no holes
+    const unsigned short *bucket;
+    int none;                      // bucket of the distances that have none; -1: all have one
+    __device__ __forceinline__ bool any() const { return np || none >= 0; }
+    __device__ __forceinline__ bool operator()(int d) const { return (np && !np[d]) || bucket[d] == none; }
+};
 
 // Shared memory, in bytes: table, buckets, zeros, barriers of the copies, then the rings.
 struct LwSmem {
@@ -760,12 +784,11 @@ __device__ __forceinline__ void lw_reduce(float (&v)[4]) {
     for (int k = 0; k < 4; k++) v[k] = __shfl_sync(0xffffffffu, c, (k >> 1) * 16 + (k & 1) * 8 + g);
 }
 
-// scores of masked places inside the span to -inf (each lane its own places)
+// scores of places that are not allowed inside the span to -inf (each lane its own places)
 template <int G, bool kExact>
-__device__ __forceinline__ void lw_punch(const LwRow &r, float *buf, int H, const LinksMask &mk) {
-    const unsigned char *np = mk.nonpad + r.row + 1;   // b * L + i + 1
+__device__ __forceinline__ void lw_punch(const LwRow &r, float *buf, int H, const LwDead &dead) {
     for (int v = threadIdx.x & 31; v < r.nj * G; v += 32)
-        if (!np[v / G]) lw_put<G, kExact>(buf, v, H, lb_ninf4());
+        if (dead(v / G)) lw_put<G, kExact>(buf, v, H, lb_ninf4());
 }
 
 // the four heads of lane group g of a row of [.., H], -inf for those that are not there
@@ -848,15 +871,15 @@ __device__ __noinline__ float4 lw_full_share(float4 t, const float (&g2)[4], flo
     return tot != 0.f ? make_float4(p.x * k, p.y * k, p.z * k, p.w * k) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
-// What both kernels begin with: table, barriers, zeros.
+// What both kernels begin with: table, barriers, zeros.  Returns the bucket of distances that have none, -1 if all have.
 template <int G, int NT>
-__device__ __forceinline__ void lw_begin(const LwSmem &lay, unsigned char *sm, const LinksBias &lb, int H, int K) {
-    lw_load_table<G, NT>(lb, reinterpret_cast<float *>(sm), reinterpret_cast<unsigned short *>(sm + lay.bucket), H, K);
+__device__ __forceinline__ int lw_begin(const LwSmem &lay, unsigned char *sm, const LinksBias &lb, int H, int K) {
+    const bool bad = lw_load_table<G, NT>(lb, reinterpret_cast<float *>(sm), reinterpret_cast<unsigned short *>(sm + lay.bucket), H, K);
     for (int x = threadIdx.x; x < kLwZeros / 16; x += NT)
         reinterpret_cast<float4 *>(sm + lay.zeros)[x] = make_float4(0.f, 0.f, 0.f, 0.f);
     if (threadIdx.x < NT / 32) umma::mbar_init(reinterpret_cast<uint64_t *>(sm + lay.mbar) + threadIdx.x, 1);
     umma::fence_smem_to_async();
-    __syncthreads();
+    return __syncthreads_or(bad) ? lb.n : -1;
 }
 
 // NG groups of four vertices at work in a CTA
@@ -872,7 +895,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
     const unsigned short *const bucket = reinterpret_cast<const unsigned short *>(lwsm + lay.bucket);
     unsigned char *const ring = lwsm + lay.rings + warp * lay.ring;
     uint64_t *const mbar = reinterpret_cast<uint64_t *>(lwsm + lay.mbar) + warp;
-    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, H, K);
+    const int none = lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, H, K);
     pdl_wait();   // the spans
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = warp / kLwRows * gridDim.x + blockIdx.x;
@@ -905,9 +928,9 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             const int nvec = r0.nj * G;
             float *const buf = reinterpret_cast<float *>(ring + s0.at) + s0.front;
             const float *const src = content + (r0.row * L + r0.i + 1) * (int64_t)H;
-            const unsigned char *const np = r0.holes ? mk.nonpad + r0.row + 1 : nullptr;
-            if (r0.holes) {
-                lw_punch<G, kExact>(r0, buf, H, mk);
+            const LwDead dead{r0.holes ? mk.nonpad + r0.row + 1 : nullptr, bucket, none};   // b * L + i + 1
+            if (dead.any()) {
+                lw_punch<G, kExact>(r0, buf, H, dead);
                 __syncwarp();
             }
             // r_h in log2 units
@@ -942,7 +965,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
             if (__any_sync(0xffffffffu, bad)) {   // the exact maximum of each head takes the place of r_h
                 float m[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
                 for (int v = lane; v < nvec; v += 32)
-                    if (!(np && !np[v / G])) {
+                    if (!dead(v / G)) {
                         const float4 c = lw_get<G, kExact>(src, v, H, -INFINITY), t = lw_bias<G>(table, bucket, v);
                         m[0] = fmaxf(m[0], fmaf(c.x, kLog2e, t.x));
                         m[1] = fmaxf(m[1], fmaf(c.y, kLog2e, t.y));
@@ -956,7 +979,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                 for (int k = 0; k < 4; k++) r[k] = m[k] > -INFINITY ? m[k] : 0.f;
                 for (int v = lane; v < nvec; v += 32) {
                     float4 e = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (!(np && !np[v / G])) {
+                    if (!dead(v / G)) {
                         const float4 t = lb_shifted(lw_get<G, kExact>(src, v, H, -INFINITY), lw_bias<G>(table, bucket, v), r);
                         e = make_float4(ex2(t.x), ex2(t.y), ex2(t.z), ex2(t.w));
                         fadd2_rn(sum[0], sum[1], sum[0], sum[1], e.x, e.y);
@@ -1011,7 +1034,7 @@ lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_g
                     for (int u = 0; u < N; u++) {
                         const int x = v + 32 * u;
                         float t[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                        if (x < nvec && !(np && !np[x / G])) {   // log2 of e f without the exponential's flush
+                        if (x < nvec && !dead(x / G)) {   // log2 of e f without the exponential's flush
                             const float4 z = lb_shifted(lw_get<G, kExact>(src, x, H, -INFINITY), lw_bias<G>(table, bucket, x), r);
                             if (ls[0] != INFINITY) t[0] = z.x + (g2[0] - ls[0]);
                             if (ls[1] != INFINITY) t[1] = z.y + (g2[1] - ls[1]);
@@ -1066,7 +1089,7 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     const bool wide = (reinterpret_cast<uintptr_t>(grad_links) & 15) == 0;
     const int set = warp / kLwRows, set_tid = tid - set * (kLwRows * 32);
     const auto set_sync = [&] { asm volatile("bar.sync %0, %1;" ::"r"(set + 1), "n"(kLwRows * 32) : "memory"); };
-    lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, H, K);
+    const int none = lw_begin<G, NG * kLwRows * 32>(lay, lwsm, lb, H, K);
     pdl_trigger();
     const int groups = B * ((L + kLwRows - 1) / kLwRows), step = gridDim.x * NG;
     int group = blockIdx.x * NG + set;
@@ -1095,10 +1118,10 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
         const int nvec = r0.nj * G;
         float *const buf = reinterpret_cast<float *>(ring + s0.at + s0.window) + s0.front;
         const float *const src = content + (r0.row * L + r0.i + 1) * (int64_t)H;
-        const unsigned char *const np = r0.holes ? mk.nonpad + r0.row + 1 : nullptr;
+        const LwDead dead{r0.holes ? mk.nonpad + r0.row + 1 : nullptr, bucket, none};
         float *const weight = reinterpret_cast<float *>(ring + s0.at) + s0.skip;   // G_d, then w_d
-        if (r0.holes) {
-            lw_punch<G, kExact>(r0, buf, H, mk);
+        if (dead.any()) {
+            lw_punch<G, kExact>(r0, buf, H, dead);
             __syncwarp();
         }
         const float ls[4] = {lb_lse(lse.x), lb_lse(lse.y), lb_lse(lse.z), lb_lse(lse.w)};
@@ -1187,14 +1210,14 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
                 if (__any_sync(0xffffffffu, full)) {   // see the first pass
                     for (int u = 0; u < N; u++) {
                         const int x = min(v + 32 * u, nvec - 1);
-                        const bool dead = np && !np[x / G];
-                        const float4 t = dead ? lb_ninf4() : lb_shifted(lw_get<G, kExact>(src, x, H, -INFINITY), lw_bias<G>(table, bucket, x), ls);
+                        const bool out = dead(x / G);
+                        const float4 t = out ? lb_ninf4() : lb_shifted(lw_get<G, kExact>(src, x, H, -INFINITY), lw_bias<G>(table, bucket, x), ls);
                         const float4 p = lw_full_share<G>(t, g2, __ldg(grad_links + r0.row * (int64_t)K + x / G));
                         float4 k = lb_grad(o[u], lw_gated(o[u], eg), w[u], S);
                         if (__float_as_uint(w[u]) == kLwFull)
                             k = make_float4(fmaf(-S[0], o[u].x, p.x), fmaf(-S[1], o[u].y, p.y), fmaf(-S[2], o[u].z, p.z),
                                             fmaf(-S[3], o[u].w, p.w));
-                        if (dead) k = make_float4(0.f, 0.f, 0.f, 0.f);   // also beside NaN
+                        if (out) k = make_float4(0.f, 0.f, 0.f, 0.f);   // also beside NaN
                         if (v + 32 * u < nvec) lw_put<G, kExact>(buf, v + 32 * u, H, k);
                     }
                 } else {

@@ -12,7 +12,7 @@ struct LinksMask {
 };
 
 // Learned relative position bias: content[b,i,j,h] + table[bucket[j-i-1], h] takes the place of the score.
-// A bucket outside the table forbids the transition (score -inf) and sets a bit of the status word.
+// A bucket outside the table forbids the transition (score -inf, whatever the content is) and sets a bit of the status word.
 struct LinksBias {
     const float *table;      // [n, H]
     const int64_t *bucket;   // [K]: bucket[d] belongs to the distance d + 1
@@ -30,6 +30,10 @@ __device__ __forceinline__ int links_jhi(int i, int L, int K, const LinksMask &m
     return jhi;
 }
 
+__device__ __forceinline__ bool links_bucket_ok(const LinksBias &lb, int d) {
+    const int64_t k = __ldg(lb.bucket + d);
+    return k >= 0 && k < lb.n;
+}
 __device__ __forceinline__ float links_bias1(const LinksBias &lb, int d, int h, int H, bool &bad) {
     const int64_t k = __ldg(lb.bucket + d);
     if (k >= 0 && k < lb.n) return __ldg(lb.table + k * H + h);

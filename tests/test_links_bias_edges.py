@@ -10,6 +10,7 @@ import torch
 
 import da_transformer_b200 as dat
 from test_links_bias import make, oracle
+from util import assert_rel
 
 DEV = "cuda:0"
 NEG_INF = float("-inf")
@@ -169,3 +170,64 @@ def test_valid_scores_that_are_no_numbers_show(H, buckets, value):
     assert np.isnan(gt[reached]).all()
     others = np.setdiff1d(np.arange(buckets), reached)
     assert np.array_equal(gt[others], clean[3][others])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,buckets", FORMS)
+def test_distances_without_a_bucket_may_hold_anything(H, buckets):
+    """The scores of a distance whose bucket lies outside the table are as good as masked."""
+    B, L = 2, 40
+    content, gates, table, grad, _, nonpad = make(B, L, H, L - 1, buckets=buckets, seed=H + 4)
+    bk = some_buckets(L - 1, buckets)
+    bk[0], bk[5], bk[17] = -1, buckets, 2 ** 40
+    content[1, 2, 5, H // 2], content[0, 8, 10, 0] = NAN, NAN              # valid ones: these vertices are NaN where they reach
+    want = run(content, gates, table, bk, L - 1, grad, nonpad_mask=nonpad)
+    assert (want[0][:, :, [0, 5, 17]] == NEG_INF).all()
+    for b, i in ((1, 2), (0, 8)):
+        ok = want[0][b, i] != NEG_INF
+        assert np.isnan(want[0][b, i][ok]).all() and np.isnan(want[1][b, i, i + 1:][ok[:L - 1 - i]]).all()
+        assert not want[1][b, i, i + 1:][~ok[:L - 1 - i]].any()
+    d = torch.arange(L, device=DEV).view(1, L) - torch.arange(L, device=DEV).view(L, 1) - 1
+    out = (d == 0) | (d == 5) | (d == 17)
+    for value in (NAN, float("inf"), NEG_INF, torch.finfo(torch.float32).max):
+        dirty = torch.where(out.view(1, L, L, 1), torch.full((), value, device=DEV), content)
+        g = torch.where(torch.from_numpy(want[0] != NEG_INF).to(DEV), grad, torch.full((), value, device=DEV))
+        for a, b in zip(run(dirty, gates, table, bk, L - 1, g, nonpad_mask=nonpad), want):
+            assert np.array_equal(a, b, equal_nan=True), value
+    dat.last_status(DEV)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,buckets", FORMS)
+def test_bias_of_minus_infinity(H, buckets):
+    """A bias of -inf is a score of -inf (a head without a finite score takes no part, for which the definition has no number),
+    and a score that is no number stays none beside it."""
+    B, L = 2, 26
+    content, gates, table, grad, _, nonpad = make(B, L, H, L - 1, buckets=buckets, seed=H + 5)
+    bk = some_buckets(L - 1, buckets)
+    table[int(bk[3])] = NEG_INF
+    table[int(bk[7]), H // 2] = NEG_INF
+    links, gc, gg, gt = run(content, gates, table, bk, L - 1, grad, nonpad_mask=nonpad)
+    # in 64 bits, in the probability domain
+    c, g, t = (x.double().cpu() for x in (content, gates, table))
+    i = torch.arange(L).view(L, 1)
+    j = i + 1 + torch.arange(L - 1).view(1, L - 1)
+    ok = (j < L) & nonpad.cpu()[:, j.clamp(max=L - 1)]
+    e = (c[:, i, j.clamp(max=L - 1)] + t[bk.cpu()]).exp() * ok.unsqueeze(-1)
+    tot = e.sum(2, keepdim=True)
+    soft = e / torch.where(tot > 0, tot, torch.ones_like(tot))
+    w = soft * g.exp().unsqueeze(2)
+    p = w.sum(3, keepdim=True)
+    gp = grad.double().cpu().unsqueeze(-1) * w / torch.where(p > 0, p, torch.ones_like(p))
+    S = gp.sum(2)
+    dc = gp - soft * S.unsqueeze(2)
+    assert_rel(links, p.squeeze(3).log().numpy(), 1e-5, "links")
+    dense = torch.zeros(B, L, 2 * L, H, dtype=torch.float64)
+    dense[:, i, j] = dc
+    assert_rel(gc, dense[:, :, :L].numpy(), 1e-4, "gradient of content")
+    assert_rel(gg, S.numpy(), 1e-4, "gradient of gates")
+    dt = torch.zeros(t.shape, dtype=torch.float64).index_add_(0, bk.cpu(), dc.sum((0, 1)))
+    assert_rel(gt, dt.numpy(), 1e-4, "gradient of table")
+    content[0, 2, 2 + 1 + 3, 0] = NAN
+    links = run(content, gates, table, bk, L - 1, grad, nonpad_mask=nonpad)[0]
+    assert np.isnan(links[0, 2, :L - 3]).all()
