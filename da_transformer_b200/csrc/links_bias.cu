@@ -577,7 +577,7 @@ __device__ __forceinline__ LwRow lw_row(Walk &walk, int L, const LinksMask &mk, 
     if (r.i >= L) return r;
     r.exists = true;
     r.row = (int64_t)b * L + r.i;
-    if (mk.nonpad) r.sp = __ldg(span + b);
+    if (mk.nonpad) r.sp = __ldcg(span + b);   // (a coherent load: the kernel that writes it may have run beside this one)
     if (mk.bound_end) r.bound = __ldg(mk.bound_end + r.row);
     return r;
 }
@@ -886,7 +886,7 @@ __device__ __forceinline__ int lw_begin(const LwSmem &lay, unsigned char *sm, co
 template <int G, bool kExact, int NG>
 __global__ void __launch_bounds__(NG * kLwRows * 32, NG == 2 ? 2 : 1)
 lw_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk,
-              const int2 *__restrict__ span, LinksBias lb, LwSmem lay, float *__restrict__ links,
+              const int2 *span, LinksBias lb, LwSmem lay, float *__restrict__ links,
               float *__restrict__ head_lse, int B, int L, int heads, int K) {
     const int H = kExact ? 4 * G : heads;
     extern __shared__ __align__(16) unsigned char lwsm[];
@@ -1074,7 +1074,7 @@ template <int G, bool kExact, int UA, int NG>
 __global__ void __launch_bounds__(NG * kLwRows * 32, UA <= 4 ? 2 : 1)
 lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ content,
               const float *__restrict__ log_gates, const float *__restrict__ head_lse, LinksMask mk,
-              const int2 *__restrict__ span, LinksBias lb, LwSmem lay, float *__restrict__ grad_content,
+              const int2 *span, LinksBias lb, LwSmem lay, float *__restrict__ grad_content,
               float *__restrict__ grad_log_gates, float *__restrict__ part, int B, int L, int heads, int K) {
     const int H = kExact ? 4 * G : heads;
     const bool whole = kExact || (H & 3) == 0;   // rows of 16-byte pieces
@@ -1308,10 +1308,12 @@ lw_bwd_kernel(const float *__restrict__ grad_links, const float *__restrict__ co
     }
 }
 
+// What the kernel before has written is read by coherent loads (__ldcg) in the following three, which may have begun beside
+// it: the read-only path is for what nobody writes while a kernel runs.
 // by_distance[x] = sum of part[n][x] over the n CTAs, x = d * H + h: 32 columns per CTA, 16 lanes of rows each
 constexpr int kLbSumCols = 32, kLbSumLanes = 16;
 __global__ void __launch_bounds__(kLbSumCols * kLbSumLanes)
-lb_sum_kernel(const float *__restrict__ part, double *__restrict__ by_distance, int n, int KH) {
+lb_sum_kernel(const float *part, double *by_distance, int n, int KH) {
     __shared__ double lane_s[kLbSumLanes][kLbSumCols];
     const int c = threadIdx.x % kLbSumCols, q = threadIdx.x / kLbSumCols, x = blockIdx.x * kLbSumCols + c;
     double acc = 0.0;
@@ -1319,7 +1321,7 @@ lb_sum_kernel(const float *__restrict__ part, double *__restrict__ by_distance, 
     pdl_wait();
     if (x < KH) {
 #pragma unroll 8
-        for (int k = q; k < n; k += kLbSumLanes) acc += (double)part[(size_t)k * KH + x];
+        for (int k = q; k < n; k += kLbSumLanes) acc += (double)__ldcg(part + (size_t)k * KH + x);
     }
     lane_s[q][c] = acc;
     __syncthreads();
@@ -1332,7 +1334,7 @@ lb_sum_kernel(const float *__restrict__ part, double *__restrict__ by_distance, 
 
 // The same sums from the dense gradient: by_distance[d * H + h] = sum of dc[b,i,i+1+d,h] over the vertices (b,i)
 __global__ void __launch_bounds__(kLbSumCols * kLbSumLanes)
-lb_diag_kernel(const float *__restrict__ grad_content, double *__restrict__ by_distance, int B, int L, int H, int K) {
+lb_diag_kernel(const float *grad_content, double *by_distance, int B, int L, int H, int K) {
     __shared__ double lane_s[kLbSumLanes][kLbSumCols];
     const int c = threadIdx.x % kLbSumCols, q = threadIdx.x / kLbSumCols, x = blockIdx.x * kLbSumCols + c;
     double acc = 0.0;
@@ -1343,7 +1345,7 @@ lb_diag_kernel(const float *__restrict__ grad_content, double *__restrict__ by_d
         for (int b = 0; b < B; b++) {
             const float *p = grad_content + ((int64_t)b * L * L + 1) * H + x;
 #pragma unroll 8
-            for (int i = q; i < n; i += kLbSumLanes) acc += (double)p[(int64_t)i * (L + 1) * H];
+            for (int i = q; i < n; i += kLbSumLanes) acc += (double)__ldcg(p + (int64_t)i * (L + 1) * H);
         }
     }
     lane_s[q][c] = acc;
@@ -1358,8 +1360,7 @@ lb_diag_kernel(const float *__restrict__ grad_content, double *__restrict__ by_d
 // grad_table[k, h]: one CTA per bucket, the distances dealt to P lanes of a head
 constexpr int kLbJoinThreads = 256;
 __global__ void __launch_bounds__(kLbJoinThreads)
-lb_join_kernel(const double *__restrict__ by_distance, const int64_t *__restrict__ bucket, float *__restrict__ grad_table,
-               int H, int K) {
+lb_join_kernel(const double *by_distance, const int64_t *__restrict__ bucket, float *__restrict__ grad_table, int H, int K) {
     __shared__ double lane_s[kLbJoinThreads];
     const int k = blockIdx.x, P = kLbJoinThreads / H, h = threadIdx.x % H, p = threadIdx.x / H;
     double acc = 0.0;
@@ -1367,7 +1368,7 @@ lb_join_kernel(const double *__restrict__ by_distance, const int64_t *__restrict
     if (p < P) {
 #pragma unroll 8
         for (int d = p; d < K; d += P) {
-            const double v = by_distance[(size_t)d * H + h];
+            const double v = __ldcg(by_distance + (size_t)d * H + h);
             acc += __ldg(bucket + d) == k ? v : 0.0;
         }
     }

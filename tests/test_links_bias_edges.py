@@ -231,3 +231,31 @@ def test_bias_of_minus_infinity(H, buckets):
     content[0, 2, 2 + 1 + 3, 0] = NAN
     links = run(content, gates, table, bk, L - 1, grad, nonpad_mask=nonpad)[0]
     assert np.isnan(links[0, 2, :L - 3]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H", [6, 8])
+def test_spans_of_the_call_before_are_not_seen(H):
+    """The kernel that reads the sentences' spans begins while the one that writes them may still run, into memory that held
+    the spans of the call before: calls with masks in turn, none waited for."""
+    B, L = 40, 48
+    content, gates, table, grad, _, _ = make(B, L, H, L - 1, seed=5)
+    bk = some_buckets(L - 1, 8)
+    gen = torch.Generator().manual_seed(6)
+    masks = [(torch.rand(B, L, generator=gen) < p).to(DEV) for p in (0.1, 0.5, 0.9, 2.0)]
+    masks.append(torch.zeros(B, L, dtype=torch.bool, device=DEV))
+    call = lambda m: dat.dag_links_from_heads(content, gates, nonpad_mask=m, relative_bias=table, relative_buckets=bk)  # noqa: E731
+    want = []
+    for m in masks:
+        torch.cuda.synchronize()
+        want.append(call(m))
+        torch.cuda.synchronize()
+    leaves = [t.detach().clone().requires_grad_() for t in (content, gates, table)]
+    first = None
+    for n in range(60):
+        m = n % len(masks)
+        assert torch.equal(call(masks[m]), want[m])
+        links = dat.dag_links_from_heads(leaves[0], leaves[1], nonpad_mask=masks[1], relative_bias=leaves[2], relative_buckets=bk)
+        got = torch.autograd.grad(links, leaves, grad)
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(got, first))
