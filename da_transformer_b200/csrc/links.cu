@@ -9,7 +9,7 @@
 // column allowed by the mask); invalid entries and vertices without any successor are -inf.
 // The reference materialises [B,L,K,H] three times on the way (gather, log_softmax, + gates).
 // Here one warp owns one vertex (b,i) (head counts that are 4, 8, 16 or 32; a CTA per vertex with the
-// scores staged in shared memory otherwise): it streams the H x (valid successors) scores, reduces per
+// scores staged in shared memory otherwise, read again from L2 where a row does not fit it): it streams the H x (valid successors) scores, reduces per
 // head, streams them again from L2 and writes the K band entries; nothing else touches HBM.
 //
 // HBM-bound.  Algorithmic bytes: forward reads the upper triangle of content once
@@ -64,11 +64,43 @@ __device__ __forceinline__ void links_stage_row(const float *__restrict__ crow, 
     }
 }
 
-// Per-head log-sum-exp (natural log; kBias: log2) over the staged successors.  Thread (h = tid % H, part = tid / H)
+// The scores of a vertex's row by place x = (j-i-1)*H + h, staged in shared memory or, where they do not fit it, from memory
+// each time (the L2 cache, after the first).
+template <bool kBias, bool kStage>
+struct LinksRow {
+    const float *sm;             // kStage: the row
+    const float *src;            // first successor's scores
+    const unsigned char *np;     // mask of the successors, or null
+    LinksBias lb;
+    int H;
+    __device__ __forceinline__ bool dead(int d) const { return (np && !np[d]) || (kBias && !links_bucket_ok(lb, d)); }
+    __device__ __forceinline__ float operator()(int x) const {
+        if (kStage) return sm[x];
+        const int d = x / H;
+        if (dead(d)) return -INFINITY;
+        if (!kBias) return src[x];
+        bool bad = false;
+        return fmaf(src[x], kLog2e, links_bias1(lb, d, x - d * H, H, bad) * kLog2e);
+    }
+};
+template <bool kBias, bool kStage>
+__device__ __forceinline__ LinksRow<kBias, kStage> links_row(const float *crow, float *sm, int i, int jhi, int H,
+                                                             const unsigned char *np_row, const LinksBias &lb) {
+    if (kStage) {
+        links_stage_row<kBias>(crow, sm, i, jhi, H, np_row, lb);
+    } else if (kBias) {
+        bool bad = false;
+        for (int d = threadIdx.x; d < jhi - i; d += kLinksThreads) bad |= !links_bucket_ok(lb, d);
+        if (bad && lb.status) atomicOr(lb.status, DAT_STATUS_BAD_INDEX);
+    }
+    return {sm, crow + (size_t)(i + 1) * H, np_row ? np_row + i + 1 : nullptr, lb, H};
+}
+
+// Per-head log-sum-exp (natural log; kBias: log2) over the row's successors.  Thread (h = tid % H, part = tid / H)
 // walks the successors part, part + P, ...; partial (max, sum) pairs meet in shared memory.
 // Result in lse_s[h] (-inf when the head sees no finite score).  Needs H <= kLinksThreads.
-template <bool kBias>
-__device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, float *part_m, float *part_s,
+template <bool kBias, bool kStage>
+__device__ __forceinline__ void links_head_lse(const LinksRow<kBias, kStage> &score, int nj, int H, float *part_m, float *part_s,
                                                float *lse_s) {
     const int tid = threadIdx.x;
     const int P = kLinksThreads / H;
@@ -76,7 +108,7 @@ __device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, f
     float m = kNegBig, s = 0.f;
     if (part < P) {
         for (int j = part; j < nj; j += P) {
-            const float v = kBias ? sm[j * H + h] : sm[j * H + h] * kLog2e;
+            const float v = kBias ? score(j * H + h) : score(j * H + h) * kLog2e;
             if (v > m) {
                 s *= ex2(m - v);
                 m = v;
@@ -96,7 +128,7 @@ __device__ __forceinline__ void links_head_lse(const float *sm, int nj, int H, f
     __syncthreads();
 }
 
-template <bool kBias>
+template <bool kBias, bool kStage>
 __global__ void __launch_bounds__(kLinksThreads)
 links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ log_gates, LinksMask mk, LinksBias lb,
                  float *__restrict__ links, float *__restrict__ head_lse, int L, int H, int K) {
@@ -105,18 +137,18 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
     const int i = (int)(row % L);
     const int64_t b = row / L;
     const int tid = threadIdx.x;
-    float *sm = lsm;                          // [(L-1) * H] staged scores
-    float *part_m = sm + (size_t)(L - 1) * H; // [P * H]
+    float *sm = lsm;                          // [min(K, L-1) * H] staged scores
+    float *part_m = sm + (kStage ? (size_t)min(K, L - 1) * H : 0);   // [P * H]
     float *part_s = part_m + kLinksThreads;
     float *lse_s = part_s + kLinksThreads;    // [H]
     float *gate_s = lse_s + H;                // [H]
     const int jhi = links_jhi(i, L, K, mk, row);
     const int nj = jhi - i > 0 ? jhi - i : 0;
     const unsigned char *np_row = mk.nonpad ? mk.nonpad + b * L : nullptr;
-    links_stage_row<kBias>(content + row * (size_t)L * H, sm, i, jhi, H, np_row, lb);
+    const auto score = links_row<kBias, kStage>(content + row * (size_t)L * H, sm, i, jhi, H, np_row, lb);
     if (tid < H) gate_s[tid] = log_gates[row * H + tid];
     __syncthreads();
-    links_head_lse<kBias>(sm, nj, H, part_m, part_s, lse_s);
+    links_head_lse(score, nj, H, part_m, part_s, lse_s);
     if (head_lse && tid < H) head_lse[row * H + tid] = lse_s[tid];
     // per head, what is added to a score: (gate - lse) in log2 units (kBias: the gate, after the lse); a head whose every
     // score is -inf (lse = -inf) takes no part
@@ -130,7 +162,7 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
     }
     __syncthreads();
     const auto term = [&](int d, int h) {
-        return kBias ? (sm[d * H + h] - lse_s[h]) + gate_s[h] : fmaf(sm[d * H + h], kLog2e, gate_s[h]);
+        return kBias ? (score(d * H + h) - lse_s[h]) + gate_s[h] : fmaf(score(d * H + h), kLog2e, gate_s[h]);
     };
     float *out = links + row * (size_t)K;
     for (int d = tid; d < K; d += kLinksThreads) {
@@ -146,7 +178,7 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
                 v = (m + lg2(s)) * kLn2;
             }
             // a vertex with NaN: the places that are not allowed are -inf all the same
-            if (kBias && v != v && ((np_row && !np_row[i + 1 + d]) || !links_bucket_ok(lb, d))) v = -INFINITY;
+            if (kBias && v != v && score.dead(d)) v = -INFINITY;
         }
         out[d] = v;
     }
@@ -157,9 +189,9 @@ links_fwd_kernel(const float *__restrict__ content, const float *__restrict__ lo
 //     S_h          = sum_j G[j] p[j,h]                          = d / d log_gates[h]
 //     d / d c[j,h] = G[j] p[j,h] - exp(c[j,h] - lse_h) * S_h
 // grad_content is written for the whole [L,H] row (zeros outside the valid successors); it may alias
-// content (a CTA has its row in shared memory before it writes).  kBias: G p is rounded the same way in the sum and in
+// content (a CTA has its row in shared memory before it writes, or reads a place for the last time right before it does).  kBias: G p is rounded the same way in the sum and in
 // the difference, so that a vertex with one successor (p the same, soft = 1) has the gradient 0.
-template <bool kBias>
+template <bool kBias, bool kStage>
 __global__ void __launch_bounds__(kLinksThreads)
 links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
                  const float *__restrict__ log_gates, const float *__restrict__ links,
@@ -170,21 +202,24 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
     const int i = (int)(row % L);
     const int64_t b = row / L;
     const int tid = threadIdx.x;
-    float *sm = lsm;                           // [(L-1) * H]
-    float *gl_s = sm + (size_t)(L - 1) * H;    // [L-1] incoming gradient per successor
-    float *lk_s = gl_s + (L - 1);              // [L-1] forward value per successor
-    float *part = lk_s + (L - 1);              // [kLinksThreads]
+    const int N = kStage ? min(K, L - 1) : 0;
+    float *sm = lsm;                           // [N * H]
+    float *gl_s = sm + (size_t)N * H;          // [N] incoming gradient per successor
+    float *lk_s = gl_s + N;                    // [N] forward value per successor
+    float *part = lk_s + N;                    // [kLinksThreads]
     float *lse_s = part + kLinksThreads;       // [H]
     float *gate_s = lse_s + H;                 // [H]
     float *S_s = gate_s + H;                   // [H]
     const int jhi = links_jhi(i, L, K, mk, row);
     const int nj = jhi - i > 0 ? jhi - i : 0;
     const unsigned char *np_row = mk.nonpad ? mk.nonpad + b * L : nullptr;
-    links_stage_row<kBias>(content + row * (size_t)L * H, sm, i, jhi, H, np_row, lb);
-    for (int d = tid; d < nj; d += kLinksThreads) {
+    const auto score = links_row<kBias, kStage>(content + row * (size_t)L * H, sm, i, jhi, H, np_row, lb);
+    for (int d = tid; kStage && d < nj; d += kLinksThreads) {
         gl_s[d] = grad_links[row * (size_t)K + d];
         lk_s[d] = links[row * (size_t)K + d];
     }
+    const auto grad_of = [&](int d) { return kStage ? gl_s[d] : grad_links[row * (size_t)K + d]; };
+    const auto link_of = [&](int d) { return kStage ? lk_s[d] : links[row * (size_t)K + d]; };
     if (tid < H) {
         gate_s[tid] = log_gates[row * H + tid];
         lse_s[tid] = head_lse[row * H + tid];
@@ -198,10 +233,10 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
         const float k = (gate_s[h] - lse_s[h]) * kLog2e;
         if (kBias ? lse_s[h] != -INFINITY : lse_s[h] > -INFINITY)
             for (int j = pt; j < nj; j += P) {
-                const float lk = lk_s[j];
+                const float lk = link_of(j);
                 if (kBias ? lk == -INFINITY : !(lk > -INFINITY)) continue;
-                if (kBias) acc = __fadd_rn(acc, __fmul_rn(gl_s[j], ex2((sm[j * H + h] - lse_s[h]) + (gate_s[h] - lk) * kLog2e)));
-                else acc += gl_s[j] * ex2(fmaf(sm[j * H + h], kLog2e, k) - lk * kLog2e);
+                if (kBias) acc = __fadd_rn(acc, __fmul_rn(grad_of(j), ex2((score(j * H + h) - lse_s[h]) + (gate_s[h] - lk) * kLog2e)));
+                else acc += grad_of(j) * ex2(fmaf(score(j * H + h), kLog2e, k) - lk * kLog2e);
             }
         part[pt * H + h] = acc;
     }
@@ -221,15 +256,15 @@ links_bwd_kernel(const float *__restrict__ grad_links, const float *content,
         float v = 0.f;
         const int d = j - i - 1;
         if (d >= 0 && d < nj) {
-            const float c = sm[d * H + hh], lse = lse_s[hh], lk = lk_s[d];
+            const float c = score(d * H + hh), lse = lse_s[hh], lk = link_of(d);
             if (kBias) {
                 // (a link of -inf: masked, or no head with a gate above -inf reaches it, and what the others lose, S, is 0)
                 if (lk != -INFINITY && lse != -INFINITY)
-                    v = __fmaf_rn(-ex2(c - lse), S_s[hh], __fmul_rn(gl_s[d], ex2((c - lse) + (gate_s[hh] - lk) * kLog2e)));
+                    v = __fmaf_rn(-ex2(c - lse), S_s[hh], __fmul_rn(grad_of(d), ex2((c - lse) + (gate_s[hh] - lk) * kLog2e)));
             } else if (c > -INFINITY && lse > -INFINITY) {
                 const float soft = ex2((c - lse) * kLog2e);
                 float pg = 0.f;
-                if (lk > -INFINITY) pg = gl_s[d] * ex2(((c - lse) + gate_s[hh] - lk) * kLog2e);
+                if (lk > -INFINITY) pg = grad_of(d) * ex2(((c - lse) + gate_s[hh] - lk) * kLog2e);
                 v = pg - soft * S_s[hh];
             }
         }
@@ -499,27 +534,27 @@ static bool links_warp_form(int H, const void *a, const void *b) {
            ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b)) & 15) == 0;
 }
 
-static size_t links_smem_fwd(int L, int H) {
-    return ((size_t)(L - 1) * H + 2 * kLinksThreads + 2 * H) * sizeof(float) + 16;
-}
-static size_t links_smem_bwd(int L, int H) {
-    return ((size_t)(L - 1) * H + 2 * (size_t)(L - 1) + kLinksThreads + 3 * H) * sizeof(float) + 16;
+// n: successors that are staged
+static size_t links_smem_fwd(int n, int H) { return ((size_t)n * H + 2 * kLinksThreads + 2 * H) * sizeof(float) + 16; }
+static size_t links_smem_bwd(int n, int H) {
+    return ((size_t)n * H + 2 * (size_t)n + kLinksThreads + 3 * H) * sizeof(float) + 16;
 }
 
-// The kernels of one CTA per vertex row, any head count up to kLinksThreads.
+// The kernels of one CTA per vertex row, any head count up to kLinksThreads; the row is staged where it fits.
 template <bool kBias>
 int links_fwd_rows(const float *content, const float *log_gates, const LinksMask &mk, const LinksBias &lb, float *links,
                    float *head_lse, int bsz, int prelen, int heads, int translen, cudaStream_t st, const DeviceInfo &di,
                    const char *who) {
     DAT_REQUIRE(heads <= kLinksThreads, DAT_ERR_UNSUPPORTED, "%s: heads=%d exceeds %d", who, heads, kLinksThreads);
-    const size_t smem = links_smem_fwd(prelen, heads);
-    DAT_REQUIRE(smem <= (size_t)di.max_smem_optin, DAT_ERR_UNSUPPORTED,
-                "%s: prelen*heads = %d*%d needs %zu bytes of shared memory", who, prelen, heads, smem);
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(links_fwd_kernel<kBias>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)smem) != cudaSuccess)
+    const size_t staged = links_smem_fwd(translen < prelen ? translen : prelen - 1, heads);
+    const bool stage = staged <= (size_t)di.max_smem_optin;
+    const size_t smem = stage ? staged : links_smem_fwd(0, heads);
+    const auto kernel = stage ? links_fwd_kernel<kBias, true> : links_fwd_kernel<kBias, false>;
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return check_launch(who);
-    links_fwd_kernel<kBias><<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, st>>>(
-        content, log_gates, mk, lb, links, head_lse, prelen, heads, translen);
+    kernel<<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, st>>>(content, log_gates, mk, lb, links, head_lse, prelen,
+                                                                          heads, translen);
     return check_launch(who);
 }
 template <bool kBias>
@@ -528,14 +563,15 @@ int links_bwd_rows(const float *grad_links, const float *content, const float *l
                    float *grad_log_gates, int bsz, int prelen, int heads, int translen, cudaStream_t st,
                    const DeviceInfo &di, const char *who) {
     DAT_REQUIRE(heads <= kLinksThreads, DAT_ERR_UNSUPPORTED, "%s: heads=%d exceeds %d", who, heads, kLinksThreads);
-    const size_t smem = links_smem_bwd(prelen, heads);
-    DAT_REQUIRE(smem <= (size_t)di.max_smem_optin, DAT_ERR_UNSUPPORTED,
-                "%s: prelen*heads = %d*%d needs %zu bytes of shared memory", who, prelen, heads, smem);
-    if (smem > 48 * 1024 && cudaFuncSetAttribute(links_bwd_kernel<kBias>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 (int)smem) != cudaSuccess)
+    const size_t staged = links_smem_bwd(translen < prelen ? translen : prelen - 1, heads);
+    const bool stage = staged <= (size_t)di.max_smem_optin;
+    const size_t smem = stage ? staged : links_smem_bwd(0, heads);
+    const auto kernel = stage ? links_bwd_kernel<kBias, true> : links_bwd_kernel<kBias, false>;
+    if (smem > 48 * 1024 &&
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess)
         return check_launch(who);
-    links_bwd_kernel<kBias><<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, st>>>(
-        grad_links, content, log_gates, links, head_lse, mk, lb, grad_content, grad_log_gates, prelen, heads, translen);
+    kernel<<<(unsigned)((size_t)bsz * prelen), kLinksThreads, smem, st>>>(grad_links, content, log_gates, links, head_lse, mk, lb,
+                                                                          grad_content, grad_log_gates, prelen, heads, translen);
     return check_launch(who);
 }
 template int links_fwd_rows<true>(const float *, const float *, const LinksMask &, const LinksBias &, float *, float *,

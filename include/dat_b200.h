@@ -282,7 +282,7 @@ int dat_sentence_mean(const float *loss, const int64_t *target_length, double *s
  * ([bsz,prelen] int64, the decoding mask, :390-393) is given, and nonpad[b,j] != 0 when nonpad
  * ([bsz,prelen] uint8, prev_output_tokens != pad, the training mask, :394-395) is given; either may be NULL.
  * head_lse (optional output, [bsz,prelen,heads] fp32): the per-head log-sum-exp the backward needs.
- * heads <= 256; (prelen-1)*heads*4 bytes must fit in shared memory (about 220 KB).
+ * heads <= 128 (4, 8, 16 and 32 have kernels of their own).
  */
 int dat_links_from_heads(const float *content, const float *log_gates, const int64_t *bound_end,
                          const unsigned char *nonpad, float *links, float *head_lse,

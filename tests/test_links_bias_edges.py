@@ -259,3 +259,58 @@ def test_spans_of_the_call_before_are_not_seen(H):
         got = torch.autograd.grad(links, leaves, grad)
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(got, first))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,L,H,K", [(1, 448, 128, 447), (1, 460, 128, 459), (1, 900, 100, 40), (1, 470, 127, 469)])
+def test_rows_beside_the_shared_memory(B, L, H, K):
+    """Rows that fit the forward's shared memory and not the backward's, rows that fit neither, and long graphs whose band is
+    short."""
+    content, gates, table, grad, bk, nonpad = make(B, L, H, K, seed=H)
+    against_64_bits(content, gates, table, bk, K, grad, 16.0, nonpad_mask=nonpad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,L,H,K", [(1, 448, 127, 447), (1, 470, 127, 469), (1, 900, 101, 40)])
+def test_rows_beside_the_shared_memory_without_a_bias(B, L, H, K):
+    content, gates, table, grad, bk, nonpad = make(B, L, H, K, seed=H)
+    leaves = [t.detach().clone().requires_grad_() for t in (content, gates)]
+    links = dat.dag_links_from_heads(*leaves, nonpad_mask=nonpad, max_transition_length=K)
+    got = torch.autograd.grad(links, leaves, torch.where(links.isfinite(), grad, 0))
+    want = oracle(content, gates, torch.zeros_like(table), bk, K, nonpad_mask=nonpad, grad=grad)
+    fin = np.isfinite(want[0])
+    a = links.detach().cpu().numpy()
+    assert np.array_equal(a[~fin], want[0][~fin]) and np.abs(a[fin] - want[0][fin]).max() <= 1e-5 * np.abs(want[0][fin]).max()
+    for u, v in zip(got, want[1:3]):
+        assert np.abs(u.cpu().numpy() - v).max() <= 1e-4 * np.abs(v).max()
+
+
+@pytest.mark.gpu
+def test_a_bias_wherever_the_links_work_without_one():
+    """2048 vertices and 32 heads, every transition: the links without a bias of the scores with the bias added."""
+    B, L, H, K = 1, 2048, 32, 2047
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    content = torch.randn(B, L, L, H, generator=gen, device=DEV)
+    gates = torch.log_softmax(torch.randn(B, L, H, generator=gen, device=DEV), -1)
+    table = torch.randn(16, H, generator=gen, device=DEV) * 0.5
+    grad = torch.randn(B, L, K, generator=gen, device=DEV)
+    bk = dat.dag_relative_buckets(K, 16, 512, device=DEV)
+    leaves = [t.detach().clone().requires_grad_() for t in (content, gates, table)]
+    links = dat.dag_links_from_heads(leaves[0], leaves[1], relative_bias=leaves[2], relative_buckets=bk)
+    got = torch.autograd.grad(links, leaves, grad)
+    i = torch.arange(L, device=DEV)
+    d = (i.view(1, L) - i.view(L, 1) - 1).clamp(0, K - 1)
+    both = content.clone()
+    for n in range(0, L, 64):
+        both[0, n:n + 64] += table[bk[d[n:n + 64]]]
+    plain = [both.requires_grad_(), gates.clone().requires_grad_()]
+    other = dat.dag_links_from_heads(*plain)
+    want = torch.autograd.grad(other, plain, grad)
+    fin = other.isfinite()
+    assert torch.equal(links.isfinite(), fin)
+    assert float((links - other)[fin].detach().abs().max()) <= 1e-5 * float(other[fin].detach().abs().max())
+    for a, b in zip(got, want):
+        assert float((a - b).abs().max()) <= 1e-4 * float(b.abs().max())
+    by = torch.stack([torch.diagonal(want[0][0], d + 1, 0, 1).double().sum(-1) for d in range(K)])
+    dt = torch.zeros(16, H, dtype=torch.float64, device=DEV).index_add_(0, bk, by)
+    assert float((got[2] - dt).abs().max()) <= 1e-4 * float(dt.abs().max())
