@@ -1380,6 +1380,22 @@ lb_join_kernel(const double *by_distance, const int64_t *__restrict__ bucket, fl
     }
 }
 
+// shared memory of a CTA per vertex with NT threads, and the partial bands of the backward's CTAs by size alone: at most two
+// CTAs per SM with a warp per vertex, as many as their shared memory lets run (and 16) with a CTA per vertex, where the head
+// count has that form; the kernels of links.cu leave none
+static size_t lb_smem(int K, int H, int NT) { return ((size_t)3 * K * H + 2 * (NT / 32) * H) * sizeof(float); }
+constexpr int kLbMaxPerSm = 16;
+static bool lb_vectors(int K, int H) {
+    const int G = H / 4;
+    return H % 4 == 0 && (G == 1 || G == 2 || G == 4 || G == 8) && (int64_t)K * G <= kLbMaxVec;
+}
+static int lb_bands_per_sm(int K, int H, const DeviceInfo &di) {
+    const int warp = H <= 32 && (int64_t)K * lw_lanes(H) <= kLwMaxVec ? 2 : 0;
+    if (!lb_vectors(K, H)) return warp;
+    const int64_t fit = di.max_smem_optin / (int64_t)lb_smem(K, H, 128);
+    return fit > kLbMaxPerSm ? kLbMaxPerSm : fit > 2 ? (int)fit : 2;
+}
+
 // a warp per vertex: by size alone, so that a forward and its backward agree on who fills the spans
 static bool lw_fits(int K, int H, int n, const DeviceInfo &di) {
     return H <= 32 && (int64_t)K * lw_lanes(H) <= kLwMaxVec && (int64_t)n * 4 * lw_lanes(H) <= kLwMaxTable &&
@@ -1389,9 +1405,7 @@ static bool lw_fits(int K, int H, int n, const DeviceInfo &di) {
 // the kernels of this file: a warp or a CTA per vertex, by size, on 16-byte boundaries
 static bool lb_own_form(int heads, int translen, int n, const DeviceInfo &di, const void *a, const void *b, const void *c,
                         const void *d) {
-    const int G = heads / 4;
-    const bool vectors = heads % 4 == 0 && (G == 1 || G == 2 || G == 4 || G == 8) && (int64_t)translen * G <= kLbMaxVec;
-    return (lw_fits(translen, heads, n, di) || vectors) &&
+    return (lw_fits(translen, heads, n, di) || lb_vectors(translen, heads)) &&
            ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | reinterpret_cast<uintptr_t>(c) |
              reinterpret_cast<uintptr_t>(d)) & 15) == 0;
 }
@@ -1410,8 +1424,6 @@ static int lb_grid(F kernel, int threads, size_t smem, int64_t rows, const Devic
     return DAT_OK;
 }
 
-constexpr int kLbMaxPerSm = 16;   // CTAs per SM that the workspace has room for
-
 struct LbArgs {
     const float *grad_links, *content, *log_gates, *head_lse_in;
     LinksMask mk;
@@ -1426,13 +1438,14 @@ template <int G, int NT, int U>
 static int lb_launch(const LbArgs &a, bool backward, int &grid, cudaStream_t st, const DeviceInfo &di, const char *who) {
     const int H = 4 * G;
     const int64_t rows = (int64_t)a.B * a.L;
-    const size_t smem = ((size_t)3 * a.K * H + 2 * (NT / 32) * H) * sizeof(float);
+    const size_t smem = lb_smem(a.K, H, NT);
     if (!backward) {
         if (int rc = lb_grid(lb_fwd_kernel<G, NT, U>, NT, smem, rows, di, grid, who)) return rc;
         lb_fwd_kernel<G, NT, U><<<grid, NT, smem, st>>>(a.content, a.log_gates, a.mk, a.lb, a.links, a.head_lse, a.B, a.L, a.K);
     } else {
         if (int rc = lb_grid(lb_bwd_kernel<G, NT, U>, NT, smem, rows, di, grid, who)) return rc;
-        if (grid > di.sm_count * kLbMaxPerSm) grid = di.sm_count * kLbMaxPerSm;
+        const int most = di.sm_count * lb_bands_per_sm(a.K, a.H, di);
+        if (grid > most) grid = most;
         lb_bwd_kernel<G, NT, U><<<grid, NT, smem, st>>>(a.grad_links, a.content, a.log_gates, a.head_lse_in, a.mk, a.lb,
                                                         a.grad_content, a.grad_log_gates, a.part, a.B, a.L, a.K);
     }
@@ -1530,7 +1543,7 @@ size_t dat_links_bias_workspace_bytes(int bsz, int prelen, int heads, int transl
     if (bsz < 0 || prelen < 1 || heads < 1 || translen < 1) return 0;
     DeviceInfo di;
     if (!device_info(&di)) return 0;
-    int64_t n = (int64_t)di.sm_count * kLbMaxPerSm;
+    int64_t n = (int64_t)di.sm_count * lb_bands_per_sm(translen, heads, di);
     const int64_t rows = (int64_t)bsz * prelen + 3;   // a CTA per vertex, or groups of up to four in CTAs of three
     if (n > rows) n = rows;
     return (size_t)translen * heads * (sizeof(double) + (size_t)n * sizeof(float)) + 16;

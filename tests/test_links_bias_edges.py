@@ -314,3 +314,17 @@ def test_a_bias_wherever_the_links_work_without_one():
     by = torch.stack([torch.diagonal(want[0][0], d + 1, 0, 1).double().sum(-1) for d in range(K)])
     dt = torch.zeros(16, H, dtype=torch.float64, device=DEV).index_add_(0, bk, by)
     assert float((got[2] - dt).abs().max()) <= 1e-4 * float(dt.abs().max())
+
+
+@pytest.mark.gpu
+def test_workspace_has_no_more_bands_than_ctas_that_run_at_once():
+    """Partial sums of the table's gradient: a band for each CTA.  At most two to an SM with a warp per vertex; a CTA per
+    vertex keeps three rows of scores in shared memory (227 KB); none for head counts that neither takes."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    size = dat._native.lib().dat_links_bias_workspace_bytes
+    for B, L, H, K in ((64, 512, 8, 511), (8, 1024, 16, 1023), (16, 1024, 8, 256), (64, 300, 3, 299), (4, 440, 128, 439), (4, 100, 40, 99)):
+        band, sums = 4 * K * H, 8 * K * H
+        bands = 0 if H > 32 else 2 * sms
+        if H in (4, 8, 16, 32):
+            bands = max(bands, sms * min(16, 232448 // (3 * band)))
+        assert sums <= size(B, L, H, K) <= sums + bands * band + 64, (B, L, H, K)
