@@ -19,10 +19,21 @@
 // (policy_fwd_kernel).
 //
 // Numerics: sums in fp32 with exact differences to a reference (the running maximum; in the ring kernel the
-// token's logit, so that lp = -log S needs no further difference).  policy_fwd_kernel puts log-probabilities,
-// ratios and the KL of a row together in 64 bits (a maximum and a log-sum near 10 carry 5e-7, which would show
-// in the ratio).  Sums over rows in 64 bits in a fixed order.  d is taken relative to its value at one place of
-// the row, so that a constant between the two models' logits does not cancel.
+// token's logit, so that lp = -log S needs no further difference): a rounding of 2^-24 in each of a thread's additions,
+// below 1e-6 of the sum together with the exponentials' own.  The log-probability and the KL of a row are
+// put together in 64 bits (a maximum and a log-sum near 10 carry 5e-7, which would show in the ratio); the ring kernel takes
+// the ratio, its term and the gradient's factors from there in 32 bits (1e-7 of each), because the gradient of a row waits
+// for them: with all of it in 64 bits 32768 rows of 32000 took 3 % longer.  Sums over rows in 64 bits in a fixed order.  d is
+// taken relative to its value at one place of the row, so that a constant between the two models' logits does not cancel.
+//
+// The KL over the vocabulary is E_p d + log(S_y / S), whose parts cancel where the models are close: the rounding of the
+// sums leaves some 1e-7 of them, more than a KL near 0 has.  A row whose KL comes out below kPoNear is gone over
+// again.  With u = d - o, o the mean of d from the first time, and phi(u) = e^-u - 1 + u,
+//     KL = m + log(1 + f - m),   m = E_p u (near 0),   f = E_p phi(u),
+// for any o, since E_p e^-u = e^o S_y / S.  phi is not negative and near u^2 / 2, by its power series for small u: nothing
+// cancels but m with itself.  policy_fwd_kernel does it from the cache; after policy_ring_kernel a kernel of its own
+// (policy_near_kernel) reads such rows again from memory.  32768 rows of 32000 bf16 logits, none and all of them close:
+// 1.13 and 2.0 ms; with the second time inside the ring 1.25 and 1.73, since the code for it slowed the loops of all rows.
 #include "cluster_util.cuh"
 #include "dat_common.cuh"
 #include "umma.cuh"
@@ -33,6 +44,7 @@ constexpr int kPoThreads = 256;
 constexpr int kPoWarps = kPoThreads / 32;
 constexpr int kPoChunk = 256;   // rows whose results are summed together
 constexpr int kPoSums = 5;      // terms, KL, ratios, clipped, active
+constexpr float kPoNear = 0.0625f;   // KL below which a row is gone over again: above, 5e-7 is 1e-5 of it
 
 // start of the caller's workspace
 struct PolicyHead {
@@ -58,7 +70,7 @@ struct PolicyArgs {
     void *grad;                   // [rows, V] or null
     PolicyHead *head;
     int *done;                    // [chunks]
-    float4 *row_sums;             // [rows]: term, KL, ratio, clipped
+    float4 *row_sums;             // [rows]: term, KL, ratio, clipped; of the ring kernel with y: see PolicyNear
     double *chunk_sums;           // [chunks, kPoSums]
     int32_t *status;
     int64_t rows;
@@ -141,6 +153,130 @@ struct PolicyState {
         }
     }
 };
+
+// A pair of fp32 numbers in one 64-bit register, so that the two-lane instructions need no moves between them.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_get(F2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+    F2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ F2 f2_ex2(F2 v) {
+    float a, b;
+    f2_get(v, a, b);
+    return f2(ex2(a), ex2(b));
+}
+__device__ __forceinline__ F2 f2_floor(F2 v) {   // what is below -1e30, or NaN, becomes -1e30
+    float a, b;
+    f2_get(v, a, b);
+    return f2(fmaxf(a, kNegBig), fmaxf(b, kNegBig));
+}
+
+// 16 bytes of logits less a reference, as pairs (sm_100 subtracts an fp32 number from a 16-bit one in one instruction,
+// rounded once)
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[2], float r, const float *) {
+    p[0] = f2_add(f2(__uint_as_float(u.x), __uint_as_float(u.y)), f2(-r, -r));
+    p[1] = f2_add(f2(__uint_as_float(u.z), __uint_as_float(u.w)), f2(-r, -r));
+}
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], float r, const __nv_bfloat16 *) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a, b;
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.bf16 %0, l, %3;\n\tsub.rn.f32.bf16 %1, h, %3;\n\t}" : "=f"(a), "=f"(b) : "r"(w[i]), "f"(r));
+        p[i] = f2(a, b);
+    }
+}
+__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], float r, const __half *) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        float a, b;
+        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %3;\n\t}" : "=f"(a), "=f"(b) : "r"(w[i]), "f"(r));
+        p[i] = f2(a, b);
+    }
+}
+
+// (e^-u - 1 + u) / u^2 for |u| < 1: the power series, whose first term left out is below 2^-23 of it
+constexpr float kPoSmall = 1.f;
+__device__ __forceinline__ F2 policy_phi(F2 u) {
+    constexpr float c[8] = {-1.f / 362880.f, 1.f / 40320.f, -1.f / 5040.f, 1.f / 720.f, -1.f / 120.f, 1.f / 24.f, -1.f / 6.f, 0.5f};
+    F2 p = f2(1.f / 3628800.f, 1.f / 3628800.f);
+#pragma unroll
+    for (int k = 0; k < 8; k++) p = f2_fma(u, p, f2(c[k], c[k]));
+    return p;
+}
+// A thread's sums of e = e^(x - r), e u and e phi(u) with u = x - y - o
+struct PolicyNearAcc {
+    F2 s = 0, u_sum = 0, f_sum = 0;   // (0, 0)
+    template <int N>
+    __device__ __forceinline__ void add(const F2 (&x)[N], const F2 (&y)[N], float r, float o) {
+        const auto both = [](float v) { return f2(v, v); };
+        F2 e[N], u[N];
+        float most = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+            e[i] = f2_ex2(f2_fma(x[i], both(kLog2e), both(-r * kLog2e)));   // (what r log2e is rounded by divides out)
+            u[i] = f2_add(f2_fma(y[i], both(-1.f), x[i]), both(-o));
+            float u0, u1;
+            f2_get(u[i], u0, u1);
+            asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(most) : "f"(most), "f"(u0), "f"(u1));
+            s = f2_add(s, e[i]);
+        }
+        if (most < kPoSmall) {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                const F2 eu = f2_mul(e[i], u[i]);
+                u_sum = f2_add(u_sum, eu);
+                f_sum = f2_fma(f2_mul(eu, u[i]), policy_phi(u[i]), f_sum);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; i++) {
+                float e0, e1, u0, u1, y0, y1, p0, p1;
+                // (x = -inf: u is made a number, e is 0, and what is left of the term is what the reference has there)
+                u[i] = f2_floor(u[i]);
+                u_sum = f2_fma(e[i], u[i], u_sum);
+                f2_get(e[i], e0, e1);
+                f2_get(u[i], u0, u1);
+                f2_get(y[i], y0, y1);
+                f2_get(policy_phi(u[i]), p0, p1);
+                f_sum = f2_add(f_sum, f2(term(e0, u0, y0 - r + o, p0), term(e1, u1, y1 - r + o, p1)));
+            }
+        }
+    }
+    __device__ __forceinline__ void add1(float x, float y, float r, float o) {   // (a place without weight beside it)
+        const F2 px[1] = {f2(x, -INFINITY)}, py[1] = {f2(y, -INFINITY)};
+        add(px, py, r, o);
+    }
+    // e e^-u = e^(y - r + o), which holds where e^-u alone would not
+    static __device__ __forceinline__ float term(float e, float u, float yr, float phi) {
+        return fabsf(u) < kPoSmall ? e * (u * u) * phi : ex2(yr * kLog2e) - e + e * u;
+    }
+    static __device__ __forceinline__ float both(F2 v) {
+        float a, b;
+        f2_get(v, a, b);
+        return a + b;
+    }
+};
+// the KL from the sums
+__device__ __forceinline__ double policy_near_kl(double S, double U, double F) { return U / S + log1p((F - U) / S); }
 
 // d at v = 0, or 0 where that is no number
 template <typename T>
@@ -273,7 +409,7 @@ template <typename T, bool kRef>
 __global__ void __launch_bounds__(kPoThreads)
 policy_fwd_kernel(PolicyArgs a) {
     constexpr int kVec = Elem<T>::kVec;
-    __shared__ float red[5][kPoWarps];
+    __shared__ float red[5][kPoWarps], red_near[3][kPoWarps];
     __shared__ PolicyRow row_s;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t row = blockIdx.x;
@@ -348,6 +484,40 @@ policy_fwd_kernel(PolicyArgs a) {
         red[4][warp] = wsy;
     }
     __syncthreads();
+    bool near = false;
+    float shift = 0.f;   // o
+    if (kRef) {
+        float S = 0.f, Tt = 0.f, Sy = 0.f;
+        for (int w = 0; w < kPoWarps; w++) {
+            S += red[2][w];
+            Tt += red[3][w];
+            Sy += red[4][w];
+        }
+        const float mean = Tt / S;
+        shift = off + mean;
+        near = mean - ((M - off - My) + logf(S / Sy)) < kPoNear;   // the same in all threads
+        if (near) {
+            PolicyNearAcc acc;
+            for (int q = tid; q < nvec; q += kPoThreads) {
+                F2 px[kVec / 2], py[kVec / 2];
+                policy_pairs(xv[q], px, 0.f, x);
+                policy_pairs(yv[q], py, 0.f, x);
+                acc.add(px, py, M, shift);
+            }
+            for (int part = 0; part < 2; part++) {
+                const int e0 = part ? head + nvec * kVec : 0, e1 = part ? V : head;
+                for (int e = e0 + tid; e < e1; e += kPoThreads)
+                    acc.add1(Elem<T>::to_float(x[e]), Elem<T>::to_float(y[e]), M, shift);
+            }
+            const float we = warp_sum(acc.both(acc.s)), wu = warp_sum(acc.both(acc.u_sum)), wf = warp_sum(acc.both(acc.f_sum));
+            if (lane == 0) {
+                red_near[0][warp] = we;
+                red_near[1][warp] = wu;
+                red_near[2][warp] = wf;
+            }
+            __syncthreads();
+        }
+    }
     const int64_t tok = a.tokens[row];
     if (tid == 0) {
         double S = 0.0, Tt = 0.0, Sy = 0.0;
@@ -372,6 +542,13 @@ policy_fwd_kernel(PolicyArgs a) {
         if (kRef) {
             mean_d = Tt / S;
             kl = mean_d - (((double)M - (double)off - (double)My) + log_s - log(Sy));
+            if (near) {
+                double t[3] = {};
+                for (int k = 0; k < 3; k++)
+                    for (int w = 0; w < kPoWarps; w++) t[k] += red_near[k][w];
+                kl = policy_near_kl(t[0], t[1], t[2]);
+                mean_d = t[1] / t[0] + ((double)shift - (double)off);
+            }
         } else if (a.ref_logp) {
             const double u = (double)a.ref_logp[row] - lp, eu = expm1(u);
             kl = eu - u;
@@ -452,40 +629,6 @@ struct PolicyTurn {
         }
     }
 };
-
-// A pair of fp32 numbers in one 64-bit register, so that the two-lane instructions need no moves between them.
-using F2 = unsigned long long;
-__device__ __forceinline__ F2 f2(float a, float b) {
-    F2 r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void f2_get(F2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
-    F2 r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
-    F2 r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-    return r;
-}
-__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
-    F2 r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-    return r;
-}
-__device__ __forceinline__ F2 f2_ex2(F2 v) {
-    float a, b;
-    f2_get(v, a, b);
-    return f2(ex2(a), ex2(b));
-}
-__device__ __forceinline__ F2 f2_floor(F2 v) {   // what is below -1e30, or NaN, becomes -1e30
-    float a, b;
-    f2_get(v, a, b);
-    return f2(fmaxf(a, kNegBig), fmaxf(b, kNegBig));
-}
 
 // Waits for a phase of a barrier.  false: gave up.
 __device__ __forceinline__ bool policy_wait(uint64_t *mbar, uint32_t parity, int polls) {
@@ -583,31 +726,6 @@ struct PolicyAcc {
     }
 };
 
-// 16 bytes of logits less a reference, as pairs (sm_100 subtracts an fp32 number from a 16-bit one in one instruction,
-// rounded once)
-__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[2], float r, const float *) {
-    p[0] = f2_add(f2(__uint_as_float(u.x), __uint_as_float(u.y)), f2(-r, -r));
-    p[1] = f2_add(f2(__uint_as_float(u.z), __uint_as_float(u.w)), f2(-r, -r));
-}
-__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], float r, const __nv_bfloat16 *) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float a, b;
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.bf16 %0, l, %3;\n\tsub.rn.f32.bf16 %1, h, %3;\n\t}" : "=f"(a), "=f"(b) : "r"(w[i]), "f"(r));
-        p[i] = f2(a, b);
-    }
-}
-__device__ __forceinline__ void policy_pairs(const uint4 &u, F2 (&p)[4], float r, const __half *) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; i++) {
-        float a, b;
-        asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tsub.rn.f32.f16 %0, l, %3;\n\tsub.rn.f32.f16 %1, h, %3;\n\t}" : "=f"(a), "=f"(b) : "r"(w[i]), "f"(r));
-        p[i] = f2(a, b);
-    }
-}
-
 // the gradient of pairs of logits
 template <bool kRef, bool kCareful, int N>
 __device__ __forceinline__ void policy_grad_pairs(const PolicyRow &p, const F2 (&x)[N], const F2 (&y)[N], float (&out)[2 * N]) {
@@ -663,8 +781,7 @@ __device__ __forceinline__ PolicyNumbers policy_numbers(const PolicyArgs &a, con
     n.kl = n.mean = 0.f;
     n.inv_s = 1.f / p.S;
     if (kRef) {
-        n.mean = p.T / p.S;
-        n.kl = n.mean - logf(p.S / p.Sy);
+        n.mean = p.T / p.S;   // the KL apart: the gradient does not wait for it
     } else if (a.ref_logp) {
         const float z = (float)((double)ref - lp), em = expm1f(z);
         n.kl = policy_excess(z, em);
@@ -672,6 +789,13 @@ __device__ __forceinline__ PolicyNumbers policy_numbers(const PolicyArgs &a, con
     }
     return n;
 }
+
+// A row for policy_near_kernel: r and o (NaN: the row is not close), and the KL that the sums have got
+struct PolicyNear {
+    float r, o;
+    double kl;
+};
+static_assert(sizeof(PolicyNear) == sizeof(float4), "a PolicyNear for each of row_sums");
 
 // NT threads in each half, kPpVecs pieces of a chunk to each, three warps beside them
 template <typename T, bool kRef, int NT, int kPpVecs>
@@ -697,6 +821,7 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
         umma::mbar_init(hand_bar + tid, 1);
     }
     if (tid < 2) umma::mbar_init(cluster_bar + tid, 1);
+    pdl_trigger();   // (policy_near_kernel, which waits for all of this)
     umma::fence_smem_to_async();
     __syncthreads();
     if (ranks > 1) cluster_barrier();   // every CTA's barriers stand before a neighbour's sums arrive on them
@@ -836,10 +961,16 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
                 policy_arrive(hand_bar + n % kPpDepth);
                 if (rank == 0) {
                     if (!ok && a.status) atomicOr(a.status, DAT_STATUS_BAD_INDEX);
+                    double kl = m.kl;
+                    if (kRef) {
+                        kl = (double)p.T / p.S - log((double)p.S / p.Sy);
+                        const float o = kl < (double)kPoNear ? (p.r - p.ry) + m.mean : __int_as_float(0x7fc00000);
+                        reinterpret_cast<PolicyNear *>(a.row_sums)[row] = PolicyNear{p.r, o, kl};
+                    }
                     a.logp[row] = m.lp;
-                    a.kl[row] = m.kl;
+                    a.kl[row] = (float)kl;
                     sums[0] += (double)m.term;
-                    sums[1] += (double)m.kl;
+                    sums[1] += kl;
                     sums[2] += (double)m.u;
                     sums[3] += m.clipped ? 1.0 : 0.0;
                     sums[4] += 1.0;
@@ -1061,6 +1192,92 @@ policy_ring_kernel(PolicyArgs a, PolicyRing ring) {
     if (lane == 0) *a.loss = (float)((total[0] + (double)a.beta * total[1]) * a.head->inv_n);
 }
 
+// The KL of the rows whose models are close, after policy_ring_kernel: a CTA a row, from memory (see the top).  The KL
+// takes the place of what the ring kernel has put down, and the differences are added to the sums in the order of the CTAs.
+// HBM (4.2 GB that the ring kernel has read before) and the fp32 units: 32768 rows of 32000 bf16 logits, all close, 0.88 ms; a
+// handful of them 30 us (a row is 128 KB for one CTA).
+constexpr int kPnThreads = 256, kPnWarps = kPnThreads / 32, kPnPerSm = 5;   // (3 and 4 per SM, with more loads ahead: 3 to 13 % slower)
+template <typename T>
+__global__ void __launch_bounds__(kPnThreads, kPnPerSm)
+policy_near_kernel(PolicyArgs a) {
+    constexpr int kVec = Elem<T>::kVec;
+    __shared__ float red[2][3][kPnWarps];
+    __shared__ unsigned close_s[kPnWarps];
+    __shared__ int last_s;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    double more = 0.0;   // (thread 0)
+    int par = 0;
+    const auto gone_over = [&](int64_t row) {
+        const float4 raw = __ldcg(a.row_sums + row);
+        const float r = raw.x, o = raw.y;
+        const T *x = static_cast<const T *>(a.x) + row * a.V, *y = static_cast<const T *>(a.y) + row * a.V;
+        int head, nvec;
+        policy_split(true, x, a.V, head, nvec);
+        const uint4 *xv = reinterpret_cast<const uint4 *>(x + head), *yv = reinterpret_cast<const uint4 *>(y + head);
+        PolicyNearAcc acc;
+        for (int v = tid; v < nvec; v += kPnThreads) {
+            F2 px[kVec / 2], py[kVec / 2];
+            const uint4 ux = ld_stream16(xv + v), uy = ld_stream16(yv + v);
+            policy_pairs(ux, px, 0.f, x);
+            policy_pairs(uy, py, 0.f, x);
+            acc.add(px, py, r, o);
+        }
+        for (int part = 0; part < 2; part++) {
+            const int e0 = part ? head + nvec * kVec : 0, e1 = part ? a.V : head;
+            for (int e = e0 + tid; e < e1; e += kPnThreads) acc.add1(Elem<T>::to_float(x[e]), Elem<T>::to_float(y[e]), r, o);
+        }
+        const float sums[3] = {warp_sum(acc.both(acc.s)), warp_sum(acc.both(acc.u_sum)), warp_sum(acc.both(acc.f_sum))};
+        if (lane == 0) {
+#pragma unroll
+            for (int k = 0; k < 3; k++) red[par][k][warp] = sums[k];
+        }
+        __syncthreads();
+        if (tid == 0) {
+            double t[3] = {};
+            for (int k = 0; k < 3; k++)
+                for (int w = 0; w < kPnWarps; w++) t[k] += red[par][k][w];
+            const double kl = policy_near_kl(t[0], t[1], t[2]);
+            a.kl[row] = (float)kl;
+            more += kl - __hiloint2double(__float_as_int(raw.w), __float_as_int(raw.z));
+        }
+        par ^= 1;   // (the next row's barrier stands between this row's reads and the writes of the row after it)
+    };
+    pdl_wait();
+    // 256 rows at a time: which of them are close
+    for (int64_t first = blockIdx.x; first < a.rows; first += (int64_t)kPnThreads * gridDim.x) {
+        const int64_t mine = first + (int64_t)tid * gridDim.x;
+        bool is_close = mine < a.rows && !(a.mask && !a.mask[mine]);
+        if (is_close) {
+            const float o = __ldcg(&a.row_sums[mine].y);
+            is_close = o == o;
+        }
+        const unsigned b = __ballot_sync(0xffffffffu, is_close);
+        __syncthreads();   // the bits of the rows before have been read
+        if (lane == 0) close_s[warp] = b;
+        __syncthreads();
+        for (int w = 0; w < kPnWarps; w++)
+            for (unsigned bits = close_s[w]; bits; bits &= bits - 1)
+                gone_over(first + (int64_t)(32 * w + __ffs(bits) - 1) * gridDim.x);
+    }
+    if (tid == 0) {
+        a.chunk_sums[blockIdx.x] = more;   // whose first use is over
+        __threadfence();
+        last_s = atomicAdd(a.done, 1) == (int)gridDim.x - 1;
+    }
+    __syncthreads();
+    if (!last_s || warp > 0) return;
+    __threadfence();
+    double t = 0.0;
+    for (int c = lane; c < (int)gridDim.x; c += 32) t += __ldcg(a.chunk_sums + c);
+#pragma unroll
+    for (int q = 16; q > 0; q >>= 1) t += __shfl_xor_sync(0xffffffffu, t, q);
+    if (lane == 0 && t != 0.0) {
+        const double kl = __ldcg(a.stats + 1) + t;
+        a.stats[1] = kl;
+        *a.loss = (float)((__ldcg(a.stats) + (double)a.beta * kl) * a.head->inv_n);
+    }
+}
+
 struct PolicyBackwardArgs {
     const void *x, *y;
     const int64_t *tokens;
@@ -1152,6 +1369,13 @@ static int policy_ring_launch(const PolicyArgs &a, const PolicyRing &ring, int s
     if (cudaFuncSetAttribute(policy_ring_kernel<T, kRef, NT, kPpVecs>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
         return check_launch(who);
     launch_after(policy_ring_kernel<T, kRef, NT, kPpVecs>, (unsigned)n * ring.ranks, 2 * NT + 96, smem, st, ring.ranks, a, ring);
+    if (kRef) {
+        int64_t grid = (int64_t)di.sm_count * kPnPerSm;
+        if (grid > a.rows) grid = a.rows;
+        if (grid > kPoMaxCtas) grid = kPoMaxCtas;
+        if (int rc = check_launch(who)) return rc;
+        launch_after(policy_near_kernel<T>, (unsigned)grid, kPnThreads, 0, st, 1, a);
+    }
     return check_launch(who);
 }
 

@@ -1,0 +1,74 @@
+"""``dag_policy_loss`` at the edges of its numerics, against plain torch in 64 bits, row by row."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from test_policy_preference import policy_call, policy_inputs, policy_oracle, row_tolerance, run_policy
+
+DEV = "cuda:0"
+U = 2.0 ** -24          # half a step of fp32 relative to the value
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def kl_in_64_bits(x, y):
+    """The KL of softmax(x) to softmax(y) as a sum of terms that are not negative: sum p (e^-u - 1 + u) with u = log p - log q
+    does not cancel."""
+    p, q = torch.log_softmax(x.double(), -1), torch.log_softmax(y.double(), -1)
+    u = p - q
+    return (p.exp() * torch.where(u.abs() < 1e-2, u * u * (0.5 - u / 6 + u * u / 24 - u ** 3 / 120), torch.expm1(-u) + u)).sum(-1)
+
+
+def check_kl(x, y, kw, V, name):
+    """Each term of the sum is off by as much as its probability (row_tolerance, with an exponent below 16) and by a few
+    roundings of its own, and none is negative: the KL is off by that part of itself."""
+    loss, logp, kl, stats = policy_call(x, kl_coef=0.1, **{**kw, "ref_logits": y})
+    want = kl_in_64_bits(x, y)
+    off = (kl.double() - want).abs()
+    assert (off <= 2 * row_tolerance(V) * want).all(), (name, float((off / want.clamp(min=1e-300)).max()), float(want.min()))
+    assert abs(float(stats[1]) - float(want.sum())) <= 2 * row_tolerance(V) * float(want.sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("B,L,V", [(1, 3, 1000), (2, 100, 1500), (1, 2, 9001), (2, 250, 5003), (1, 3, 32000), (1, 160, 30001),
+                                   (1, 1, 128000)])
+def test_kl_of_a_reference_close_to_the_policy(B, L, V, dtype):
+    """Where training with a reference model starts: logits that differ by a thousandth to a tenth, by a constant beside,
+    or not at all."""
+    x, kw = policy_inputs(B, L, V, dtype, seed=V)
+    noise = torch.randn(B, L, V, generator=torch.Generator().manual_seed(3)).to(DEV)
+    for size in (1e-3, 1e-2, 1e-1, 0.3, 1.0):
+        check_kl(x, (x.float() + size * noise).to(dtype), kw, V, size)
+    if dtype == torch.float32:
+        check_kl(x, x + 0.01 * noise + 2, kw, V, "constant")
+    same = policy_call(x, kl_coef=0.1, **{**kw, "ref_logits": x.clone()})
+    assert not same[2].any() and float(same[3][1]) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [1000, 9001, 30001, 100000])
+def test_kl_of_models_that_differ_at_the_token(V, dtype):
+    """The token's own logit far from the reference's, at tokens of any probability, and all others close."""
+    x, kw = policy_inputs(1, 8, V, dtype, seed=V + 1)
+    tok = kw["tokens"].unsqueeze(-1)
+    noise = torch.randn(1, 8, V, generator=torch.Generator().manual_seed(4)).to(DEV)
+    y = (x.float() + 0.05 * noise).to(dtype)
+    up = torch.tensor([3.0, -3.0, 0.5, -0.5, 6.0, -6.0, 1.0, 0.1], device=DEV).view(1, 8, 1)
+    y = y.scatter(-1, tok, (x.float().gather(-1, tok) + up).to(dtype))
+    check_kl(x, y, kw, V, "token")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [1000, 9001, 30001])
+def test_gradient_of_a_reference_close_to_the_policy(V):
+    """The gradient of the KL alone (no advantage): p (d - E d)."""
+    x, kw = policy_inputs(1, 6, V, torch.float32, seed=V + 2)
+    kw["adv"].zero_()
+    kw["ref_logits"] = x + 0.01 * torch.randn(1, 6, V, generator=torch.Generator().manual_seed(5)).to(DEV)
+    got, want = run_policy(x, kw, kl_coef=1.0)[4].double().cpu().numpy(), policy_oracle(x, kl_coef=1.0, **kw)[4]
+    # d is a difference of logits below 16, rounded there, and d - E d is about 0.03 at most
+    for a, b in zip(got[0], want[0]):
+        assert np.abs(a - b).max() <= 1e-3 * np.abs(b).max()
