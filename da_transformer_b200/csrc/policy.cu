@@ -585,14 +585,15 @@ policy_fwd_kernel(PolicyArgs a) {
 // and as many of the reference took 1.42 ms.)  Measured there: 1.12 to 1.16 ms, 5.3 to 5.5 TB/s of the bytes that it
 // cannot do without; 32768 rows of 42000 fp16 logits, one in eight active: 0.63 ms for the whole call, 5.4 TB/s.
 // The sums are taken relative to the token's logits r = x[token], ry = y[token] in place of the maxima: they are at
-// least 1, and a row where one overflows (or the token's logit is no number) takes the maxima after all.  One
+// least 1, and a row where one passes kPpHuge (a token less likely than e^-41, or no number) takes the maxima after all.  One
 // barrier per row; every thread puts the row's numbers together for itself.
 // Next to HBM the special-function unit bounds it: three exponentials per logit pair with the full KL, 24 of its
 // cycles per 32 pairs and scheduler against 33 that HBM takes for the 6 bytes of each at 16 bits.
 // ---------------------------------------------------------------------------------------------------
 constexpr int kPpPolls = 1 << 20;      // bound of a wait (never reached)
 constexpr int kPpZeros = 4096;         // bytes of zeros
-constexpr float kPpHuge = 0x1p100f;
+// sums up to here keep the gradient's factors, c / (N S), normal numbers for any c / N above 2^-66
+constexpr float kPpHuge = 0x1p60f;
 
 constexpr int kPpDepth = 4;            // rows under way in a CTA
 constexpr int kPpRanks = 8;            // CTAs that share a row at most

@@ -72,3 +72,24 @@ def test_gradient_of_a_reference_close_to_the_policy(V):
     # d is a difference of logits below 16, rounded there, and d - E d is about 0.03 at most
     for a, b in zip(got[0], want[0]):
         assert np.abs(a - b).max() <= 1e-3 * np.abs(b).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [700, 9001, 40000])
+@pytest.mark.parametrize("ref", [False, True])
+def test_small_gradients_of_unlikely_tokens(V, ref):
+    """A token whose log-probability is -41 to -69 (in the reference model too) and a coefficient of 1e-13: the gradient of
+    the likely logits is c p, whatever the sums are taken relative to."""
+    x, kw = policy_inputs(1, 8, V, torch.float32, seed=V + 3)
+    tok = kw["tokens"].unsqueeze(-1)
+    low = x.amax(-1, keepdim=True) - torch.tensor([30., 41., 43., 50., 60., 66., 68., 75.], device=DEV).view(1, 8, 1)
+    x = x.scatter(-1, tok, low)
+    if ref:
+        kw["ref_logits"] = x * 0.95 + 0.1 * torch.randn(1, 8, V, generator=torch.Generator().manual_seed(6)).to(DEV)
+    kw["old"] = (torch.log_softmax(x.double(), -1).gather(-1, tok).squeeze(-1) - 0.05).float()
+    kw["adv"] = torch.full_like(kw["adv"], 1e-13)
+    coef = 1e-13 if ref else 0.0
+    got, want = run_policy(x, kw, kl_coef=coef)[4].double().cpu().numpy(), policy_oracle(x, kl_coef=coef, **kw)[4]
+    # log-probabilities near -70 are rounded by 2^-24 of them twice, the ratio with them
+    for a, b in zip(got[0], want[0]):
+        assert np.abs(a - b).max() <= (1e-4 + 300 * U) * np.abs(b).max()
