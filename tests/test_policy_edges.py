@@ -93,3 +93,43 @@ def test_small_gradients_of_unlikely_tokens(V, ref):
     # log-probabilities near -70 are rounded by 2^-24 of them twice, the ratio with them
     for a, b in zip(got[0], want[0]):
         assert np.abs(a - b).max() <= (1e-4 + 300 * U) * np.abs(b).max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [700, 9001, 40000])
+@pytest.mark.parametrize("ref", [False, True])
+def test_logits_far_apart_row_by_row(V, ref):
+    """The token's logit 60 to 200 below the largest, which no sum relative to it holds in 32 bits: each row against bounds
+    of its own numbers, far below its own gradient."""
+    rows = [0.0, 60.0, 80.0, 100.0, 150.0, 200.0]
+    x, kw = policy_inputs(1, len(rows), V, torch.float32, seed=V + 4)
+    tok = kw["tokens"].unsqueeze(-1)
+    top = (tok + 1) % V
+    x = x.scatter_add(-1, top, torch.tensor(rows, device=DEV).view(1, -1, 1))
+    if ref:
+        kw["ref_logits"] = x * 0.9 + 0.5 * torch.randn(1, len(rows), V, generator=torch.Generator().manual_seed(7)).to(DEV)
+    every = torch.log_softmax(x.double(), -1)
+    kw["old"] = (every.gather(-1, tok).squeeze(-1) - 0.05).float()
+    kw["adv"] = torch.linspace(0.5, 2, len(rows), device=DEV).view(1, -1)
+    beta = 0.1 if ref else 0.0
+    got = run_policy(x, kw, kl_coef=beta)
+    want = policy_oracle(x, kl_coef=beta, **kw)
+    p = every.exp()[0].cpu().numpy()
+    d = (x.double() - kw["ref_logits"].double())[0].cpu().numpy() if ref else np.zeros_like(p)
+    tol = row_tolerance(V)
+    for n in range(len(rows)):
+        lp, kl, g = float(got[1][0, n]), float(got[2][0, n]), got[4][0, n].double().cpu().numpy()
+        wlp, wkl, wg = want[1][0, n], want[2][0, n], want[4][0, n]
+        near = p[n] > 1e-12                                   # the logits that carry the row
+        reach = np.abs(d[n] - d[n][near].mean())[near].max()   # how far their d are apart
+        far = np.abs(d[n]).max()                              # what d is rounded at
+        assert abs(lp - wlp) <= tol + 3 * U * abs(wlp)
+        if ref:
+            bound = 2 * tol * (1 + reach) + 4 * U * far
+            assert abs(kl - wkl) <= bound
+            assert bound < 0.05 * want[2].max()
+        # the ratio is off by as much as the log-probability; the coefficient is below 2 of 1/N, p off by the exponent's part
+        ratio = 2 * (tol + 4 * U * (abs(wlp) + abs(float(kw["old"][0, n]))))
+        bound = (ratio + 2 * tol + beta * (2 * tol * (1 + reach) + 4 * U * far)) / len(rows)
+        assert bound < 0.05 * np.abs(wg).max()
+        assert np.abs(g - wg).max() <= bound, (n, np.abs(g - wg).max(), bound)
