@@ -8,11 +8,12 @@
 //     dT[k,h] = sum over (b,i,d) with bucket[d] = k of dc[b,i,i+1+d,h].
 //
 // HBM-bound: the scores of the valid transitions are read once forward and once backward, the band is written
-// forward, the dense gradient backward.  A CTA owns a vertex at a time and keeps its scores in registers, a
-// thread the same distances and heads (16 bytes: four heads of one distance) for every vertex it meets, so that
-// the bias is expanded by distance once per CTA (shared memory, log2 units) and the table's gradient gathers in
-// its registers; the partial sums of the CTAs are added in a fixed order (no atomics: results repeat bit for
-// bit).  One exponential per score and direction:
+// forward, the dense gradient backward.  A vertex's scores lie in shared memory while it is worked on, and the exponentials
+// and then the gradient take their place (a warp per vertex), or in registers (a CTA per vertex).  The bias is added in log2
+// units; the table's gradient is gathered by distance over the vertices that a thread meets, and the partial sums of the CTAs
+// are added in a fixed order in 64 bits (no atomics: results repeat bit for bit).  A thread's own sums are fp32, over some
+// hundred vertices: 2^-24 of the sum in each addition, less than what the scores' gradients are rounded by.  One
+// exponential per score and direction:
 //   forward   e = exp(z - r_h), r_h the score of the nearest successor in place of the maximum over all of them:
 //             the sum is at least 1, and a vertex where it overflows (a score 60 above r_h) or whose nearest
 //             successor is masked takes the maximum after all.  links = log sum_h e_h exp(g_h) / S_h,
@@ -192,6 +193,8 @@ __device__ __forceinline__ float4 lb_grad(float4 soft, float4 q, float w, const 
     return q;
 }
 
+// A CTA per vertex.  A thread holds the same distances and heads (16 bytes: four heads of one distance) of every vertex, the
+// scores in registers; the bias is expanded by distance once per CTA.
 // Shared memory of both kernels: the bias by distance [K * H], two rows of scores [K * H], red [2][NT / 32][H].
 // A row's scores are copied while the row before is worked on, its mask is read one row earlier still.
 // G = H / 4 vectors per distance; thread t holds the vectors t, t + NT, ... of a vertex's row (U of them).
@@ -1483,10 +1486,12 @@ static int lw_launch(const LbArgs &a, bool backward, int &parts, cudaStream_t st
                                              a.head_lse_in, a.mk, a.span, a.lb, std::ref(lay), a.grad_content,
                                              a.grad_log_gates, a.part, a.B, a.L, a.H, a.K);
     };
-    // Two CTAs per SM, of eight warps, where their rings hold more than the longest row; else one of twelve; longer rows
-    // leave room for eight.  (16 graphs of 1024 vertices, band of 256, forward: 30 us with 16 warps per SM, 43 with 12.)
+    // Two CTAs per SM, of eight warps, where their rings hold the longest row; else one of twelve; longer rows leave room
+    // for eight.  Forward alone in a graph, 16 against 12 warps per SM: 16 graphs of 1024 vertices and 8 heads, bands of 256,
+    // 300, 340 and 380 (the largest that fits) 39 / 43 / 47 / 49 against 43 / 47 / 49 / 53 us; 64 of 512 and 4 heads 49
+    // against 55; 32 of 512, 12 heads and a band of 200 64 against 66, 16 heads and bands of 150 and 190 45 / 51 against 47 / 53.
     if (!backward) {
-        if (two >= row + row / 4) return fwd(lw_fwd_kernel<G, kExact, 2>, LwInt<2>(), 2);
+        if (two >= row) return fwd(lw_fwd_kernel<G, kExact, 2>, LwInt<2>(), 2);
         if (one >= row) return fwd(lw_fwd_kernel<G, kExact, 3>, LwInt<3>(), 1);
         return fwd(lw_fwd_kernel<G, kExact, 2>, LwInt<2>(), 1);
     }

@@ -328,3 +328,12 @@ def test_workspace_has_no_more_bands_than_ctas_that_run_at_once():
         if H in (4, 8, 16, 32):
             bands = max(bands, sms * min(16, 232448 // (3 * band)))
         assert sums <= size(B, L, H, K) <= sums + bands * band + 64, (B, L, H, K)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("B,L,H,K", [(2, 400, 8, 380), (2, 400, 8, 383), (2, 400, 8, 386), (3, 360, 8, 340), (2, 640, 4, 630),
+                                     (2, 200, 16, 195)])
+def test_rows_that_all_but_fill_their_ring(B, L, H, K):
+    """A ring with no room for the next row beside the longest: its copy begins when the row before has been worked off."""
+    content, gates, table, grad, bk, nonpad = make(B, L, H, K, buckets=32, seed=K)
+    against_64_bits(content, gates, table, bk, K, grad, 16.0, nonpad_mask=nonpad)
