@@ -133,3 +133,115 @@ def test_logits_far_apart_row_by_row(V, ref):
         bound = (ratio + 2 * tol + beta * (2 * tol * (1 + reach) + 4 * U * far)) / len(rows)
         assert bound < 0.05 * np.abs(wg).max()
         assert np.abs(g - wg).max() <= bound, (n, np.abs(g - wg).max(), bound)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [1001, 9001, 40000])
+def test_close_reference_with_forbidden_tokens(V, dtype):
+    """Tokens that both models forbid, and tokens that the policy alone forbids, to which the reference gives little: the KL
+    counts what the reference has there."""
+    x, kw = policy_inputs(2, 6, V, dtype, seed=V + 5)
+    y = (x.float() + 0.05 * torch.randn(2, 6, V, generator=torch.Generator().manual_seed(8)).to(DEV)).to(dtype)
+    gen = torch.Generator().manual_seed(9)
+    ban = (torch.rand(V, generator=gen) < 0.2).to(DEV)
+    ban[kw["tokens"].unique()] = False
+    for alone in (False, True):
+        xx, yy = x.clone(), y.clone()
+        xx[..., ban] = float("-inf")
+        yy[..., ban] = float("-inf")
+        if alone:
+            some = ban.nonzero()[:40, 0]
+            yy[1][..., some] = y[1][..., some] - 9
+        kw["old"] = (torch.log_softmax(xx.double(), -1).gather(-1, kw["tokens"].unsqueeze(-1)).squeeze(-1) - 0.1).float()
+        loss, _, kl, stats = policy_call(xx, kl_coef=0.1, **{**kw, "ref_logits": yy})
+        p, q = torch.log_softmax(xx.double(), -1), torch.log_softmax(yy.double(), -1)
+        u = torch.where(p > float("-inf"), p - q, 0)
+        # sum p (e^-u - 1 + u), plus what the reference has where the policy has nothing
+        want = (p.exp() * torch.where(u.abs() < 1e-2, u * u * (0.5 - u / 6 + u * u / 24 - u ** 3 / 120), torch.expm1(-u) + u)).sum(-1)
+        want += torch.where(p > float("-inf"), 0, q.exp()).sum(-1)
+        assert float(want.max()) < 0.05 and float(want.min()) > 1e-4
+        assert ((kl.double() - want).abs() <= 2 * row_tolerance(V) * want).all(), float(((kl.double() - want).abs() / want).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [900, 9001])
+def test_sums_and_loss_take_the_close_rows_as_they_are_returned(V):
+    """Some rows close, some not, some masked: the loss and the sums are those of the returned KL; twice the same bits."""
+    B, L = 3, 70
+    x, kw = policy_inputs(B, L, V, torch.float32, seed=V + 6, link=True, mask=0.6)
+    noise = torch.randn(B, L, V, generator=torch.Generator().manual_seed(10)).to(DEV)
+    size = 10.0 ** torch.linspace(-4, 0, L, device=DEV).view(1, L, 1)
+    kw["ref_logits"] = x + size * noise
+    got = run_policy(x, kw, kl_coef=0.7)
+    again = run_policy(x, kw, kl_coef=0.7)
+    assert all(torch.equal(a, b) for a, b in zip(got, again))
+    loss, _, kl, stats = got[:4]
+    n = int(kw["mask"].sum())
+    want = kl_in_64_bits(x, kw["ref_logits"])
+    on = kw["mask"]
+    assert ((kl.double() - want)[on].abs() <= 2 * row_tolerance(V) * want[on]).all() and not kl[~on].any()
+    # the sum is of 64-bit numbers that are returned rounded once
+    assert abs(float(stats[1]) - float(kl.double().sum())) <= 1.01 * U * float(kl.double().sum())
+    total = (float(stats[0]) + 0.7 * float(stats[1])) / n
+    assert abs(float(loss) - total) <= 2 * U * abs(total) + 1e-9 * 0.7
+    assert int(stats[4]) == n
+
+
+@pytest.mark.gpu
+def test_close_rows_of_a_batch_longer_than_a_round():
+    """More rows than the CTAs look at in one round (256 each), close ones in all rounds."""
+    B, L, V = 2, 110000, 4100
+    gen = torch.Generator(device=DEV).manual_seed(11)
+    x = torch.randn(B, L, V, generator=gen, device=DEV, dtype=torch.bfloat16).mul_(2)
+    y = torch.randn(B, L, V, generator=gen, device=DEV, dtype=torch.bfloat16).mul_(0.05).add_(x)
+    far = torch.arange(L, device=DEV) % 3 == 1
+    for b in range(B):
+        y[b, far] *= 0.5
+    tokens = torch.randint(0, V, (B, L), generator=gen, device=DEV)
+    zero = torch.zeros(B, L, device=DEV)
+    mask = torch.rand(B, L, generator=gen, device=DEV) < 0.8
+    with torch.no_grad():
+        loss, logp, kl, stats = policy_call(x, tokens, zero - 8, zero + 1, mask=mask, ref_logits=y, kl_coef=0.1)
+    assert not kl[~mask].any()
+    at = torch.cat([torch.arange(0, L, 997, device=DEV), torch.arange(L - 50, L, device=DEV)])
+    for b in range(B):
+        want = kl_in_64_bits(x[b, at], y[b, at])
+        on = mask[b, at]
+        assert ((kl[b, at].double() - want)[on].abs() <= 2 * row_tolerance(V) * want[on]).all()
+    assert abs(float(stats[1]) - float(kl.double().sum())) <= 1.01 * U * float(kl.double().sum())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("V", [500, 20000])
+def test_close_rows_on_streams_and_in_graphs(V):
+    x, kw = policy_inputs(2, 40, V, torch.bfloat16, seed=14, link=True, mask=0.5)
+    kw["ref_logits"] = (x.float() + 0.05 * torch.randn(2, 40, V, generator=torch.Generator().manual_seed(12)).to(DEV)).to(x.dtype)
+    want = run_policy(x, kw, kl_coef=0.1)
+    stat = {n: t.clone() for n, t in kw.items()}
+    xs = torch.zeros_like(x).requires_grad_()
+    stat["link"].requires_grad_()
+
+    def step():
+        loss, logp, kl, st = policy_call(xs, kl_coef=0.1, **stat)
+        return (loss.detach(), logp, kl, st) + torch.autograd.grad(loss, (xs, stat["link"]))
+
+    side = torch.cuda.Stream(DEV)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+        for a, b in zip(run_policy(x, kw, kl_coef=0.1), want):
+            assert torch.equal(a, b)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        graphs.append((graph, out))
+    with torch.no_grad():
+        xs.copy_(x)
+    for graph, out in graphs + graphs[:1]:
+        graph.replay()
+        for a, b in zip(out, want):
+            assert torch.equal(a, b)
