@@ -275,8 +275,11 @@ struct PolicyNearAcc {
         return a + b;
     }
 };
-// the KL from the sums
-__device__ __forceinline__ double policy_near_kl(double S, double U, double F) { return U / S + log1p((F - U) / S); }
+// the KL from the sums (what the 64-bit roundings may leave below 0 is 0; NaN stays)
+__device__ __forceinline__ double policy_near_kl(double S, double U, double F) {
+    const double kl = U / S + log1p((F - U) / S);
+    return kl < 0.0 ? 0.0 : kl;
+}
 
 // d at v = 0, or 0 where that is no number
 template <typename T>

@@ -48,6 +48,26 @@ def test_kl_of_a_reference_close_to_the_policy(B, L, V, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("V", [2, 3, 50, 9001])
+def test_kl_is_not_negative(V):
+    """One token carries all but nothing of the row: KLs of 1e-25 to 1, below what the sums resolve."""
+    x, kw = policy_inputs(1, 3000 if V < 100 else 300, V, torch.float32, seed=V + 9)
+    x = x.scatter_add(-1, kw["tokens"].unsqueeze(-1), torch.full_like(kw["old"], 25.0).unsqueeze(-1))
+    size = 10.0 ** torch.linspace(-5, 0.5, x.shape[1], device=DEV).view(1, -1, 1)
+    y = x + size * torch.randn(x.shape, generator=torch.Generator().manual_seed(13)).to(DEV)
+    kl = policy_call(x, kl_coef=0.1, **{**kw, "ref_logits": y})[2]
+    want = kl_in_64_bits(x, y)
+    assert (kl >= 0).all()
+    # The KL lies with the other tokens, whose exponents reach 25 log2 e = 36: the exponential of one is off by 2 U, by U of its
+    # argument in the difference and by U of it in the product, U (2 + 2 * 36) in all.  A term e e^-u - e + e u carries that
+    # (e^-u + 1) / phi(u) times, below 6 for |u| >= 1 (5.2 at -1); the sums add as in row_tolerance.  A KL of 1/16 and more is
+    # a difference of log-sum-exps and of the mean of d, of row_tolerance each.  64-bit sums near 1 leave 1e-15.
+    d = float((x - y).abs().max())
+    bound = U * (V / 256 + 16 + 6 * 74) * want + torch.where(want >= 0.06, row_tolerance(V) * (2 + d), 0)
+    assert ((kl.double() - want).abs() <= bound + 1e-15).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("V", [1000, 9001, 30001, 100000])
 def test_kl_of_models_that_differ_at_the_token(V, dtype):
@@ -189,8 +209,8 @@ def test_sums_and_loss_take_the_close_rows_as_they_are_returned(V):
 
 
 @pytest.mark.gpu
-def test_close_rows_of_a_batch_longer_than_a_round():
-    """More rows than the CTAs look at in one round (256 each), close ones in all rounds."""
+def test_close_rows_of_a_long_batch():
+    """More rows than the CTAs look at together (256 each): they come back for the rest, with close ones among them."""
     B, L, V = 2, 110000, 4100
     gen = torch.Generator(device=DEV).manual_seed(11)
     x = torch.randn(B, L, V, generator=gen, device=DEV, dtype=torch.bfloat16).mul_(2)
